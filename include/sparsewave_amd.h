@@ -462,6 +462,47 @@ int sw_attention_tile_floor(const int32_t *row_offsets,
                             int value_bytes, void *stream);
 
 /*
+ * Causal attention over a sliding window with sinks, an operator without a
+ * counterpart in the reference, for packed sequences: sequence i holds the
+ * queries query_offsets[i] .. query_offsets[i+1] - 1 and the keys
+ * key_offsets[i] .. key_offsets[i+1] - 1, its queries being the last of its
+ * keys (nq queries and nk keys: query r stands at place p = r + nk - nq).  A
+ * query sees key j <= p where p - j < window or j < sinks, and
+ *   output = sum exp(alpha q.k - m) v / l,  l = sum exp(alpha q.k - m),
+ *   log_sum = m + ln l,  m the largest alpha q.k that it sees.
+ *
+ * query[query_tokens][query_heads][d] and output alike, key and value
+ * [key_tokens][key_heads][d], log_sum[query_heads][query_tokens] fp32 (NULL:
+ * not wanted).  query_heads is a multiple of key_heads; consecutive query
+ * heads share a key head.  d is a multiple of 8 from 8 to 128.  `strides`
+ * holds the token and the head stride, in elements, of query, key, value and
+ * output (NULL: as the shapes above); rows start on 16 bytes, a token stride
+ * is at least d and at most 2^23 bytes, a head stride of 0 shares one head
+ * between all (not in the output).
+ *
+ * A query that sees no key (nq > nk) gets zeros and a log_sum of -inf.  Tokens
+ * outside every sequence are left as they were.  Offsets are clamped to the
+ * operands, so no contents of them reach outside.  An infinity or NaN of a
+ * key or value changes those queries alone that see it.  fp32 arithmetic;
+ * bf16 probabilities are rounded to bf16 for the matrix cores, their sum is
+ * not.  No atomics: repeated calls give the same bits.
+ */
+int sw_window_attention_f32(
+    const int32_t *query_offsets, const int32_t *key_offsets,
+    const float *query, const float *key, const float *value, float *output,
+    float *log_sum, int64_t sequences, int64_t query_tokens,
+    int64_t key_tokens, int64_t query_heads, int64_t key_heads, int64_t d,
+    const int64_t *strides, int64_t window, int64_t sinks, float alpha,
+    void *stream);
+int sw_window_attention_bf16(
+    const int32_t *query_offsets, const int32_t *key_offsets,
+    const uint16_t *query, const uint16_t *key, const uint16_t *value,
+    uint16_t *output, float *log_sum, int64_t sequences, int64_t query_tokens,
+    int64_t key_tokens, int64_t query_heads, int64_t key_heads, int64_t d,
+    const int64_t *strides, int64_t window, int64_t sinks, float alpha,
+    void *stream);
+
+/*
  * sparsewave.csr_row_at_position for a batch of positions:
  * out_rows[i] = (first j in [1, rows+1) with row_offsets[j] > positions[i]) - 1,
  * the row search of SparsePositionToSCF.cpp:225-271 that the position

@@ -20,8 +20,8 @@ __all__ = [
     "load_library", "spmv",
     "coo_spmv", "spmv_gather_floor", "bsr_slab_floor", "attention_tile_floor",
     "spmm", "bsr_spmm", "sddmm", "csr_row_reduce", "csr_rowwise_map",
-    "sparse_attention", "csr_row_at_position", "SDDMM_MUL", "SDDMM_AFFINE",
-    "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV", "MAP_SUB", "MAP_MUL",
+    "sparse_attention", "window_attention", "csr_row_at_position",
+    "SDDMM_MUL", "SDDMM_AFFINE", "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV", "MAP_SUB", "MAP_MUL",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -42,6 +42,7 @@ EXPORTED_SYMBOLS = (
     "sw_sddmm_csr_bf16_ws", "sw_csr_row_reduce_f32", "sw_csr_row_reduce_bf16",
     "sw_csr_rowwise_map_f32", "sw_csr_rowwise_map_bf16",
     "sw_sparse_attention_f32", "sw_sparse_attention_bf16",
+    "sw_window_attention_f32", "sw_window_attention_bf16",
     "sw_csr_row_at_position", "sw_attention_tile_floor",
     "sw_host_matrix_free", "sw_host_bsr_free", "sw_matrix_market_read",
     "sw_csr_binary_write", "sw_coo_binary_write", "sw_csr_binary_read",
@@ -171,6 +172,9 @@ def load_library():
                                                     I64, F, F, OP, P]),
         "sw_csr_row_at_position": (ctypes.c_int, [P, I64, P, P, I64, P]),
     }
+    for dt in ("_f32", "_bf16"):
+        sig["sw_window_attention" + dt] = (
+            ctypes.c_int, [P] * 7 + [I64] * 6 + [P, I64, I64, F, P])
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -616,6 +620,96 @@ def sparse_attention(row_offsets, column_indices, mask_values, query,
         _dev(scores, dt, "scores"), _dev(row_maximum, dt, "row_maximum"),
         _dev(row_sum, dt, "row_sum"), _dev(output, dt, "output"), rows, cols,
         nnz, d, dv, alpha, beta, _opts(options), _stream(stream)))
+    return output
+
+
+def _heads(t, dtype, name):
+    """Address and (row, head) strides of a [rows, heads, d] operand, whose
+    rows of d elements are consecutive."""
+    torch = _torch or _load_torch()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor, got {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    *outer, row, head, last = t.stride()
+    if last != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have consecutive elements in its last "
+                         "dimension")
+    # (a dimension of one has any stride: its packed one)
+    if t.shape[-2] == 1:
+        head = t.shape[-1]
+    if t.shape[-3] == 1:
+        row = max(head, t.shape[-1]) * t.shape[-2]
+    return (t.data_ptr(), *outer, row, head)
+
+
+def _one_device(stream, *tensors):
+    """All operands on the device whose stream the call goes to."""
+    torch = _torch or _load_torch()
+    at = None
+    for t in tensors:
+        if t is None or not t.is_cuda:
+            continue  # (not a device tensor: refused where it is taken)
+        if at is None:
+            at = (torch.cuda.current_device() if stream is None
+                  else stream.device.index)
+        if t.get_device() != at:
+            raise ValueError(
+                f"an operand is on {t.device}, but the call goes to a stream "
+                f"of cuda:{at}")
+
+
+def _window_shapes(query_offsets, key_offsets, query, key, value):
+    _need(query.dim() == 3 and key.dim() == 3 and
+          tuple(key.shape) == tuple(value.shape) and
+          query.shape[2] == key.shape[2],
+          "expected query [query_tokens, query_heads, d] and key and value "
+          "[key_tokens, key_heads, d]")
+    sequences = _rows_of(query_offsets, "query_offsets")
+    _need(tuple(key_offsets.shape) == (sequences + 1,),
+          "query and key offsets must have the same length")
+    return (sequences, query.shape[0], key.shape[0], query.shape[1],
+            key.shape[1], query.shape[2])
+
+
+def window_attention(query_offsets, key_offsets, query, key, value, output,
+                     log_sum, alpha, window, sinks=0, stream=None):
+    """Causal attention over a sliding window with sinks (no counterpart in
+    the reference): softmax(alpha q.k) v over the keys that a query sees.
+
+    Sequence i holds queries query_offsets[i] .. query_offsets[i + 1] - 1 of
+    query [query_tokens, query_heads, d] and the keys of the same places in
+    key_offsets of key and value [key_tokens, key_heads, d]; its queries are
+    the last of its keys.  A query at place p sees key j <= p where
+    p - j < window or j < sinks.  query_heads is a multiple of key_heads and
+    consecutive query heads share one; d is a multiple of 8 up to 128.
+    float32 or bfloat16, any strides of 16 bytes between rows and heads.
+
+    log_sum [query_heads, query_tokens] float32 receives the logarithms of
+    the softmax's sums, which the backward pass reads; None leaves them out.
+    A query that sees no key gets zeros and -inf; tokens of no sequence are
+    left as they were."""
+    torch = _torch or _load_torch()
+    shape = _window_shapes(query_offsets, key_offsets, query, key, value)
+    dt = _value_dtype(query, "query")
+    _need(tuple(output.shape) == tuple(query.shape),
+          "output must have query's shape")
+    if log_sum is not None:
+        _need(tuple(log_sum.shape) == (shape[3], shape[1]),
+              "log_sum must be [query_heads, query_tokens]")
+    _one_device(stream, query_offsets, key_offsets, query, key, value, output,
+                log_sum)
+    q, k, v, o = (_heads(t, dt, n) for t, n in (
+        (query, "query"), (key, "key"), (value, "value"),
+        (output, "output")))
+    strides = (ctypes.c_int64 * 8)(*q[1:], *k[1:], *v[1:], *o[1:])
+    _check(_fn("sw_window_attention", dt)(
+        _dev(query_offsets, torch.int32, "query_offsets"),
+        _dev(key_offsets, torch.int32, "key_offsets"), q[0], k[0], v[0], o[0],
+        None if log_sum is None else _dev(log_sum, torch.float32, "log_sum"),
+        *shape, strides, window, sinks, alpha, _stream(stream)))
     return output
 
 

@@ -25,6 +25,7 @@ SOURCES = [
     "sw_spmm.hip",
     "sw_bsr.hip",
     "sw_attention.hip",
+    "sw_window_attention.hip",
 ]
 
 # -packed-fp32-ops: keep hipcc from forming v_pk_{add,mul,fma}_f32.

@@ -1,0 +1,267 @@
+// Device-side building blocks of attention over [tokens][heads][d] operands:
+// fragments of the matrix cores, tiles of rows in LDS that are read both
+// along and across their rows, and the search for a packed sequence.
+//
+// A matrix product of 32 x 32 with K = 16 takes from lane l the eight
+// elements k = 8 (l / 32) + i of row (A) or column (B) l % 32, and leaves in
+// accumulator r of lane l the element of row 8 (r / 4) + 4 (l / 32) + r % 4
+// and column l % 32.  The eight accumulators 8 s .. 8 s + 7 of a result are
+// therefore a B operand of the next product as they stand, for the K indices
+// 16 s + 8 (i / 4) + 4 (l / 32) + i % 4: scores are computed as K Q^T, keys
+// in rows and queries in columns, and the probabilities stay in registers.
+// The A operand of that product runs across the rows of a tile (V^T, or K^T
+// in a gradient): bf16 tiles are read by the transposing LDS load, which
+// gives lane i of 16 column i of four rows.
+#pragma once
+
+#include "sw_device.h"
+
+namespace swd {
+
+typedef float v8f __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <typename T> struct FragOf;
+template <> struct FragOf<float> { using type = v8f; };
+template <> struct FragOf<uint16_t> { using type = v4u; };
+template <typename T> using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ v16f mma32(v4u a, v4u b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+      __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+      0);
+}
+// fp32 has K = 2 a product, one index of each half of the wave: element i of
+// both halves is product i, so the fragments are those of bf16
+__device__ __forceinline__ v16f mma32(v8f a, v8f b, v16f c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ v4f mma16(v4u a, v4u b, v4f c) {
+  return mfma_16x16x32_bf16(a, b, c);
+}
+__device__ __forceinline__ v4f mma16(v8f a, v8f b, v4f c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+// Eight fp32 values as a fragment (bf16: each rounded to nearest even).
+template <typename T> __device__ __forceinline__ Frag<T> make_frag(const float *x) {
+  if constexpr (sizeof(T) == 4)
+    return v8f{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+  else
+    return v4u{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+template <typename T> __device__ __forceinline__ Frag<T> zero_frag() {
+  if constexpr (sizeof(T) == 4)
+    return v8f{0, 0, 0, 0, 0, 0, 0, 0};
+  else
+    return v4u{0, 0, 0, 0};
+}
+// The fragment with element i alone, in the lanes where `keep` holds.
+template <typename T>
+__device__ __forceinline__ Frag<T> one_of_frag(Frag<T> f, int i, bool keep) {
+  Frag<T> r = zero_frag<T>();
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      r[e] = keep && e == i ? f[e] : 0.0f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      r[e] = keep && e == i / 2 ? f[e] & (i % 2 ? 0xFFFF0000u : 0xFFFFu) : 0u;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> negate_frag(Frag<T> f) {
+  if constexpr (sizeof(T) == 4)
+    return -f;
+  else
+    return f ^ 0x80008000u;
+}
+// sum of the products of two fragments' elements
+template <typename T>
+__device__ __forceinline__ float dot_frag(Frag<T> a, Frag<T> b, float c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      c = fmaf(a[e], b[e], c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c = fmaf(bf16_to_f32(a[e] & 0xFFFFu), bf16_to_f32(b[e] & 0xFFFFu), c);
+      c = fmaf(__uint_as_float(a[e] & 0xFFFF0000u),
+               __uint_as_float(b[e] & 0xFFFF0000u), c);
+    }
+  }
+  return c;
+}
+
+// Eight elements from 16-byte aligned global memory.
+__device__ __forceinline__ v4u ld_frag(const uint16_t *p) {
+  return *reinterpret_cast<const v4u *>(p);
+}
+__device__ __forceinline__ v8f ld_frag(const float *p) {
+  const v4f a = *reinterpret_cast<const v4f *>(p);
+  const v4f b = *reinterpret_cast<const v4f *>(p + 4);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Four consecutive fp32 values to an 8 (bf16) or 16 (fp32) byte aligned place.
+__device__ __forceinline__ void st4(float *p, float a, float b, float c,
+                                    float d) {
+  *reinterpret_cast<v4f *>(p) = v4f{a, b, c, d};
+}
+__device__ __forceinline__ void st4(uint16_t *p, float a, float b, float c,
+                                    float d) {
+  *reinterpret_cast<v2u *>(p) = v2u{pack_bf16x2(a, b), pack_bf16x2(c, d)};
+}
+
+// The value of lane l ^ 32 combined with the lane's own, in both.
+__device__ __forceinline__ float both_halves_max(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(
+      __float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float both_halves_sum(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(
+      __float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// ---- tiles of rows in LDS ----------------------------------------------------
+// Rows of D elements without padding, in chunks of 16 bytes; chunk c of row r
+// lies at place c ^ swizzle(r).  The swizzle keeps three reads free of bank
+// conflicts (64 banks of 4 bytes): 16 consecutive rows at one chunk (a
+// fragment along the rows), and, for bf16, two chunks of each of four
+// consecutive rows (a transposing load); the chunk's lowest bit must
+// therefore not be what alone tells neighbouring rows apart.  ROWS is a
+// multiple of 32 and a tile is filled by THREADS threads.
+template <typename T, int D, int ROWS, int THREADS> struct RowTile {
+  static constexpr int kChunks = D * (int)sizeof(T) / 16;
+  static constexpr int kPitch = D * (int)sizeof(T);
+  static constexpr int kBytes = ROWS * kPitch;
+  static constexpr int kPasses = ROWS * kChunks / THREADS;
+  static constexpr int kPassRows = THREADS / kChunks;
+  static_assert(ROWS * kChunks % THREADS == 0 && THREADS % kChunks == 0, "");
+
+  __device__ static __forceinline__ int swizzle(int row) {
+    if constexpr (sizeof(T) == 4)
+      return row & 15;
+    else if constexpr (kChunks == 16)
+      return ((row & 7) << 1) | ((row >> 3) & 1);
+    else
+      return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+  }
+  __device__ static __forceinline__ int place(int row, int chunk) {
+    return row * kPitch + ((chunk ^ swizzle(row)) << 4);
+  }
+
+  // A thread's part of a tile on its way from memory to LDS.
+  struct Staged { v4u x[kPasses]; };
+
+  // Rows 0 .. rows - 1 of the matrix at `base` (wave-uniform; row_bytes apart,
+  // d elements of each); elements past d and rows past the end are zero.  The
+  // descriptor bounds what is read: (ROWS - 1) row_bytes + 4 D < 2^31 is the
+  // host's check.
+  __device__ static __forceinline__ Staged fetch(const T *base, int rows,
+                                                 uint32_t row_bytes, int d) {
+    Staged s;
+    rows = rows < 0 ? 0 : rows > ROWS ? ROWS : rows;
+    const uint32_t bytes =
+        rows == 0 ? 0u : (uint32_t)(rows - 1) * row_bytes + d * sizeof(T);
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(base, bytes);
+    const int c = threadIdx.x % kChunks, row = threadIdx.x / kChunks;
+    // (an offset past every descriptor: reads zero)
+    const uint32_t at =
+        c * 16 < d * (int)sizeof(T) ? row * row_bytes + c * 16 : 0x80000000u;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+      s.x[p] = __builtin_bit_cast(
+          v4u, __builtin_amdgcn_raw_buffer_load_b128(
+                   r, (int)(at + p * kPassRows * row_bytes), 0, 0));
+    return s;
+  }
+  __device__ static __forceinline__ void put(char *lds, const Staged &s) {
+    const int c = threadIdx.x % kChunks, row = threadIdx.x / kChunks;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+      *reinterpret_cast<v4u *>(lds + place(row + p * kPassRows, c)) = s.x[p];
+  }
+
+  // Row 32 rb + l % 32, elements 16 s + 8 (l / 32) + i: the A operand with
+  // the tile's rows as rows.
+  __device__ static __forceinline__ Frag<T> along(const char *lds, int rb,
+                                                  int s) {
+    const int l = lane_id(), row = 32 * rb + (l & 31), h = l >> 5;
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const v4u *>(lds + place(row, 2 * s + h));
+    } else {
+      const v4f a = *reinterpret_cast<const v4f *>(lds + place(row, 4 * s + 2 * h));
+      const v4f b =
+          *reinterpret_cast<const v4f *>(lds + place(row, 4 * s + 2 * h + 1));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // Element 32 db + l % 32 of the rows 16 st + 8 (i / 4) + 4 (l / 32) + i % 4:
+  // the A operand with the tile's columns as rows, whose K indices are those
+  // of accumulators 8 (st % 2) .. of row block st / 2.
+  __device__ static __forceinline__ Frag<T> across(const char *lds, int st,
+                                                   int db) {
+    const int l = lane_id(), h = l >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) v4s lds_v4s;
+      const int i = l & 15;
+      const int row = 16 * st + 4 * h + (i >> 2);
+      const int chunk = 4 * db + 2 * ((l >> 4) & 1) + ((i & 3) >> 1);
+      const int sub = (i & 1) * 8;
+      const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_v4s *)(lds + place(row, chunk) + sub));
+      const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_v4s *)(lds + place(row + 8, chunk) + sub));
+      const v2u x = __builtin_bit_cast(v2u, a), y = __builtin_bit_cast(v2u, b);
+      return v4u{x.x, x.y, y.x, y.y};
+    } else {
+      v8f r;
+      const int col = 32 * db + (l & 31);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 16 * st + 8 * (i >> 2) + 4 * h + (i & 3);
+        r[i] = *reinterpret_cast<const float *>(
+            lds + place(row, col >> 2) + (col & 3) * 4);
+      }
+      return r;
+    }
+  }
+};
+
+// ---- packed sequences ----------------------------------------------------------
+// Sequence i of n holds tokens offsets[i] .. offsets[i + 1] - 1, and, cut into
+// tiles of 1 << shift tokens, the tile numbers (offsets[i] >> shift) + i up to
+// that of i + 1: at least as many as it has tiles, without a count of the
+// tiles before it.  Returns the sequence of tile number `tile`, which is
+// wave-uniform, by 64 probes a trip.
+__device__ __forceinline__ int sequence_of_tile(
+    const int32_t *__restrict__ offsets, int n, int tile, int shift) {
+  const int l = lane_id();
+  int from = 0, count = n; // the answer lies in [from, from + count)
+  while (count > 1) {
+    const int step = (count + kWave - 1) / kWave;
+    const int at = from + l * step;
+    const bool in = l * (int64_t)step < count;
+    const int32_t first = (offsets[in ? at : from] >> shift) + (in ? at : from);
+    // (probe 0 is at or before the tile: `from` starts there)
+    const uint64_t before = ballot(in && first <= tile);
+    const int k = before ? 63 - __builtin_clzll(before) : 0;
+    count = count - k * step < step ? count - k * step : step;
+    from += k * step;
+  }
+  return __builtin_amdgcn_readfirstlane(from);
+}
+
+} // namespace swd

@@ -1,0 +1,208 @@
+"""Window attention on the GPU against float64, element by element within
+bounds that the arithmetic gives (tests/_window_check.py)."""
+import math
+
+import pytest
+import torch
+
+import sparsewavecomp_amd as sw
+from _window_check import check, gradients, half_step, softmax, visible
+from gpu_util import DEV, say
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def offsets(lengths, start=0):
+    out = [start]
+    for n in lengths:
+        out.append(out[-1] + n)
+    return torch.tensor(out, dtype=torch.int32)
+
+
+def inputs(dtype, nq, nk, h, hk, d, seed=0, lead=0, tail=0):
+    """CPU operands for sequences of nq[i] queries and nk[i] keys, `lead`
+    tokens before the first and `tail` behind the last."""
+    gen = torch.Generator().manual_seed(seed)
+    def values(n, heads):
+        return torch.randn(lead + n + tail, heads, d, generator=gen).to(
+            DTYPES[dtype])
+    return (offsets(nq, lead), offsets(nk, lead), values(sum(nq), h),
+            values(sum(nk), hk), values(sum(nk), hk))
+
+
+def forward(qo, ko, q, k, v, alpha, window, sinks, fill=7.0):
+    out = torch.full(q.shape, fill, dtype=q.dtype, device=DEV)
+    lse = torch.full((q.shape[1], q.shape[0]), fill, device=DEV)
+    got = sw.window_attention(qo.to(DEV), ko.to(DEV), q.to(DEV), k.to(DEV),
+                              v.to(DEV), out, lse, alpha, window, sinks)
+    torch.cuda.synchronize()
+    assert got is out
+    return out.cpu(), lse.cpu()
+
+
+def expect(qo, ko, q, k, v, out, lse, alpha, window, sinks, fill=7.0):
+    t = half_step(q.dtype)
+    g = q.shape[1] // k.shape[1]
+    qd, kd, vd = q.double(), k.double(), v.double()
+    inside = torch.zeros(q.shape[0], dtype=torch.bool)
+    for i in range(len(qo) - 1):
+        a, b, c, e = int(qo[i]), int(qo[i + 1]), int(ko[i]), int(ko[i + 1])
+        inside[a:b] = True
+        see = visible(b - a, e - c, window, sinks)
+        for h in range(q.shape[1]):
+            o, ob, _, l, lb, _ = softmax(qd[a:b, h], kd[c:e, h // g],
+                                         vd[c:e, h // g], see, alpha, t)
+            check(f"output of sequence {i}, head {h}", out[a:b, h], o, ob)
+            check(f"log_sum of sequence {i}, head {h}", lse[h, a:b], l, lb)
+    assert torch.equal(out[~inside], torch.full_like(out[~inside], fill))
+    assert torch.equal(lse[:, ~inside], torch.full_like(lse[:, ~inside], fill))
+
+
+# (queries, keys), window, sinks: one token; a window of one; a window that
+# starts inside a tile; sinks that touch it, lie apart and fill more than a
+# tile; rows that see nothing (more queries than keys); empty sequences;
+# keys before the queries; tile borders at 32, 64 and 128 from both sides
+CASES = [
+    (([1], [1]), 1, 0),
+    (([1], [1]), 4096, 4),
+    (([5], [5]), 1, 0),
+    (([130], [130]), 1, 1),
+    (([33, 0, 127, 1, 129], [33, 0, 127, 1, 129]), 40, 3),
+    (([300], [300]), 64, 0),
+    (([257], [257]), 31, 100),
+    (([400], [400]), 100, 4),
+    (([400], [400]), 33, 65),
+    (([10, 200], [3, 150]), 50, 2),
+    (([7], [0]), 50, 2),
+    (([1, 20, 64], [500, 333, 64]), 128, 16),
+    (([128, 64], [256, 192]), 128, 0),
+    (([500], [500]), 2 ** 31 + 5, 0),
+    (([500], [500]), 10, 2 ** 40),
+    (([2] * 150, [2] * 150), 2, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_forward(dev, dtype, case):
+    (nq, nk), window, sinks = CASES[case]
+    say(f"window forward {dtype} {CASES[case]}")
+    x = inputs(dtype, nq, nk, 2, 1, 64, seed=case)
+    out, lse = forward(*x, 0.125, window, sinks)
+    expect(*x, out, lse, 0.125, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("h,hk,d", [(1, 1, 8), (3, 3, 24), (6, 2, 64),
+                                    (4, 1, 72), (2, 2, 96), (8, 2, 128),
+                                    (5, 1, 128)])
+def test_forward_heads(dev, dtype, h, hk, d):
+    say(f"window forward heads {dtype} {h} {hk} {d}")
+    x = inputs(dtype, [70, 131], [90, 131], h, hk, d, seed=d + h)
+    out, lse = forward(*x, 1 / math.sqrt(d), 48, 5)
+    expect(*x, out, lse, 1 / math.sqrt(d), 48, 5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_forward_leaves_other_tokens(dev, dtype):
+    say(f"window forward lead and tail {dtype}")
+    x = inputs(dtype, [40, 3, 150], [40, 9, 150], 2, 2, 64, seed=3, lead=13,
+               tail=200)
+    out, lse = forward(*x, 0.2, 30, 2)
+    expect(*x, out, lse, 0.2, 30, 2)
+
+
+@pytest.mark.parametrize("alpha", [-0.3, 0.0, 4.0])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_forward_alpha(dev, dtype, alpha):
+    say(f"window forward alpha {dtype} {alpha}")
+    x = inputs(dtype, [200], [200], 2, 1, 64, seed=5)
+    out, lse = forward(*x, alpha, 70, 2)
+    expect(*x, out, lse, alpha, 70, 2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_forward_strides(dev, dtype):
+    """Slices of one projection's output, heads before tokens, and one key
+    head shared by a stride of zero."""
+    say(f"window forward strides {dtype}")
+    gen = torch.Generator().manual_seed(11)
+    t, h, d = 150, 4, 64
+    packed = torch.randn(t, 3 * h, d, generator=gen).to(DTYPES[dtype]).to(DEV)
+    q, k, v = packed[:, :h], packed[:, h:2 * h], packed[:, 2 * h:]
+    qo = offsets([t]).to(DEV)
+    plain = torch.empty(t, h, d, dtype=q.dtype, device=DEV)
+    sw.window_attention(qo, qo, q.contiguous(), k.contiguous(), v.contiguous(),
+                        plain, None, 0.125, 40, 3)
+    wide = torch.full((h, t, d), 7.0, dtype=q.dtype, device=DEV)
+    sw.window_attention(qo, qo, q, k, v, wide.transpose(0, 1), None, 0.125,
+                        40, 3)
+    assert torch.equal(wide.transpose(0, 1), plain)
+    one_k, one_v = k[:, :1].expand(-1, h, -1), v[:, :1].expand(-1, h, -1)
+    shared = torch.empty_like(plain)
+    sw.window_attention(qo, qo, q, one_k, one_v, shared, None, 0.125, 40, 3)
+    sw.window_attention(qo, qo, q, k[:, :1], v[:, :1], plain, None, 0.125, 40, 3)
+    assert torch.equal(shared, plain)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("at", [0, 60, 100, 199])
+def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at):
+    """An infinity or NaN of one key and value reaches the queries that see
+    it, and no others."""
+    say(f"window forward {bad} at {at} {dtype}")
+    qo, ko, q, k, v = inputs(dtype, [200], [200], 2, 2, 64, seed=at)
+    window, sinks = 50, 2
+    sees = visible(200, 200, window, sinks)[:, at]
+    clean, clean_lse = forward(qo, ko, q, k, v, 0.125, window, sinks)
+    for what in ("value", "key"):
+        kk, vv = k.clone(), v.clone()
+        (vv if what == "value" else kk)[at, 1, 5] = bad
+        out, lse = forward(qo, ko, q, kk, vv, 0.125, window, sinks)
+        expect(qo, ko, q[:, :1], kk[:, :1], vv[:, :1], out[:, :1], lse[:1],
+               0.125, window, sinks)
+        x, y = out[~sees, 1].float(), clean[~sees, 1].float()
+        assert torch.isfinite(x).all()
+        # (a repeated pass may add up in another order)
+        if not sees.all():
+            assert (x - y).abs().max() <= 4 * half_step(q.dtype) * y.abs().max()
+        assert torch.isfinite(lse[1][~sees]).all()
+        if what == "value":
+            hit = out[sees, 1, 5].float()
+            assert torch.isnan(hit).all() if math.isnan(bad) else \
+                (hit == bad).all()
+            others = torch.cat([out[sees, 1, :5], out[sees, 1, 6:]], 1)
+            assert torch.isfinite(others).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_forward_repeats_and_graph(dev, dtype):
+    """The same bits again, on another stream, and from a captured graph that
+    is replayed with eager work between."""
+    say(f"window forward graph {dtype}")
+    qo, ko, q, k, v = (x.to(DEV) for x in inputs(
+        dtype, [100, 300], [100, 300], 4, 2, 128, seed=2))
+    out = torch.empty_like(q)
+    call = lambda o, **kw: sw.window_attention(qo, ko, q, k, v, o, None, 0.1,
+                                               64, 4, **kw)
+    call(out)
+    side = torch.cuda.Stream()
+    other = torch.empty_like(q)
+    side.wait_stream(torch.cuda.current_stream())
+    call(other, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(out, other)
+    replayed = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(replayed)
+    for i in range(3):
+        q.mul_(1.5)
+        call(out)
+        replayed.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, replayed)

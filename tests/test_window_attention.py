@@ -1,0 +1,83 @@
+"""What the window attention entry points refuse, before any launch."""
+import ctypes
+
+import pytest
+
+import sparsewavecomp_amd as sw
+
+A = 1 << 20  # an aligned address that no call here reaches
+
+
+def c_forward(strides=None, dt="_bf16", **kw):
+    a = dict(query_offsets=A, key_offsets=A, query=A, key=A, value=A, output=A,
+             log_sum=None, sequences=1, query_tokens=10, key_tokens=10,
+             query_heads=4, key_heads=2, d=64, window=8, sinks=1, alpha=1.0)
+    a.update(kw)
+    s = (ctypes.c_int64 * 8)(*strides) if strides else None
+    rc = getattr(sw.load_library(), "sw_window_attention" + dt)(
+        a["query_offsets"], a["key_offsets"], a["query"], a["key"],
+        a["value"], a["output"], a["log_sum"], a["sequences"],
+        a["query_tokens"], a["key_tokens"], a["query_heads"], a["key_heads"],
+        a["d"], s, a["window"], a["sinks"], a["alpha"], None)
+    return rc, sw.load_library().sw_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,code,needle", [
+    (dict(sequences=-1), -2, "sequences and tokens"),
+    (dict(query_tokens=2 ** 31), -2, "sequences and tokens"),
+    (dict(query_heads=3), -2, "multiple of key heads"),
+    (dict(key_heads=0), -2, "multiple of key heads"),
+    (dict(d=60), -2, "multiple of 8"),
+    (dict(d=136), -2, "multiple of 8"),
+    (dict(d=0), -2, "multiple of 8"),
+    (dict(window=0), -2, "window of at least 1"),
+    (dict(sinks=-1), -2, "no negative sinks"),
+    (dict(alpha=float("nan")), -3, "alpha must be finite"),
+    (dict(alpha=float("inf")), -3, "alpha must be finite"),
+    (dict(query_offsets=None), -3, "offsets pointer is null"),
+    (dict(key=None), -3, "key pointer is null"),
+    (dict(output=None), -3, "output pointer is null"),
+    (dict(value=A + 2), -3, "value must be 16-byte aligned"),
+    (dict(log_sum=A + 2), -3, "not aligned"),
+    (dict(strides=[256, 64, 128, 4, 128, 64, 256, 64]), -3, "key must be 16-byte"),
+    (dict(strides=[32, 64, 128, 64, 128, 64, 256, 64]), -2, "query strides"),
+    (dict(strides=[256, -64, 128, 64, 128, 64, 256, 64]), -2, "query strides"),
+    (dict(strides=[1 << 23, 64, 128, 64, 128, 64, 256, 64]), -2, "2^23 bytes"),
+    (dict(strides=[256, 64, 128, 64, 128, 64, 256, 0]), -2, "output rows overlap"),
+    (dict(strides=[256, 64, 128, 64, 128, 64, 128, 64]), -2, "output rows overlap"),
+    (dict(strides=[256, 64, 128, 64, 128, 64, 64, 320]), -2, "output rows overlap"),
+])
+@pytest.mark.parametrize("dt", ["_f32", "_bf16"])
+def test_refused(dt, kw, code, needle):
+    if dt == "_f32" and "strides" in kw and code == -3:
+        kw = dict(kw, strides=[256, 64, 128, 2, 128, 64, 256, 64])
+    rc, message = c_forward(dt=dt, **kw)
+    assert rc == code and needle in message
+
+
+def test_nothing_to_do():
+    assert c_forward(sequences=0, query_offsets=None, key_offsets=None)[0] == 0
+    assert c_forward(query_tokens=0, query=None, output=None)[0] == 0
+
+
+def test_mirror_refuses():
+    import torch
+    off = torch.zeros(2, dtype=torch.int32)
+    q, k = torch.zeros(4, 4, 64), torch.zeros(4, 2, 64)
+
+    def call(qo=off, ko=off, query=q, key=k, value=k, output=q, log_sum=None):
+        sw.window_attention(qo, ko, query, key, value, output, log_sum, 1.0, 4)
+    with pytest.raises(ValueError, match="device tensor"):
+        call()
+    with pytest.raises(sw.ShapeError, match="expected query"):
+        call(value=k[:3])
+    with pytest.raises(sw.ShapeError, match="expected query"):
+        call(key=k[..., :32], value=k[..., :32])
+    with pytest.raises(sw.ShapeError, match="same length"):
+        call(ko=off[:1])
+    with pytest.raises(sw.ShapeError, match="query's shape"):
+        call(output=k)
+    with pytest.raises(sw.ShapeError, match="log_sum"):
+        call(log_sum=torch.zeros(4, 5))
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        call(query=q.half())
