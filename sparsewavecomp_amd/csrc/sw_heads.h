@@ -49,13 +49,21 @@ __device__ __forceinline__ v4f mma16(v8f a, v8f b, v4f c) {
   return c;
 }
 
+// Two fp32 values as bf16 in one instruction, the first in the low half.
+__device__ __forceinline__ uint32_t cvt_pk_bf16(float lo, float hi) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_convertvector(v2f{lo, hi}, bf16x2));
+}
+
 // Eight fp32 values as a fragment (bf16: each rounded to nearest even).
 template <typename T> __device__ __forceinline__ Frag<T> make_frag(const float *x) {
   if constexpr (sizeof(T) == 4)
     return v8f{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
   else
-    return v4u{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    return v4u{cvt_pk_bf16(x[0], x[1]), cvt_pk_bf16(x[2], x[3]),
+               cvt_pk_bf16(x[4], x[5]), cvt_pk_bf16(x[6], x[7])};
 }
 template <typename T> __device__ __forceinline__ Frag<T> zero_frag() {
   if constexpr (sizeof(T) == 4)
@@ -119,7 +127,7 @@ __device__ __forceinline__ void st4(float *p, float a, float b, float c,
 }
 __device__ __forceinline__ void st4(uint16_t *p, float a, float b, float c,
                                     float d) {
-  *reinterpret_cast<v2u *>(p) = v2u{pack_bf16x2(a, b), pack_bf16x2(c, d)};
+  *reinterpret_cast<v2u *>(p) = v2u{cvt_pk_bf16(a, b), cvt_pk_bf16(c, d)};
 }
 
 // The value of lane l ^ 32 combined with the lane's own, in both.
@@ -134,111 +142,179 @@ __device__ __forceinline__ float both_halves_sum(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// ---- LDS by address ----------------------------------------------------------
+// Addresses are byte offsets in the workgroup's LDS: a lane's part and a part
+// known when the kernel is built, which becomes the instruction's offset.
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t lane, uint32_t at) {
+  return *(const __attribute__((address_space(3))) V *)(uintptr_t)(lane + at);
+}
+template <typename V>
+__device__ __forceinline__ void lds_write(uint32_t at, V v) {
+  *(__attribute__((address_space(3))) V *)(uintptr_t)at = v;
+}
+// the transposing load of 16-bit elements: lane i of 16 reads 8 bytes, and gets
+// the elements i % 4 of what lanes i / 4, i / 4 + 4, + 8, + 12 of its 16 read
+__device__ __forceinline__ v2u lds_read_across(uint32_t lane, uint32_t at) {
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                     (lds_v4s *)(uintptr_t)(lane + at)));
+}
+
+// The words of buffer_rsrc(p, n), for an instruction written out.
+__device__ __forceinline__ v4u buffer_words(const void *p, uint32_t n) {
+  const uint64_t a = (uint64_t)p;
+  return v4u{(uint32_t)__builtin_amdgcn_readfirstlane((int)a),
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xFFFFu,
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+}
+// Starts a copy of 16 bytes a lane from the buffer to 1024 consecutive bytes
+// of LDS at the wave-uniform address.  Written out because the compiler waits
+// for every copy that its builtin has under way before the next LDS read, of
+// whichever tile (which made each tile wait for the next one's copy); this one
+// returns no register, and landed() waits for it.  It sets m0, which nothing
+// else in the kernels that call it uses (LDS instructions do not on gfx9).
+__device__ __forceinline__ void copy_to_lds(v4u buffer, uint32_t at,
+                                            uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+               "buffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at),
+                 "s"(buffer)
+               : "memory");
+}
+
 // ---- tiles of rows in LDS ----------------------------------------------------
 // Rows of D elements without padding, in chunks of 16 bytes; chunk c of row r
-// lies at place c ^ swizzle(r).  The swizzle keeps three reads free of bank
+// lies at place c ^ swizzle(r).  The swizzle keeps these reads free of bank
 // conflicts (64 banks of 4 bytes): 16 consecutive rows at one chunk (a
-// fragment along the rows), and, for bf16, two chunks of each of four
-// consecutive rows (a transposing load); the chunk's lowest bit must
-// therefore not be what alone tells neighbouring rows apart.  ROWS is a
-// multiple of 32 and a tile is filled by THREADS threads.
+// fragment along the rows), and, for bf16, four consecutive chunks of each of
+// four consecutive rows (half a wave's transposing load).  ROWS is a multiple
+// of 32 and a tile is filled by THREADS threads.
 template <typename T, int D, int ROWS, int THREADS> struct RowTile {
   static constexpr int kChunks = D * (int)sizeof(T) / 16;
   static constexpr int kPitch = D * (int)sizeof(T);
   static constexpr int kBytes = ROWS * kPitch;
   static constexpr int kPasses = ROWS * kChunks / THREADS;
-  static constexpr int kPassRows = THREADS / kChunks;
-  static_assert(ROWS * kChunks % THREADS == 0 && THREADS % kChunks == 0, "");
+  static constexpr int kSteps = D / 16; // products along a row
+  static_assert(ROWS * kChunks % THREADS == 0 && 1024 % kPitch == 0, "");
 
   __device__ static __forceinline__ int swizzle(int row) {
     if constexpr (sizeof(T) == 4)
       return row & 15;
     else if constexpr (kChunks == 16)
-      return ((row & 7) << 1) | ((row >> 3) & 1);
+      return ((row & 3) << 2) | ((row >> 2) & 3);
     else
-      return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+      return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   }
   __device__ static __forceinline__ int place(int row, int chunk) {
     return row * kPitch + ((chunk ^ swizzle(row)) << 4);
   }
 
-  // A thread's part of a tile on its way from memory to LDS.
-  struct Staged { v4u x[kPasses]; };
-
-  // Rows 0 .. rows - 1 of the matrix at `base` (wave-uniform; row_bytes apart,
-  // d elements of each); elements past d and rows past the end are zero.  The
-  // descriptor bounds what is read: (ROWS - 1) row_bytes + 4 D < 2^31 is the
-  // host's check.
-  __device__ static __forceinline__ Staged fetch(const T *base, int rows,
-                                                 uint32_t row_bytes, int d) {
-    Staged s;
+  // Starts the copy of rows 0 .. rows - 1 of the matrix at `base`
+  // (wave-uniform; row_bytes apart, d elements of each) to the tile at `lds`,
+  // without registers between: a wave's load writes 1024 consecutive bytes of
+  // LDS, and each lane picks the chunk that belongs at its place.  Elements
+  // past d and rows past the end are written as zeros (the descriptor bounds
+  // what is read: (ROWS - 1) row_bytes + 4 D < 2^31 is the host's check).
+  // landed() waits for it.
+  __device__ static __forceinline__ void copy(uint32_t lds, const T *base,
+                                              int rows, uint32_t row_bytes,
+                                              int d) {
+    const int l = lane_id(), w = wave_in_group();
+    constexpr int kStep = (THREADS / kWave) * (1024 / kPitch); // rows a pass
     rows = rows < 0 ? 0 : rows > ROWS ? ROWS : rows;
     const uint32_t bytes =
         rows == 0 ? 0u : (uint32_t)(rows - 1) * row_bytes + d * sizeof(T);
-    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(base, bytes);
-    const int c = threadIdx.x % kChunks, row = threadIdx.x / kChunks;
-    // (an offset past every descriptor: reads zero)
-    const uint32_t at =
-        c * 16 < d * (int)sizeof(T) ? row * row_bytes + c * 16 : 0x80000000u;
+    const v4u buffer = buffer_words(base, bytes);
+    uint32_t at = 0;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p)
-      s.x[p] = __builtin_bit_cast(
-          v4u, __builtin_amdgcn_raw_buffer_load_b128(
-                   r, (int)(at + p * kPassRows * row_bytes), 0, 0));
-    return s;
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = w * (1024 / kPitch) + l / kChunks;
+      if (p == 0 || kStep % 16 != 0) { // (the swizzle has a period of 16 rows)
+        const int c = (l % kChunks) ^ swizzle(row + p * kStep);
+        // (an offset past every descriptor: reads zero)
+        at = c * 16 < d * (int)sizeof(T) ? row * row_bytes + c * 16
+                                         : 0x80000000u;
+      }
+      copy_to_lds(buffer, at + p * kStep * row_bytes,
+                  lds + (p * (THREADS / kWave) + w) * 1024);
+    }
   }
-  __device__ static __forceinline__ void put(char *lds, const Staged &s) {
-    const int c = threadIdx.x % kChunks, row = threadIdx.x / kChunks;
+
+  // A lane's addresses within any tile, which a kernel computes once: what is
+  // left of a read's address is a constant that the load instruction adds.
+  struct Lane {
+    uint32_t along[kSteps * (int)sizeof(T) / 2];
+    uint32_t across[2 * (D / 32)]; // (bf16)
+    __device__ __forceinline__ Lane() {
+      const int l = lane_id(), h = l >> 5;
+      if constexpr (sizeof(T) == 2) {
+        const int i = l & 15;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p)
-      *reinterpret_cast<v4u *>(lds + place(row + p * kPassRows, c)) = s.x[p];
-  }
+        for (int s = 0; s < kSteps; ++s)
+          along[s] = place(l & 31, 2 * s + h);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db)
+            across[e * (D / 32) + db] =
+                place(8 * e + 4 * h + (i >> 2),
+                      4 * db + 2 * ((l >> 4) & 1) + ((i & 3) >> 1)) +
+                (i & 1) * 8;
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2 * kSteps; ++s)
+          along[s] = place(l & 31, 4 * (s / 2) + 2 * h + s % 2);
+      }
+    }
+  };
 
   // Row 32 rb + l % 32, elements 16 s + 8 (l / 32) + i: the A operand with
   // the tile's rows as rows.
-  __device__ static __forceinline__ Frag<T> along(const char *lds, int rb,
-                                                  int s) {
-    const int l = lane_id(), row = 32 * rb + (l & 31), h = l >> 5;
+  __device__ static __forceinline__ Frag<T> along(uint32_t lds, const Lane &n,
+                                                  int rb, int s) {
+    const uint32_t at = lds + 32 * rb * kPitch;
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const v4u *>(lds + place(row, 2 * s + h));
+      return lds_read<v4u>(n.along[s], at);
     } else {
-      const v4f a = *reinterpret_cast<const v4f *>(lds + place(row, 4 * s + 2 * h));
-      const v4f b =
-          *reinterpret_cast<const v4f *>(lds + place(row, 4 * s + 2 * h + 1));
+      const v4f a = lds_read<v4f>(n.along[2 * s], at);
+      const v4f b = lds_read<v4f>(n.along[2 * s + 1], at);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
   // Element 32 db + l % 32 of the rows 16 st + 8 (i / 4) + 4 (l / 32) + i % 4:
   // the A operand with the tile's columns as rows, whose K indices are those
   // of accumulators 8 (st % 2) .. of row block st / 2.
-  __device__ static __forceinline__ Frag<T> across(const char *lds, int st,
-                                                   int db) {
-    const int l = lane_id(), h = l >> 5;
+  __device__ static __forceinline__ Frag<T> across(uint32_t lds, const Lane &n,
+                                                   int st, int db) {
+    const uint32_t at = lds + 16 * st * kPitch;
     if constexpr (sizeof(T) == 2) {
-      typedef __attribute__((address_space(3))) v4s lds_v4s;
-      const int i = l & 15;
-      const int row = 16 * st + 4 * h + (i >> 2);
-      const int chunk = 4 * db + 2 * ((l >> 4) & 1) + ((i & 3) >> 1);
-      const int sub = (i & 1) * 8;
-      const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_v4s *)(lds + place(row, chunk) + sub));
-      const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_v4s *)(lds + place(row + 8, chunk) + sub));
-      const v2u x = __builtin_bit_cast(v2u, a), y = __builtin_bit_cast(v2u, b);
+      const v2u x = lds_read_across(n.across[db], at);
+      const v2u y = lds_read_across(n.across[D / 32 + db], at);
       return v4u{x.x, x.y, y.x, y.y};
     } else {
       v8f r;
-      const int col = 32 * db + (l & 31);
+      const int l = lane_id(), col = 32 * db + (l & 31);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = 16 * st + 8 * (i >> 2) + 4 * h + (i & 3);
-        r[i] = *reinterpret_cast<const float *>(
-            lds + place(row, col >> 2) + (col & 3) * 4);
-      }
+      for (int i = 0; i < 8; ++i)
+        r[i] = lds_read<float>(place(8 * (i >> 2) + 4 * (l >> 5) + (i & 3),
+                                     col >> 2) + (col & 3) * 4, at);
       return r;
     }
   }
 };
+
+// Waits until this wave's copies and its reads of earlier tiles are done, and
+// then for the workgroup's other waves.
+__device__ __forceinline__ void landed() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // ---- packed sequences ----------------------------------------------------------
 // Sequence i of n holds tokens offsets[i] .. offsets[i + 1] - 1, and, cut into
