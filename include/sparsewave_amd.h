@@ -503,6 +503,46 @@ int sw_window_attention_bf16(
     void *stream);
 
 /*
+ * The gradients of sw_window_attention: from its operands, its output and
+ * log_sum, and the output's gradient, with p = exp(alpha q.k - log_sum),
+ *   value_gradient = sum p do,      ds = p (do.v - do.o),
+ *   query_gradient = alpha sum ds k, key_gradient = alpha sum ds q,
+ * the last two sums over the queries that see a key, of all query heads that
+ * share its head.  `strides` holds sixteen: of query, key, value, output,
+ * output gradient, query gradient, key gradient and value gradient.  Nothing
+ * outside the sequences is written.  bf16 rounds p and ds to bf16 for the
+ * matrix cores and each gradient once.  No atomics.
+ *
+ * The workspace (16-byte aligned, of at least
+ * sw_window_attention_backward_workspace_bytes, 0 for sizes that the call
+ * refuses) belongs to the call until its work on `stream` is done; two calls
+ * or two captured graphs that may run at once need one each.
+ */
+int64_t sw_window_attention_backward_workspace_bytes(
+    int64_t sequences, int64_t query_tokens, int64_t key_tokens,
+    int64_t query_heads, int64_t key_heads, int64_t d, int64_t window,
+    int64_t sinks);
+int sw_window_attention_backward_f32(
+    const int32_t *query_offsets, const int32_t *key_offsets,
+    const float *query, const float *key, const float *value,
+    const float *output, const float *log_sum, const float *output_gradient,
+    float *query_gradient, float *key_gradient, float *value_gradient,
+    int64_t sequences, int64_t query_tokens, int64_t key_tokens,
+    int64_t query_heads, int64_t key_heads, int64_t d, const int64_t *strides,
+    int64_t window, int64_t sinks, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream);
+int sw_window_attention_backward_bf16(
+    const int32_t *query_offsets, const int32_t *key_offsets,
+    const uint16_t *query, const uint16_t *key, const uint16_t *value,
+    const uint16_t *output, const float *log_sum,
+    const uint16_t *output_gradient, uint16_t *query_gradient,
+    uint16_t *key_gradient, uint16_t *value_gradient, int64_t sequences,
+    int64_t query_tokens, int64_t key_tokens, int64_t query_heads,
+    int64_t key_heads, int64_t d, const int64_t *strides, int64_t window,
+    int64_t sinks, float alpha, void *workspace, int64_t workspace_bytes,
+    void *stream);
+
+/*
  * sparsewave.csr_row_at_position for a batch of positions:
  * out_rows[i] = (first j in [1, rows+1) with row_offsets[j] > positions[i]) - 1,
  * the row search of SparsePositionToSCF.cpp:225-271 that the position

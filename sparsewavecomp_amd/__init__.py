@@ -20,7 +20,8 @@ __all__ = [
     "load_library", "spmv",
     "coo_spmv", "spmv_gather_floor", "bsr_slab_floor", "attention_tile_floor",
     "spmm", "bsr_spmm", "sddmm", "csr_row_reduce", "csr_rowwise_map",
-    "sparse_attention", "window_attention", "csr_row_at_position",
+    "sparse_attention", "window_attention",
+    "window_attention_backward", "csr_row_at_position",
     "SDDMM_MUL", "SDDMM_AFFINE", "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV", "MAP_SUB", "MAP_MUL",
 ]
 
@@ -43,6 +44,8 @@ EXPORTED_SYMBOLS = (
     "sw_csr_rowwise_map_f32", "sw_csr_rowwise_map_bf16",
     "sw_sparse_attention_f32", "sw_sparse_attention_bf16",
     "sw_window_attention_f32", "sw_window_attention_bf16",
+    "sw_window_attention_backward_workspace_bytes",
+    "sw_window_attention_backward_f32", "sw_window_attention_backward_bf16",
     "sw_csr_row_at_position", "sw_attention_tile_floor",
     "sw_host_matrix_free", "sw_host_bsr_free", "sw_matrix_market_read",
     "sw_csr_binary_write", "sw_coo_binary_write", "sw_csr_binary_read",
@@ -175,6 +178,9 @@ def load_library():
     for dt in ("_f32", "_bf16"):
         sig["sw_window_attention" + dt] = (
             ctypes.c_int, [P] * 7 + [I64] * 6 + [P, I64, I64, F, P])
+        sig["sw_window_attention_backward" + dt] = (
+            ctypes.c_int, [P] * 11 + [I64] * 6 + [P, I64, I64, F, P, I64, P])
+    sig["sw_window_attention_backward_workspace_bytes"] = (I64, [I64] * 8)
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -711,6 +717,73 @@ def window_attention(query_offsets, key_offsets, query, key, value, output,
         None if log_sum is None else _dev(log_sum, torch.float32, "log_sum"),
         *shape, strides, window, sinks, alpha, _stream(stream)))
     return output
+
+
+def _scratch(nbytes, like, workspace, stream):
+    """The workspace that a call cannot do without: the caller's, or one of
+    torch's allocator for the call's stream (under graph capture, of the
+    graph's own pool)."""
+    torch = _torch or _load_torch()
+    if workspace is not None:
+        _dev(workspace, torch.uint8, "workspace")
+        _need(workspace.numel() >= nbytes,
+              f"workspace must hold {nbytes} bytes")
+        _one_device(stream, workspace)
+        return workspace
+    if nbytes == 0:
+        return None
+    if stream is not None:
+        if not isinstance(stream, torch.cuda.Stream):
+            raise ValueError("a stream that is not torch's needs a workspace")
+        with torch.cuda.stream(stream):
+            return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+
+
+def window_attention_backward(query_offsets, key_offsets, query, key, value,
+                              output, log_sum, output_gradient,
+                              query_gradient, key_gradient, value_gradient,
+                              alpha, window, sinks=0, workspace=None,
+                              stream=None):
+    """The gradients of :func:`window_attention`, from its operands, its
+    output and log_sum, and the output's gradient.  The key's and value's are
+    summed over the query heads that share them.  Tokens of no sequence are
+    left as they were.  The scratch memory of
+    sw_window_attention_backward_workspace_bytes is taken from torch's
+    allocator where `workspace` (uint8) is not given."""
+    torch = _torch or _load_torch()
+    shape = _window_shapes(query_offsets, key_offsets, query, key, value)
+    dt = _value_dtype(query, "query")
+    for t, n in ((output, "output"), (output_gradient, "output_gradient"),
+                 (query_gradient, "query_gradient")):
+        _need(tuple(t.shape) == tuple(query.shape),
+              f"{n} must have query's shape")
+    for t, n in ((key_gradient, "key_gradient"),
+                 (value_gradient, "value_gradient")):
+        _need(tuple(t.shape) == tuple(key.shape), f"{n} must have key's shape")
+    _need(tuple(log_sum.shape) == (shape[3], shape[1]),
+          "log_sum must be [query_heads, query_tokens]")
+    _one_device(stream, query_offsets, key_offsets, query, key, value, output,
+                log_sum, output_gradient, query_gradient, key_gradient,
+                value_gradient)
+    ops = [_heads(t, dt, n) for t, n in (
+        (query, "query"), (key, "key"), (value, "value"), (output, "output"),
+        (output_gradient, "output_gradient"),
+        (query_gradient, "query_gradient"), (key_gradient, "key_gradient"),
+        (value_gradient, "value_gradient"))]
+    strides = (ctypes.c_int64 * 16)(*(x for o in ops for x in o[1:]))
+    offsets = (_dev(query_offsets, torch.int32, "query_offsets"),
+               _dev(key_offsets, torch.int32, "key_offsets"))
+    lse = _dev(log_sum, torch.float32, "log_sum")
+    need = load_library().sw_window_attention_backward_workspace_bytes(
+        *shape, window, sinks)
+    scratch = _scratch(need, query, workspace, stream)
+    p = [o[0] for o in ops]
+    _check(_fn("sw_window_attention_backward", dt)(
+        *offsets, *p[:4], lse, *p[4:], *shape, strides, window, sinks, alpha,
+        None if scratch is None else scratch.data_ptr(), need,
+        _stream(stream)))
+    return query_gradient, key_gradient, value_gradient
 
 
 def csr_row_at_position(row_offsets, positions, out_rows, stream=None):

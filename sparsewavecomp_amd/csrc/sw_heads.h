@@ -187,6 +187,17 @@ __device__ __forceinline__ void copy_to_lds(v4u buffer, uint32_t at,
                : "memory");
 }
 
+// The same of 4 bytes a lane, to 256 consecutive bytes.
+__device__ __forceinline__ void copy_words_to_lds(v4u buffer, uint32_t at,
+                                                  uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+               "buffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at),
+                 "s"(buffer)
+               : "memory");
+}
+
 // ---- tiles of rows in LDS ----------------------------------------------------
 // Rows of D elements without padding, in chunks of 16 bytes; chunk c of row r
 // lies at place c ^ swizzle(r).  The swizzle keeps these reads free of bank
@@ -247,9 +258,11 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
 
   // A lane's addresses within any tile, which a kernel computes once: what is
   // left of a read's address is a constant that the load instruction adds.
+  // (The swizzle reaches the chunk's four low bits: fp32 reads that differ in
+  // higher ones share an address.)
   struct Lane {
-    uint32_t along[kSteps * (int)sizeof(T) / 2];
-    uint32_t across[2 * (D / 32)]; // (bf16)
+    uint32_t along[sizeof(T) == 2 ? kSteps : 8];
+    uint32_t across[sizeof(T) == 2 ? 2 * (D / 32) : 4];
     __device__ __forceinline__ Lane() {
       const int l = lane_id(), h = l >> 5;
       if constexpr (sizeof(T) == 2) {
@@ -267,8 +280,11 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
                 (i & 1) * 8;
       } else {
 #pragma unroll
-        for (int s = 0; s < 2 * kSteps; ++s)
+        for (int s = 0; s < 8; ++s)
           along[s] = place(l & 31, 4 * (s / 2) + 2 * h + s % 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          across[e] = place(4 * h + e, (l & 31) >> 2) + (l & 3) * 4;
       }
     }
   };
@@ -281,8 +297,9 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
     if constexpr (sizeof(T) == 2) {
       return lds_read<v4u>(n.along[s], at);
     } else {
-      const v4f a = lds_read<v4f>(n.along[2 * s], at);
-      const v4f b = lds_read<v4f>(n.along[2 * s + 1], at);
+      const uint32_t up = at + 256 * (s / 4);
+      const v4f a = lds_read<v4f>(n.along[2 * (s % 4)], up);
+      const v4f b = lds_read<v4f>(n.along[2 * (s % 4) + 1], up);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -298,11 +315,12 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
       return v4u{x.x, x.y, y.x, y.y};
     } else {
       v8f r;
-      const int l = lane_id(), col = 32 * db + (l & 31);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        r[i] = lds_read<float>(place(8 * (i >> 2) + 4 * (l >> 5) + (i & 3),
-                                     col >> 2) + (col & 3) * 4, at);
+      for (int i = 0; i < 8; ++i) // (row bit 3 swaps chunks 8 apart)
+        r[i] = lds_read<float>(n.across[i & 3],
+                               at + 8 * (i >> 2) * kPitch +
+                                   128 * ((db ^ (i >> 2)) & 1) +
+                                   256 * (db >> 1));
       return r;
     }
   }

@@ -6,6 +6,12 @@
 //   s = alpha q.k,  m = max s,  l = sum exp(s - m),
 //   o = sum exp(s - m) v / l,  log_sum = m + log l.
 // Query heads g G .. g G + G - 1 share key head g, G = query_heads / key_heads.
+// With p = exp(s - log_sum) and the output's gradient do:
+//   dv = sum p do,  dp = do.v,  delta = do.o,  ds = p (dp - delta),
+//   dq = alpha sum ds k,  dk = alpha sum ds q,
+// the sums for keys over all queries that see them, of all heads that share
+// the key head.  The scores are computed again, once for dq and once for dk
+// and dv, so that every sum has one owner: no atomics, the same bits again.
 #include "sw_heads.h"
 #include "sw_internal.h"
 
@@ -56,6 +62,32 @@ __device__ __forceinline__ Sequence sequence(const A &a, int i) {
   s.nk = clamped(a.key_offsets[i + 1], s.k0, a.key_tokens) - s.k0;
   return s;
 }
+
+// A workgroup's rows: 128 queries of one head, 32 a wave.  Neighbouring
+// workgroups of an XCD take the heads that share a key head, then the next
+// rows, whose windows overlap (65,536 queries, window 4096: 2222 us; in plain
+// order 2351 us).
+struct Rows {
+  Sequence s;
+  int head, key_head, row0, row_lo, count, shift;
+  __device__ __forceinline__ explicit Rows(const WindowArgs &a) {
+    const int group = a.query_heads / a.key_heads;
+    int64_t item = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int g = (int)(item % group);
+    item /= group;
+    const int tile = (int)(item % a.tiles);
+    key_head = (int)(item / a.tiles);
+    head = key_head * group + g;
+    const int i =
+        sequence_of_tile(a.query_offsets, a.sequences, tile, kRowShift);
+    s = sequence(a, i);
+    row0 = (tile - (a.query_offsets[i] >> kRowShift) - i) << kRowShift;
+    // (none in the numbers between one sequence's tiles and the next's)
+    count = row0 < 0 ? 0 : s.nq - row0 < kRows ? s.nq - row0 : kRows;
+    row_lo = row0 + 32 * wave_in_group();
+    shift = s.nk - s.nq; // a query's place less its index
+  }
+};
 
 // The keys that a workgroup's rows see between them, as tiles of KT: the sinks
 // before the window first where they do not touch it, then the window from its
@@ -134,6 +166,40 @@ __device__ __forceinline__ v16f mma32_seen(Frag<T> a, Frag<T> b, v16f acc,
   return acc;
 }
 
+// the rows of a fragment's lane: 32 of an operand, zeros past the end
+template <typename T, int STEPS>
+__device__ __forceinline__ void load_rows(Frag<T> (&f)[STEPS], const T *p,
+                                          bool live, int d, bool negate) {
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) {
+    const int c = 16 * st + 8 * h;
+    f[st] = live && c < d ? ld_frag(p + c) : zero_frag<T>();
+    if (negate)
+      f[st] = negate_frag<T>(f[st]);
+  }
+}
+template <typename T, int BLOCKS>
+__device__ __forceinline__ bool all_finite(const v16f (&acc)[BLOCKS]) {
+  float x = 0.0f;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      x = fmaf(acc[b][r], 0.0f, x);
+  return x == 0.0f;
+}
+// Whether a wave of the workgroup says so; every thread must call it.
+__device__ __forceinline__ bool any_wave(bool says, int *verdict) {
+  if (threadIdx.x == 0)
+    *verdict = 0;
+  __syncthreads();
+  if (ballot(says) != 0 && lane_id() == 0)
+    *verdict = 1;
+  __syncthreads();
+  return *verdict != 0;
+}
+
 // ---- forward -------------------------------------------------------------------
 
 template <typename T, int D> struct Forward {
@@ -153,51 +219,29 @@ window_forward(WindowArgs a) {
   using Tile = typename F::Tile;
   constexpr int KT = F::kTile;
   __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
-  __shared__ int spoiled;
+  __shared__ int verdict;
 
-  const int group = a.query_heads / a.key_heads;
-  int64_t item = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int g = (int)(item % group);
-  item /= group;
-  const int tile = (int)(item % a.tiles);
-  const int hk = (int)(item / a.tiles);
-  const int head = hk * group + g;
-
-  const int seq = sequence_of_tile(a.query_offsets, a.sequences, tile, kRowShift);
-  const Sequence s = sequence(a, seq);
-  const int row0 =
-      (tile - (a.query_offsets[seq] >> kRowShift) - seq) << kRowShift;
-  if (row0 < 0 || row0 >= s.nq)
+  const Rows w(a);
+  if (w.count <= 0)
     return;
-  const int rows = s.nq - row0 < kRows ? s.nq - row0 : kRows;
-  const int shift = s.nk - s.nq; // a query's place less its index
-
-  const int lane = lane_id(), h = lane >> 5, wave = wave_in_group();
-  const int row = row0 + 32 * wave + (lane & 31);
+  const Sequence &s = w.s;
+  const int lane = lane_id(), h = lane >> 5;
+  const int place_lo = w.row_lo + w.shift, place_hi = place_lo + 31;
+  const int row = w.row_lo + (lane & 31), place = row + w.shift;
   const bool live = row < s.nq;
-  const int place = row + shift;
-  const int place_lo = row0 + 32 * wave + shift, place_hi = place_lo + 31;
+  const int head = w.head, hk = w.key_head;
 
   // the wave's queries, negated where alpha is negative, and zero for an alpha
   // too small to scale a masked score of -inf
-  Frag<T> q[F::kSteps];
   const bool tiny = fabsf(a.alpha) < 0x1p-126f;
-  {
-    const T *p = static_cast<const T *>(a.query) +
-                 (int64_t)(s.q0 + (live ? row : row0)) * a.q.token +
-                 head * a.q.head;
-#pragma unroll
-    for (int st = 0; st < F::kSteps; ++st) {
-      const int c = 16 * st + 8 * h;
-      q[st] = live && c < a.d && !tiny ? ld_frag(p + c) : zero_frag<T>();
-      if (a.alpha < 0.0f)
-        q[st] = negate_frag<T>(q[st]);
-    }
-  }
+  Frag<T> q[F::kSteps];
+  load_rows<T>(q, static_cast<const T *>(a.query) +
+                      (int64_t)(s.q0 + (live ? row : w.row0)) * a.q.token +
+                      head * a.q.head, live && !tiny, a.d, a.alpha < 0.0f);
   const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
 
-  const KeyTiles<KT> keys(row0 + shift, row0 + rows - 1 + shift, a.window,
-                          a.sinks, s.nk);
+  const KeyTiles<KT> keys(w.row0 + w.shift, w.row0 + w.count - 1 + w.shift,
+                          a.window, a.sinks, s.nk);
   const T *kbase = static_cast<const T *>(a.key) + (int64_t)s.k0 * a.k.token +
                    hk * a.k.head;
   const T *vbase = static_cast<const T *>(a.value) + (int64_t)s.k0 * a.v.token +
@@ -334,22 +378,8 @@ window_forward(WindowArgs a) {
   pass(std::false_type{});
   // A finite result has met no infinity or NaN.  Others are computed again
   // with the keys at the edges of the mask kept apart.
-  {
-    float x = 0.0f;
-#pragma unroll
-    for (int b = 0; b < F::kBlocks; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        x = fmaf(acc[b][r], 0.0f, x);
-    if (threadIdx.x == 0)
-      spoiled = 0;
-    __syncthreads();
-    if (ballot(x != 0.0f) != 0 && lane == 0)
-      spoiled = 1;
-    __syncthreads();
-    if (spoiled)
-      pass(std::true_type{});
-  }
+  if (any_wave(!all_finite<T>(acc), &verdict))
+    pass(std::true_type{});
 
   sum = both_halves_sum(sum);
   const bool empty = place < 0 || s.nk == 0; // a row that sees no key
@@ -374,14 +404,492 @@ window_forward(WindowArgs a) {
   }
 }
 
+// ---- backward ------------------------------------------------------------------
+
+struct BackwardArgs {
+  WindowArgs w; // o: the output's strides; log_sum: the forward pass's
+  const void *output_gradient;
+  void *query_gradient, *key_gradient, *value_gradient;
+  Operand go, gq, gk, gv;
+  float *log2_sum, *delta; // [query_heads][query_tokens], of the first kernel
+  // sums of the sinks' gradients in fp32, [..][key_heads][sink_rows][2][d]:
+  // those of the window, for each sequence, and of the queries past it, for
+  // each chunk of 1 << chunk_shift queries
+  float *sink_window, *sink_chunks;
+  int key_tiles, chunks, chunk_shift, sink_rows; // sink_rows: a multiple of 32
+};
+
+// dq of a tile of rows, and for the second kernel log_sum in powers of two
+// and delta of its rows.  The forward pass's loop with one product more:
+// ds^T = K Q^T and V dO^T element by element, dq^T += K^T ds^T.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (Forward<T, D>::kWaves)) void
+window_query_gradient(BackwardArgs b) {
+  const WindowArgs &a = b.w;
+  using F = Forward<T, D>;
+  using Tile = typename F::Tile;
+  constexpr int KT = F::kTile;
+  __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
+  __shared__ int verdict;
+
+  const Rows w(a);
+  if (w.count <= 0)
+    return;
+  const Sequence &s = w.s;
+  const int lane = lane_id(), h = lane >> 5;
+  const int place_lo = w.row_lo + w.shift, place_hi = place_lo + 31;
+  const int row = w.row_lo + (lane & 31), place = row + w.shift;
+  const bool live = row < s.nq;
+  const int head = w.head, hk = w.key_head;
+  const int64_t token = s.q0 + (live ? row : w.row0);
+
+  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
+  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+  Frag<T> q[F::kSteps], go[F::kSteps];
+  load_rows<T>(q, static_cast<const T *>(a.query) + token * a.q.token +
+                      head * a.q.head, live && !tiny, a.d, a.alpha < 0.0f);
+  load_rows<T>(go, static_cast<const T *>(b.output_gradient) +
+                       token * b.go.token + head * b.go.head, live, a.d, false);
+  float delta = 0.0f, log2_sum = 0.0f;
+  {
+    Frag<T> o[F::kSteps];
+    load_rows<T>(o, static_cast<const T *>(a.output) + token * a.o.token +
+                        head * a.o.head, live, a.d, false);
+#pragma unroll
+    for (int st = 0; st < F::kSteps; ++st)
+      delta = dot_frag<T>(go[st], o[st], delta);
+    delta = both_halves_sum(delta);
+    if (live) {
+      const int64_t at = (int64_t)head * a.query_tokens + token;
+      log2_sum = a.log_sum[at] * kLog2e;
+      if (h == 0) {
+        b.log2_sum[at] = log2_sum;
+        b.delta[at] = delta;
+      }
+    }
+  }
+
+  const KeyTiles<KT> keys(w.row0 + w.shift, w.row0 + w.count - 1 + w.shift,
+                          a.window, a.sinks, s.nk);
+  const T *kbase = static_cast<const T *>(a.key) + (int64_t)s.k0 * a.k.token +
+                   hk * a.k.head;
+  const T *vbase = static_cast<const T *>(a.value) + (int64_t)s.k0 * a.v.token +
+                   hk * a.v.head;
+  const uint32_t kbytes = (uint32_t)(a.k.token * sizeof(T));
+  const uint32_t vbytes = (uint32_t)(a.v.token * sizeof(T));
+  const typename Tile::Lane at;
+  const uint32_t base = lds_address(lds);
+  auto copy = [&](int t) __attribute__((always_inline)) {
+    const int64_t j = keys.from(t);
+    const int n = keys.end(t) - (int)j;
+    const uint32_t to = base + (t & 1) * 2 * Tile::kBytes;
+    Tile::copy(to, kbase + j * a.k.token, n, kbytes, a.d);
+    Tile::copy(to + Tile::kBytes, vbase + j * a.v.token, n, vbytes, a.d);
+  };
+
+  v16f acc[F::kBlocks];
+  auto products = [&](uint32_t kt, int t, auto careful)
+                      __attribute__((always_inline)) {
+    const uint32_t vt = kt + Tile::kBytes;
+    const bool all = keys.all(t, place_lo, place_hi, a.window, a.sinks);
+    const bool sink = keys.sink(t);
+    const int j0 = keys.from(t) + 4 * h;
+    const int back = sink ? 1 << 30 : place - j0;
+    const uint32_t window = sink ? 0 : a.window;
+    const int left = (sink ? keys.end(t) : a.sinks) - j0;
+#pragma unroll
+    for (int kb = 0; kb < F::kKeyBlocks; ++kb) {
+      v16f p = {}, ds = {};
+#pragma unroll
+      for (int st = 0; st < F::kSteps; ++st)
+        p = mma32(Tile::along(kt, at, kb, st), q[st], p);
+#pragma unroll
+      for (int st = 0; st < F::kSteps; ++st)
+        ds = mma32(Tile::along(vt, at, kb, st), go[st], ds);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ds[r] = __builtin_amdgcn_exp2f(fmaf(p[r], scale, -log2_sum)) *
+                (ds[r] - delta);
+      uint32_t seen = 0;
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = 32 * kb + 8 * (r >> 2) + (r & 3);
+          const bool see = ((uint32_t)(back - j) < window) |
+                           ((back >= j) & (left > j));
+          ds[r] = see ? ds[r] : 0.0f;
+          if constexpr (decltype(careful)::value)
+            seen |= (uint32_t)see << r;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = ds[8 * half + i];
+        // bf16: rounded once more, as the matrix core takes it
+        const Frag<T> f = make_frag<T>(x);
+#pragma unroll
+        for (int c = 0; c < F::kBlocks; ++c) {
+          const Frag<T> kf = Tile::across(kt, at, 2 * kb + half, c);
+          if (decltype(careful)::value && !all)
+            acc[c] = mma32_seen<T>(kf, f, acc[c], seen >> (8 * half));
+          else
+            acc[c] = mma32(kf, f, acc[c]);
+        }
+      }
+    }
+  };
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < F::kBlocks; ++c)
+      acc[c] = v16f{};
+    if (keys.count > 0)
+      copy(0);
+    auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+      landed();
+      if (t + 1 < keys.count)
+        copy(t + 1);
+      if (keys.any(t, place_lo, place_hi, a.window, a.sinks))
+        products(base + decltype(parity)::value * 2 * Tile::kBytes, t,
+                 careful);
+    };
+    for (int t = 0; t < keys.count; t += 2) {
+      step(t, std::integral_constant<int, 0>{});
+      if (t + 1 < keys.count)
+        step(t + 1, std::integral_constant<int, 1>{});
+    }
+  };
+  pass(std::false_type{});
+  if (any_wave(!all_finite<T>(acc), &verdict))
+    pass(std::true_type{});
+  if (live) {
+    T *out = static_cast<T *>(b.query_gradient) + token * b.gq.token +
+             head * b.gq.head;
+#pragma unroll
+    for (int c = 0; c < F::kBlocks; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        if (32 * c + acc_row(r) < a.d)
+          st4(out + 32 * c + acc_row(r), acc[c][r] * a.alpha,
+              acc[c][r + 1] * a.alpha, acc[c][r + 2] * a.alpha,
+              acc[c][r + 3] * a.alpha);
+  }
+}
+
+// dk and dv.  A workgroup holds 128 keys of one key head, 32 a wave, and goes
+// through the queries that see them, head by head: S = Q K^T and dP = dO V^T
+// with queries in rows and keys in columns, dv^T += dO^T p, dk^T += Q^T ds.
+// The queries past the window that see the sinks are as many as the sequence
+// has, so they are split: a workgroup of those takes 32 sinks and a chunk of
+// queries, its waves blocks of 32 queries in turn, and leaves its sums to
+// window_sink_gradient.
+template <typename T, int D> struct Backward {
+  static constexpr int kTile = sizeof(T) == 2 ? 64 : 32; // queries
+  using Tile = RowTile<T, D, kTile, kThreads>;
+  static constexpr int kSteps = D / 16;
+  static constexpr int kBlocks = D / 32;
+  static constexpr int kWaves = D > 64 ? 1 : 2;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (Backward<T, D>::kWaves)) void
+window_key_gradient(BackwardArgs b) {
+  const WindowArgs &a = b.w;
+  using F = Backward<T, D>;
+  using Tile = typename F::Tile;
+  constexpr int QT = F::kTile;
+  __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
+  __shared__ __align__(16) float stats[2][2][64];
+  __shared__ int verdict;
+
+  const int lane = lane_id(), h = lane >> 5, wave = wave_in_group();
+  const int group = a.query_heads / a.key_heads;
+  const int sink_blocks = b.sink_rows / 32;
+  const int64_t sink_items = (int64_t)b.chunks * a.key_heads * sink_blocks;
+  const bool sink = blockIdx.x < sink_items;
+  int hk, i, key0, first, last; // keys from key0; queries first .. last
+  Sequence s;
+  int64_t item;
+  if (sink) {
+    item = blockIdx.x;
+    const int block = (int)(item % sink_blocks);
+    hk = (int)(item / sink_blocks % a.key_heads);
+    const int chunk = (int)(item / sink_blocks / a.key_heads);
+    item = chunk;
+    i = sequence_of_tile(a.query_offsets, a.sequences, chunk, b.chunk_shift);
+    s = sequence(a, i);
+    const int row0 = (chunk - (a.query_offsets[i] >> b.chunk_shift) - i)
+                     << b.chunk_shift;
+    key0 = 32 * block;
+    first = row0;
+    last = row0 + (1 << b.chunk_shift) - 1;
+    last = last < s.nq - 1 ? last : s.nq - 1;
+    if (row0 < 0 || last < first || last + s.nk - s.nq < a.window)
+      return; // (no query, or none past the window: the sum leaves it out)
+    const int far = key0 + a.window - (s.nk - s.nq);
+    first = far > first ? far : first;
+  } else {
+    item = xcd_contiguous(blockIdx.x - sink_items, gridDim.x - sink_items);
+    const int tile = (int)(item % b.key_tiles);
+    hk = (int)(item / b.key_tiles);
+    i = sequence_of_tile(a.key_offsets, a.sequences, tile, kRowShift);
+    s = sequence(a, i);
+    key0 = (tile - (a.key_offsets[i] >> kRowShift) - i) << kRowShift;
+    if (key0 < 0 || key0 >= s.nk)
+      return;
+    const int shift = s.nk - s.nq;
+    const int end = (s.nk < key0 + kRows ? s.nk : key0 + kRows) - 1;
+    first = key0 - shift > 0 ? key0 - shift : 0;
+    last = s.nk - 1 - end < a.window ? s.nq - 1 : end + a.window - 1 - shift;
+    key0 += 32 * wave;
+  }
+  const int shift = s.nk - s.nq;
+  const int key = key0 + (lane & 31);
+  const bool live = key < s.nk && (!sink || key < a.sinks);
+
+  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
+  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+  Frag<T> k[F::kSteps], v[F::kSteps];
+  {
+    const int64_t token = s.k0 + (live ? key : 0);
+    load_rows<T>(k, static_cast<const T *>(a.key) + token * a.k.token +
+                        hk * a.k.head, live && !tiny, a.d, a.alpha < 0.0f);
+    load_rows<T>(v, static_cast<const T *>(a.value) + token * a.v.token +
+                        hk * a.v.head, live, a.d, false);
+  }
+
+  const T *qbase = static_cast<const T *>(a.query) + (int64_t)s.q0 * a.q.token;
+  const T *obase = static_cast<const T *>(b.output_gradient) +
+                   (int64_t)s.q0 * b.go.token;
+  const uint32_t qbytes = (uint32_t)(a.q.token * sizeof(T));
+  const uint32_t obytes = (uint32_t)(b.go.token * sizeof(T));
+  const int tiles = last < first ? 0 : (last - first) / QT + 1;
+  const int count = tiles * group;
+  const typename Tile::Lane at;
+  const uint32_t base = lds_address(lds), sbase = lds_address(stats);
+  auto copy = [&](int t) __attribute__((always_inline)) {
+    const int head = hk * group + t / tiles;
+    const int64_t r = first + t % tiles * QT;
+    const int n = last + 1 - (int)r;
+    const uint32_t to = base + (t & 1) * 2 * Tile::kBytes;
+    Tile::copy(to, qbase + r * a.q.token + head * a.q.head, n, qbytes, a.d);
+    Tile::copy(to + Tile::kBytes, obase + r * b.go.token + head * b.go.head, n,
+               obytes, a.d);
+    if (wave < 2) { // a row's two numbers, 64 of each
+      const float *x = (wave == 0 ? b.log2_sum : b.delta) +
+                       (int64_t)head * a.query_tokens + s.q0 + r;
+      const int m = n < QT ? n : QT;
+      copy_words_to_lds(buffer_words(x, 4 * m), 4 * lane,
+                        sbase + ((t & 1) * 2 + wave) * 256);
+    }
+  };
+
+  v16f dk[F::kBlocks], dv[F::kBlocks];
+  auto products = [&](int t, auto parity, auto careful)
+                      __attribute__((always_inline)) {
+    constexpr int P = decltype(parity)::value;
+    const uint32_t qt = base + P * 2 * Tile::kBytes, ot = qt + Tile::kBytes;
+    const int r0 = first + t % tiles * QT;
+#pragma unroll
+    for (int rb = 0; rb < QT / 32; ++rb) {
+      const int lo = r0 + 32 * rb; // this block's first query
+      if (sink ? ((t * (QT / 32) + rb) & 3) != wave
+               : lo + 31 + shift < key0 || lo + shift - (key0 + 31) >= a.window)
+        continue; // another wave's, or hidden
+      if (lo > last)
+        continue;
+      const bool all =
+          lo + 31 <= last &&
+          (sink ? lo + shift - (key0 + 31) >= a.window && key0 + 32 <= a.sinks
+                : lo + shift >= key0 + 31 &&
+                      lo + 31 + shift - key0 < a.window);
+      v16f p = {}, ds = {};
+#pragma unroll
+      for (int st = 0; st < F::kSteps; ++st)
+        p = mma32(Tile::along(qt, at, rb, st), k[st], p);
+#pragma unroll
+      for (int st = 0; st < F::kSteps; ++st)
+        ds = mma32(Tile::along(ot, at, rb, st), v[st], ds);
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        // (rows acc_row(r) .. + 3 of the block)
+        const v4f l4 = lds_read<v4f>(16 * h, sbase + P * 512 + 128 * rb + 8 * r);
+        const v4f d4 =
+            lds_read<v4f>(16 * h, sbase + P * 512 + 256 + 128 * rb + 8 * r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[r + e] = __builtin_amdgcn_exp2f(fmaf(p[r + e], scale, -l4[e]));
+          ds[r + e] = p[r + e] * (ds[r + e] - d4[e]);
+        }
+      }
+      uint32_t seen = 0;
+      if (!all) {
+        const int back = lo + shift + 4 * h - key; // of accumulator row 0
+        const int rows = last - lo - 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = 8 * (r >> 2) + (r & 3);
+          const bool see =
+              ((sink ? (back + j >= a.window) & live
+                     : (uint32_t)(back + j) < (uint32_t)a.window)) &
+              (j <= rows);
+          p[r] = see ? p[r] : 0.0f;
+          ds[r] = see ? ds[r] : 0.0f;
+          if constexpr (decltype(careful)::value)
+            seen |= (uint32_t)see << r;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = p[8 * half + e];
+          y[e] = ds[8 * half + e];
+        }
+        // bf16: rounded once more each, as the matrix core takes them
+        const Frag<T> pf = make_frag<T>(x), df = make_frag<T>(y);
+#pragma unroll
+        for (int c = 0; c < F::kBlocks; ++c) {
+          const Frag<T> of = Tile::across(ot, at, 2 * rb + half, c);
+          const Frag<T> qf = Tile::across(qt, at, 2 * rb + half, c);
+          if (decltype(careful)::value && !all) {
+            dv[c] = mma32_seen<T>(of, pf, dv[c], seen >> (8 * half));
+            dk[c] = mma32_seen<T>(qf, df, dk[c], seen >> (8 * half));
+          } else {
+            dv[c] = mma32(of, pf, dv[c]);
+            dk[c] = mma32(qf, df, dk[c]);
+          }
+        }
+      }
+    }
+  };
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < F::kBlocks; ++c)
+      dk[c] = dv[c] = v16f{};
+    if (count > 0)
+      copy(0);
+    auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+      landed();
+      if (t + 1 < count)
+        copy(t + 1);
+      products(t, parity, careful);
+    };
+    for (int t = 0; t < count; t += 2) {
+      step(t, std::integral_constant<int, 0>{});
+      if (t + 1 < count)
+        step(t + 1, std::integral_constant<int, 1>{});
+    }
+  };
+  pass(std::false_type{});
+  if (any_wave(!(all_finite<T>(dk) && all_finite<T>(dv)), &verdict))
+    pass(std::true_type{});
+
+  if (sink) {
+    // the waves' sums, one after the other, in the tiles' memory
+    static_assert(sizeof(lds) >= 2 * F::kBlocks * 16 * 64 * 4, "");
+    float *sums = reinterpret_cast<float *>(lds);
+    for (int turn = 0; turn < 4; ++turn) {
+      __syncthreads();
+      if (turn == wave) {
+#pragma unroll
+        for (int c = 0; c < F::kBlocks; ++c)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float *x = sums + ((c * 16 + r) * 2) * 64 + lane;
+            if (turn > 0) {
+              dk[c][r] += x[0];
+              dv[c][r] += x[64];
+            }
+            x[0] = dk[c][r];
+            x[64] = dv[c][r];
+          }
+      }
+    }
+    if (wave != 3)
+      return;
+  }
+  if (!live)
+    return;
+  // a sink's sums wait for those of the queries past the window
+  if (sink || key < b.sink_rows) {
+    const int64_t of = (sink ? item : i) * a.key_heads + hk;
+    float *out = (sink ? b.sink_chunks : b.sink_window) +
+                 (of * b.sink_rows + key) * 2 * a.d;
+#pragma unroll
+    for (int c = 0; c < F::kBlocks; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        if (32 * c + acc_row(r) < a.d) {
+          float *x = out + 32 * c + acc_row(r);
+          st4(x, dk[c][r], dk[c][r + 1], dk[c][r + 2], dk[c][r + 3]);
+          st4(x + a.d, dv[c][r], dv[c][r + 1], dv[c][r + 2], dv[c][r + 3]);
+        }
+    if (sink || key < a.sinks)
+      return;
+  }
+  const int64_t token = s.k0 + key;
+  T *kout = static_cast<T *>(b.key_gradient) + token * b.gk.token +
+            hk * b.gk.head;
+  T *vout = static_cast<T *>(b.value_gradient) + token * b.gv.token +
+            hk * b.gv.head;
+#pragma unroll
+  for (int c = 0; c < F::kBlocks; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      if (32 * c + acc_row(r) < a.d) {
+        st4(kout + 32 * c + acc_row(r), dk[c][r] * a.alpha,
+            dk[c][r + 1] * a.alpha, dk[c][r + 2] * a.alpha,
+            dk[c][r + 3] * a.alpha);
+        st4(vout + 32 * c + acc_row(r), dv[c][r], dv[c][r + 1], dv[c][r + 2],
+            dv[c][r + 3]);
+      }
+}
+
+// The sinks' gradients: the window's sums and every chunk's, in order.  One
+// workgroup of d threads for a sink of one sequence and key head.
+template <typename T>
+__global__ void window_sink_gradient(BackwardArgs b) {
+  const WindowArgs &a = b.w;
+  const int key = blockIdx.x % a.sinks;
+  const int hk = blockIdx.x / a.sinks % a.key_heads;
+  const int i = blockIdx.x / a.sinks / a.key_heads;
+  const Sequence s = sequence(a, i);
+  const int c = threadIdx.x;
+  if (key >= s.nk || c >= a.d)
+    return;
+  const int64_t row = (int64_t)b.sink_rows * 2 * a.d;
+  const int64_t own = (int64_t)key * 2 * a.d + c;
+  const float *x = b.sink_window + ((int64_t)i * a.key_heads + hk) * row + own;
+  float dk = x[0], dv = x[a.d];
+  const int begin = (a.query_offsets[i] >> b.chunk_shift) + i;
+  for (int r = 0; r < s.nq; r += 1 << b.chunk_shift) {
+    int last = r + (1 << b.chunk_shift) - 1;
+    last = last < s.nq - 1 ? last : s.nq - 1;
+    const int chunk = begin + (r >> b.chunk_shift);
+    if (last + s.nk - s.nq < a.window || chunk >= b.chunks)
+      continue;
+    const float *y = b.sink_chunks + ((int64_t)chunk * a.key_heads + hk) * row + own;
+    dk += y[0];
+    dv += y[a.d];
+  }
+  const int64_t token = s.k0 + key;
+  stv(static_cast<T *>(b.key_gradient) + token * b.gk.token + hk * b.gk.head + c,
+      dk * a.alpha);
+  stv(static_cast<T *>(b.value_gradient) + token * b.gv.token +
+          hk * b.gv.head + c, dv);
+}
+
 // ---- host ------------------------------------------------------------------------
 
 // Strides of one operand: rows of d elements, 16-byte aligned, close enough
 // that a tile of rows spans 2^30 bytes (descriptor offsets are 32 bits).
 int check_operand(const char *name, const void *p, const Operand &s, int64_t d,
-                  int64_t elem, bool some, bool output, int64_t tokens,
-                  int64_t heads) {
-  if (!some)
+                  int64_t elem, bool output, int64_t tokens, int64_t heads) {
+  if (tokens == 0)
     return SW_OK;
   if (!p)
     return sw::fail(SW_ERR_INVALID_ARGUMENT, "%s pointer is null", name);
@@ -441,6 +949,61 @@ int check_window(int64_t sequences, int64_t query_tokens, int64_t key_tokens,
   return SW_OK;
 }
 
+// Checks what both directions take and fills `a`; `some` says whether there
+// is anything to launch.
+int fill_window(WindowArgs &a, size_t elem, const int32_t *query_offsets,
+                const int32_t *key_offsets, const void *query, const void *key,
+                const void *value, const void *output, const float *log_sum,
+                int64_t sequences, int64_t query_tokens, int64_t key_tokens,
+                int64_t query_heads, int64_t key_heads, int64_t d,
+                const int64_t *strides, int64_t window, int64_t sinks,
+                float alpha, bool writes) {
+  if (int rc = check_window(sequences, query_tokens, key_tokens, query_heads,
+                            key_heads, d, window, sinks, alpha))
+    return rc;
+  if (sequences > 0 && (!query_offsets || !key_offsets))
+    return sw::fail(SW_ERR_INVALID_ARGUMENT, "sequence offsets pointer is null");
+  a.q = operand(strides, 0, query_heads, d);
+  a.k = operand(strides, 1, key_heads, d);
+  a.v = operand(strides, 2, key_heads, d);
+  a.o = operand(strides, 3, query_heads, d);
+  if (int rc = check_operand("query", query, a.q, d, elem, false, query_tokens,
+                             query_heads))
+    return rc;
+  if (int rc = check_operand("key", key, a.k, d, elem, false, key_tokens,
+                             key_heads))
+    return rc;
+  if (int rc = check_operand("value", value, a.v, d, elem, false, key_tokens,
+                             key_heads))
+    return rc;
+  if (int rc = check_operand("output", output, a.o, d, elem, writes,
+                             query_tokens, query_heads))
+    return rc;
+  if (int rc = sw::check_value_alignment(4, {query_offsets, key_offsets,
+                                             log_sum}))
+    return rc;
+  a.query_offsets = query_offsets;
+  a.key_offsets = key_offsets;
+  a.query = query;
+  a.key = key;
+  a.value = value;
+  a.output = const_cast<void *>(output);
+  a.log_sum = const_cast<float *>(log_sum);
+  a.sequences = (int)sequences;
+  a.query_tokens = (int)query_tokens;
+  a.key_tokens = (int)key_tokens;
+  a.query_heads = (int)query_heads;
+  a.key_heads = (int)key_heads;
+  a.d = (int)d;
+  // (no key lies past a window of all keys, so there are no sinks apart then)
+  a.window = (int)std::min(window, std::max<int64_t>(key_tokens, 1));
+  a.sinks = window >= key_tokens ? 0 : (int)std::min(sinks, key_tokens);
+  a.alpha = alpha;
+  a.tiles = (int)((query_tokens >> kRowShift) + sequences);
+  return sw::check_flat_grid((int64_t)a.tiles * query_heads, kThreads,
+                             "window attention");
+}
+
 template <typename T>
 int forward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
                   const T *query, const T *key, const T *value, T *output,
@@ -449,55 +1012,141 @@ int forward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
                   int64_t d, const int64_t *strides, int64_t window,
                   int64_t sinks, float alpha, void *stream) {
   sw::clear_error();
-  if (int rc = check_window(sequences, query_tokens, key_tokens, query_heads,
-                            key_heads, d, window, sinks, alpha))
-    return rc;
-  if (sequences > 0 && (!query_offsets || !key_offsets))
-    return sw::fail(SW_ERR_INVALID_ARGUMENT, "sequence offsets pointer is null");
   WindowArgs a{};
-  a.q = operand(strides, 0, query_heads, d);
-  a.k = operand(strides, 1, key_heads, d);
-  a.v = operand(strides, 2, key_heads, d);
-  a.o = operand(strides, 3, query_heads, d);
-  if (int rc = check_operand("query", query, a.q, d, sizeof(T), query_tokens > 0, false, query_tokens, query_heads))
-    return rc;
-  if (int rc = check_operand("key", key, a.k, d, sizeof(T), key_tokens > 0, false, key_tokens, key_heads))
-    return rc;
-  if (int rc = check_operand("value", value, a.v, d, sizeof(T), key_tokens > 0, false, key_tokens, key_heads))
-    return rc;
-  if (int rc = check_operand("output", output, a.o, d, sizeof(T), query_tokens > 0, true, query_tokens, query_heads))
-    return rc;
-  if (int rc = sw::check_value_alignment(4, {log_sum}))
+  if (int rc = fill_window(a, sizeof(T), query_offsets, key_offsets, query, key,
+                           value, output, log_sum, sequences, query_tokens,
+                           key_tokens, query_heads, key_heads, d, strides,
+                           window, sinks, alpha, true))
     return rc;
   if (sequences == 0 || query_tokens == 0)
     return SW_OK;
-  a.query_offsets = query_offsets;
-  a.key_offsets = key_offsets;
-  a.query = query;
-  a.key = key;
-  a.value = value;
-  a.output = output;
-  a.log_sum = log_sum;
-  a.sequences = (int)sequences;
-  a.query_tokens = (int)query_tokens;
-  a.key_tokens = (int)key_tokens;
-  a.query_heads = (int)query_heads;
-  a.key_heads = (int)key_heads;
-  a.d = (int)d;
-  a.window = (int)std::min(window, std::max<int64_t>(key_tokens, 1));
-  a.sinks = (int)std::min(sinks, key_tokens);
-  a.alpha = alpha;
-  const int64_t tiles = (query_tokens >> kRowShift) + sequences;
-  a.tiles = (int)tiles;
-  const int64_t grid = tiles * query_heads;
-  if (int rc = sw::check_flat_grid(grid, kThreads, "window attention"))
-    return rc;
+  const dim3 grid((unsigned)((int64_t)a.tiles * query_heads));
   const hipStream_t st = sw::as_stream(stream);
   if (d <= 64)
-    window_forward<T, 64><<<dim3((unsigned)grid), kThreads, 0, st>>>(a);
+    window_forward<T, 64><<<grid, kThreads, 0, st>>>(a);
   else
-    window_forward<T, 128><<<dim3((unsigned)grid), kThreads, 0, st>>>(a);
+    window_forward<T, 128><<<grid, kThreads, 0, st>>>(a);
   return sw::launch_check("window attention");
+}
+
+// The backward pass's scratch memory: [2][query_heads][query_tokens] of the
+// queries' numbers, then the sinks' sums.
+struct Scratch {
+  int64_t stats, sink_window, sink_chunks; // floats of each
+  int64_t chunks;
+  int chunk_shift, sink_rows;
+  int64_t bytes() const { return 4 * (2 * stats + sink_window + sink_chunks); }
+};
+Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
+                         int64_t key_tokens, int64_t query_heads,
+                         int64_t key_heads, int64_t d, int64_t window,
+                         int64_t sinks) {
+  Scratch c{};
+  // (whole 16 bytes, so that what follows stays aligned)
+  c.stats = sw::ceil_div(query_heads * query_tokens, 4) * 4;
+  const int64_t s = window >= key_tokens ? 0 : std::min(sinks, key_tokens);
+  if (s == 0)
+    return c;
+  c.sink_rows = (int)sw::ceil_div(s, 32) * 32;
+  // 1024 queries a chunk, more where there are more than 64 sinks: the sums
+  // then stay below the keys' own size
+  c.chunk_shift = 10;
+  while (((int64_t)64 << (c.chunk_shift - 10)) < s)
+    ++c.chunk_shift;
+  c.chunks = (query_tokens >> c.chunk_shift) + sequences;
+  const int64_t one = key_heads * c.sink_rows * 2 * d;
+  c.sink_window = sequences * one;
+  c.sink_chunks = c.chunks * one;
+  return c;
+}
+
+template <typename T>
+int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
+                   const T *query, const T *key, const T *value,
+                   const T *output, const float *log_sum,
+                   const T *output_gradient, T *query_gradient,
+                   T *key_gradient, T *value_gradient, int64_t sequences,
+                   int64_t query_tokens, int64_t key_tokens,
+                   int64_t query_heads, int64_t key_heads, int64_t d,
+                   const int64_t *strides, int64_t window, int64_t sinks,
+                   float alpha, void *workspace, int64_t workspace_bytes,
+                   void *stream) {
+  sw::clear_error();
+  BackwardArgs b{};
+  WindowArgs &a = b.w;
+  if (int rc = fill_window(a, sizeof(T), query_offsets, key_offsets, query, key,
+                           value, output, log_sum, sequences, query_tokens,
+                           key_tokens, query_heads, key_heads, d, strides,
+                           window, sinks, alpha, false))
+    return rc;
+  b.go = operand(strides, 4, query_heads, d);
+  b.gq = operand(strides, 5, query_heads, d);
+  b.gk = operand(strides, 6, key_heads, d);
+  b.gv = operand(strides, 7, key_heads, d);
+  if (int rc = check_operand("output gradient", output_gradient, b.go, d,
+                             sizeof(T), false, query_tokens, query_heads))
+    return rc;
+  if (int rc = check_operand("query gradient", query_gradient, b.gq, d,
+                             sizeof(T), true, query_tokens, query_heads))
+    return rc;
+  if (int rc = check_operand("key gradient", key_gradient, b.gk, d, sizeof(T),
+                             true, key_tokens, key_heads))
+    return rc;
+  if (int rc = check_operand("value gradient", value_gradient, b.gv, d,
+                             sizeof(T), true, key_tokens, key_heads))
+    return rc;
+  if (sequences == 0 || (query_tokens == 0 && key_tokens == 0))
+    return SW_OK;
+  if (!log_sum && query_tokens > 0)
+    return sw::fail(SW_ERR_INVALID_ARGUMENT, "log_sum pointer is null");
+  const Scratch c = backward_scratch(sequences, query_tokens, key_tokens,
+                                     query_heads, key_heads, d, window, sinks);
+  if (c.bytes() > 0 && (!workspace || !sw::aligned16(workspace) ||
+                        workspace_bytes < c.bytes()))
+    return sw::fail(SW_ERR_INVALID_ARGUMENT,
+                    "the backward pass needs a 16-byte aligned workspace of "
+                    "%lld bytes", (long long)c.bytes());
+  b.output_gradient = output_gradient;
+  b.query_gradient = query_gradient;
+  b.key_gradient = key_gradient;
+  b.value_gradient = value_gradient;
+  b.log2_sum = static_cast<float *>(workspace);
+  b.delta = b.log2_sum + c.stats;
+  b.sink_window = b.delta + c.stats;
+  b.sink_chunks = b.sink_window + c.sink_window;
+  b.chunks = (int)c.chunks;
+  b.chunk_shift = c.chunk_shift;
+  b.sink_rows = c.sink_rows;
+  b.key_tiles = (int)((key_tokens >> kRowShift) + sequences);
+  const int64_t grid = (int64_t)b.key_tiles * key_heads +
+                       c.chunks * key_heads * (c.sink_rows / 32);
+  const int64_t rows = sequences * key_heads * a.sinks;
+  if (int rc = sw::check_flat_grid(std::max(grid, rows), kThreads,
+                                   "window attention's gradient"))
+    return rc;
+  const hipStream_t st = sw::as_stream(stream);
+  const dim3 rows_grid((unsigned)((int64_t)a.tiles * query_heads));
+  if (query_tokens > 0) {
+    if (d <= 64)
+      window_query_gradient<T, 64><<<rows_grid, kThreads, 0, st>>>(b);
+    else
+      window_query_gradient<T, 128><<<rows_grid, kThreads, 0, st>>>(b);
+    if (int rc = sw::launch_check("window attention's query gradient"))
+      return rc;
+  }
+  if (key_tokens == 0)
+    return SW_OK;
+  if (d <= 64)
+    window_key_gradient<T, 64><<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
+  else
+    window_key_gradient<T, 128><<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
+  if (int rc = sw::launch_check("window attention's key gradient"))
+    return rc;
+  if (a.sinks > 0) {
+    window_sink_gradient<T><<<dim3((unsigned)rows), 128, 0, st>>>(b);
+    return sw::launch_check("window attention's sink gradient");
+  }
+  return SW_OK;
 }
 
 } // namespace
@@ -526,4 +1175,48 @@ extern "C" int sw_window_attention_bf16(
                                  output, log_sum, sequences, query_tokens,
                                  key_tokens, query_heads, key_heads, d,
                                  strides, window, sinks, alpha, stream);
+}
+
+extern "C" int64_t sw_window_attention_backward_workspace_bytes(
+    int64_t sequences, int64_t query_tokens, int64_t key_tokens,
+    int64_t query_heads, int64_t key_heads, int64_t d, int64_t window,
+    int64_t sinks) {
+  if (check_window(sequences, query_tokens, key_tokens, query_heads, key_heads,
+                   d, window, sinks, 0.0f) != SW_OK)
+    return 0;
+  return backward_scratch(sequences, query_tokens, key_tokens, query_heads,
+                          key_heads, d, window, sinks).bytes();
+}
+
+extern "C" int sw_window_attention_backward_f32(
+    const int32_t *query_offsets, const int32_t *key_offsets,
+    const float *query, const float *key, const float *value,
+    const float *output, const float *log_sum, const float *output_gradient,
+    float *query_gradient, float *key_gradient, float *value_gradient,
+    int64_t sequences, int64_t query_tokens, int64_t key_tokens,
+    int64_t query_heads, int64_t key_heads, int64_t d, const int64_t *strides,
+    int64_t window, int64_t sinks, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream) {
+  return backward_entry<float>(
+      query_offsets, key_offsets, query, key, value, output, log_sum,
+      output_gradient, query_gradient, key_gradient, value_gradient, sequences,
+      query_tokens, key_tokens, query_heads, key_heads, d, strides, window,
+      sinks, alpha, workspace, workspace_bytes, stream);
+}
+
+extern "C" int sw_window_attention_backward_bf16(
+    const int32_t *query_offsets, const int32_t *key_offsets,
+    const uint16_t *query, const uint16_t *key, const uint16_t *value,
+    const uint16_t *output, const float *log_sum,
+    const uint16_t *output_gradient, uint16_t *query_gradient,
+    uint16_t *key_gradient, uint16_t *value_gradient, int64_t sequences,
+    int64_t query_tokens, int64_t key_tokens, int64_t query_heads,
+    int64_t key_heads, int64_t d, const int64_t *strides, int64_t window,
+    int64_t sinks, float alpha, void *workspace, int64_t workspace_bytes,
+    void *stream) {
+  return backward_entry<uint16_t>(
+      query_offsets, key_offsets, query, key, value, output, log_sum,
+      output_gradient, query_gradient, key_gradient, value_gradient, sequences,
+      query_tokens, key_tokens, query_heads, key_heads, d, strides, window,
+      sinks, alpha, workspace, workspace_bytes, stream);
 }

@@ -206,3 +206,249 @@ def test_forward_repeats_and_graph(dev, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, replayed)
+
+
+# ---- the backward pass ---------------------------------------------------------
+
+def backward(qo, ko, q, k, v, do, alpha, window, sinks, fill=7.0):
+    """Forward and backward as a training step makes them; the gradients."""
+    dev = [x.to(DEV) for x in (qo, ko, q, k, v)]
+    out = torch.full_like(dev[2], fill)
+    lse = torch.full((q.shape[1], q.shape[0]), fill, device=DEV)
+    sw.window_attention(*dev, out, lse, alpha, window, sinks)
+    grads = [torch.full_like(x, fill) for x in dev[2:]]
+    got = sw.window_attention_backward(*dev, out, lse, do.to(DEV), *grads,
+                                       alpha, window, sinks)
+    torch.cuda.synchronize()
+    assert all(a is b for a, b in zip(got, grads))
+    return [g.cpu() for g in grads]
+
+
+def expect_gradients(qo, ko, q, k, v, do, grads, alpha, window, sinks,
+                     fill=7.0):
+    t = half_step(q.dtype)
+    h, hk = q.shape[1], k.shape[1]
+    g = h // hk
+    qd, kd, vd, dod = (x.double() for x in (q, k, v, do))
+    queries = torch.zeros(q.shape[0], dtype=torch.bool)
+    keys = torch.zeros(k.shape[0], dtype=torch.bool)
+    for i in range(len(qo) - 1):
+        a, b, c, e = int(qo[i]), int(qo[i + 1]), int(ko[i]), int(ko[i + 1])
+        queries[a:b], keys[c:e] = True, True
+        see = visible(b - a, e - c, window, sinks)
+        for j in range(hk):
+            total = [torch.zeros(e - c, q.shape[2], dtype=torch.float64)
+                     for _ in range(4)]
+            for x in range(j * g, j * g + g):
+                (dq, *kv), (bound, *kv_bound) = gradients(
+                    qd[a:b, x], kd[c:e, j], vd[c:e, j], dod[a:b, x], see,
+                    alpha, t)
+                check(f"dq of sequence {i}, head {x}", grads[0][a:b, x], dq,
+                      bound)
+                for n, y in enumerate(kv + kv_bound):
+                    total[n] += y
+            check(f"dk of sequence {i}, head {j}", grads[1][c:e, j], total[0],
+                  total[2] + t * total[0].abs())
+            check(f"dv of sequence {i}, head {j}", grads[2][c:e, j], total[1],
+                  total[3] + t * total[1].abs())
+    for x, inside in zip(grads, (queries, keys, keys)):
+        assert torch.equal(x[~inside], torch.full_like(x[~inside], fill))
+
+
+def output_gradient(x, seed=1):
+    gen = torch.Generator().manual_seed(seed + 1000)
+    return torch.randn(x[2].shape, generator=gen).to(x[2].dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_backward(dev, dtype, case):
+    (nq, nk), window, sinks = CASES[case]
+    say(f"window backward {dtype} {CASES[case]}")
+    x = inputs(dtype, nq, nk, 2, 1, 64, seed=case)
+    do = output_gradient(x)
+    grads = backward(*x, do, 0.125, window, sinks)
+    expect_gradients(*x, do, grads, 0.125, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("h,hk,d", [(1, 1, 8), (3, 3, 24), (6, 2, 64),
+                                    (4, 1, 72), (2, 2, 96), (8, 2, 128),
+                                    (5, 1, 128)])
+def test_backward_heads(dev, dtype, h, hk, d):
+    say(f"window backward heads {dtype} {h} {hk} {d}")
+    x = inputs(dtype, [70, 131], [90, 131], h, hk, d, seed=d + h)
+    do = output_gradient(x)
+    grads = backward(*x, do, 1 / math.sqrt(d), 48, 5)
+    expect_gradients(*x, do, grads, 1 / math.sqrt(d), 48, 5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(100, 4), (40, 33), (700, 70)])
+def test_backward_sinks_over_chunks(dev, dtype, d, window, sinks):
+    """Sinks that queries of several chunks see from past the window, in
+    sequences that start inside a chunk and one that has no such queries."""
+    say(f"window backward sinks {dtype} {d} {window} {sinks}")
+    x = inputs(dtype, [1500, 30, 1100], [1500, 30, 1200], 2, 1, d, seed=d,
+               lead=5, tail=9)
+    do = output_gradient(x)
+    grads = backward(*x, do, 1 / math.sqrt(d), window, sinks)
+    expect_gradients(*x, do, grads, 1 / math.sqrt(d), window, sinks)
+
+
+@pytest.mark.parametrize("alpha", [-0.3, 0.0])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_backward_alpha(dev, dtype, alpha):
+    say(f"window backward alpha {dtype} {alpha}")
+    x = inputs(dtype, [200], [200], 2, 1, 64, seed=5)
+    do = output_gradient(x)
+    grads = backward(*x, do, alpha, 70, 2)
+    expect_gradients(*x, do, grads, alpha, 70, 2)
+
+
+def test_backward_against_differences(dev):
+    """Directional derivatives of sum(output * do), by central differences in
+    fp32: the step 2^-6 leaves a cubic term of about 2^-12 of the derivative,
+    and the sum's rounding, about 2^-20 of its terms' size, is divided by the
+    step."""
+    say("window backward differences")
+    x = inputs("f32", [150], [170], 4, 2, 32, seed=8)
+    do = output_gradient(x)
+    alpha, window, sinks = 0.2, 40, 3
+    grads = backward(*x, do, alpha, window, sinks)
+    gen = torch.Generator().manual_seed(77)
+    for n in range(3):
+        way = torch.randn(x[2 + n].shape, generator=gen)
+        way /= way.norm()
+        step = 2.0 ** -6
+        sides = []
+        for sign in (1, -1):
+            y = list(x)
+            y[2 + n] = x[2 + n] + sign * step * way
+            out, _ = forward(*y, alpha, window, sinks)
+            sides.append((out.double() * do.double()).sum())
+        slope = (sides[0] - sides[1]) / (2 * step)
+        want = (grads[n].double() * way.double()).sum()
+        size = grads[n].double().norm()
+        assert abs(slope - want) <= 2.0 ** -10 * size
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_backward_strides(dev, dtype):
+    """Gradients into the slices of a projection's gradient, of operands that
+    are slices too, from a broadcast output gradient."""
+    say(f"window backward strides {dtype}")
+    gen = torch.Generator().manual_seed(11)
+    t, h, d = 150, 4, 64
+    packed = torch.randn(t, 3 * h, d, generator=gen).to(DTYPES[dtype]).to(DEV)
+    q, k, v = packed[:, :h], packed[:, h:2 * h], packed[:, 2 * h:]
+    do = torch.randn(t, 1, d, generator=gen).to(DTYPES[dtype]).to(DEV)
+    do = do.expand(t, h, d)
+    off = offsets([t]).to(DEV)
+    out = torch.empty(h, t, d, dtype=q.dtype, device=DEV).transpose(0, 1)
+    lse = torch.empty(h, t, device=DEV)
+    sw.window_attention(off, off, q, k, v, out, lse, 0.125, 40, 3)
+    full = torch.full_like(packed, 7.0)
+    sw.window_attention_backward(
+        off, off, q, k, v, out, lse, do, full[:, :h], full[:, h:2 * h],
+        full[:, 2 * h:], 0.125, 40, 3)
+    dense = [x.contiguous() for x in (q, k, v, out)]
+    plain = [torch.empty_like(x) for x in dense[:3]]
+    sw.window_attention_backward(off, off, *dense, lse, do.contiguous(),
+                                 *plain, 0.125, 40, 3)
+    assert torch.equal(full, torch.cat(plain, 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("what", ["query", "key", "value", "do"])
+def test_backward_keeps_what_is_masked_apart(dev, dtype, bad, what):
+    """An infinity or NaN at one token reaches the gradients of the tokens
+    that it sees or that see it, and of those alone that share a query with
+    them; the rest are those of clean operands."""
+    say(f"window backward {bad} in {what} {dtype}")
+    qo, ko, q, k, v = inputs(dtype, [260], [260], 1, 1, 64, seed=4)
+    do = output_gradient((qo, ko, q, k, v))
+    window, sinks, at = 40, 2, 101
+    clean = backward(qo, ko, q, k, v, do, 0.125, window, sinks)
+    y = {"query": q.clone(), "key": k.clone(), "value": v.clone(),
+         "do": do.clone()}
+    y[what][at, 0, 3] = bad
+    got = backward(qo, ko, y["query"], y["key"], y["value"], y["do"], 0.125,
+                   window, sinks)
+    see = visible(260, 260, window, sinks)
+    rows = torch.zeros(260, dtype=torch.bool)
+    if what in ("query", "do"):
+        rows[at] = True
+    else:
+        rows = see[:, at].clone()
+    cols = see[rows].any(0)
+    for n, (x, c) in enumerate(zip(got, clean)):
+        free = ~rows if n == 0 else ~cols
+        x, c = x[free].float(), c[free].float()
+        assert torch.isfinite(x).all()
+        # (a repeated pass may add up in another order)
+        assert (x - c).abs().max() <= 8 * half_step(q.dtype) * c.abs().max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_training_step_repeats_and_graphs(dev, dtype):
+    """Forward and backward together: the same bits again, from a given
+    workspace, on another stream, and from two captured graphs replayed in
+    turn with eager work between."""
+    say(f"window training step graph {dtype}")
+    x = inputs(dtype, [100, 1300], [100, 1300], 4, 2, 128, seed=2)
+    qo, ko, q, k, v = (y.to(DEV) for y in x)
+    do = output_gradient(x).to(DEV)
+
+    def buffers():
+        return [torch.empty_like(q), torch.empty(4, 1400, device=DEV),
+                torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]
+
+    def step(b, stream=None, **kw):
+        sw.window_attention(qo, ko, q, k, v, b[0], b[1], 0.1, 64, 4,
+                            stream=stream)
+        sw.window_attention_backward(qo, ko, q, k, v, b[0], b[1], do, *b[2:],
+                                     0.1, 64, 4, stream=stream, **kw)
+    want, other = buffers(), buffers()
+    step(want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    step(other, stream=side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, other))
+    need = sw.load_library().sw_window_attention_backward_workspace_bytes(
+        2, 1400, 1400, 4, 2, 128, 64, 4)
+    step(other, workspace=torch.full((need,), 255, dtype=torch.uint8,
+                                     device=DEV))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, other))
+    graphs, held = [], []
+    for _ in range(2):
+        held.append(buffers())
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            step(held[-1])
+    for i in range(3):
+        q.mul_(1.25)
+        step(want)
+        for b in held:
+            for y in b:
+                y.zero_()
+        graphs[i % 2].replay()
+        graphs[1 - i % 2].replay()
+        torch.cuda.synchronize()
+        for b in held:
+            assert all(torch.equal(a, c) for a, c in zip(want, b))
+
+
+def test_backward_refuses_a_short_workspace(dev):
+    x = inputs("f32", [10], [10], 1, 1, 64)
+    qo, ko, q, k, v = (y.to(DEV) for y in x)
+    lse = torch.zeros(1, 10, device=DEV)
+    g = [torch.zeros_like(q) for _ in range(3)]
+    with pytest.raises(sw.ShapeError, match="workspace must hold"):
+        sw.window_attention_backward(
+            qo, ko, q, k, v, q, lse, q, *g, 1.0, 4, 1,
+            workspace=torch.zeros(16, dtype=torch.uint8, device=DEV))

@@ -55,7 +55,65 @@ def test_refused(dt, kw, code, needle):
     assert rc == code and needle in message
 
 
+def c_backward(strides=None, dt="_bf16", **kw):
+    a = dict(query_offsets=A, key_offsets=A, query=A, key=A, value=A, output=A,
+             log_sum=A, output_gradient=A, query_gradient=A, key_gradient=A,
+             value_gradient=A, sequences=1, query_tokens=10, key_tokens=10,
+             query_heads=4, key_heads=2, d=64, window=8, sinks=1, alpha=1.0,
+             workspace=A, workspace_bytes=1 << 30)
+    a.update(kw)
+    v = list(a.values())
+    s = (ctypes.c_int64 * 16)(*strides) if strides else None
+    rc = getattr(sw.load_library(), "sw_window_attention_backward" + dt)(
+        *v[:17], s, *v[17:], None)
+    return rc, sw.load_library().sw_last_error().decode()
+
+
+FULL = [256, 64, 128, 64, 128, 64, 256, 64, 256, 64, 256, 64, 128, 64, 128, 64]
+
+
+@pytest.mark.parametrize("kw,code,needle", [
+    (dict(d=12), -2, "multiple of 8"),
+    (dict(window=-3), -2, "window of at least 1"),
+    (dict(log_sum=None), -3, "log_sum pointer is null"),
+    (dict(output_gradient=None), -3, "output gradient pointer is null"),
+    (dict(key_gradient=None), -3, "key gradient pointer is null"),
+    (dict(workspace=None), -3, "workspace of"),
+    (dict(workspace=A + 8), -3, "workspace of"),
+    (dict(workspace_bytes=100), -3, "workspace of"),
+    (dict(strides=FULL[:10] + [256, 0] + FULL[12:]), -2, "query gradient rows overlap"),
+    (dict(strides=FULL[:12] + [64, 64] + FULL[14:]), -2, "key gradient rows overlap"),
+    (dict(strides=FULL[:14] + [120, 64]), -2, "value gradient rows overlap"),
+])
+@pytest.mark.parametrize("dt", ["_f32", "_bf16"])
+def test_backward_refused(dt, kw, code, needle):
+    rc, message = c_backward(dt=dt, **kw)
+    assert rc == code and needle in message
+
+
+def test_backward_workspace_rule():
+    need = sw.load_library().sw_window_attention_backward_workspace_bytes
+    # two numbers of each query and head
+    assert need(1, 100, 100, 4, 2, 64, 100, 7) == 2 * 4 * 100 * 4
+    # sinks apart: those of the window and of one chunk a sequence more than
+    # whole ones, 32 rows each
+    rows = 2 * 32 * 2 * 64
+    assert need(3, 100, 100, 4, 2, 64, 99, 7) == 2 * 4 * 100 * 4 + \
+        4 * rows * (3 + 3)
+    assert need(3, 5000, 100, 4, 2, 64, 99, 7) == 2 * 4 * 5000 * 4 + \
+        4 * rows * (3 + 4 + 3)
+    # at least the keys' own size apart from one chunk a sequence, however
+    # many sinks
+    for sinks in (64, 100, 1000, 5000):
+        assert need(1, 1 << 20, 1 << 20, 1, 1, 128, 64, sinks) <= \
+            2 * 4 * (1 << 20) + 2 * 4 * (1 << 20) * 128 + 3 * 4 * 256 * (
+                sinks + 31)
+    assert need(1, 100, 100, 4, 3, 64, 100, 7) == 0
+
+
 def test_nothing_to_do():
+    assert c_backward(sequences=0, workspace=None)[0] == 0
+    assert c_backward(query_tokens=0, key_tokens=0, workspace=None)[0] == 0
     assert c_forward(sequences=0, query_offsets=None, key_offsets=None)[0] == 0
     assert c_forward(query_tokens=0, query=None, output=None)[0] == 0
 
@@ -81,3 +139,18 @@ def test_mirror_refuses():
         call(log_sum=torch.zeros(4, 5))
     with pytest.raises(TypeError, match="float32 or bfloat16"):
         call(query=q.half())
+
+    def back(**kw):
+        a = dict(query_offsets=off, key_offsets=off, query=q, key=k, value=k,
+                 output=q, log_sum=torch.zeros(4, 4), output_gradient=q,
+                 query_gradient=q, key_gradient=k, value_gradient=k,
+                 alpha=1.0, window=4)
+        sw.window_attention_backward(**{**a, **kw})
+    with pytest.raises(ValueError, match="device tensor"):
+        back()
+    with pytest.raises(sw.ShapeError, match="output_gradient must"):
+        back(output_gradient=k)
+    with pytest.raises(sw.ShapeError, match="value_gradient must"):
+        back(value_gradient=q)
+    with pytest.raises(sw.ShapeError, match="log_sum"):
+        back(log_sum=torch.zeros(4, 3))
