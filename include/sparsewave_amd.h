@@ -543,6 +543,72 @@ int sw_window_attention_backward_bf16(
     void *stream);
 
 /*
+ * One step of sw_window_attention for each sequence, against a key-value
+ * cache: query[sequences][query_heads][d], the query of sequence i at the place
+ * of its last key, over the last `window` of its key_lengths[i] keys and its
+ * first `sinks`.  Key j is row j % page_size of page
+ * page_table[i][j / page_size] of key_cache and value_cache
+ * [pages][page_size][key_heads][d]; page_table[sequences][table_width] may be
+ * NULL: sequence i then has page i to itself.  A page number outside 0 ..
+ * pages - 1 is not read: its keys are not there.  Lengths are clamped to 0 ..
+ * page_size * table_width; a sequence without keys gets zeros.
+ *
+ * Heads, d, types and alignment as in sw_window_attention; `strides` holds, in
+ * elements, the token and head stride of query and of output, and the page,
+ * token and head stride of key_cache and of value_cache (NULL: as the shapes
+ * above).  Offsets into a cache are 64 bits.  No atomics.  The workspace
+ * (16-byte aligned, of sw_window_attention_decode_workspace_bytes; none where
+ * that is 0) belongs to the call until its work on `stream` is done.
+ */
+int64_t sw_window_attention_decode_workspace_bytes(
+    int64_t sequences, int64_t page_size, int64_t table_width,
+    int64_t query_heads, int64_t key_heads, int64_t d, int64_t window,
+    int64_t sinks);
+int sw_window_attention_decode_f32(
+    const int32_t *key_lengths, const int32_t *page_table, const float *query,
+    const float *key_cache, const float *value_cache, float *output,
+    int64_t sequences, int64_t pages, int64_t page_size, int64_t table_width,
+    int64_t query_heads, int64_t key_heads, int64_t d, const int64_t *strides,
+    int64_t window, int64_t sinks, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream);
+int sw_window_attention_decode_bf16(
+    const int32_t *key_lengths, const int32_t *page_table,
+    const uint16_t *query, const uint16_t *key_cache,
+    const uint16_t *value_cache, uint16_t *output, int64_t sequences,
+    int64_t pages, int64_t page_size, int64_t table_width,
+    int64_t query_heads, int64_t key_heads, int64_t d, const int64_t *strides,
+    int64_t window, int64_t sinks, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream);
+
+/*
+ * One query for each sequence over a prefix that all of them share,
+ * prefix_key and prefix_value [prefix_tokens][key_heads][d], and behind it the
+ * sequence's own keys, all key_lengths[i] of a cache as above.  The prefix is
+ * read once for the whole batch.  `strides` holds four more: the token and
+ * head stride of prefix_key and of prefix_value.
+ */
+int64_t sw_shared_prefix_attention_workspace_bytes(
+    int64_t sequences, int64_t prefix_tokens, int64_t page_size,
+    int64_t table_width, int64_t query_heads, int64_t key_heads, int64_t d);
+int sw_shared_prefix_attention_f32(
+    const int32_t *key_lengths, const int32_t *page_table, const float *query,
+    const float *prefix_key, const float *prefix_value,
+    const float *key_cache, const float *value_cache, float *output,
+    int64_t sequences, int64_t prefix_tokens, int64_t pages,
+    int64_t page_size, int64_t table_width, int64_t query_heads,
+    int64_t key_heads, int64_t d, const int64_t *strides, float alpha,
+    void *workspace, int64_t workspace_bytes, void *stream);
+int sw_shared_prefix_attention_bf16(
+    const int32_t *key_lengths, const int32_t *page_table,
+    const uint16_t *query, const uint16_t *prefix_key,
+    const uint16_t *prefix_value, const uint16_t *key_cache,
+    const uint16_t *value_cache, uint16_t *output, int64_t sequences,
+    int64_t prefix_tokens, int64_t pages, int64_t page_size,
+    int64_t table_width, int64_t query_heads, int64_t key_heads, int64_t d,
+    const int64_t *strides, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream);
+
+/*
  * sparsewave.csr_row_at_position for a batch of positions:
  * out_rows[i] = (first j in [1, rows+1) with row_offsets[j] > positions[i]) - 1,
  * the row search of SparsePositionToSCF.cpp:225-271 that the position

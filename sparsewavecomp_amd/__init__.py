@@ -21,7 +21,8 @@ __all__ = [
     "coo_spmv", "spmv_gather_floor", "bsr_slab_floor", "attention_tile_floor",
     "spmm", "bsr_spmm", "sddmm", "csr_row_reduce", "csr_rowwise_map",
     "sparse_attention", "window_attention",
-    "window_attention_backward", "csr_row_at_position",
+    "window_attention_backward", "window_attention_decode",
+    "shared_prefix_attention", "csr_row_at_position",
     "SDDMM_MUL", "SDDMM_AFFINE", "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV", "MAP_SUB", "MAP_MUL",
 ]
 
@@ -45,6 +46,10 @@ EXPORTED_SYMBOLS = (
     "sw_sparse_attention_f32", "sw_sparse_attention_bf16",
     "sw_window_attention_f32", "sw_window_attention_bf16",
     "sw_window_attention_backward_workspace_bytes",
+    "sw_window_attention_decode_workspace_bytes",
+    "sw_window_attention_decode_f32", "sw_window_attention_decode_bf16",
+    "sw_shared_prefix_attention_workspace_bytes",
+    "sw_shared_prefix_attention_f32", "sw_shared_prefix_attention_bf16",
     "sw_window_attention_backward_f32", "sw_window_attention_backward_bf16",
     "sw_csr_row_at_position", "sw_attention_tile_floor",
     "sw_host_matrix_free", "sw_host_bsr_free", "sw_matrix_market_read",
@@ -180,7 +185,13 @@ def load_library():
             ctypes.c_int, [P] * 7 + [I64] * 6 + [P, I64, I64, F, P])
         sig["sw_window_attention_backward" + dt] = (
             ctypes.c_int, [P] * 11 + [I64] * 6 + [P, I64, I64, F, P, I64, P])
+        sig["sw_window_attention_decode" + dt] = (
+            ctypes.c_int, [P] * 6 + [I64] * 7 + [P, I64, I64, F, P, I64, P])
+        sig["sw_shared_prefix_attention" + dt] = (
+            ctypes.c_int, [P] * 8 + [I64] * 8 + [P, F, P, I64, P])
     sig["sw_window_attention_backward_workspace_bytes"] = (I64, [I64] * 8)
+    sig["sw_window_attention_decode_workspace_bytes"] = (I64, [I64] * 8)
+    sig["sw_shared_prefix_attention_workspace_bytes"] = (I64, [I64] * 7)
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -631,7 +642,8 @@ def sparse_attention(row_offsets, column_indices, mask_values, query,
 
 def _heads(t, dtype, name):
     """Address and (row, head) strides of a [rows, heads, d] operand, whose
-    rows of d elements are consecutive."""
+    rows of d elements are consecutive; of [pages, rows, heads, d] the page's
+    before them."""
     torch = _torch or _load_torch()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -639,16 +651,21 @@ def _heads(t, dtype, name):
         raise ValueError(f"{name} must be a device tensor, got {t.device}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    *outer, row, head, last = t.stride()
-    if last != 1 and t.shape[-1] > 1:
+    if t.is_contiguous():
+        *pages, rows, heads, d = t.shape
+        if pages:
+            return t.data_ptr(), rows * heads * d, heads * d, d
+        return t.data_ptr(), heads * d, d
+    *page, row, head, last = t.stride()
+    if last != 1:
         raise ValueError(f"{name} must have consecutive elements in its last "
                          "dimension")
-    # (a dimension of one has any stride: its packed one)
+    # (the stride of a dimension of one is any number: a packed one)
     if t.shape[-2] == 1:
         head = t.shape[-1]
     if t.shape[-3] == 1:
-        row = max(head, t.shape[-1]) * t.shape[-2]
-    return (t.data_ptr(), *outer, row, head)
+        row = t.shape[-2] * max(head, t.shape[-1])
+    return (t.data_ptr(), *page, row, head)
 
 
 def _one_device(stream, *tensors):
@@ -784,6 +801,105 @@ def window_attention_backward(query_offsets, key_offsets, query, key, value,
         None if scratch is None else scratch.data_ptr(), need,
         _stream(stream)))
     return query_gradient, key_gradient, value_gradient
+
+
+def _cache_shapes(key_lengths, page_table, query, key_cache, value_cache,
+                  output):
+    _need(query.dim() == 3 and tuple(output.shape) == tuple(query.shape),
+          "expected query and output [sequences, query_heads, d]")
+    _need(key_cache.dim() == 4 and
+          tuple(key_cache.shape) == tuple(value_cache.shape) and
+          key_cache.shape[3] == query.shape[2],
+          "expected key and value caches [pages, page_size, key_heads, d]")
+    sequences, width = query.shape[0], 1
+    _need(tuple(key_lengths.shape) == (sequences,),
+          "key_lengths must hold one length a sequence")
+    if page_table is not None:
+        _need(page_table.dim() == 2 and page_table.shape[0] == sequences,
+              "page_table must be [sequences, most_pages]")
+        width = page_table.shape[1]
+    return (sequences, key_cache.shape[0], key_cache.shape[1], width,
+            query.shape[1], key_cache.shape[2], query.shape[2])
+
+
+def window_attention_decode(key_lengths, page_table, query, key_cache,
+                            value_cache, output, alpha, window, sinks=0,
+                            workspace=None, stream=None):
+    """One step of :func:`window_attention` for each sequence, against a
+    key-value cache: query and output [sequences, query_heads, d], the query
+    at the place of its sequence's last key.  It sees the last `window` of
+    key_lengths[i] keys and the first `sinks`.
+
+    Key j of sequence i is row j % page_size of page
+    page_table[i, j // page_size] of key_cache and value_cache [pages,
+    page_size, key_heads, d], or, where page_table is None, row j of page i.
+    A page number outside the cache means that its keys are not there.
+    Lengths are clamped to what a table's row holds; a length of 0 gives
+    zeros.  float32 or bfloat16, any strides of 16 bytes.  The scratch memory
+    of sw_window_attention_decode_workspace_bytes is taken from torch's
+    allocator where `workspace` (uint8) is not given."""
+    torch = _torch or _load_torch()
+    shape = _cache_shapes(key_lengths, page_table, query, key_cache,
+                          value_cache, output)
+    dt = _value_dtype(query, "query")
+    _one_device(stream, key_lengths, page_table, query, key_cache, value_cache,
+                output)
+    q, o = _heads(query, dt, "query"), _heads(output, dt, "output")
+    k = _heads(key_cache, dt, "key_cache")
+    v = _heads(value_cache, dt, "value_cache")
+    lib = load_library()
+    need = lib.sw_window_attention_decode_workspace_bytes(
+        shape[0], *shape[2:], window, sinks)
+    lengths = _dev(key_lengths, torch.int32, "key_lengths")
+    table = (None if page_table is None else
+             _dev(page_table, torch.int32, "page_table"))
+    scratch = _scratch(need, query, workspace, stream)
+    _check(_fn("sw_window_attention_decode", dt)(
+        lengths, table, q[0], k[0], v[0], o[0], *shape,
+        (ctypes.c_int64 * 10)(*q[1:], *o[1:], *k[1:], *v[1:]), window, sinks,
+        alpha, None if scratch is None else scratch.data_ptr(), need,
+        _stream(stream)))
+    return output
+
+
+def shared_prefix_attention(key_lengths, page_table, query, prefix_key,
+                            prefix_value, key_cache, value_cache, output,
+                            alpha, workspace=None, stream=None):
+    """One query for each sequence over a prefix that all share, prefix_key
+    and prefix_value [prefix_tokens, key_heads, d], and behind it the sequence's
+    own key_lengths[i] keys in a cache laid out as
+    :func:`window_attention_decode` takes it.  The prefix is read once for the
+    whole batch.  Operands, types and workspace as there."""
+    torch = _torch or _load_torch()
+    shape = _cache_shapes(key_lengths, page_table, query, key_cache,
+                          value_cache, output)
+    _need(prefix_key.dim() == 3 and
+          tuple(prefix_key.shape) == tuple(prefix_value.shape) and
+          tuple(prefix_key.shape[1:]) == tuple(key_cache.shape[2:]),
+          "expected prefix key and value [prefix_tokens, key_heads, d]")
+    dt = _value_dtype(query, "query")
+    _one_device(stream, key_lengths, page_table, query, prefix_key,
+                prefix_value, key_cache, value_cache, output)
+    q, o = _heads(query, dt, "query"), _heads(output, dt, "output")
+    pk = _heads(prefix_key, dt, "prefix_key")
+    pv = _heads(prefix_value, dt, "prefix_value")
+    k = _heads(key_cache, dt, "key_cache")
+    v = _heads(value_cache, dt, "value_cache")
+    lib = load_library()
+    need = lib.sw_shared_prefix_attention_workspace_bytes(
+        shape[0], prefix_key.shape[0], *shape[2:])
+    lengths = _dev(key_lengths, torch.int32, "key_lengths")
+    table = (None if page_table is None else
+             _dev(page_table, torch.int32, "page_table"))
+    scratch = _scratch(need, query, workspace, stream)
+    _check(_fn("sw_shared_prefix_attention", dt)(
+        lengths, table, q[0], pk[0], pv[0], k[0], v[0], o[0], shape[0],
+        prefix_key.shape[0], *shape[1:],
+        (ctypes.c_int64 * 14)(*q[1:], *o[1:], *k[1:], *v[1:], *pk[1:],
+                              *pv[1:]),
+        alpha, None if scratch is None else scratch.data_ptr(), need,
+        _stream(stream)))
+    return output
 
 
 def csr_row_at_position(row_offsets, positions, out_rows, stream=None):

@@ -26,6 +26,7 @@ SOURCES = [
     "sw_bsr.hip",
     "sw_attention.hip",
     "sw_window_attention.hip",
+    "sw_cache_attention.hip",
 ]
 
 # -packed-fp32-ops: keep hipcc from forming v_pk_{add,mul,fma}_f32.

@@ -203,8 +203,9 @@ __device__ __forceinline__ void copy_words_to_lds(v4u buffer, uint32_t at,
 // lies at place c ^ swizzle(r).  The swizzle keeps these reads free of bank
 // conflicts (64 banks of 4 bytes): 16 consecutive rows at one chunk (a
 // fragment along the rows), and, for bf16, four consecutive chunks of each of
-// four consecutive rows (half a wave's transposing load).  ROWS is a multiple
-// of 32 and a tile is filled by THREADS threads.
+// four consecutive rows or two of each of eight (half a wave's transposing
+// load for products of 32 or 16 rows).  ROWS is a multiple of 32 and a tile is
+// filled by THREADS threads.
 template <typename T, int D, int ROWS, int THREADS> struct RowTile {
   static constexpr int kChunks = D * (int)sizeof(T) / 16;
   static constexpr int kPitch = D * (int)sizeof(T);
@@ -217,9 +218,9 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
     if constexpr (sizeof(T) == 4)
       return row & 15;
     else if constexpr (kChunks == 16)
-      return ((row & 3) << 2) | ((row >> 2) & 3);
+      return ((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1);
     else
-      return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+      return ((row << 1) & 4) | ((row >> 1) & 2) | ((row >> 3) & 1);
   }
   __device__ static __forceinline__ int place(int row, int chunk) {
     return row * kPitch + ((chunk ^ swizzle(row)) << 4);
@@ -332,6 +333,20 @@ __device__ __forceinline__ void landed() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+
+// A lane's row of 32 as fragments, zeros where it is not live and past d.
+template <typename T, int STEPS>
+__device__ __forceinline__ void load_rows(Frag<T> (&f)[STEPS], const T *p,
+                                          bool live, int d, bool negate) {
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) {
+    const int c = 16 * st + 8 * h;
+    f[st] = live && c < d ? ld_frag(p + c) : zero_frag<T>();
+    if (negate)
+      f[st] = negate_frag<T>(f[st]);
+  }
 }
 
 // ---- packed sequences ----------------------------------------------------------

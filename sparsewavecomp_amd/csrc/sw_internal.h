@@ -155,4 +155,63 @@ inline int check_csr(const int32_t *ro, const int32_t *col, const void *val,
   return SW_OK;
 }
 
+// ---- attention over [tokens][heads][d] operands ----
+
+constexpr int64_t kMostTokens = (int64_t)1 << 30;
+
+struct Operand {
+  int64_t token, head; // strides in elements
+};
+
+constexpr int64_t kMostStride = (int64_t)1 << 40;
+
+// Strides of one operand: rows of d elements, 16-byte aligned, close enough
+// that a tile of rows spans 2^30 bytes (descriptor offsets are 32 bits).
+inline int check_operand(const char *name, const void *p, const Operand &s,
+                         int64_t d, int64_t elem, bool output, int64_t tokens,
+                         int64_t heads) {
+  if (tokens == 0)
+    return SW_OK;
+  if (!p)
+    return fail(SW_ERR_INVALID_ARGUMENT, "%s pointer is null", name);
+  if (s.token < d || s.head < 0 || s.token > ((int64_t)1 << 23) / elem ||
+      s.head > kMostStride)
+    return fail(SW_ERR_INVALID_SHAPE,
+                "%s strides must be at least d = %lld (tokens; at most 2^23 "
+                "bytes) and 0 (heads; at most 2^40), but got %lld and %lld",
+                name, (long long)d, (long long)s.token, (long long)s.head);
+  if (!aligned16(p) || s.token * elem % 16 != 0 || s.head * elem % 16 != 0)
+    return fail(SW_ERR_INVALID_ARGUMENT,
+                "%s must be 16-byte aligned, its strides included", name);
+  if (output && heads > 1) {
+    // heads within a token's row, or a head's tokens within its plane
+    const bool in_row = s.head >= d && s.token >= (heads - 1) * s.head + d;
+    const bool in_plane = s.head >= (tokens - 1) * s.token + d;
+    if (!in_row && !in_plane)
+      return fail(SW_ERR_INVALID_SHAPE, "%s rows overlap", name);
+  }
+  return SW_OK;
+}
+
+inline Operand operand(const int64_t *strides, int i, int64_t heads, int64_t d) {
+  if (strides)
+    return {strides[2 * i], strides[2 * i + 1]};
+  return {heads * d, d};
+}
+
+// Query heads share key heads in groups; rows of d are whole fragments.
+inline int check_heads(int64_t query_heads, int64_t key_heads, int64_t d) {
+  if (query_heads < 1 || key_heads < 1 || query_heads > 65536 ||
+      query_heads % key_heads != 0)
+    return fail(SW_ERR_INVALID_SHAPE,
+                    "query heads must be a multiple of key heads (at most "
+                    "65536), but got %lld and %lld", (long long)query_heads,
+                    (long long)key_heads);
+  if (d < 8 || d > 128 || d % 8 != 0)
+    return fail(SW_ERR_INVALID_SHAPE,
+                    "head dimension must be a multiple of 8 up to 128, but "
+                    "got %lld", (long long)d);
+  return SW_OK;
+}
+
 } // namespace sw

@@ -19,6 +19,9 @@
 #include <cmath>
 
 using namespace swd;
+using sw::Operand;
+using sw::check_operand;
+using sw::operand;
 
 namespace {
 
@@ -29,10 +32,6 @@ constexpr float kInf = __builtin_inff();
 constexpr int kThreads = 256; // four waves of 32 rows
 constexpr int kRowShift = 7;
 constexpr int kRows = 1 << kRowShift;
-
-struct Operand {
-  int64_t token, head; // strides in elements
-};
 
 struct WindowArgs {
   const int32_t *query_offsets, *key_offsets;
@@ -166,19 +165,6 @@ __device__ __forceinline__ v16f mma32_seen(Frag<T> a, Frag<T> b, v16f acc,
   return acc;
 }
 
-// the rows of a fragment's lane: 32 of an operand, zeros past the end
-template <typename T, int STEPS>
-__device__ __forceinline__ void load_rows(Frag<T> (&f)[STEPS], const T *p,
-                                          bool live, int d, bool negate) {
-  const int h = lane_id() >> 5;
-#pragma unroll
-  for (int st = 0; st < STEPS; ++st) {
-    const int c = 16 * st + 8 * h;
-    f[st] = live && c < d ? ld_frag(p + c) : zero_frag<T>();
-    if (negate)
-      f[st] = negate_frag<T>(f[st]);
-  }
-}
 template <typename T, int BLOCKS>
 __device__ __forceinline__ bool all_finite(const v16f (&acc)[BLOCKS]) {
   float x = 0.0f;
@@ -885,60 +871,18 @@ __global__ void window_sink_gradient(BackwardArgs b) {
 
 // ---- host ------------------------------------------------------------------------
 
-// Strides of one operand: rows of d elements, 16-byte aligned, close enough
-// that a tile of rows spans 2^30 bytes (descriptor offsets are 32 bits).
-int check_operand(const char *name, const void *p, const Operand &s, int64_t d,
-                  int64_t elem, bool output, int64_t tokens, int64_t heads) {
-  if (tokens == 0)
-    return SW_OK;
-  if (!p)
-    return sw::fail(SW_ERR_INVALID_ARGUMENT, "%s pointer is null", name);
-  if (!sw::aligned16(p) || s.token * elem % 16 != 0 || s.head * elem % 16 != 0)
-    return sw::fail(SW_ERR_INVALID_ARGUMENT,
-                    "%s must be 16-byte aligned, its strides included", name);
-  if (s.token < d || s.head < 0 || s.token * elem > (int64_t)1 << 23)
-    return sw::fail(SW_ERR_INVALID_SHAPE,
-                    "%s strides must be at least d = %lld (tokens; at most "
-                    "2^23 bytes) and 0 (heads), but got %lld and %lld",
-                    name, (long long)d, (long long)s.token, (long long)s.head);
-  if (output && heads > 1) {
-    // heads within a token's row, or a head's tokens within its plane
-    const bool in_row = s.head >= d && s.token >= (heads - 1) * s.head + d;
-    const bool in_plane = s.head >= (tokens - 1) * s.token + d;
-    if (!in_row && !in_plane)
-      return sw::fail(SW_ERR_INVALID_SHAPE, "%s rows overlap", name);
-  }
-  return SW_OK;
-}
-
-constexpr int64_t kMostTokens = (int64_t)1 << 30;
-
-Operand operand(const int64_t *strides, int i, int64_t heads, int64_t d) {
-  if (strides)
-    return {strides[2 * i], strides[2 * i + 1]};
-  return {heads * d, d};
-}
-
 int check_window(int64_t sequences, int64_t query_tokens, int64_t key_tokens,
                  int64_t query_heads, int64_t key_heads, int64_t d,
                  int64_t window, int64_t sinks, float alpha) {
   if (sequences < 0 || query_tokens < 0 || key_tokens < 0 ||
-      sequences > kMostTokens || query_tokens > kMostTokens ||
-      key_tokens > kMostTokens)
+      sequences > sw::kMostTokens || query_tokens > sw::kMostTokens ||
+      key_tokens > sw::kMostTokens)
     return sw::fail(SW_ERR_INVALID_SHAPE,
                     "expected 0 to 2^30 sequences and tokens, but got %lld, "
                     "%lld and %lld", (long long)sequences,
                     (long long)query_tokens, (long long)key_tokens);
-  if (query_heads < 1 || key_heads < 1 || query_heads > 65536 ||
-      query_heads % key_heads != 0)
-    return sw::fail(SW_ERR_INVALID_SHAPE,
-                    "query heads must be a multiple of key heads (at most "
-                    "65536), but got %lld and %lld", (long long)query_heads,
-                    (long long)key_heads);
-  if (d < 8 || d > 128 || d % 8 != 0)
-    return sw::fail(SW_ERR_INVALID_SHAPE,
-                    "head dimension must be a multiple of 8 up to 128, but "
-                    "got %lld", (long long)d);
+  if (int rc = sw::check_heads(query_heads, key_heads, d))
+    return rc;
   if (window < 1 || sinks < 0)
     return sw::fail(SW_ERR_INVALID_SHAPE,
                     "expected a window of at least 1 and no negative sinks, "
