@@ -236,7 +236,7 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
   __device__ static __forceinline__ void copy(uint32_t lds, const T *base,
                                               int rows, uint32_t row_bytes,
                                               int d) {
-    const int l = lane_id(), w = wave_in_group();
+    const int l = lane_id(), w = THREADS == kWave ? 0 : wave_in_group();
     constexpr int kStep = (THREADS / kWave) * (1024 / kPitch); // rows a pass
     rows = rows < 0 ? 0 : rows > ROWS ? ROWS : rows;
     const uint32_t bytes =
@@ -257,68 +257,88 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
     }
   }
 
-  // A lane's addresses within any tile, which a kernel computes once: what is
-  // left of a read's address is a constant that the load instruction adds.
+  // A lane's addresses within any tile, in two registers: an operation for each
+  // address that is used.
+  struct FewLane {
+    uint32_t x, y;
+    __device__ __forceinline__ FewLane() {
+      const int l = lane_id(), h = l >> 5, i = l & 15;
+      if constexpr (sizeof(T) == 2) {
+        x = place(l & 31, h);
+        y = place(4 * h + (i >> 2), 2 * ((l >> 4) & 1) + ((i & 3) >> 1)) +
+            (i & 1) * 8;
+      } else {
+        x = place(l & 31, 2 * h);
+        y = place(4 * h, (l & 31) >> 2) + (l & 3) * 4;
+      }
+    }
+    // (keeps the compiler from computing every address ahead of a loop)
+    __device__ __forceinline__ void fresh() {
+      asm volatile("" : "+v"(x), "+v"(y));
+    }
+    // bf16: chunk 2 i + h; fp32: chunk 4 (i / 2) + 2 h + i % 2
+    __device__ __forceinline__ uint32_t along(int i) const {
+      return x ^ (sizeof(T) == 2 ? i << 5 : (i >> 1) << 6 | (i & 1) << 4);
+    }
+    // bf16: chunks from 4 (i % (D / 32)) on, rows from 8 (i / (D / 32)) on;
+    // fp32: row i
+    __device__ __forceinline__ uint32_t across(int i) const {
+      if constexpr (sizeof(T) == 2)
+        return (y ^ ((i % (D / 32)) << 6 | (i / (D / 32)) << 4)) +
+               i / (D / 32) * 8 * kPitch;
+      else
+        return (y ^ (i << 4)) + i * kPitch;
+    }
+  };
+  // The same computed once: what is left of a read's address is a constant that
+  // the load instruction adds.
   // (The swizzle reaches the chunk's four low bits: fp32 reads that differ in
   // higher ones share an address.)
   struct Lane {
-    uint32_t along[sizeof(T) == 2 ? kSteps : 8];
-    uint32_t across[sizeof(T) == 2 ? 2 * (D / 32) : 4];
+    uint32_t x[sizeof(T) == 2 ? kSteps : 8], y[sizeof(T) == 2 ? 2 * (D / 32) : 4];
     __device__ __forceinline__ Lane() {
-      const int l = lane_id(), h = l >> 5;
-      if constexpr (sizeof(T) == 2) {
-        const int i = l & 15;
+      const FewLane f;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-          along[s] = place(l & 31, 2 * s + h);
+      for (int i = 0; i < (int)(sizeof x / 4); ++i)
+        x[i] = f.along(i);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int db = 0; db < D / 32; ++db)
-            across[e * (D / 32) + db] =
-                place(8 * e + 4 * h + (i >> 2),
-                      4 * db + 2 * ((l >> 4) & 1) + ((i & 3) >> 1)) +
-                (i & 1) * 8;
-      } else {
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          along[s] = place(l & 31, 4 * (s / 2) + 2 * h + s % 2);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          across[e] = place(4 * h + e, (l & 31) >> 2) + (l & 3) * 4;
-      }
+      for (int i = 0; i < (int)(sizeof y / 4); ++i)
+        y[i] = f.across(i);
     }
+    __device__ __forceinline__ uint32_t along(int i) const { return x[i]; }
+    __device__ __forceinline__ uint32_t across(int i) const { return y[i]; }
   };
-
   // Row 32 rb + l % 32, elements 16 s + 8 (l / 32) + i: the A operand with
-  // the tile's rows as rows.
-  __device__ static __forceinline__ Frag<T> along(uint32_t lds, const Lane &n,
+  // the tile's rows as rows (or B, with its rows as columns).
+  template <typename L>
+  __device__ static __forceinline__ Frag<T> along(uint32_t lds, const L &n,
                                                   int rb, int s) {
     const uint32_t at = lds + 32 * rb * kPitch;
     if constexpr (sizeof(T) == 2) {
-      return lds_read<v4u>(n.along[s], at);
+      return lds_read<v4u>(n.along(s), at);
     } else {
       const uint32_t up = at + 256 * (s / 4);
-      const v4f a = lds_read<v4f>(n.along[2 * (s % 4)], up);
-      const v4f b = lds_read<v4f>(n.along[2 * (s % 4) + 1], up);
+      const v4f a = lds_read<v4f>(n.along(2 * (s % 4)), up);
+      const v4f b = lds_read<v4f>(n.along(2 * (s % 4) + 1), up);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
   // Element 32 db + l % 32 of the rows 16 st + 8 (i / 4) + 4 (l / 32) + i % 4:
   // the A operand with the tile's columns as rows, whose K indices are those
   // of accumulators 8 (st % 2) .. of row block st / 2.
-  __device__ static __forceinline__ Frag<T> across(uint32_t lds, const Lane &n,
+  template <typename L>
+  __device__ static __forceinline__ Frag<T> across(uint32_t lds, const L &n,
                                                    int st, int db) {
     const uint32_t at = lds + 16 * st * kPitch;
     if constexpr (sizeof(T) == 2) {
-      const v2u x = lds_read_across(n.across[db], at);
-      const v2u y = lds_read_across(n.across[D / 32 + db], at);
+      const v2u x = lds_read_across(n.across(db), at);
+      const v2u y = lds_read_across(n.across(D / 32 + db), at);
       return v4u{x.x, x.y, y.x, y.y};
     } else {
       v8f r;
 #pragma unroll
       for (int i = 0; i < 8; ++i) // (row bit 3 swaps chunks 8 apart)
-        r[i] = lds_read<float>(n.across[i & 3],
+        r[i] = lds_read<float>(n.across(i & 3),
                                at + 8 * (i >> 2) * kPitch +
                                    128 * ((db ^ (i >> 2)) & 1) +
                                    256 * (db >> 1));
@@ -327,6 +347,10 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
   }
 };
 
+// Waits until this wave's copies and its reads of earlier tiles are done.
+__device__ __forceinline__ void landed_wave() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
 // Waits until this wave's copies and its reads of earlier tiles are done, and
 // then for the workgroup's other waves.
 __device__ __forceinline__ void landed() {

@@ -565,48 +565,56 @@ window_query_gradient(BackwardArgs b) {
 }
 
 // dk and dv.  A workgroup holds 128 keys of one key head, 32 a wave, and goes
-// through the queries that see them, head by head: S = Q K^T and dP = dO V^T
-// with queries in rows and keys in columns, dv^T += dO^T p, dk^T += Q^T ds.
+// through the queries that see them, head by head and 32 at a time: S = Q K^T
+// and dP = dO V^T with queries in rows and keys in columns, dv^T += dO^T p,
+// dk^T += Q^T ds.  K stays in registers and V in LDS: both in registers, and
+// the sums, are more than two waves a SIMD have.
+//
 // The queries past the window that see the sinks are as many as the sequence
-// has, so they are split: a workgroup of those takes 32 sinks and a chunk of
-// queries, its waves blocks of 32 queries in turn, and leaves its sums to
-// window_sink_gradient.
-template <typename T, int D> struct Backward {
-  static constexpr int kTile = sizeof(T) == 2 ? 64 : 32; // queries
-  using Tile = RowTile<T, D, kTile, kThreads>;
+// has, so they are split (SINK): a workgroup of those takes 32 sinks and a
+// chunk of queries, its waves blocks of 32 queries in turn, each with tiles of
+// its own, and leaves its sums to window_sink_gradient.
+template <typename T, int D, bool SINK> struct Backward {
+  static constexpr int kTile = 32; // queries
+  using Tile = RowTile<T, D, kTile, SINK ? kWave : kThreads>;
+  using Values = RowTile<T, D, kRows, kThreads>;
+  static constexpr int kBuffers = SINK ? 4 : 1;
+  // (fp32 rows of 128 leave a wave's own tiles no second place)
+  static constexpr int kParities = SINK && sizeof(T) * D > 256 ? 1 : 2;
+  static constexpr int kValues = SINK ? 0 : Values::kBytes;
   static constexpr int kSteps = D / 16;
   static constexpr int kBlocks = D / 32;
-  static constexpr int kWaves = D > 64 ? 1 : 2;
+  static constexpr int kWaves = SINK || sizeof(T) * D > 256 ? 1 : 2;
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (Backward<T, D>::kWaves)) void
+template <typename T, int D, bool SINK>
+__global__ __launch_bounds__(kThreads, (Backward<T, D, SINK>::kWaves)) void
 window_key_gradient(BackwardArgs b) {
   const WindowArgs &a = b.w;
-  using F = Backward<T, D>;
+  using F = Backward<T, D, SINK>;
   using Tile = typename F::Tile;
+  using Values = typename F::Values;
   constexpr int QT = F::kTile;
-  __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
-  __shared__ __align__(16) float stats[2][2][64];
+  // [buffer of a wave, or of all][parity][q, do], then the values
+  __shared__ __align__(1024) char
+      lds[F::kBuffers * F::kParities * 2 * Tile::kBytes + F::kValues];
+  __shared__ __align__(16) float stats[F::kBuffers][2][2][64];
   __shared__ int verdict;
 
   const int lane = lane_id(), h = lane >> 5, wave = wave_in_group();
   const int group = a.query_heads / a.key_heads;
-  const int sink_blocks = b.sink_rows / 32;
-  const int64_t sink_items = (int64_t)b.chunks * a.key_heads * sink_blocks;
-  const bool sink = blockIdx.x < sink_items;
   int hk, i, key0, first, last; // keys from key0; queries first .. last
   Sequence s;
   int64_t item;
-  if (sink) {
-    item = blockIdx.x;
-    const int block = (int)(item % sink_blocks);
-    hk = (int)(item / sink_blocks % a.key_heads);
-    const int chunk = (int)(item / sink_blocks / a.key_heads);
-    item = chunk;
-    i = sequence_of_tile(a.query_offsets, a.sequences, chunk, b.chunk_shift);
+  if constexpr (SINK) {
+    const int sink_blocks = b.sink_rows / 32;
+    const int block = (int)(blockIdx.x % sink_blocks);
+    item = blockIdx.x / sink_blocks;
+    hk = (int)(item % a.key_heads);
+    item /= a.key_heads; // the chunk
+    i = sequence_of_tile(a.query_offsets, a.sequences, (int)item, b.chunk_shift);
     s = sequence(a, i);
-    const int row0 = (chunk - (a.query_offsets[i] >> b.chunk_shift) - i)
+    const int row0 = ((int)item - (a.query_offsets[i] >> b.chunk_shift) - i)
                      << b.chunk_shift;
     key0 = 32 * block;
     first = row0;
@@ -617,7 +625,7 @@ window_key_gradient(BackwardArgs b) {
     const int far = key0 + a.window - (s.nk - s.nq);
     first = far > first ? far : first;
   } else {
-    item = xcd_contiguous(blockIdx.x - sink_items, gridDim.x - sink_items);
+    item = xcd_contiguous(blockIdx.x, gridDim.x);
     const int tile = (int)(item % b.key_tiles);
     hk = (int)(item / b.key_tiles);
     i = sequence_of_tile(a.key_offsets, a.sequences, tile, kRowShift);
@@ -629,21 +637,28 @@ window_key_gradient(BackwardArgs b) {
     const int end = (s.nk < key0 + kRows ? s.nk : key0 + kRows) - 1;
     first = key0 - shift > 0 ? key0 - shift : 0;
     last = s.nk - 1 - end < a.window ? s.nq - 1 : end + a.window - 1 - shift;
-    key0 += 32 * wave;
   }
+  const int tile_key = key0;
+  if constexpr (!SINK)
+    key0 += 32 * wave;
   const int shift = s.nk - s.nq;
   const int key = key0 + (lane & 31);
-  const bool live = key < s.nk && (!sink || key < a.sinks);
+  const bool live = key < s.nk && (!SINK || key < a.sinks);
 
   const bool tiny = fabsf(a.alpha) < 0x1p-126f;
   const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
-  Frag<T> k[F::kSteps], v[F::kSteps];
+  const uint32_t vbase = lds_address(lds) + F::kBuffers * F::kParities * 2 * Tile::kBytes;
+  Frag<T> k[F::kSteps], v[SINK ? F::kSteps : 1];
   {
     const int64_t token = s.k0 + (live ? key : 0);
     load_rows<T>(k, static_cast<const T *>(a.key) + token * a.k.token +
                         hk * a.k.head, live && !tiny, a.d, a.alpha < 0.0f);
-    load_rows<T>(v, static_cast<const T *>(a.value) + token * a.v.token +
-                        hk * a.v.head, live, a.d, false);
+    const T *values = static_cast<const T *>(a.value) + hk * a.v.head;
+    if constexpr (SINK)
+      load_rows<T>(v, values + token * a.v.token, live, a.d, false);
+    else
+      Values::copy(vbase, values + (int64_t)(s.k0 + tile_key) * a.v.token,
+                   s.nk - tile_key, (uint32_t)(a.v.token * sizeof(T)), a.d);
   }
 
   const T *qbase = static_cast<const T *>(a.query) + (int64_t)s.q0 * a.q.token;
@@ -653,128 +668,152 @@ window_key_gradient(BackwardArgs b) {
   const uint32_t obytes = (uint32_t)(b.go.token * sizeof(T));
   const int tiles = last < first ? 0 : (last - first) / QT + 1;
   const int count = tiles * group;
-  const typename Tile::Lane at;
-  const uint32_t base = lds_address(lds), sbase = lds_address(stats);
-  auto copy = [&](int t) __attribute__((always_inline)) {
+  typename Tile::FewLane at;
+  const uint32_t base =
+      lds_address(lds) + (SINK ? wave * F::kParities * 2 * Tile::kBytes : 0);
+  const uint32_t sbase = lds_address(stats) + (SINK ? wave * 1024 : 0);
+  auto copy = [&](int t, int parity) __attribute__((always_inline)) {
     const int head = hk * group + t / tiles;
     const int64_t r = first + t % tiles * QT;
     const int n = last + 1 - (int)r;
-    const uint32_t to = base + (t & 1) * 2 * Tile::kBytes;
+    const uint32_t to = base + parity * 2 * Tile::kBytes;
     Tile::copy(to, qbase + r * a.q.token + head * a.q.head, n, qbytes, a.d);
     Tile::copy(to + Tile::kBytes, obase + r * b.go.token + head * b.go.head, n,
                obytes, a.d);
-    if (wave < 2) { // a row's two numbers, 64 of each
-      const float *x = (wave == 0 ? b.log2_sum : b.delta) +
-                       (int64_t)head * a.query_tokens + s.q0 + r;
-      const int m = n < QT ? n : QT;
-      copy_words_to_lds(buffer_words(x, 4 * m), 4 * lane,
-                        sbase + ((t & 1) * 2 + wave) * 256);
-    }
+    // a row's two numbers, 64 of each
+    const int64_t row = (int64_t)head * a.query_tokens + s.q0 + r;
+    const int m = n < QT ? n : QT;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (SINK || wave == e)
+        copy_words_to_lds(
+            buffer_words((e == 0 ? b.log2_sum : b.delta) + row, 4 * m),
+            4 * lane, sbase + (parity * 2 + e) * 256);
   };
 
   v16f dk[F::kBlocks], dv[F::kBlocks];
-  auto products = [&](int t, auto parity, auto careful)
+  auto products = [&](int t, int parity, auto careful)
                       __attribute__((always_inline)) {
-    constexpr int P = decltype(parity)::value;
-    const uint32_t qt = base + P * 2 * Tile::kBytes, ot = qt + Tile::kBytes;
-    const int r0 = first + t % tiles * QT;
+    const uint32_t qt = base + parity * 2 * Tile::kBytes;
+    const uint32_t ot = qt + Tile::kBytes;
+    const uint32_t st0 = sbase + parity * 512;
+    const int lo = first + t % tiles * QT; // the block's first query
+    if (!SINK &&
+        (lo + 31 + shift < key0 || lo + shift - (key0 + 31) >= a.window))
+      return; // hidden
+    const bool all =
+        lo + 31 <= last &&
+        (SINK ? lo + shift - (key0 + 31) >= a.window && key0 + 32 <= a.sinks
+              : lo + shift >= key0 + 31 && lo + 31 + shift - key0 < a.window);
+    at.fresh();
+    v16f p = {}, ds = {};
 #pragma unroll
-    for (int rb = 0; rb < QT / 32; ++rb) {
-      const int lo = r0 + 32 * rb; // this block's first query
-      if (sink ? ((t * (QT / 32) + rb) & 3) != wave
-               : lo + 31 + shift < key0 || lo + shift - (key0 + 31) >= a.window)
-        continue; // another wave's, or hidden
-      if (lo > last)
-        continue;
-      const bool all =
-          lo + 31 <= last &&
-          (sink ? lo + shift - (key0 + 31) >= a.window && key0 + 32 <= a.sinks
-                : lo + shift >= key0 + 31 &&
-                      lo + 31 + shift - key0 < a.window);
-      v16f p = {}, ds = {};
+    for (int st = 0; st < F::kSteps; ++st)
+      p = mma32(Tile::along(qt, at, 0, st), k[st], p);
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st)
-        p = mma32(Tile::along(qt, at, rb, st), k[st], p);
+    for (int st = 0; st < F::kSteps; ++st) {
+      // (a tile of 128 rows has the lane's addresses of one of 32)
+      if constexpr (SINK)
+        ds = mma32(Tile::along(ot, at, 0, st), v[st], ds);
+      else
+        ds = mma32(Tile::along(ot, at, 0, st),
+                   Tile::along(vbase + wave * 32 * Tile::kPitch, at, 0, st),
+                   ds);
+    }
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st)
-        ds = mma32(Tile::along(ot, at, rb, st), v[st], ds);
+    for (int r = 0; r < 16; r += 4) {
+      // (rows acc_row(r) .. + 3 of the block)
+      const v4f l4 = lds_read<v4f>(16 * h, st0 + 8 * r);
+      const v4f d4 = lds_read<v4f>(16 * h, st0 + 256 + 8 * r);
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        // (rows acc_row(r) .. + 3 of the block)
-        const v4f l4 = lds_read<v4f>(16 * h, sbase + P * 512 + 128 * rb + 8 * r);
-        const v4f d4 =
-            lds_read<v4f>(16 * h, sbase + P * 512 + 256 + 128 * rb + 8 * r);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[r + e] = __builtin_amdgcn_exp2f(fmaf(p[r + e], scale, -l4[e]));
-          ds[r + e] = p[r + e] * (ds[r + e] - d4[e]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        p[r + e] = __builtin_amdgcn_exp2f(fmaf(p[r + e], scale, -l4[e]));
+        ds[r + e] = p[r + e] * (ds[r + e] - d4[e]);
       }
-      uint32_t seen = 0;
-      if (!all) {
-        const int back = lo + shift + 4 * h - key; // of accumulator row 0
-        const int rows = last - lo - 4 * h;
+    }
+    uint32_t seen = 0;
+    if (!all) {
+      const int back = lo + shift + 4 * h - key; // of accumulator row 0
+      const int rows = last - lo - 4 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = 8 * (r >> 2) + (r & 3);
-          const bool see =
-              ((sink ? (back + j >= a.window) & live
-                     : (uint32_t)(back + j) < (uint32_t)a.window)) &
-              (j <= rows);
-          p[r] = see ? p[r] : 0.0f;
-          ds[r] = see ? ds[r] : 0.0f;
-          if constexpr (decltype(careful)::value)
-            seen |= (uint32_t)see << r;
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int j = 8 * (r >> 2) + (r & 3);
+        const bool see =
+            ((SINK ? (back + j >= a.window) & live
+                   : (uint32_t)(back + j) < (uint32_t)a.window)) &
+            (j <= rows);
+        p[r] = see ? p[r] : 0.0f;
+        ds[r] = see ? ds[r] : 0.0f;
+        if constexpr (decltype(careful)::value)
+          seen |= (uint32_t)see << r;
       }
+    }
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float x[8], y[8];
+    for (int half = 0; half < 2; ++half) {
+      float x[8], y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = p[8 * half + e];
-          y[e] = ds[8 * half + e];
-        }
-        // bf16: rounded once more each, as the matrix core takes them
-        const Frag<T> pf = make_frag<T>(x), df = make_frag<T>(y);
+      for (int e = 0; e < 8; ++e) {
+        x[e] = p[8 * half + e];
+        y[e] = ds[8 * half + e];
+      }
+      // bf16: both round once more, as the matrix core takes them
+      const Frag<T> pf = make_frag<T>(x), df = make_frag<T>(y);
 #pragma unroll
-        for (int c = 0; c < F::kBlocks; ++c) {
-          const Frag<T> of = Tile::across(ot, at, 2 * rb + half, c);
-          const Frag<T> qf = Tile::across(qt, at, 2 * rb + half, c);
-          if (decltype(careful)::value && !all) {
-            dv[c] = mma32_seen<T>(of, pf, dv[c], seen >> (8 * half));
-            dk[c] = mma32_seen<T>(qf, df, dk[c], seen >> (8 * half));
-          } else {
-            dv[c] = mma32(of, pf, dv[c]);
-            dk[c] = mma32(qf, df, dk[c]);
-          }
+      for (int c = 0; c < F::kBlocks; ++c) {
+        const Frag<T> of = Tile::across(ot, at, half, c);
+        const Frag<T> qf = Tile::across(qt, at, half, c);
+        if (decltype(careful)::value && !all) {
+          dv[c] = mma32_seen<T>(of, pf, dv[c], seen >> (8 * half));
+          dk[c] = mma32_seen<T>(qf, df, dk[c], seen >> (8 * half));
+        } else {
+          dv[c] = mma32(of, pf, dv[c]);
+          dk[c] = mma32(qf, df, dk[c]);
         }
       }
     }
+    __builtin_amdgcn_s_setprio(0);
   };
   auto pass = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
       dk[c] = dv[c] = v16f{};
-    if (count > 0)
-      copy(0);
-    auto step = [&](int t, auto parity) __attribute__((always_inline)) {
-      landed();
-      if (t + 1 < count)
-        copy(t + 1);
-      products(t, parity, careful);
-    };
-    for (int t = 0; t < count; t += 2) {
-      step(t, std::integral_constant<int, 0>{});
-      if (t + 1 < count)
-        step(t + 1, std::integral_constant<int, 1>{});
+    if constexpr (SINK) {
+      if (wave < count && F::kParities == 2)
+        copy(wave, 0);
+      for (int t = wave, parity = 0; t < count; t += 4) {
+        if (F::kParities == 1) {
+          landed_wave(); // (its reads of the tile before)
+          copy(t, 0);
+        }
+        landed_wave();
+        if (F::kParities == 2 && t + 4 < count)
+          copy(t + 4, parity ^ 1);
+        products(t, parity, careful);
+        parity ^= F::kParities - 1;
+      }
+    } else {
+      if (count > 0)
+        copy(0, 0);
+      auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+        constexpr int P = decltype(parity)::value;
+        landed();
+        if (t + 1 < count)
+          copy(t + 1, 1 - P);
+        products(t, P, careful);
+      };
+      for (int t = 0; t < count; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < count)
+          step(t + 1, std::integral_constant<int, 1>{});
+      }
     }
   };
   pass(std::false_type{});
   if (any_wave(!(all_finite<T>(dk) && all_finite<T>(dv)), &verdict))
     pass(std::true_type{});
 
-  if (sink) {
+  if constexpr (SINK) {
     // the waves' sums, one after the other, in the tiles' memory
     static_assert(sizeof(lds) >= 2 * F::kBlocks * 16 * 64 * 4, "");
     float *sums = reinterpret_cast<float *>(lds);
@@ -801,9 +840,9 @@ window_key_gradient(BackwardArgs b) {
   if (!live)
     return;
   // a sink's sums wait for those of the queries past the window
-  if (sink || key < b.sink_rows) {
-    const int64_t of = (sink ? item : i) * a.key_heads + hk;
-    float *out = (sink ? b.sink_chunks : b.sink_window) +
+  if (SINK || key < b.sink_rows) {
+    const int64_t of = (SINK ? item : i) * a.key_heads + hk;
+    float *out = (SINK ? b.sink_chunks : b.sink_window) +
                  (of * b.sink_rows + key) * 2 * a.d;
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
@@ -814,7 +853,7 @@ window_key_gradient(BackwardArgs b) {
           st4(x, dk[c][r], dk[c][r + 1], dk[c][r + 2], dk[c][r + 3]);
           st4(x + a.d, dv[c][r], dv[c][r + 1], dv[c][r + 2], dv[c][r + 3]);
         }
-    if (sink || key < a.sinks)
+    if (SINK || key < a.sinks)
       return;
   }
   const int64_t token = s.k0 + key;
@@ -835,32 +874,53 @@ window_key_gradient(BackwardArgs b) {
       }
 }
 
-// The sinks' gradients: the window's sums and every chunk's, in order.  One
-// workgroup of d threads for a sink of one sequence and key head.
+// The sinks' gradients: the window's sums and every chunk's, in the same order
+// each time: eight runs of chunks, then the runs.  One workgroup of 128 x 8
+// threads for a sink of one sequence and key head.
+constexpr int kSinkRuns = 8;
 template <typename T>
-__global__ void window_sink_gradient(BackwardArgs b) {
+__global__ __launch_bounds__(128 * kSinkRuns) void
+window_sink_gradient(BackwardArgs b) {
   const WindowArgs &a = b.w;
+  __shared__ float sums[2][kSinkRuns][128];
   const int key = blockIdx.x % a.sinks;
   const int hk = blockIdx.x / a.sinks % a.key_heads;
   const int i = blockIdx.x / a.sinks / a.key_heads;
   const Sequence s = sequence(a, i);
-  const int c = threadIdx.x;
-  if (key >= s.nk || c >= a.d)
+  if (key >= s.nk)
     return;
+  const int run = threadIdx.x >> 7, c = threadIdx.x & 127;
   const int64_t row = (int64_t)b.sink_rows * 2 * a.d;
   const int64_t own = (int64_t)key * 2 * a.d + c;
+  float dk = 0.0f, dv = 0.0f;
+  if (c < a.d) {
+    const int begin = (a.query_offsets[i] >> b.chunk_shift) + i;
+    const int chunks = s.nq == 0 ? 0 : ((s.nq - 1) >> b.chunk_shift) + 1;
+    // chunks that reach past the window: those from the first whose last
+    // query's place is at least a.window
+    const int far = a.window - (s.nk - s.nq); // query of that place
+    int x = far <= 0 ? 0 : far >> b.chunk_shift;
+    for (x += run; x < chunks && begin + x < b.chunks; x += kSinkRuns) {
+      if (far > s.nq - 1)
+        break;
+      const float *y = b.sink_chunks +
+                       ((int64_t)(begin + x) * a.key_heads + hk) * row + own;
+      dk += y[0];
+      dv += y[a.d];
+    }
+  }
+  sums[0][run][c] = dk;
+  sums[1][run][c] = dv;
+  __syncthreads();
+  if (run != 0 || c >= a.d)
+    return;
   const float *x = b.sink_window + ((int64_t)i * a.key_heads + hk) * row + own;
-  float dk = x[0], dv = x[a.d];
-  const int begin = (a.query_offsets[i] >> b.chunk_shift) + i;
-  for (int r = 0; r < s.nq; r += 1 << b.chunk_shift) {
-    int last = r + (1 << b.chunk_shift) - 1;
-    last = last < s.nq - 1 ? last : s.nq - 1;
-    const int chunk = begin + (r >> b.chunk_shift);
-    if (last + s.nk - s.nq < a.window || chunk >= b.chunks)
-      continue;
-    const float *y = b.sink_chunks + ((int64_t)chunk * a.key_heads + hk) * row + own;
-    dk += y[0];
-    dv += y[a.d];
+  dk = x[0];
+  dv = x[a.d];
+#pragma unroll
+  for (int r = 0; r < kSinkRuns; ++r) {
+    dk += sums[0][r][c];
+    dv += sums[1][r][c];
   }
   const int64_t token = s.k0 + key;
   stv(static_cast<T *>(b.key_gradient) + token * b.gk.token + hk * b.gk.head + c,
@@ -992,10 +1052,10 @@ Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
   if (s == 0)
     return c;
   c.sink_rows = (int)sw::ceil_div(s, 32) * 32;
-  // 1024 queries a chunk, more where there are more than 64 sinks: the sums
-  // then stay below the keys' own size
-  c.chunk_shift = 10;
-  while (((int64_t)64 << (c.chunk_shift - 10)) < s)
+  // 256 queries a chunk, more where there are more than 64 sinks: the sums
+  // then stay below the size of bf16 keys
+  c.chunk_shift = 8;
+  while (((int64_t)64 << (c.chunk_shift - 8)) < s)
     ++c.chunk_shift;
   c.chunks = (query_tokens >> c.chunk_shift) + sequences;
   const int64_t one = key_heads * c.sink_rows * 2 * d;
@@ -1062,11 +1122,14 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   b.chunk_shift = c.chunk_shift;
   b.sink_rows = c.sink_rows;
   b.key_tiles = (int)((key_tokens >> kRowShift) + sequences);
-  const int64_t grid = (int64_t)b.key_tiles * key_heads +
-                       c.chunks * key_heads * (c.sink_rows / 32);
+  const int64_t grid = (int64_t)b.key_tiles * key_heads;
+  const int64_t sink_grid = c.chunks * key_heads * (c.sink_rows / 32);
   const int64_t rows = sequences * key_heads * a.sinks;
-  if (int rc = sw::check_flat_grid(std::max(grid, rows), kThreads,
+  if (int rc = sw::check_flat_grid(std::max(grid, sink_grid), kThreads,
                                    "window attention's gradient"))
+    return rc;
+  if (int rc = sw::check_flat_grid(rows, 128 * kSinkRuns,
+                                   "window attention's sink gradient"))
     return rc;
   const hipStream_t st = sw::as_stream(stream);
   const dim3 rows_grid((unsigned)((int64_t)a.tiles * query_heads));
@@ -1080,14 +1143,27 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   }
   if (key_tokens == 0)
     return SW_OK;
+  if (sink_grid > 0) {
+    if (d <= 64)
+      window_key_gradient<T, 64, true>
+          <<<dim3((unsigned)sink_grid), kThreads, 0, st>>>(b);
+    else
+      window_key_gradient<T, 128, true>
+          <<<dim3((unsigned)sink_grid), kThreads, 0, st>>>(b);
+    if (int rc = sw::launch_check("window attention's key gradient"))
+      return rc;
+  }
   if (d <= 64)
-    window_key_gradient<T, 64><<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
+    window_key_gradient<T, 64, false>
+        <<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
   else
-    window_key_gradient<T, 128><<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
+    window_key_gradient<T, 128, false>
+        <<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
   if (int rc = sw::launch_check("window attention's key gradient"))
     return rc;
   if (a.sinks > 0) {
-    window_sink_gradient<T><<<dim3((unsigned)rows), 128, 0, st>>>(b);
+    window_sink_gradient<T>
+        <<<dim3((unsigned)rows), 128 * kSinkRuns, 0, st>>>(b);
     return sw::launch_check("window attention's sink gradient");
   }
   return SW_OK;

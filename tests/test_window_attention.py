@@ -101,12 +101,12 @@ def test_backward_workspace_rule():
     assert need(3, 100, 100, 4, 2, 64, 99, 7) == 2 * 4 * 100 * 4 + \
         4 * rows * (3 + 3)
     assert need(3, 5000, 100, 4, 2, 64, 99, 7) == 2 * 4 * 5000 * 4 + \
-        4 * rows * (3 + 4 + 3)
-    # at least the keys' own size apart from one chunk a sequence, however
+        4 * rows * (3 + 19 + 3)
+    # at most the size of bf16 keys apart from one chunk a sequence, however
     # many sinks
     for sinks in (64, 100, 1000, 5000):
         assert need(1, 1 << 20, 1 << 20, 1, 1, 128, 64, sinks) <= \
-            2 * 4 * (1 << 20) + 2 * 4 * (1 << 20) * 128 + 3 * 4 * 256 * (
+            2 * 4 * (1 << 20) + 2 * 2 * (1 << 20) * 128 + 3 * 4 * 256 * (
                 sinks + 31)
     assert need(1, 100, 100, 4, 3, 64, 100, 7) == 0
 
