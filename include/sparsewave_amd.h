@@ -514,14 +514,14 @@ int sw_window_attention_bf16(
  * matrix cores and each gradient once.  No atomics.
  *
  * The workspace (16-byte aligned, of at least
- * sw_window_attention_backward_workspace_bytes, 0 for sizes that the call
- * refuses) belongs to the call until its work on `stream` is done; two calls
+ * sw_window_attention_backward_workspace_bytes for elements of value_bytes, 0
+ * for sizes that the call refuses) belongs to the call until its work on `stream` is done; two calls
  * or two captured graphs that may run at once need one each.
  */
 int64_t sw_window_attention_backward_workspace_bytes(
     int64_t sequences, int64_t query_tokens, int64_t key_tokens,
     int64_t query_heads, int64_t key_heads, int64_t d, int64_t window,
-    int64_t sinks);
+    int64_t sinks, int value_bytes);
 int sw_window_attention_backward_f32(
     const int32_t *query_offsets, const int32_t *key_offsets,
     const float *query, const float *key, const float *value,

@@ -189,7 +189,8 @@ def load_library():
             ctypes.c_int, [P] * 6 + [I64] * 7 + [P, I64, I64, F, P, I64, P])
         sig["sw_shared_prefix_attention" + dt] = (
             ctypes.c_int, [P] * 8 + [I64] * 8 + [P, F, P, I64, P])
-    sig["sw_window_attention_backward_workspace_bytes"] = (I64, [I64] * 8)
+    sig["sw_window_attention_backward_workspace_bytes"] = (
+        I64, [I64] * 8 + [ctypes.c_int])
     sig["sw_window_attention_decode_workspace_bytes"] = (I64, [I64] * 8)
     sig["sw_shared_prefix_attention_workspace_bytes"] = (I64, [I64] * 7)
     for name, (res, args) in sig.items():
@@ -793,7 +794,7 @@ def window_attention_backward(query_offsets, key_offsets, query, key, value,
                _dev(key_offsets, torch.int32, "key_offsets"))
     lse = _dev(log_sum, torch.float32, "log_sum")
     need = load_library().sw_window_attention_backward_workspace_bytes(
-        *shape, window, sinks)
+        *shape, window, sinks, query.element_size())
     scratch = _scratch(need, query, workspace, stream)
     p = [o[0] for o in ops]
     _check(_fn("sw_window_attention_backward", dt)(

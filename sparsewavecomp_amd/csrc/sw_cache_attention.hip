@@ -424,9 +424,9 @@ shared_prefix_parts(StepArgs a) {
   auto copy = [&](int t) __attribute__((always_inline)) {
     const int64_t j = v0 + t * KT;
     const uint32_t to = base + (t & 1) * 2 * Tile::kBytes;
-    Tile::copy(to, keys + j * a.prefix.key_token, v1 - (int)j, kbytes, a.d);
+    Tile::copy(to, keys + j * a.prefix.key_token, v1 - (int)j, kbytes, a.d, wave);
     Tile::copy(to + Tile::kBytes, values + j * a.prefix.value_token,
-               v1 - (int)j, vbytes, a.d);
+               v1 - (int)j, vbytes, a.d, wave);
   };
 
   v16f acc[F::kBlocks];

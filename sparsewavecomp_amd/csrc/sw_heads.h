@@ -232,11 +232,12 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
   // LDS, and each lane picks the chunk that belongs at its place.  Elements
   // past d and rows past the end are written as zeros (the descriptor bounds
   // what is read: (ROWS - 1) row_bytes + 4 D < 2^31 is the host's check).
-  // landed() waits for it.
+  // landed() waits for it.  `w`: this wave's number among the THREADS / 64 that
+  // fill the tile.
   __device__ static __forceinline__ void copy(uint32_t lds, const T *base,
                                               int rows, uint32_t row_bytes,
-                                              int d) {
-    const int l = lane_id(), w = THREADS == kWave ? 0 : wave_in_group();
+                                              int d, int w) {
+    const int l = lane_id();
     constexpr int kStep = (THREADS / kWave) * (1024 / kPitch); // rows a pass
     rows = rows < 0 ? 0 : rows > ROWS ? ROWS : rows;
     const uint32_t bytes =
@@ -272,6 +273,11 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
         y = place(4 * h, (l & 31) >> 2) + (l & 3) * 4;
       }
     }
+    // (a multiple of 512: the operations below change bits under it)
+    __device__ __forceinline__ void offset(uint32_t by) {
+      x += by;
+      y += by;
+    }
     // (keeps the compiler from computing every address ahead of a loop)
     __device__ __forceinline__ void fresh() {
       asm volatile("" : "+v"(x), "+v"(y));
@@ -304,6 +310,14 @@ template <typename T, int D, int ROWS, int THREADS> struct RowTile {
 #pragma unroll
       for (int i = 0; i < (int)(sizeof y / 4); ++i)
         y[i] = f.across(i);
+    }
+    __device__ __forceinline__ void offset(uint32_t by) {
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof x / 4); ++i)
+        x[i] += by;
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof y / 4); ++i)
+        y[i] += by;
     }
     __device__ __forceinline__ uint32_t along(int i) const { return x[i]; }
     __device__ __forceinline__ uint32_t across(int i) const { return y[i]; }

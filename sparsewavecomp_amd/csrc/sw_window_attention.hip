@@ -29,9 +29,13 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kInf = __builtin_inff();
 
-constexpr int kThreads = 256; // four waves of 32 rows
+constexpr int kThreads = 256; // four waves, of 32 rows each
 constexpr int kRowShift = 7;
 constexpr int kRows = 1 << kRowShift;
+
+// The rows of a workgroup whose four waves take their keys in one share, 128,
+// or in two, 64 where there are few rows.
+constexpr int shared_shift(int streams) { return kRowShift + 1 - streams; }
 
 struct WindowArgs {
   const int32_t *query_offsets, *key_offsets;
@@ -62,14 +66,14 @@ __device__ __forceinline__ Sequence sequence(const A &a, int i) {
   return s;
 }
 
-// A workgroup's rows: 128 queries of one head, 32 a wave.  Neighbouring
+// A workgroup's rows: 1 << SHIFT queries of one head, 32 a wave.  Neighbouring
 // workgroups of an XCD take the heads that share a key head, then the next
 // rows, whose windows overlap (65,536 queries, window 4096: 2222 us; in plain
 // order 2351 us).
-struct Rows {
+template <int SHIFT> struct Rows {
   Sequence s;
   int head, key_head, row0, row_lo, count, shift;
-  __device__ __forceinline__ explicit Rows(const WindowArgs &a) {
+  __device__ __forceinline__ Rows(const WindowArgs &a, int block) {
     const int group = a.query_heads / a.key_heads;
     int64_t item = xcd_contiguous(blockIdx.x, gridDim.x);
     const int g = (int)(item % group);
@@ -78,12 +82,13 @@ struct Rows {
     key_head = (int)(item / a.tiles);
     head = key_head * group + g;
     const int i =
-        sequence_of_tile(a.query_offsets, a.sequences, tile, kRowShift);
+        sequence_of_tile(a.query_offsets, a.sequences, tile, SHIFT);
     s = sequence(a, i);
-    row0 = (tile - (a.query_offsets[i] >> kRowShift) - i) << kRowShift;
+    row0 = (tile - (a.query_offsets[i] >> SHIFT) - i) << SHIFT;
     // (none in the numbers between one sequence's tiles and the next's)
-    count = row0 < 0 ? 0 : s.nq - row0 < kRows ? s.nq - row0 : kRows;
-    row_lo = row0 + 32 * wave_in_group();
+    const int left = s.nq - row0;
+    count = row0 < 0 ? 0 : left < 1 << SHIFT ? left : 1 << SHIFT;
+    row_lo = row0 + 32 * block;
     shift = s.nk - s.nq; // a query's place less its index
   }
 };
@@ -188,26 +193,83 @@ __device__ __forceinline__ bool any_wave(bool says, int *verdict) {
 
 // ---- forward -------------------------------------------------------------------
 
-template <typename T, int D> struct Forward {
-  static constexpr int kTile = sizeof(T) == 2 ? 64 : 32; // keys
-  using Tile = RowTile<T, D, kTile, kThreads>;
+// The row kernels: STREAMS shares of the keys, each with tiles of its own that
+// 4 / STREAMS waves of 32 rows go through.
+template <typename T, int D, int STREAMS> struct Forward {
+  static constexpr int kTile = sizeof(T) == 2 && STREAMS == 1 ? 64 : 32; // keys
+  static constexpr int kBlocksOfRows = 4 / STREAMS;
+  using Tile = RowTile<T, D, kTile, kThreads / STREAMS>;
+  using Rows = ::Rows<shared_shift(STREAMS)>;
   static constexpr int kSteps = D / 16;   // products along d
   static constexpr int kBlocks = D / 32;  // output rows of 32
   static constexpr int kKeyBlocks = kTile / 32;
+  static constexpr int kBytes = STREAMS * 4 * Tile::kBytes;
   // waves a SIMD: fp32 rows of 128 take more than half of the registers
   static constexpr int kWaves = sizeof(T) * D > 256 ? 1 : 2;
+  static_assert(kBytes <= 128 * 1024, "");
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (Forward<T, D>::kWaves)) void
+// Adds up what the shares of the keys left in acc, in the first share's waves,
+// share by share, under their common maximum; true in those.  Every thread must
+// call it, when the tiles' memory is free.
+template <typename T, int D, int STREAMS, int BLOCKS>
+__device__ __forceinline__ bool add_shares(v16f (&acc)[BLOCKS], float &top,
+                                           float &sum, char *lds) {
+  if constexpr (STREAMS == 1) {
+    return true;
+  } else {
+    constexpr int kWords = (BLOCKS * 16 + 2) * kWave;
+    constexpr int kRowBlocks = 4 / STREAMS;
+    static_assert((4 - kRowBlocks) * kWords * 4 <=
+                  Forward<T, D, STREAMS>::kBytes, "");
+    const int wave = wave_in_group();
+    float *words = reinterpret_cast<float *>(lds) + lane_id();
+    __syncthreads();
+    if (wave >= kRowBlocks) {
+      float *x = words + (wave - kRowBlocks) * kWords;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          x[(b * 16 + r) * kWave] = acc[b][r];
+      x[BLOCKS * 16 * kWave] = top;
+      x[(BLOCKS * 16 + 1) * kWave] = sum;
+    }
+    __syncthreads();
+    if (wave >= kRowBlocks)
+      return false;
+#pragma unroll 1
+    for (int i = 0; i < STREAMS - 1; ++i) {
+      const float *x = words + (wave + i * kRowBlocks) * kWords;
+      const float other = x[BLOCKS * 16 * kWave];
+      const float to = fmaxf(top, other);
+      const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+      const float add = other == to ? 1.0f : __builtin_amdgcn_exp2f(other - to);
+      top = to;
+      sum = fmaf(x[(BLOCKS * 16 + 1) * kWave], add, sum * by);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[b][r] = fmaf(x[(b * 16 + r) * kWave], add, acc[b][r] * by);
+    }
+    return true;
+  }
+}
+
+template <typename T, int D, int STREAMS>
+__global__ __launch_bounds__(kThreads, (Forward<T, D, STREAMS>::kWaves)) void
 window_forward(WindowArgs a) {
-  using F = Forward<T, D>;
+  using F = Forward<T, D, STREAMS>;
   using Tile = typename F::Tile;
   constexpr int KT = F::kTile;
-  __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
+  __shared__ __align__(1024) char lds[F::kBytes];
   __shared__ int verdict;
 
-  const Rows w(a);
+  const int wave = wave_in_group();
+  const int share = STREAMS == 1 ? 0 : wave / F::kBlocksOfRows;
+  const int block = wave - share * F::kBlocksOfRows;
+  const typename F::Rows w(a, block);
   if (w.count <= 0)
     return;
   const Sequence &s = w.s;
@@ -234,14 +296,20 @@ window_forward(WindowArgs a) {
                    hk * a.v.head;
   const uint32_t kbytes = (uint32_t)(a.k.token * sizeof(T));
   const uint32_t vbytes = (uint32_t)(a.v.token * sizeof(T));
-  const typename Tile::Lane at;
-  const uint32_t base = lds_address(lds);
-  auto copy = [&](int t) __attribute__((always_inline)) {
+  typename Tile::Lane at;
+  const uint32_t base = lds_address(lds) + share * 4 * Tile::kBytes;
+  at.offset(base);
+  // the share's tile of a step
+  const int steps = (keys.count + STREAMS - 1) / STREAMS;
+  auto copy = [&](int step) __attribute__((always_inline)) {
+    const int t = step * STREAMS + share;
+    if (t >= keys.count)
+      return;
     const int64_t j = keys.from(t);
     const int n = keys.end(t) - (int)j;
-    const uint32_t to = base + (t & 1) * 2 * Tile::kBytes;
-    Tile::copy(to, kbase + j * a.k.token, n, kbytes, a.d);
-    Tile::copy(to + Tile::kBytes, vbase + j * a.v.token, n, vbytes, a.d);
+    const uint32_t to = base + (step & 1) * 2 * Tile::kBytes;
+    Tile::copy(to, kbase + j * a.k.token, n, kbytes, a.d, block);
+    Tile::copy(to + Tile::kBytes, vbase + j * a.v.token, n, vbytes, a.d, block);
   };
 
   v16f acc[F::kBlocks];
@@ -343,22 +411,24 @@ window_forward(WindowArgs a) {
       acc[b] = v16f{};
     top = -kInf; // the largest scaled score, in powers of two
     sum = 0.0f;  // of this half's keys
-    if (keys.count > 0)
+    if (steps > 0)
       copy(0);
     // (the tile's place in LDS is a constant of each copy of the step, and so
     // are the addresses behind the lane's)
-    auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+    auto step = [&](int i, auto parity) __attribute__((always_inline)) {
       landed();
-      if (t + 1 < keys.count)
-        copy(t + 1);
-      if (keys.any(t, place_lo, place_hi, a.window, a.sinks))
-        products(base + decltype(parity)::value * 2 * Tile::kBytes, t,
+      if (i + 1 < steps)
+        copy(i + 1);
+      const int t = i * STREAMS + share;
+      if (t < keys.count &&
+          keys.any(t, place_lo, place_hi, a.window, a.sinks))
+        products(decltype(parity)::value * 2 * Tile::kBytes, t,
                  careful);
     };
-    for (int t = 0; t < keys.count; t += 2) {
-      step(t, std::integral_constant<int, 0>{});
-      if (t + 1 < keys.count)
-        step(t + 1, std::integral_constant<int, 1>{});
+    for (int i = 0; i < steps; i += 2) {
+      step(i, std::integral_constant<int, 0>{});
+      if (i + 1 < steps)
+        step(i + 1, std::integral_constant<int, 1>{});
     }
   };
   pass(std::false_type{});
@@ -367,6 +437,8 @@ window_forward(WindowArgs a) {
   if (any_wave(!all_finite<T>(acc), &verdict))
     pass(std::true_type{});
 
+  if (!add_shares<T, D, STREAMS>(acc, top, sum, lds))
+    return;
   sum = both_halves_sum(sum);
   const bool empty = place < 0 || s.nk == 0; // a row that sees no key
   const float by = empty ? 0.0f : 1.0f / sum;
@@ -399,26 +471,30 @@ struct BackwardArgs {
   Operand go, gq, gk, gv;
   float *log2_sum, *delta; // [query_heads][query_tokens], of the first kernel
   // sums of the sinks' gradients in fp32, [..][key_heads][sink_rows][2][d]:
-  // those of the window, for each sequence, and of the queries past it, for
-  // each chunk of 1 << chunk_shift queries
+  // those of the window, for each part and sequence, and of the queries past
+  // it, for each chunk of 1 << chunk_shift queries
   float *sink_window, *sink_chunks;
-  int key_tiles, chunks, chunk_shift, sink_rows; // sink_rows: a multiple of 32
+  float *part_sums; // [parts][key_tokens][key_heads][2][d], of two and more
+  int parts, key_tiles, chunks, chunk_shift, sink_rows; // sink_rows: a multiple of 32
 };
 
 // dq of a tile of rows, and for the second kernel log_sum in powers of two
 // and delta of its rows.  The forward pass's loop with one product more:
 // ds^T = K Q^T and V dO^T element by element, dq^T += K^T ds^T.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (Forward<T, D>::kWaves)) void
+template <typename T, int D, int STREAMS>
+__global__ __launch_bounds__(kThreads, (Forward<T, D, STREAMS>::kWaves)) void
 window_query_gradient(BackwardArgs b) {
   const WindowArgs &a = b.w;
-  using F = Forward<T, D>;
+  using F = Forward<T, D, STREAMS>;
   using Tile = typename F::Tile;
   constexpr int KT = F::kTile;
-  __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
+  __shared__ __align__(1024) char lds[F::kBytes];
   __shared__ int verdict;
 
-  const Rows w(a);
+  const int wave = wave_in_group();
+  const int share = STREAMS == 1 ? 0 : wave / F::kBlocksOfRows;
+  const int block = wave - share * F::kBlocksOfRows;
+  const typename F::Rows w(a, block);
   if (w.count <= 0)
     return;
   const Sequence &s = w.s;
@@ -448,7 +524,7 @@ window_query_gradient(BackwardArgs b) {
     if (live) {
       const int64_t at = (int64_t)head * a.query_tokens + token;
       log2_sum = a.log_sum[at] * kLog2e;
-      if (h == 0) {
+      if (h == 0 && share == 0) {
         b.log2_sum[at] = log2_sum;
         b.delta[at] = delta;
       }
@@ -463,20 +539,27 @@ window_query_gradient(BackwardArgs b) {
                    hk * a.v.head;
   const uint32_t kbytes = (uint32_t)(a.k.token * sizeof(T));
   const uint32_t vbytes = (uint32_t)(a.v.token * sizeof(T));
-  const typename Tile::Lane at;
-  const uint32_t base = lds_address(lds);
-  auto copy = [&](int t) __attribute__((always_inline)) {
+  typename Tile::FewLane at;
+  const uint32_t base = lds_address(lds) + share * 4 * Tile::kBytes;
+  at.offset(base);
+  // the share's tile of a step
+  const int steps = (keys.count + STREAMS - 1) / STREAMS;
+  auto copy = [&](int step) __attribute__((always_inline)) {
+    const int t = step * STREAMS + share;
+    if (t >= keys.count)
+      return;
     const int64_t j = keys.from(t);
     const int n = keys.end(t) - (int)j;
-    const uint32_t to = base + (t & 1) * 2 * Tile::kBytes;
-    Tile::copy(to, kbase + j * a.k.token, n, kbytes, a.d);
-    Tile::copy(to + Tile::kBytes, vbase + j * a.v.token, n, vbytes, a.d);
+    const uint32_t to = base + (step & 1) * 2 * Tile::kBytes;
+    Tile::copy(to, kbase + j * a.k.token, n, kbytes, a.d, block);
+    Tile::copy(to + Tile::kBytes, vbase + j * a.v.token, n, vbytes, a.d, block);
   };
 
   v16f acc[F::kBlocks];
   auto products = [&](uint32_t kt, int t, auto careful)
                       __attribute__((always_inline)) {
     const uint32_t vt = kt + Tile::kBytes;
+    at.fresh();
     const bool all = keys.all(t, place_lo, place_hi, a.window, a.sinks);
     const bool sink = keys.sink(t);
     const int j0 = keys.from(t) + 4 * h;
@@ -531,25 +614,30 @@ window_query_gradient(BackwardArgs b) {
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
       acc[c] = v16f{};
-    if (keys.count > 0)
+    if (steps > 0)
       copy(0);
-    auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+    auto step = [&](int i, auto parity) __attribute__((always_inline)) {
       landed();
-      if (t + 1 < keys.count)
-        copy(t + 1);
-      if (keys.any(t, place_lo, place_hi, a.window, a.sinks))
-        products(base + decltype(parity)::value * 2 * Tile::kBytes, t,
+      if (i + 1 < steps)
+        copy(i + 1);
+      const int t = i * STREAMS + share;
+      if (t < keys.count &&
+          keys.any(t, place_lo, place_hi, a.window, a.sinks))
+        products(decltype(parity)::value * 2 * Tile::kBytes, t,
                  careful);
     };
-    for (int t = 0; t < keys.count; t += 2) {
-      step(t, std::integral_constant<int, 0>{});
-      if (t + 1 < keys.count)
-        step(t + 1, std::integral_constant<int, 1>{});
+    for (int i = 0; i < steps; i += 2) {
+      step(i, std::integral_constant<int, 0>{});
+      if (i + 1 < steps)
+        step(i + 1, std::integral_constant<int, 1>{});
     }
   };
   pass(std::false_type{});
   if (any_wave(!all_finite<T>(acc), &verdict))
     pass(std::true_type{});
+  float top = 0.0f, sum = 0.0f; // (the shares' gradients add up as they are)
+  if (!add_shares<T, D, STREAMS>(acc, top, sum, lds))
+    return;
   if (live) {
     T *out = static_cast<T *>(b.query_gradient) + token * b.gq.token +
              head * b.gq.head;
@@ -574,6 +662,9 @@ window_query_gradient(BackwardArgs b) {
 // has, so they are split (SINK): a workgroup of those takes 32 sinks and a
 // chunk of queries, its waves blocks of 32 queries in turn, each with tiles of
 // its own, and leaves its sums to window_sink_gradient.
+//
+// Where there are few keys, the tiles of their queries are split into `parts`,
+// one workgroup for each, whose sums window_key_join adds up.
 template <typename T, int D, bool SINK> struct Backward {
   static constexpr int kTile = 32; // queries
   using Tile = RowTile<T, D, kTile, SINK ? kWave : kThreads>;
@@ -582,30 +673,31 @@ template <typename T, int D, bool SINK> struct Backward {
   // (fp32 rows of 128 leave a wave's own tiles no second place)
   static constexpr int kParities = SINK && sizeof(T) * D > 256 ? 1 : 2;
   static constexpr int kValues = SINK ? 0 : Values::kBytes;
+  static constexpr int kBytes =
+      kBuffers * kParities * 2 * Tile::kBytes + kValues;
   static constexpr int kSteps = D / 16;
   static constexpr int kBlocks = D / 32;
   static constexpr int kWaves = SINK || sizeof(T) * D > 256 ? 1 : 2;
 };
 
-template <typename T, int D, bool SINK>
-__global__ __launch_bounds__(kThreads, (Backward<T, D, SINK>::kWaves)) void
-window_key_gradient(BackwardArgs b) {
+// True: a sum is not finite, and nothing is written; CAREFUL computes those,
+// with the queries at the edges of the mask kept apart.
+template <typename T, int D, bool SINK, bool CAREFUL>
+__device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
+                                                  char *lds, float *stats,
+                                                  int *verdict) {
   const WindowArgs &a = b.w;
   using F = Backward<T, D, SINK>;
   using Tile = typename F::Tile;
   using Values = typename F::Values;
   constexpr int QT = F::kTile;
-  // [buffer of a wave, or of all][parity][q, do], then the values
-  __shared__ __align__(1024) char
-      lds[F::kBuffers * F::kParities * 2 * Tile::kBytes + F::kValues];
-  __shared__ __align__(16) float stats[F::kBuffers][2][2][64];
-  __shared__ int verdict;
 
   const int lane = lane_id(), h = lane >> 5, wave = wave_in_group();
   const int group = a.query_heads / a.key_heads;
   int hk, i, key0, first, last; // keys from key0; queries first .. last
   Sequence s;
   int64_t item;
+  int part = 0;
   if constexpr (SINK) {
     const int sink_blocks = b.sink_rows / 32;
     const int block = (int)(blockIdx.x % sink_blocks);
@@ -621,18 +713,20 @@ window_key_gradient(BackwardArgs b) {
     last = row0 + (1 << b.chunk_shift) - 1;
     last = last < s.nq - 1 ? last : s.nq - 1;
     if (row0 < 0 || last < first || last + s.nk - s.nq < a.window)
-      return; // (no query, or none past the window: the sum leaves it out)
+      return false; // (no query, or none past the window: the sum leaves it out)
     const int far = key0 + a.window - (s.nk - s.nq);
     first = far > first ? far : first;
   } else {
     item = xcd_contiguous(blockIdx.x, gridDim.x);
+    part = (int)(item % b.parts);
+    item /= b.parts;
     const int tile = (int)(item % b.key_tiles);
     hk = (int)(item / b.key_tiles);
     i = sequence_of_tile(a.key_offsets, a.sequences, tile, kRowShift);
     s = sequence(a, i);
     key0 = (tile - (a.key_offsets[i] >> kRowShift) - i) << kRowShift;
     if (key0 < 0 || key0 >= s.nk)
-      return;
+      return false;
     const int shift = s.nk - s.nq;
     const int end = (s.nk < key0 + kRows ? s.nk : key0 + kRows) - 1;
     first = key0 - shift > 0 ? key0 - shift : 0;
@@ -658,7 +752,7 @@ window_key_gradient(BackwardArgs b) {
       load_rows<T>(v, values + token * a.v.token, live, a.d, false);
     else
       Values::copy(vbase, values + (int64_t)(s.k0 + tile_key) * a.v.token,
-                   s.nk - tile_key, (uint32_t)(a.v.token * sizeof(T)), a.d);
+                   s.nk - tile_key, (uint32_t)(a.v.token * sizeof(T)), a.d, wave);
   }
 
   const T *qbase = static_cast<const T *>(a.query) + (int64_t)s.q0 * a.q.token;
@@ -667,19 +761,38 @@ window_key_gradient(BackwardArgs b) {
   const uint32_t qbytes = (uint32_t)(a.q.token * sizeof(T));
   const uint32_t obytes = (uint32_t)(b.go.token * sizeof(T));
   const int tiles = last < first ? 0 : (last - first) / QT + 1;
-  const int count = tiles * group;
+  // tiles of all heads, and this part's
+  const int begin = SINK ? 0 : (int)((int64_t)tiles * group * part / b.parts);
+  const int count =
+      (SINK ? tiles * group
+            : (int)((int64_t)tiles * group * (part + 1) / b.parts)) - begin;
   typename Tile::FewLane at;
   const uint32_t base =
       lds_address(lds) + (SINK ? wave * F::kParities * 2 * Tile::kBytes : 0);
   const uint32_t sbase = lds_address(stats) + (SINK ? wave * 1024 : 0);
-  auto copy = [&](int t, int parity) __attribute__((always_inline)) {
-    const int head = hk * group + t / tiles;
-    const int64_t r = first + t % tiles * QT;
+  // the head and first query of the tile that is copied next, and of the one
+  // that is computed next
+  int next_head = 0, next = 0, now = 0;
+  auto ahead = [&](int n) __attribute__((always_inline)) { // n tiles on
+    next += n * QT;
+    while (next > last) {
+      next -= tiles * QT;
+      ++next_head;
+    }
+  };
+  if (count > 0) {
+    next_head = hk * group + begin / tiles;
+    next = first + begin % tiles * QT;
+  }
+  auto copy = [&](int parity) __attribute__((always_inline)) {
+    const int head = next_head;
+    const int64_t r = next;
     const int n = last + 1 - (int)r;
     const uint32_t to = base + parity * 2 * Tile::kBytes;
-    Tile::copy(to, qbase + r * a.q.token + head * a.q.head, n, qbytes, a.d);
+    Tile::copy(to, qbase + r * a.q.token + head * a.q.head, n, qbytes, a.d,
+               SINK ? 0 : wave);
     Tile::copy(to + Tile::kBytes, obase + r * b.go.token + head * b.go.head, n,
-               obytes, a.d);
+               obytes, a.d, SINK ? 0 : wave);
     // a row's two numbers, 64 of each
     const int64_t row = (int64_t)head * a.query_tokens + s.q0 + r;
     const int m = n < QT ? n : QT;
@@ -692,12 +805,11 @@ window_key_gradient(BackwardArgs b) {
   };
 
   v16f dk[F::kBlocks], dv[F::kBlocks];
-  auto products = [&](int t, int parity, auto careful)
+  auto products = [&](int lo, int parity)
                       __attribute__((always_inline)) {
     const uint32_t qt = base + parity * 2 * Tile::kBytes;
     const uint32_t ot = qt + Tile::kBytes;
     const uint32_t st0 = sbase + parity * 512;
-    const int lo = first + t % tiles * QT; // the block's first query
     if (!SINK &&
         (lo + 31 + shift < key0 || lo + shift - (key0 + 31) >= a.window))
       return; // hidden
@@ -744,7 +856,7 @@ window_key_gradient(BackwardArgs b) {
             (j <= rows);
         p[r] = see ? p[r] : 0.0f;
         ds[r] = see ? ds[r] : 0.0f;
-        if constexpr (decltype(careful)::value)
+        if constexpr (CAREFUL)
           seen |= (uint32_t)see << r;
       }
     }
@@ -763,7 +875,7 @@ window_key_gradient(BackwardArgs b) {
       for (int c = 0; c < F::kBlocks; ++c) {
         const Frag<T> of = Tile::across(ot, at, half, c);
         const Frag<T> qf = Tile::across(qt, at, half, c);
-        if (decltype(careful)::value && !all) {
+        if (CAREFUL && !all) {
           dv[c] = mma32_seen<T>(of, pf, dv[c], seen >> (8 * half));
           dk[c] = mma32_seen<T>(qf, df, dk[c], seen >> (8 * half));
         } else {
@@ -774,33 +886,42 @@ window_key_gradient(BackwardArgs b) {
     }
     __builtin_amdgcn_s_setprio(0);
   };
-  auto pass = [&](auto careful) __attribute__((always_inline)) {
+  {
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
       dk[c] = dv[c] = v16f{};
     if constexpr (SINK) {
+      if (wave < count)
+        ahead(wave);
       if (wave < count && F::kParities == 2)
-        copy(wave, 0);
+        copy(0);
       for (int t = wave, parity = 0; t < count; t += 4) {
+        now = next;
         if (F::kParities == 1) {
           landed_wave(); // (its reads of the tile before)
-          copy(t, 0);
+          copy(0);
         }
         landed_wave();
-        if (F::kParities == 2 && t + 4 < count)
-          copy(t + 4, parity ^ 1);
-        products(t, parity, careful);
+        if (t + 4 < count) {
+          ahead(4);
+          if (F::kParities == 2)
+            copy(parity ^ 1);
+        }
+        products(now, parity);
         parity ^= F::kParities - 1;
       }
     } else {
       if (count > 0)
-        copy(0, 0);
+        copy(0);
       auto step = [&](int t, auto parity) __attribute__((always_inline)) {
         constexpr int P = decltype(parity)::value;
         landed();
-        if (t + 1 < count)
-          copy(t + 1, 1 - P);
-        products(t, P, careful);
+        now = next;
+        if (t + 1 < count) {
+          ahead(1);
+          copy(1 - P);
+        }
+        products(now, P);
       };
       for (int t = 0; t < count; t += 2) {
         step(t, std::integral_constant<int, 0>{});
@@ -808,14 +929,13 @@ window_key_gradient(BackwardArgs b) {
           step(t + 1, std::integral_constant<int, 1>{});
       }
     }
-  };
-  pass(std::false_type{});
-  if (any_wave(!(all_finite<T>(dk) && all_finite<T>(dv)), &verdict))
-    pass(std::true_type{});
+  }
+  if (!CAREFUL && any_wave(!(all_finite<T>(dk) && all_finite<T>(dv)), verdict))
+    return true;
 
   if constexpr (SINK) {
     // the waves' sums, one after the other, in the tiles' memory
-    static_assert(sizeof(lds) >= 2 * F::kBlocks * 16 * 64 * 4, "");
+    static_assert(F::kBytes >= 2 * F::kBlocks * 16 * 64 * 4, "");
     float *sums = reinterpret_cast<float *>(lds);
     for (int turn = 0; turn < 4; ++turn) {
       __syncthreads();
@@ -835,15 +955,20 @@ window_key_gradient(BackwardArgs b) {
       }
     }
     if (wave != 3)
-      return;
+      return false;
   }
   if (!live)
-    return;
-  // a sink's sums wait for those of the queries past the window
-  if (SINK || key < b.sink_rows) {
-    const int64_t of = (SINK ? item : i) * a.key_heads + hk;
-    float *out = (SINK ? b.sink_chunks : b.sink_window) +
-                 (of * b.sink_rows + key) * 2 * a.d;
+    return false;
+  // A sink's sums wait for those of the queries past the window, and a part's
+  // for the other parts'.
+  if (SINK || b.parts > 1 || key < a.sinks) {
+    float *out = SINK || key < a.sinks
+                     ? (SINK ? b.sink_chunks : b.sink_window) +
+                           (((SINK ? item : (int64_t)part * a.sequences + i) *
+                                 a.key_heads + hk) * b.sink_rows + key) *
+                               2 * a.d
+                     : b.part_sums + (((int64_t)part * a.key_tokens + s.k0 +
+                                       key) * a.key_heads + hk) * 2 * a.d;
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
 #pragma unroll
@@ -853,8 +978,7 @@ window_key_gradient(BackwardArgs b) {
           st4(x, dk[c][r], dk[c][r + 1], dk[c][r + 2], dk[c][r + 3]);
           st4(x + a.d, dv[c][r], dv[c][r + 1], dv[c][r + 2], dv[c][r + 3]);
         }
-    if (SINK || key < a.sinks)
-      return;
+    return false;
   }
   const int64_t token = s.k0 + key;
   T *kout = static_cast<T *>(b.key_gradient) + token * b.gk.token +
@@ -872,6 +996,31 @@ window_key_gradient(BackwardArgs b) {
         st4(vout + 32 * c + acc_row(r), dv[c][r], dv[c][r + 1], dv[c][r + 2],
             dv[c][r + 3]);
       }
+  return false;
+}
+
+// CAREFUL is a function that is called and reads the kernel's arguments where
+// they lie: inlined beside the plain one it takes registers of its loop, and a
+// spilled register read back there waits for every copy under way (16,384
+// tokens, window 1024: 351 us, inlined 370 to 506 us).
+template <typename T, int D, bool SINK>
+__device__ __noinline__ void key_gradient_again(const void *args, char *lds,
+                                                float *stats, int *verdict) {
+  key_gradient_rows<T, D, SINK, true>(*static_cast<const BackwardArgs *>(args),
+                                      lds, stats, verdict);
+}
+template <typename T, int D, bool SINK>
+__global__ __launch_bounds__(kThreads, (Backward<T, D, SINK>::kWaves)) void
+window_key_gradient(BackwardArgs b) {
+  using F = Backward<T, D, SINK>;
+  // [buffer of a wave, or of all][parity][q, do], then the values
+  __shared__ __align__(1024) char lds[F::kBytes];
+  __shared__ __align__(16) float stats[F::kBuffers * 2 * 2 * 64];
+  __shared__ int verdict;
+  if (key_gradient_rows<T, D, SINK, false>(b, lds, stats, &verdict))
+    key_gradient_again<T, D, SINK>(
+        (const void *)__builtin_amdgcn_kernarg_segment_ptr(), lds, stats,
+        &verdict);
 }
 
 // The sinks' gradients: the window's sums and every chunk's, in the same order
@@ -914,9 +1063,13 @@ window_sink_gradient(BackwardArgs b) {
   __syncthreads();
   if (run != 0 || c >= a.d)
     return;
-  const float *x = b.sink_window + ((int64_t)i * a.key_heads + hk) * row + own;
-  dk = x[0];
-  dv = x[a.d];
+  dk = dv = 0.0f;
+  for (int p = 0; p < b.parts; ++p) {
+    const float *x = b.sink_window + (((int64_t)p * a.sequences + i) *
+                                          a.key_heads + hk) * row + own;
+    dk += x[0];
+    dv += x[a.d];
+  }
 #pragma unroll
   for (int r = 0; r < kSinkRuns; ++r) {
     dk += sums[0][r][c];
@@ -927,6 +1080,48 @@ window_sink_gradient(BackwardArgs b) {
       dk * a.alpha);
   stv(static_cast<T *>(b.value_gradient) + token * b.gv.token +
           hk * b.gv.head + c, dv);
+}
+
+// The sums of the parts of the keys that are no sinks, in order: four elements
+// of a key and head a thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_key_join(BackwardArgs b) {
+  const WindowArgs &a = b.w;
+  const int per_row = a.d / 4;
+  const int64_t x = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t row = x / per_row;
+  const int c = (int)(x % per_row) * 4;
+  const int token = (int)(row / a.key_heads), hk = (int)(row % a.key_heads);
+  if (token >= a.key_tokens)
+    return;
+  // the sequence of the token: the last that starts at or before it
+  int lo = 0, n = a.sequences;
+  while (n > 1) {
+    const int half = n / 2;
+    if (a.key_offsets[lo + half] <= token) {
+      lo += half;
+      n -= half;
+    } else {
+      n = half;
+    }
+  }
+  const Sequence s = sequence(a, lo);
+  const int key = token - s.k0;
+  if (key < a.sinks || key >= s.nk)
+    return; // (a sink's, or of no sequence)
+  const float *p = b.part_sums + row * 2 * a.d + c;
+  const int64_t step = (int64_t)a.key_tokens * a.key_heads * 2 * a.d;
+  v4f dk = {}, dv = {};
+#pragma unroll 4
+  for (int i = 0; i < b.parts; ++i) {
+    dk += ld4(p + i * step);
+    dv += ld4(p + i * step + a.d);
+  }
+  st4(static_cast<T *>(b.key_gradient) + (int64_t)token * b.gk.token +
+          hk * b.gk.head + c, dk[0] * a.alpha, dk[1] * a.alpha,
+      dk[2] * a.alpha, dk[3] * a.alpha);
+  st4(static_cast<T *>(b.value_gradient) + (int64_t)token * b.gv.token +
+          hk * b.gv.head + c, dv[0], dv[1], dv[2], dv[3]);
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -1003,9 +1198,35 @@ int fill_window(WindowArgs &a, size_t elem, const int32_t *query_offsets,
   a.window = (int)std::min(window, std::max<int64_t>(key_tokens, 1));
   a.sinks = window >= key_tokens ? 0 : (int)std::min(sinks, key_tokens);
   a.alpha = alpha;
-  a.tiles = (int)((query_tokens >> kRowShift) + sequences);
-  return sw::check_flat_grid((int64_t)a.tiles * query_heads, kThreads,
-                             "window attention");
+  return SW_OK;
+}
+
+// Shares of the keys for each workgroup of the row kernels.  The chip holds
+// 512 workgroups (two waves a SIMD); about half of them and fewer are split.
+// 4096 queries, window 1024, bf16 heads of 128, one share / two: 4 heads (132
+// workgroups) 34.9 / 26.9 us, 8 heads (264) 39.5 / 36.0, 12 heads (396) 45.2 /
+// 51.7, 32 heads (1056) 93.1 / 113.7; 2501 queries of 12 heads (288), window
+// 2000: 63.9 / 72.8.
+int choose_streams(WindowArgs &a) {
+  auto tiles = [&](int streams) {
+    return ((int64_t)a.query_tokens >> shared_shift(streams)) + a.sequences;
+  };
+  const int streams = tiles(1) * a.query_heads < 272 ? 2 : 1;
+  a.tiles = (int)tiles(streams);
+  return streams;
+}
+
+template <typename T, int D>
+int launch_forward(WindowArgs &a, int streams, hipStream_t st) {
+  const int64_t grid = (int64_t)a.tiles * a.query_heads;
+  if (int rc = sw::check_flat_grid(grid, kThreads, "window attention"))
+    return rc;
+  const dim3 g((unsigned)grid);
+  if (streams == 1)
+    window_forward<T, D, 1><<<g, kThreads, 0, st>>>(a);
+  else
+    window_forward<T, D, 2><<<g, kThreads, 0, st>>>(a);
+  return sw::launch_check("window attention");
 }
 
 template <typename T>
@@ -1024,44 +1245,116 @@ int forward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
     return rc;
   if (sequences == 0 || query_tokens == 0)
     return SW_OK;
-  const dim3 grid((unsigned)((int64_t)a.tiles * query_heads));
+  const int streams = choose_streams(a);
   const hipStream_t st = sw::as_stream(stream);
-  if (d <= 64)
-    window_forward<T, 64><<<grid, kThreads, 0, st>>>(a);
-  else
-    window_forward<T, 128><<<grid, kThreads, 0, st>>>(a);
-  return sw::launch_check("window attention");
+  return d <= 64 ? launch_forward<T, 64>(a, streams, st)
+                 : launch_forward<T, 128>(a, streams, st);
 }
 
 // The backward pass's scratch memory: [2][query_heads][query_tokens] of the
-// queries' numbers, then the sinks' sums.
+// queries' numbers, the sinks' sums, the parts' sums.
 struct Scratch {
-  int64_t stats, sink_window, sink_chunks; // floats of each
+  int64_t stats, sink_window, sink_chunks, part_sums; // floats of each
   int64_t chunks;
-  int chunk_shift, sink_rows;
-  int64_t bytes() const { return 4 * (2 * stats + sink_window + sink_chunks); }
+  int parts, chunk_shift, sink_rows;
+  int64_t bytes() const {
+    return 4 * (2 * stats + sink_window + sink_chunks + part_sums);
+  }
 };
 Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
                          int64_t key_tokens, int64_t query_heads,
                          int64_t key_heads, int64_t d, int64_t window,
-                         int64_t sinks) {
+                         int64_t sinks, int64_t elem) {
   Scratch c{};
   // (whole 16 bytes, so that what follows stays aligned)
   c.stats = sw::ceil_div(query_heads * query_tokens, 4) * 4;
+  // The chip holds 512 workgroups of 128 keys (256 of fp32 rows past 64).
+  // Fewer are split until they are as many, as long as each part has eight
+  // tiles of queries; a little more than half of them too, where a second part
+  // of at least 32 tiles is worth its sums.  4096 keys, window 1024, bf16 heads
+  // of 128, one part / the rule's: 8 heads over 4 (132 workgroups) 164 / 100 us
+  // (3 parts; 4: 128 us), 24 over 8 (264) 243 / 200 (2), 12 over 12 (396)
+  // 115 (2 parts: 150).
+  const int64_t groups = ((key_tokens >> kRowShift) + sequences) * key_heads;
+  const int64_t slots = elem == 4 && d > 64 ? 256 : 512;
+  const int64_t tiles = query_heads / key_heads *
+                        (std::min({window, key_tokens, query_tokens}) + kRows) /
+                        32;
+  int64_t parts = std::min(slots / std::max<int64_t>(groups, 1), tiles / 8);
+  if (parts == 1 && groups * 8 <= slots * 5 && tiles >= 64)
+    parts = 2;
+  c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(parts, 16));
+  if (c.parts > 1)
+    c.part_sums = c.parts * key_tokens * key_heads * 2 * d;
   const int64_t s = window >= key_tokens ? 0 : std::min(sinks, key_tokens);
   if (s == 0)
     return c;
   c.sink_rows = (int)sw::ceil_div(s, 32) * 32;
   // 256 queries a chunk, more where there are more than 64 sinks: the sums
-  // then stay below the size of bf16 keys
+  // then stay below the size of bf16 keys; fewer, to 64, where that makes
+  // fewer workgroups than the chip has units.
   c.chunk_shift = 8;
   while (((int64_t)64 << (c.chunk_shift - 8)) < s)
     ++c.chunk_shift;
+  while (c.chunk_shift > 6 && (query_tokens >> c.chunk_shift) * key_heads *
+                                      (c.sink_rows / 32) < 256)
+    --c.chunk_shift;
   c.chunks = (query_tokens >> c.chunk_shift) + sequences;
   const int64_t one = key_heads * c.sink_rows * 2 * d;
-  c.sink_window = sequences * one;
+  c.sink_window = c.parts * sequences * one;
   c.sink_chunks = c.chunks * one;
   return c;
+}
+
+template <typename T, int D>
+int launch_backward(BackwardArgs &b, hipStream_t st) {
+  WindowArgs &a = b.w;
+  const char *what = "window attention's gradient";
+  const int streams = choose_streams(a);
+  const int64_t rows = (int64_t)a.tiles * a.query_heads;
+  const int64_t sinks = (int64_t)b.chunks * a.key_heads * (b.sink_rows / 32);
+  const int64_t keys = (int64_t)b.key_tiles * a.key_heads * b.parts;
+  const int64_t part_rows = sw::ceil_div(
+      b.parts > 1 ? (int64_t)a.key_tokens * a.key_heads * (a.d / 4) : 0,
+      kThreads);
+  const int64_t join = (int64_t)a.sequences * a.key_heads * a.sinks;
+  if (int rc = sw::check_flat_grid(std::max({rows, sinks, keys, part_rows}),
+                                   kThreads, what))
+    return rc;
+  if (int rc = sw::check_flat_grid(join, 128 * kSinkRuns, what))
+    return rc;
+  if (a.query_tokens > 0) {
+    const dim3 g((unsigned)rows);
+    if (streams == 1)
+      window_query_gradient<T, D, 1><<<g, kThreads, 0, st>>>(b);
+    else
+      window_query_gradient<T, D, 2><<<g, kThreads, 0, st>>>(b);
+    if (int rc = sw::launch_check(what))
+      return rc;
+  }
+  if (a.key_tokens == 0)
+    return SW_OK;
+  if (sinks > 0) {
+    window_key_gradient<T, D, true>
+        <<<dim3((unsigned)sinks), kThreads, 0, st>>>(b);
+    if (int rc = sw::launch_check(what))
+      return rc;
+  }
+  window_key_gradient<T, D, false>
+      <<<dim3((unsigned)keys), kThreads, 0, st>>>(b);
+  if (int rc = sw::launch_check(what))
+    return rc;
+  if (part_rows > 0) {
+    window_key_join<T><<<dim3((unsigned)part_rows), kThreads, 0, st>>>(b);
+    if (int rc = sw::launch_check(what))
+      return rc;
+  }
+  if (join > 0) {
+    window_sink_gradient<T>
+        <<<dim3((unsigned)join), 128 * kSinkRuns, 0, st>>>(b);
+    return sw::launch_check(what);
+  }
+  return SW_OK;
 }
 
 template <typename T>
@@ -1104,7 +1397,8 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   if (!log_sum && query_tokens > 0)
     return sw::fail(SW_ERR_INVALID_ARGUMENT, "log_sum pointer is null");
   const Scratch c = backward_scratch(sequences, query_tokens, key_tokens,
-                                     query_heads, key_heads, d, window, sinks);
+                                     query_heads, key_heads, d, window, sinks,
+                                     sizeof(T));
   if (c.bytes() > 0 && (!workspace || !sw::aligned16(workspace) ||
                         workspace_bytes < c.bytes()))
     return sw::fail(SW_ERR_INVALID_ARGUMENT,
@@ -1121,52 +1415,12 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   b.chunks = (int)c.chunks;
   b.chunk_shift = c.chunk_shift;
   b.sink_rows = c.sink_rows;
+  b.part_sums = b.sink_chunks + c.sink_chunks;
+  b.parts = c.parts;
   b.key_tiles = (int)((key_tokens >> kRowShift) + sequences);
-  const int64_t grid = (int64_t)b.key_tiles * key_heads;
-  const int64_t sink_grid = c.chunks * key_heads * (c.sink_rows / 32);
-  const int64_t rows = sequences * key_heads * a.sinks;
-  if (int rc = sw::check_flat_grid(std::max(grid, sink_grid), kThreads,
-                                   "window attention's gradient"))
-    return rc;
-  if (int rc = sw::check_flat_grid(rows, 128 * kSinkRuns,
-                                   "window attention's sink gradient"))
-    return rc;
   const hipStream_t st = sw::as_stream(stream);
-  const dim3 rows_grid((unsigned)((int64_t)a.tiles * query_heads));
-  if (query_tokens > 0) {
-    if (d <= 64)
-      window_query_gradient<T, 64><<<rows_grid, kThreads, 0, st>>>(b);
-    else
-      window_query_gradient<T, 128><<<rows_grid, kThreads, 0, st>>>(b);
-    if (int rc = sw::launch_check("window attention's query gradient"))
-      return rc;
-  }
-  if (key_tokens == 0)
-    return SW_OK;
-  if (sink_grid > 0) {
-    if (d <= 64)
-      window_key_gradient<T, 64, true>
-          <<<dim3((unsigned)sink_grid), kThreads, 0, st>>>(b);
-    else
-      window_key_gradient<T, 128, true>
-          <<<dim3((unsigned)sink_grid), kThreads, 0, st>>>(b);
-    if (int rc = sw::launch_check("window attention's key gradient"))
-      return rc;
-  }
-  if (d <= 64)
-    window_key_gradient<T, 64, false>
-        <<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
-  else
-    window_key_gradient<T, 128, false>
-        <<<dim3((unsigned)grid), kThreads, 0, st>>>(b);
-  if (int rc = sw::launch_check("window attention's key gradient"))
-    return rc;
-  if (a.sinks > 0) {
-    window_sink_gradient<T>
-        <<<dim3((unsigned)rows), 128 * kSinkRuns, 0, st>>>(b);
-    return sw::launch_check("window attention's sink gradient");
-  }
-  return SW_OK;
+  return d <= 64 ? launch_backward<T, 64>(b, st)
+                 : launch_backward<T, 128>(b, st);
 }
 
 } // namespace
@@ -1200,12 +1454,13 @@ extern "C" int sw_window_attention_bf16(
 extern "C" int64_t sw_window_attention_backward_workspace_bytes(
     int64_t sequences, int64_t query_tokens, int64_t key_tokens,
     int64_t query_heads, int64_t key_heads, int64_t d, int64_t window,
-    int64_t sinks) {
-  if (check_window(sequences, query_tokens, key_tokens, query_heads, key_heads,
+    int64_t sinks, int value_bytes) {
+  if ((value_bytes != 4 && value_bytes != 2) ||
+      check_window(sequences, query_tokens, key_tokens, query_heads, key_heads,
                    d, window, sinks, 0.0f) != SW_OK)
     return 0;
   return backward_scratch(sequences, query_tokens, key_tokens, query_heads,
-                          key_heads, d, window, sinks).bytes();
+                          key_heads, d, window, sinks, value_bytes).bytes();
 }
 
 extern "C" int sw_window_attention_backward_f32(

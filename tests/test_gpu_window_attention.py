@@ -419,7 +419,7 @@ def test_training_step_repeats_and_graphs(dev, dtype):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, other))
     need = sw.load_library().sw_window_attention_backward_workspace_bytes(
-        2, 1400, 1400, 4, 2, 128, 64, 4)
+        2, 1400, 1400, 4, 2, 128, 64, 4, q.element_size())
     step(other, workspace=torch.full((need,), 255, dtype=torch.uint8,
                                      device=DEV))
     torch.cuda.synchronize()

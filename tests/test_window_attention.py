@@ -94,21 +94,30 @@ def test_backward_refused(dt, kw, code, needle):
 def test_backward_workspace_rule():
     need = sw.load_library().sw_window_attention_backward_workspace_bytes
     # two numbers of each query and head
-    assert need(1, 100, 100, 4, 2, 64, 100, 7) == 2 * 4 * 100 * 4
-    # sinks apart: those of the window and of one chunk a sequence more than
-    # whole ones, 32 rows each
+    assert need(1, 100, 100, 4, 2, 64, 100, 7, 2) == 2 * 4 * 100 * 4
+    # sinks apart: those of the window, and of one chunk of 64 queries a
+    # sequence more than whole ones, 32 rows each
     rows = 2 * 32 * 2 * 64
-    assert need(3, 100, 100, 4, 2, 64, 99, 7) == 2 * 4 * 100 * 4 + \
-        4 * rows * (3 + 3)
-    assert need(3, 5000, 100, 4, 2, 64, 99, 7) == 2 * 4 * 5000 * 4 + \
-        4 * rows * (3 + 19 + 3)
-    # at most the size of bf16 keys apart from one chunk a sequence, however
-    # many sinks
+    assert need(3, 100, 100, 4, 2, 64, 99, 7, 2) == 2 * 4 * 100 * 4 + \
+        4 * rows * (3 + 1 + 3)
+    assert need(3, 5000, 100, 4, 2, 64, 99, 7, 2) == 2 * 4 * 5000 * 4 + \
+        4 * rows * (3 + 78 + 3)
+    assert need(3, 99000, 100, 4, 2, 64, 99, 7, 2) == 2 * 4 * 99000 * 4 + \
+        4 * rows * (3 + 386 + 3)
+    # parts of few keys: dk and dv of each
+    one = need(1, 4096, 4096, 8, 4, 128, 4096, 0, 2)
+    assert one == 2 * 4 * 8 * 4096 + 3 * 4 * 4096 * 4 * 2 * 128
+    assert need(1, 4096, 4096, 8, 4, 128, 4096, 0, 4) == \
+        2 * 4 * 8 * 4096 + 2 * 4 * 4096 * 4 * 2 * 128
+    assert need(1, 4096, 4096, 12, 12, 128, 4096, 0, 2) == 2 * 4 * 12 * 4096
+    # many sinks: at most the size of bf16 keys apart from a chunk a sequence
+    # and the window's
+    n = 1 << 20
     for sinks in (64, 100, 1000, 5000):
-        assert need(1, 1 << 20, 1 << 20, 1, 1, 128, 64, sinks) <= \
-            2 * 4 * (1 << 20) + 2 * 2 * (1 << 20) * 128 + 3 * 4 * 256 * (
-                sinks + 31)
-    assert need(1, 100, 100, 4, 3, 64, 100, 7) == 0
+        assert need(1, n, n, 1, 1, 128, 64, sinks, 2) <= 2 * 4 * n + \
+            2 * 2 * n * 128 + 3 * 4 * 256 * (sinks + 31)
+    assert need(1, 100, 100, 4, 3, 64, 100, 7, 2) == 0
+    assert need(1, 100, 100, 4, 2, 64, 100, 7, 8) == 0
 
 
 def test_nothing_to_do():
