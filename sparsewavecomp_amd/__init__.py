@@ -23,7 +23,8 @@ __all__ = [
     "sparse_attention", "window_attention",
     "window_attention_backward", "window_attention_decode",
     "shared_prefix_attention", "csr_row_at_position",
-    "SDDMM_MUL", "SDDMM_AFFINE", "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV", "MAP_SUB", "MAP_MUL",
+    "SDDMM_MUL", "SDDMM_AFFINE", "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV",
+    "MAP_SUB", "MAP_MUL",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -641,61 +642,70 @@ def sparse_attention(row_offsets, column_indices, mask_values, query,
     return output
 
 
-def _heads(t, dtype, name):
-    """Address and (row, head) strides of a [rows, heads, d] operand, whose
-    rows of d elements are consecutive; of [pages, rows, heads, d] the page's
-    before them."""
+def _heads(dtype, at, *named):
+    """Addresses and strides of [rows, heads, d] operands, given as tensor and
+    name in turn, whose rows of d elements are consecutive, on device `at`:
+    a list of addresses, and the (row, head) strides of all as a C array, of
+    [pages, rows, heads, d] the page's before them; None where every operand is
+    packed, which is what the C functions take it for."""
     torch = _torch or _load_torch()
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a device tensor, got {t.device}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.is_contiguous():
-        *pages, rows, heads, d = t.shape
-        if pages:
-            return t.data_ptr(), rows * heads * d, heads * d, d
-        return t.data_ptr(), heads * d, d
-    *page, row, head, last = t.stride()
-    if last != 1:
-        raise ValueError(f"{name} must have consecutive elements in its last "
-                         "dimension")
-    # (the stride of a dimension of one is any number: a packed one)
-    if t.shape[-2] == 1:
-        head = t.shape[-1]
-    if t.shape[-3] == 1:
-        row = t.shape[-2] * max(head, t.shape[-1])
-    return (t.data_ptr(), *page, row, head)
-
-
-def _one_device(stream, *tensors):
-    """All operands on the device whose stream the call goes to."""
-    torch = _torch or _load_torch()
-    at = None
-    for t in tensors:
-        if t is None or not t.is_cuda:
-            continue  # (not a device tensor: refused where it is taken)
-        if at is None:
-            at = (torch.cuda.current_device() if stream is None
-                  else stream.device.index)
+    pointers, packed = [], True
+    for t, name in zip(named[::2], named[1::2]):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
         if t.get_device() != at:
-            raise ValueError(
-                f"an operand is on {t.device}, but the call goes to a stream "
-                f"of cuda:{at}")
+            if not t.is_cuda:
+                raise ValueError(
+                    f"{name} must be a device tensor, got {t.device}")
+            raise ValueError(f"{name} is on {t.device}, but the call goes to "
+                             f"a stream of cuda:{at}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if packed and not t.is_contiguous():
+            packed = False
+        pointers.append(t.data_ptr())
+    if packed:
+        return pointers, None
+    strides = []
+    for t, name in zip(named[::2], named[1::2]):
+        *page, row, head, last = t.stride()
+        if last != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{name} must have consecutive elements in its "
+                             "last dimension")
+        # (the stride of a dimension of one is any number: a packed one)
+        if t.shape[-2] == 1:
+            head = t.shape[-1]
+        if t.shape[-3] == 1:
+            row = t.shape[-2] * max(head, t.shape[-1])
+        strides += [*page, row, head]
+    return pointers, (ctypes.c_int64 * len(strides))(*strides)
+
+
+def _device_of(stream):
+    """The device that a call on `stream` goes to."""
+    torch = _torch or _load_torch()
+    return (torch.cuda.current_device() if stream is None
+            else stream.device.index) if torch.cuda.is_initialized() else -2
+
+
+def _flat(t, dtype, at, name):
+    """Address of a contiguous operand on device `at`."""
+    p = _dev(t, dtype, name)
+    if t.get_device() != at:
+        raise ValueError(f"{name} is on {t.device}, but the call goes to a "
+                         f"stream of cuda:{at}")
+    return p
 
 
 def _window_shapes(query_offsets, key_offsets, query, key, value):
-    _need(query.dim() == 3 and key.dim() == 3 and
-          tuple(key.shape) == tuple(value.shape) and
-          query.shape[2] == key.shape[2],
-          "expected query [query_tokens, query_heads, d] and key and value "
-          "[key_tokens, key_heads, d]")
+    q, k = query.shape, key.shape
+    if not (len(q) == len(k) == 3 and k == value.shape and q[2] == k[2]):
+        raise ShapeError("expected query [query_tokens, query_heads, d] and "
+                         "key and value [key_tokens, key_heads, d]")
     sequences = _rows_of(query_offsets, "query_offsets")
-    _need(tuple(key_offsets.shape) == (sequences + 1,),
-          "query and key offsets must have the same length")
-    return (sequences, query.shape[0], key.shape[0], query.shape[1],
-            key.shape[1], query.shape[2])
+    if key_offsets.shape != query_offsets.shape:
+        raise ShapeError("query and key offsets must have the same length")
+    return sequences, q[0], k[0], q[1], k[1], q[2]
 
 
 def window_attention(query_offsets, key_offsets, query, key, value, output,
@@ -723,16 +733,15 @@ def window_attention(query_offsets, key_offsets, query, key, value, output,
     if log_sum is not None:
         _need(tuple(log_sum.shape) == (shape[3], shape[1]),
               "log_sum must be [query_heads, query_tokens]")
-    _one_device(stream, query_offsets, key_offsets, query, key, value, output,
-                log_sum)
-    q, k, v, o = (_heads(t, dt, n) for t, n in (
-        (query, "query"), (key, "key"), (value, "value"),
-        (output, "output")))
-    strides = (ctypes.c_int64 * 8)(*q[1:], *k[1:], *v[1:], *o[1:])
+    at = _device_of(stream)
+    (q, k, v, o), strides = _heads(dt, at, query, "query", key, "key", value,
+                                   "value", output, "output")
+    lse = None
+    if log_sum is not None:
+        lse = _flat(log_sum, torch.float32, at, "log_sum")
     _check(_fn("sw_window_attention", dt)(
-        _dev(query_offsets, torch.int32, "query_offsets"),
-        _dev(key_offsets, torch.int32, "key_offsets"), q[0], k[0], v[0], o[0],
-        None if log_sum is None else _dev(log_sum, torch.float32, "log_sum"),
+        _flat(query_offsets, torch.int32, at, "query_offsets"),
+        _flat(key_offsets, torch.int32, at, "key_offsets"), q, k, v, o, lse,
         *shape, strides, window, sinks, alpha, _stream(stream)))
     return output
 
@@ -746,7 +755,8 @@ def _scratch(nbytes, like, workspace, stream):
         _dev(workspace, torch.uint8, "workspace")
         _need(workspace.numel() >= nbytes,
               f"workspace must hold {nbytes} bytes")
-        _one_device(stream, workspace)
+        if workspace.get_device() != like.get_device():
+            raise ValueError("workspace must be on the operands' device")
         return workspace
     if nbytes == 0:
         return None
@@ -781,22 +791,17 @@ def window_attention_backward(query_offsets, key_offsets, query, key, value,
         _need(tuple(t.shape) == tuple(key.shape), f"{n} must have key's shape")
     _need(tuple(log_sum.shape) == (shape[3], shape[1]),
           "log_sum must be [query_heads, query_tokens]")
-    _one_device(stream, query_offsets, key_offsets, query, key, value, output,
-                log_sum, output_gradient, query_gradient, key_gradient,
-                value_gradient)
-    ops = [_heads(t, dt, n) for t, n in (
-        (query, "query"), (key, "key"), (value, "value"), (output, "output"),
-        (output_gradient, "output_gradient"),
-        (query_gradient, "query_gradient"), (key_gradient, "key_gradient"),
-        (value_gradient, "value_gradient"))]
-    strides = (ctypes.c_int64 * 16)(*(x for o in ops for x in o[1:]))
-    offsets = (_dev(query_offsets, torch.int32, "query_offsets"),
-               _dev(key_offsets, torch.int32, "key_offsets"))
-    lse = _dev(log_sum, torch.float32, "log_sum")
+    at = _device_of(stream)
+    p, strides = _heads(
+        dt, at, query, "query", key, "key", value, "value", output, "output",
+        output_gradient, "output_gradient", query_gradient, "query_gradient",
+        key_gradient, "key_gradient", value_gradient, "value_gradient")
+    offsets = (_flat(query_offsets, torch.int32, at, "query_offsets"),
+               _flat(key_offsets, torch.int32, at, "key_offsets"))
+    lse = _flat(log_sum, torch.float32, at, "log_sum")
     need = load_library().sw_window_attention_backward_workspace_bytes(
         *shape, window, sinks, query.element_size())
     scratch = _scratch(need, query, workspace, stream)
-    p = [o[0] for o in ops]
     _check(_fn("sw_window_attention_backward", dt)(
         *offsets, *p[:4], lse, *p[4:], *shape, strides, window, sinks, alpha,
         None if scratch is None else scratch.data_ptr(), need,
@@ -806,21 +811,21 @@ def window_attention_backward(query_offsets, key_offsets, query, key, value,
 
 def _cache_shapes(key_lengths, page_table, query, key_cache, value_cache,
                   output):
-    _need(query.dim() == 3 and tuple(output.shape) == tuple(query.shape),
-          "expected query and output [sequences, query_heads, d]")
-    _need(key_cache.dim() == 4 and
-          tuple(key_cache.shape) == tuple(value_cache.shape) and
-          key_cache.shape[3] == query.shape[2],
-          "expected key and value caches [pages, page_size, key_heads, d]")
-    sequences, width = query.shape[0], 1
-    _need(tuple(key_lengths.shape) == (sequences,),
-          "key_lengths must hold one length a sequence")
+    q, c = query.shape, key_cache.shape
+    if len(q) != 3 or output.shape != q:
+        raise ShapeError("expected query and output [sequences, query_heads, "
+                         "d]")
+    if len(c) != 4 or value_cache.shape != c or c[3] != q[2]:
+        raise ShapeError("expected key and value caches [pages, page_size, "
+                         "key_heads, d]")
+    if key_lengths.shape != q[:1]:
+        raise ShapeError("key_lengths must hold one length a sequence")
+    width = 1
     if page_table is not None:
-        _need(page_table.dim() == 2 and page_table.shape[0] == sequences,
-              "page_table must be [sequences, most_pages]")
+        if page_table.dim() != 2 or page_table.shape[0] != q[0]:
+            raise ShapeError("page_table must be [sequences, most_pages]")
         width = page_table.shape[1]
-    return (sequences, key_cache.shape[0], key_cache.shape[1], width,
-            query.shape[1], key_cache.shape[2], query.shape[2])
+    return q[0], c[0], c[1], width, q[1], c[2], q[2]
 
 
 def window_attention_decode(key_lengths, page_table, query, key_cache,
@@ -843,22 +848,19 @@ def window_attention_decode(key_lengths, page_table, query, key_cache,
     shape = _cache_shapes(key_lengths, page_table, query, key_cache,
                           value_cache, output)
     dt = _value_dtype(query, "query")
-    _one_device(stream, key_lengths, page_table, query, key_cache, value_cache,
-                output)
-    q, o = _heads(query, dt, "query"), _heads(output, dt, "output")
-    k = _heads(key_cache, dt, "key_cache")
-    v = _heads(value_cache, dt, "value_cache")
-    lib = load_library()
-    need = lib.sw_window_attention_decode_workspace_bytes(
+    at = _device_of(stream)
+    (q, o, k, v), strides = _heads(dt, at, query, "query", output, "output",
+                                   key_cache, "key_cache", value_cache,
+                                   "value_cache")
+    need = load_library().sw_window_attention_decode_workspace_bytes(
         shape[0], *shape[2:], window, sinks)
-    lengths = _dev(key_lengths, torch.int32, "key_lengths")
+    lengths = _flat(key_lengths, torch.int32, at, "key_lengths")
     table = (None if page_table is None else
-             _dev(page_table, torch.int32, "page_table"))
+             _flat(page_table, torch.int32, at, "page_table"))
     scratch = _scratch(need, query, workspace, stream)
     _check(_fn("sw_window_attention_decode", dt)(
-        lengths, table, q[0], k[0], v[0], o[0], *shape,
-        (ctypes.c_int64 * 10)(*q[1:], *o[1:], *k[1:], *v[1:]), window, sinks,
-        alpha, None if scratch is None else scratch.data_ptr(), need,
+        lengths, table, q, k, v, o, *shape, strides, window, sinks, alpha,
+        None if scratch is None else scratch.data_ptr(), need,
         _stream(stream)))
     return output
 
@@ -879,26 +881,21 @@ def shared_prefix_attention(key_lengths, page_table, query, prefix_key,
           tuple(prefix_key.shape[1:]) == tuple(key_cache.shape[2:]),
           "expected prefix key and value [prefix_tokens, key_heads, d]")
     dt = _value_dtype(query, "query")
-    _one_device(stream, key_lengths, page_table, query, prefix_key,
-                prefix_value, key_cache, value_cache, output)
-    q, o = _heads(query, dt, "query"), _heads(output, dt, "output")
-    pk = _heads(prefix_key, dt, "prefix_key")
-    pv = _heads(prefix_value, dt, "prefix_value")
-    k = _heads(key_cache, dt, "key_cache")
-    v = _heads(value_cache, dt, "value_cache")
-    lib = load_library()
-    need = lib.sw_shared_prefix_attention_workspace_bytes(
+    at = _device_of(stream)
+    (q, o, k, v, pk, pv), strides = _heads(
+        dt, at, query, "query", output, "output", key_cache, "key_cache",
+        value_cache, "value_cache", prefix_key, "prefix_key", prefix_value,
+        "prefix_value")
+    need = load_library().sw_shared_prefix_attention_workspace_bytes(
         shape[0], prefix_key.shape[0], *shape[2:])
-    lengths = _dev(key_lengths, torch.int32, "key_lengths")
+    lengths = _flat(key_lengths, torch.int32, at, "key_lengths")
     table = (None if page_table is None else
-             _dev(page_table, torch.int32, "page_table"))
+             _flat(page_table, torch.int32, at, "page_table"))
     scratch = _scratch(need, query, workspace, stream)
     _check(_fn("sw_shared_prefix_attention", dt)(
-        lengths, table, q[0], pk[0], pv[0], k[0], v[0], o[0], shape[0],
-        prefix_key.shape[0], *shape[1:],
-        (ctypes.c_int64 * 14)(*q[1:], *o[1:], *k[1:], *v[1:], *pk[1:],
-                              *pv[1:]),
-        alpha, None if scratch is None else scratch.data_ptr(), need,
+        lengths, table, q, pk, pv, k, v, o, shape[0], prefix_key.shape[0],
+        *shape[1:], strides, alpha,
+        None if scratch is None else scratch.data_ptr(), need,
         _stream(stream)))
     return output
 

@@ -55,7 +55,8 @@ struct StepArgs {
   int chunk, parts, prefix_chunk, prefix_parts;
   int rows, prefix_rows; // of one part: a multiple of 16, of 16 or 128
   float *sums, *stats, *prefix_sums, *prefix_stats;
-  int64_t prefix_items; // workgroups of the prefix in window_cache_parts
+  // workgroups of the prefix: by cache_part and by prefix_part
+  int64_t prefix_items, wide_items;
 };
 
 // The keys that sequence i's query sees: the first `lead`, and those from
@@ -88,25 +89,34 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
 }
 
 // One chunk of keys against up to 16 query rows: 16 x 16 products of K Q^T, 32
-// keys a wave at a time, the next 32 on their way to registers meanwhile; V
-// goes through LDS to be read across its rows.  The four waves' results are
-// joined in LDS.
+// keys a wave at a time; V goes through LDS to be read across its rows.  The
+// four waves' results are joined in LDS.  The keys of a wave's next tile are
+// not fetched ahead: the registers hold another wave a SIMD instead, whose
+// fetches go on meanwhile (64 sequences, window 4096: 201 us with two waves
+// and fetches ahead, 195 us with three; four waves' registers spill, 306 us).
+template <typename T, int D> struct CacheParts {
+  using Tile = RowTile<T, D, kTile, kWave>;
+  static constexpr int kWaveBytes =
+      Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
+  static constexpr int kBytes = 4 * kWaveBytes;
+  static constexpr int kWaves = sizeof(T) * D > 256 ? 1 : 3;
+};
+struct Totals {
+  float top[4][kRows], sum[4][kRows];
+};
+
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, sizeof(T) * D > 256 ? 1 : 2) void
-window_cache_parts(StepArgs a) {
+__device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
+                                           char *lds, Totals &found) {
   using Tile = RowTile<T, D, kTile, kWave>;
   constexpr int kSteps = D / 32;  // products along d
   constexpr int kBlocks = D / 16; // output rows of 16
   constexpr int kPieces = Tile::kBytes / 1024;
   constexpr int kPieceRows = 1024 / Tile::kPitch;
-  constexpr int kWaveBytes =
-      Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
-  __shared__ __align__(1024) char lds[4][kWaveBytes];
-  __shared__ float tops[4][kRows], totals[4][kRows];
+  constexpr int kWaveBytes = CacheParts<T, D>::kWaveBytes;
 
   const int lane = lane_id(), g = lane >> 4, wave = wave_in_group();
   // ---- which rows, which keys
-  int64_t item = blockIdx.x;
   const bool shared = item < a.prefix_items;
   int hk, part, first_row, rows, total, v0, v1, seq = 0;
   float *sums, *stats;
@@ -246,14 +256,8 @@ window_cache_parts(StepArgs a) {
 
   bool some = false; // whether a key was there (wave-uniform)
   int v = v0 + wave * kTile;
-  Data now;
-  if (v < v1)
-    now = fetch(rows_of(v));
   while (v < v1) {
-    const int next = v + 4 * kTile;
-    Data then;
-    if (next < v1)
-      then = fetch(rows_of(next));
+    const Data now = fetch(rows_of(v));
     v4f score[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -313,8 +317,7 @@ window_cache_parts(StepArgs a) {
       acc[b] = mma16(vf, pf, acc[b]);
     }
     some |= ballot(((~now.none) & 0xFF) != 0) != 0;
-    now = then;
-    v = next;
+    v += 4 * kTile;
   }
   if (some && top == -kInf)
     top = kLowest;
@@ -322,8 +325,8 @@ window_cache_parts(StepArgs a) {
   // ---- the four waves' results, joined
   sum = rows16_sum(sum);
   if (g == 0) {
-    tops[wave][lane] = top;
-    totals[wave][lane] = sum;
+    found.top[wave][lane] = top;
+    found.sum[wave][lane] = sum;
   }
   // o[row][d] of each wave, in its own part of LDS
 #pragma unroll
@@ -334,19 +337,19 @@ window_cache_parts(StepArgs a) {
     const int r = x / (D / 4), c = x % (D / 4) * 4;
     if (r >= rows)
       break;
-    float m = tops[0][r];
+    float m = found.top[0][r];
 #pragma unroll
     for (int w = 1; w < 4; ++w)
-      m = fmaxf(m, tops[w][r]);
+      m = fmaxf(m, found.top[w][r]);
     float l = 0.0f;
     v4f o = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float by =
-          tops[w][r] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(tops[w][r] - m);
+          found.top[w][r] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(found.top[w][r] - m);
       const v4f y =
           lds_read<v4f>(lds_address(lds) + w * kWaveBytes + (r * D + c) * 4, 0);
-      l = fmaf(totals[w][r], by, l);
+      l = fmaf(found.sum[w][r], by, l);
       o += y * by;
     }
     if (only) {
@@ -368,6 +371,14 @@ window_cache_parts(StepArgs a) {
   }
 }
 
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (CacheParts<T, D>::kWaves)) void
+window_cache_parts(StepArgs a) {
+  __shared__ __align__(1024) char lds[CacheParts<T, D>::kBytes];
+  __shared__ Totals found;
+  cache_part<T, D>(a, blockIdx.x, lds, found);
+}
+
 // The prefix against many query rows: 128 rows, 32 a wave, and one chunk of
 // the prefix, in tiles of LDS that the four waves share; 32 x 32 products of
 // K Q^T as in the window's forward pass.
@@ -378,19 +389,18 @@ template <typename T, int D> struct Prefix {
   static constexpr int kBlocks = D / 32;
   static constexpr int kKeyBlocks = kTile / 32;
   static constexpr int kWaves = sizeof(T) * D > 256 ? 1 : 2;
+  static constexpr int kBytes = std::max(4 * Tile::kBytes,
+                                         CacheParts<T, D>::kBytes);
 };
 constexpr int kPrefixRows = 128;
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (Prefix<T, D>::kWaves)) void
-shared_prefix_parts(StepArgs a) {
+__device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
+                                            char *lds) {
   using F = Prefix<T, D>;
   using Tile = typename F::Tile;
   constexpr int KT = F::kTile;
-  __shared__ __align__(1024) char lds[2][2][Tile::kBytes];
 
-  // (the row tiles of a chunk next to each other on one XCD)
-  int64_t item = xcd_contiguous(blockIdx.x, gridDim.x);
   const int tiles = a.prefix_rows / kPrefixRows;
   const int first_row = (int)(item % tiles) * kPrefixRows;
   item /= tiles;
@@ -522,67 +532,83 @@ shared_prefix_parts(StepArgs a) {
   }
 }
 
-// Joins the parts of a query head's softmax: one wave for each, its halves
-// taking the parts in turn; DIM / 32 consecutive elements a lane.
+// Both kinds of parts in one launch, spread evenly among each other: the
+// prefix's multiply while the caches' are read (128 sequences behind 16,384
+// keys: 157 us and 44 us one after the other, 173 us together).
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (Prefix<T, D>::kWaves)) void
+shared_prefix_parts(StepArgs a) {
+  __shared__ __align__(1024) char lds[Prefix<T, D>::kBytes];
+  __shared__ Totals found;
+  const int64_t all = gridDim.x, prefix = a.wide_items;
+  const int64_t before = blockIdx.x * prefix / all;
+  if ((blockIdx.x + (int64_t)1) * prefix / all > before)
+    // (the row tiles of a chunk next to each other on one XCD)
+    prefix_part<T, D>(a, xcd_contiguous(before, prefix), lds);
+  else
+    cache_part<T, D>(a, blockIdx.x - before, lds, found);
+}
+
+// Joins the parts of a query head's softmax: one workgroup for each, whose
+// eight half waves take the parts in turn, DIM / 32 consecutive elements a
+// lane, and are joined in LDS.
 template <typename T, int DIM>
 __global__ __launch_bounds__(kThreads) void window_cache_join(StepArgs a) {
-  constexpr int N = DIM / 32;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / kWave) + wave_in_group();
-  if (item >= (int64_t)a.sequences * a.query_heads)
-    return;
-  const int seq = (int)(item / a.query_heads);
-  const int head = (int)(item % a.query_heads);
+  constexpr int N = DIM / 32, kHalves = kThreads / 32;
+  __shared__ float outs[kHalves][DIM], tops[kHalves], totals[kHalves];
+  const int seq = (int)(blockIdx.x / a.query_heads);
+  const int head = (int)(blockIdx.x % a.query_heads);
   const int hk = head / a.group, row = head % a.group;
   const Visible see(a, seq);
   const int own = see.count == 0 ? 0 : (see.count - 1) / a.chunk + 1;
   const int parts = own + a.prefix_parts;
-  // row of part i in the buffers of sums and statistics
-  auto at = [&](int i, const float *&sums, const float *&stats) {
-    int64_t r;
-    if (i < own) {
-      r = (((int64_t)seq * a.key_heads + hk) * a.parts + i) * a.rows + row;
-      sums = a.sums + r * DIM;
-      stats = a.stats + r * 2;
-    } else {
-      r = ((int64_t)hk * a.prefix_parts + i - own) * a.prefix_rows +
-          (int64_t)seq * a.group + row;
-      sums = a.prefix_sums + r * DIM;
-      stats = a.prefix_stats + r * 2;
-    }
-  };
-  const int lane = lane_id(), h = lane >> 5, c = (lane & 31) * N;
-  const float *sums, *stats;
-  float top = -kInf;
-  for (int i = lane; i < parts; i += kWave) {
-    at(i, sums, stats);
-    top = fmaxf(top, stats[0]);
-  }
-  top = rows16_max(top);
-#pragma unroll
-  for (int s = 8; s > 0; s >>= 1)
-    top = fmaxf(top, __shfl_xor(top, s));
-  float l = 0.0f, o[N] = {};
-  for (int i = h; i < parts; i += 2) {
-    at(i, sums, stats);
-    const float m = stats[0];
-    const float by = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    l = fmaf(stats[1], by, l);
+  const int half = threadIdx.x / 32, c = (threadIdx.x % 32) * N;
+  float top = -kInf, l = 0.0f, o[N] = {};
+#pragma unroll 4
+  for (int i = half; i < parts; i += kHalves) {
+    // row of part i in the buffers of sums and statistics
+    const int64_t r =
+        i < own ? (((int64_t)seq * a.key_heads + hk) * a.parts + i) * a.rows + row
+                : ((int64_t)hk * a.prefix_parts + i - own) * a.prefix_rows +
+                      (int64_t)seq * a.group + row;
+    const float *sums = (i < own ? a.sums : a.prefix_sums) + r * DIM + c;
+    const float *stats = (i < own ? a.stats : a.prefix_stats) + r * 2;
+    const float m = stats[0], to = fmaxf(top, m);
+    const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+    const float add = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    top = to;
+    l = fmaf(stats[1], add, l * by);
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      o[e] = fmaf(sums[c + e], by, o[e]);
+      o[e] = fmaf(sums[e], add, o[e] * by);
   }
-  l = both_halves_sum(l);
-  const float by = 1.0f / l;
-  T *out = static_cast<T *>(a.output) + seq * a.output_token +
-           head * a.output_head;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float x = both_halves_sum(o[e]);
-    if (h == 0 && c + e < a.d)
-      stv(out + c + e, top == -kInf ? 0.0f : x * by);
+  for (int e = 0; e < N; ++e)
+    outs[half][c + e] = o[e];
+  if (threadIdx.x % 32 == 0) {
+    tops[half] = top;
+    totals[half] = l;
   }
+  __syncthreads();
+  if (threadIdx.x >= a.d)
+    return;
+  top = tops[0];
+#pragma unroll
+  for (int i = 1; i < kHalves; ++i)
+    top = fmaxf(top, tops[i]);
+  float x = 0.0f;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kHalves; ++i) {
+    const float by =
+        tops[i] == top ? 1.0f : __builtin_amdgcn_exp2f(tops[i] - top);
+    l = fmaf(totals[i], by, l);
+    x = fmaf(outs[i][threadIdx.x], by, x);
+  }
+  stv(static_cast<T *>(a.output) + seq * a.output_token +
+          head * a.output_head + threadIdx.x,
+      top == -kInf ? 0.0f : x * (1.0f / l));
 }
-
 
 // ---- host ------------------------------------------------------------------------
 
@@ -613,8 +639,12 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
     const int64_t chunk = std::max(least, sw::ceil_div(n, parts));
     return std::min<int64_t>(sw::ceil_div(chunk, step) * step, 1 << 30);
   };
-  p.chunk = cut(visible, sequences * key_heads * (p.rows / kRows), 1024, 256,
-                128);
+  // Few keys are one part: a second one and the join of both cost more (one
+  // sequence, 260 keys: 6.1 + 3.5 us in two parts, 6.4 us in one).
+  p.chunk = visible <= 512
+                ? 512
+                : cut(visible, sequences * key_heads * (p.rows / kRows), 512,
+                      256, 128);
   p.parts = std::max<int64_t>(1, sw::ceil_div(visible, p.chunk));
   if (prefix_tokens > 0) {
     const int64_t rows = sequences * group;
@@ -622,7 +652,7 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
     const int64_t step = p.wide ? kPrefixRows : kRows;
     p.prefix_rows = sw::ceil_div(rows, step) * step;
     p.prefix_chunk = cut(prefix_tokens, key_heads * (p.prefix_rows / step),
-                         p.wide ? 512 : 1024, 256, 128);
+                         p.wide ? 256 : 1024, 256, 128);
     p.prefix_parts = sw::ceil_div(prefix_tokens, p.prefix_chunk);
   }
   if (p.parts == 1 && p.prefix_parts == 0)
@@ -775,26 +805,23 @@ int step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.prefix_stats = a.prefix_sums + p.prefix_sums;
   a.prefix_items = p.wide ? 0
                           : key_heads * (p.prefix_rows / kRows) * p.prefix_parts;
-  const int64_t grid =
-      a.prefix_items + sequences * key_heads * (p.rows / kRows) * p.parts;
-  const int64_t wide =
+  a.wide_items =
       p.wide ? key_heads * (p.prefix_rows / kPrefixRows) * p.prefix_parts : 0;
-  const int64_t join = sw::ceil_div(sequences * query_heads, kThreads / kWave);
-  if (int rc = sw::check_flat_grid(std::max({grid, wide, join}), kThreads, what))
+  const int64_t grid = a.prefix_items + a.wide_items +
+                       sequences * key_heads * (p.rows / kRows) * p.parts;
+  const int64_t join = sequences * query_heads;
+  if (int rc = sw::check_flat_grid(std::max(grid, join), kThreads, what))
     return rc;
   const hipStream_t st = sw::as_stream(stream);
-  if (p.wide) {
-    if (d <= 64)
-      shared_prefix_parts<T, 64><<<dim3((unsigned)wide), kThreads, 0, st>>>(a);
-    else
-      shared_prefix_parts<T, 128><<<dim3((unsigned)wide), kThreads, 0, st>>>(a);
-    if (int rc = sw::launch_check(what))
-      return rc;
-  }
-  if (d <= 64)
-    window_cache_parts<T, 64><<<dim3((unsigned)grid), kThreads, 0, st>>>(a);
+  const dim3 g((unsigned)grid);
+  if (p.wide && d <= 64)
+    shared_prefix_parts<T, 64><<<g, kThreads, 0, st>>>(a);
+  else if (p.wide)
+    shared_prefix_parts<T, 128><<<g, kThreads, 0, st>>>(a);
+  else if (d <= 64)
+    window_cache_parts<T, 64><<<g, kThreads, 0, st>>>(a);
   else
-    window_cache_parts<T, 128><<<dim3((unsigned)grid), kThreads, 0, st>>>(a);
+    window_cache_parts<T, 128><<<g, kThreads, 0, st>>>(a);
   if (int rc = sw::launch_check(what))
     return rc;
   if (p.parts == 1 && p.prefix_parts == 0)
