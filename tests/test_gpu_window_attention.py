@@ -42,7 +42,9 @@ def forward(qo, ko, q, k, v, alpha, window, sinks, fill=7.0):
     return out.cpu(), lse.cpu()
 
 
-def expect(qo, ko, q, k, v, out, lse, alpha, window, sinks, fill=7.0):
+def expect(qo, ko, q, k, v, out, lse, alpha, window, sinks, fill=7.0,
+           heads=None):
+    """Every head's results, or those of `heads`."""
     t = half_step(q.dtype)
     g = q.shape[1] // k.shape[1]
     qd, kd, vd = q.double(), k.double(), v.double()
@@ -51,7 +53,7 @@ def expect(qo, ko, q, k, v, out, lse, alpha, window, sinks, fill=7.0):
         a, b, c, e = int(qo[i]), int(qo[i + 1]), int(ko[i]), int(ko[i + 1])
         inside[a:b] = True
         see = visible(b - a, e - c, window, sinks)
-        for h in range(q.shape[1]):
+        for h in heads or range(q.shape[1]):
             o, ob, _, l, lb, _ = softmax(qd[a:b, h], kd[c:e, h // g],
                                          vd[c:e, h // g], see, alpha, t)
             check(f"output of sequence {i}, head {h}", out[a:b, h], o, ob)
@@ -95,14 +97,27 @@ def test_forward(dev, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_forward_many_heads(dev, dtype, case):
+    """The same with so many heads that a workgroup takes 128 rows, whose keys
+    are not shared out among its waves."""
+    (nq, nk), window, sinks = CASES[case]
+    say(f"window forward many heads {dtype} {CASES[case]}")
+    x = inputs(dtype, nq, nk, 288, 144, 64, seed=case)
+    out, lse = forward(*x, 0.125, window, sinks)
+    expect(*x, out, lse, 0.125, window, sinks, heads=[0, 131, 287])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("h,hk,d", [(1, 1, 8), (3, 3, 24), (6, 2, 64),
                                     (4, 1, 72), (2, 2, 96), (8, 2, 128),
-                                    (5, 1, 128)])
+                                    (5, 1, 128), (290, 145, 128)])
 def test_forward_heads(dev, dtype, h, hk, d):
     say(f"window forward heads {dtype} {h} {hk} {d}")
     x = inputs(dtype, [70, 131], [90, 131], h, hk, d, seed=d + h)
     out, lse = forward(*x, 1 / math.sqrt(d), 48, 5)
-    expect(*x, out, lse, 1 / math.sqrt(d), 48, 5)
+    expect(*x, out, lse, 1 / math.sqrt(d), 48, 5,
+           heads=None if h < 10 else [0, 3, h - 1])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -150,11 +165,12 @@ def test_forward_strides(dev, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("at", [0, 60, 100, 199])
-def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at):
+@pytest.mark.parametrize("heads", [2, 288])
+def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at, heads):
     """An infinity or NaN of one key and value reaches the queries that see
     it, and no others."""
-    say(f"window forward {bad} at {at} {dtype}")
-    qo, ko, q, k, v = inputs(dtype, [200], [200], 2, 2, 64, seed=at)
+    say(f"window forward {bad} at {at} {dtype} {heads}")
+    qo, ko, q, k, v = inputs(dtype, [200], [200], heads, heads, 64, seed=at)
     window, sinks = 50, 2
     sees = visible(200, 200, window, sinks)[:, at]
     clean, clean_lse = forward(qo, ko, q, k, v, 0.125, window, sinks)
@@ -162,8 +178,9 @@ def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at):
         kk, vv = k.clone(), v.clone()
         (vv if what == "value" else kk)[at, 1, 5] = bad
         out, lse = forward(qo, ko, q, kk, vv, 0.125, window, sinks)
-        expect(qo, ko, q[:, :1], kk[:, :1], vv[:, :1], out[:, :1], lse[:1],
-               0.125, window, sinks)
+        others = [i for i in range(heads) if i != 1]
+        assert torch.equal(out[:, others], clean[:, others])
+        assert torch.equal(lse[others], clean_lse[others])
         x, y = out[~sees, 1].float(), clean[~sees, 1].float()
         assert torch.isfinite(x).all()
         # (a repeated pass may add up in another order)
@@ -174,8 +191,8 @@ def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at):
             hit = out[sees, 1, 5].float()
             assert torch.isnan(hit).all() if math.isnan(bad) else \
                 (hit == bad).all()
-            others = torch.cat([out[sees, 1, :5], out[sees, 1, 6:]], 1)
-            assert torch.isfinite(others).all()
+            rest = torch.cat([out[sees, 1, :5], out[sees, 1, 6:]], 1)
+            assert torch.isfinite(rest).all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -225,7 +242,8 @@ def backward(qo, ko, q, k, v, do, alpha, window, sinks, fill=7.0):
 
 
 def expect_gradients(qo, ko, q, k, v, do, grads, alpha, window, sinks,
-                     fill=7.0):
+                     fill=7.0, heads=None):
+    """The gradients of every key head and its query heads, or of `heads`."""
     t = half_step(q.dtype)
     h, hk = q.shape[1], k.shape[1]
     g = h // hk
@@ -236,7 +254,7 @@ def expect_gradients(qo, ko, q, k, v, do, grads, alpha, window, sinks,
         a, b, c, e = int(qo[i]), int(qo[i + 1]), int(ko[i]), int(ko[i + 1])
         queries[a:b], keys[c:e] = True, True
         see = visible(b - a, e - c, window, sinks)
-        for j in range(hk):
+        for j in heads or range(hk):
             total = [torch.zeros(e - c, q.shape[2], dtype=torch.float64)
                      for _ in range(4)]
             for x in range(j * g, j * g + g):
@@ -272,15 +290,45 @@ def test_backward(dev, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_backward_many_heads(dev, dtype, case):
+    """The same with so many heads that neither rows nor keys are split."""
+    (nq, nk), window, sinks = CASES[case]
+    say(f"window backward many heads {dtype} {CASES[case]}")
+    x = inputs(dtype, nq, nk, 288, 144, 64, seed=case)
+    do = output_gradient(x)
+    grads = backward(*x, do, 0.125, window, sinks)
+    expect_gradients(*x, do, grads, 0.125, window, sinks, heads=[0, 77, 143])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window,sinks", [(300, 0), (300, 3), (64, 40)])
+def test_backward_parts(dev, dtype, window, sinks):
+    """Few keys and many query heads on each: the tiles of their queries are
+    split into parts, which end inside a head's tiles."""
+    say(f"window backward parts {dtype} {window} {sinks}")
+    x = inputs(dtype, [333, 0, 50], [350, 20, 50], 10, 1, 72, seed=12, lead=3,
+               tail=5)
+    need = sw.load_library().sw_window_attention_backward_workspace_bytes
+    one, many = (need(3, 391, 428, h, 1, 72, window, 0,
+                      4 if dtype == "f32" else 2) for h in (1, 10))
+    assert many - 10 * one > 2 * 4 * 428 * 2 * 72
+    do = output_gradient(x)
+    grads = backward(*x, do, 0.2, window, sinks)
+    expect_gradients(*x, do, grads, 0.2, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("h,hk,d", [(1, 1, 8), (3, 3, 24), (6, 2, 64),
                                     (4, 1, 72), (2, 2, 96), (8, 2, 128),
-                                    (5, 1, 128)])
+                                    (5, 1, 128), (290, 145, 128)])
 def test_backward_heads(dev, dtype, h, hk, d):
     say(f"window backward heads {dtype} {h} {hk} {d}")
     x = inputs(dtype, [70, 131], [90, 131], h, hk, d, seed=d + h)
     do = output_gradient(x)
     grads = backward(*x, do, 1 / math.sqrt(d), 48, 5)
-    expect_gradients(*x, do, grads, 1 / math.sqrt(d), 48, 5)
+    expect_gradients(*x, do, grads, 1 / math.sqrt(d), 48, 5,
+                     heads=None if h < 10 else [0, 100, hk - 1])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -363,12 +411,13 @@ def test_backward_strides(dev, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("what", ["query", "key", "value", "do"])
-def test_backward_keeps_what_is_masked_apart(dev, dtype, bad, what):
+@pytest.mark.parametrize("heads", [1, 288])
+def test_backward_keeps_what_is_masked_apart(dev, dtype, bad, what, heads):
     """An infinity or NaN at one token reaches the gradients of the tokens
     that it sees or that see it, and of those alone that share a query with
     them; the rest are those of clean operands."""
-    say(f"window backward {bad} in {what} {dtype}")
-    qo, ko, q, k, v = inputs(dtype, [260], [260], 1, 1, 64, seed=4)
+    say(f"window backward {bad} in {what} {dtype} {heads}")
+    qo, ko, q, k, v = inputs(dtype, [260], [260], heads, heads, 64, seed=4)
     do = output_gradient((qo, ko, q, k, v))
     window, sinks, at = 40, 2, 101
     clean = backward(qo, ko, q, k, v, do, 0.125, window, sinks)
@@ -385,8 +434,9 @@ def test_backward_keeps_what_is_masked_apart(dev, dtype, bad, what):
         rows = see[:, at].clone()
     cols = see[rows].any(0)
     for n, (x, c) in enumerate(zip(got, clean)):
+        assert torch.equal(x[:, 1:], c[:, 1:])
         free = ~rows if n == 0 else ~cols
-        x, c = x[free].float(), c[free].float()
+        x, c = x[free, 0].float(), c[free, 0].float()
         assert torch.isfinite(x).all()
         # (a repeated pass may add up in another order)
         assert (x - c).abs().max() <= 8 * half_step(q.dtype) * c.abs().max()
