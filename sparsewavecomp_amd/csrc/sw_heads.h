@@ -198,6 +198,23 @@ __device__ __forceinline__ void copy_words_to_lds(v4u buffer, uint32_t at,
                : "memory");
 }
 
+// For N products of this stretch of code, each with one LDS read of its own:
+// four reads first, then a product and a read in turn, so that a product waits
+// for a read of four before it.  (The compiler otherwise leaves two reads in
+// flight.)
+template <int N> __device__ __forceinline__ void schedule_reads() {
+  constexpr int kProduct = 0x8, kRead = 0x100, kAhead = 4;
+  if constexpr (N > kAhead) {
+    __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < N - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kProduct, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kProduct, kAhead, 0);
+  }
+}
+
 // ---- tiles of rows in LDS ----------------------------------------------------
 // Rows of D elements without padding, in chunks of 16 bytes; chunk c of row r
 // lies at place c ^ swizzle(r).  The swizzle keeps these reads free of bank

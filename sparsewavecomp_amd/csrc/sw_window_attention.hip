@@ -327,12 +327,14 @@ window_forward(WindowArgs a) {
     const bool all = keys.all(t, place_lo, place_hi, a.window, a.sinks);
     v16f score[N];
 #pragma unroll
-    for (int kb = 0; kb < N; ++kb) {
+    for (int kb = 0; kb < N; ++kb)
       score[kb] = v16f{};
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st)
+    for (int st = 0; st < F::kSteps; ++st)
+#pragma unroll
+      for (int kb = 0; kb < N; ++kb)
         score[kb] = mma32(Tile::along(kt, at, kb, st), q[st], score[kb]);
-    }
+    schedule_reads<sizeof(T) == 2 ? N * F::kSteps : 0>(); // (fp32: two reads each)
     uint32_t seen[N];
     if (!all) {
       // places before this lane's query (a sink tile's: any), and sinks left,
@@ -570,11 +572,10 @@ window_query_gradient(BackwardArgs b) {
     for (int kb = 0; kb < F::kKeyBlocks; ++kb) {
       v16f p = {}, ds = {};
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st)
+      for (int st = 0; st < F::kSteps; ++st) {
         p = mma32(Tile::along(kt, at, kb, st), q[st], p);
-#pragma unroll
-      for (int st = 0; st < F::kSteps; ++st)
         ds = mma32(Tile::along(vt, at, kb, st), go[st], ds);
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         ds[r] = __builtin_amdgcn_exp2f(fmaf(p[r], scale, -log2_sum)) *
@@ -820,10 +821,8 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
     at.fresh();
     v16f p = {}, ds = {};
 #pragma unroll
-    for (int st = 0; st < F::kSteps; ++st)
-      p = mma32(Tile::along(qt, at, 0, st), k[st], p);
-#pragma unroll
     for (int st = 0; st < F::kSteps; ++st) {
+      p = mma32(Tile::along(qt, at, 0, st), k[st], p);
       // (a tile of 128 rows has the lane's addresses of one of 32)
       if constexpr (SINK)
         ds = mma32(Tile::along(ot, at, 0, st), v[st], ds);
