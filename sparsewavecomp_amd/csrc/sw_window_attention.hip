@@ -1048,9 +1048,11 @@ window_sink_gradient(BackwardArgs b) {
     // query's place is at least a.window
     const int far = a.window - (s.nk - s.nq); // query of that place
     int x = far <= 0 ? 0 : far >> b.chunk_shift;
-    for (x += run; x < chunks && begin + x < b.chunks; x += kSinkRuns) {
-      if (far > s.nq - 1)
-        break;
+    if (far > s.nq - 1)
+      x = chunks; // (no query is past the window)
+    for (x += run; x < chunks; x += kSinkRuns) {
+      if (begin + x < 0 || begin + x >= b.chunks)
+        continue; // (offsets outside the operands)
       const float *y = b.sink_chunks +
                        ((int64_t)(begin + x) * a.key_heads + hk) * row + own;
       dk += y[0];

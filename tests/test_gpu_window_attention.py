@@ -502,3 +502,52 @@ def test_backward_refuses_a_short_workspace(dev):
         sw.window_attention_backward(
             qo, ko, q, k, v, q, lse, q, *g, 1.0, 4, 1,
             workspace=torch.zeros(16, dtype=torch.uint8, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_nothing_on_one_side(dev, dtype):
+    """No queries at all: keys' gradients of zero.  No keys: zeros and -inf.
+    No sequences: nothing is written."""
+    say(f"window empty sides {dtype}")
+    x = inputs(dtype, [0, 0], [5, 40], 2, 1, 64)
+    for window, sinks in ((10, 3), (100, 0)):
+        grads = backward(*x, torch.empty_like(x[2]), 0.1, window, sinks)
+        assert all((g == 0).all() for g in grads)
+    x = inputs(dtype, [5, 40], [0, 0], 2, 1, 64)
+    out, lse = forward(*x, 0.1, 10, 3)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    grads = backward(*x, output_gradient(x), 0.1, 10, 3)
+    assert (grads[0] == 0).all()
+    x = inputs(dtype, [5], [5], 2, 1, 64)
+    none = torch.zeros(1, dtype=torch.int32)
+    out, lse = forward(none, none, *x[2:], 0.1, 10, 3)
+    assert (out == 7).all() and (lse == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_offsets_outside_the_operands(dev, dtype):
+    """Offsets that lead outside are clamped: sequences in place keep their
+    results, and nothing outside the operands is touched."""
+    say(f"window bad offsets {dtype}")
+    x = inputs(dtype, [300, 200], [300, 200], 2, 1, 64, seed=3)
+    do = output_gradient(x)
+    good = backward(*x, do, 0.125, 64, 4)
+    bad = torch.tensor([0, 300, 2 ** 31 - 1], dtype=torch.int32)
+    got = backward(bad, bad, *x[2:], do, 0.125, 64, 4)
+    assert all(torch.equal(a, b) for a, b in zip(good, got))
+    for bad in ([-1000, 300, 500], [400, 100, 600], [-2 ** 31, 2 ** 31 - 1, 0]):
+        bad = torch.tensor(bad, dtype=torch.int32)
+        # rows of one projection, so that neighbours show what is written
+        wide = torch.full((500, 6, 64), 7.0, dtype=x[2].dtype, device=DEV)
+        wide[:, :2] = x[2].to(DEV)
+        off = bad.to(DEV)
+        lse = torch.full((2, 500), 7.0, device=DEV)
+        k, v = x[3].to(DEV), x[4].to(DEV)
+        sw.window_attention(off, off, wide[:, :2], k, v, wide[:, 2:4], lse,
+                            0.125, 64, 4)
+        g = torch.full((500, 5, 64), 7.0, dtype=x[2].dtype, device=DEV)
+        sw.window_attention_backward(off, off, wide[:, :2], k, v,
+                                     wide[:, 2:4], lse, do.to(DEV), g[:, :2],
+                                     g[:, 2:3], g[:, 3:4], 0.125, 64, 4)
+        torch.cuda.synchronize()
+        assert (wide[:, 4:] == 7).all() and (g[:, 4:] == 7).all()
