@@ -485,7 +485,8 @@ int sw_attention_tile_floor(const int32_t *row_offsets,
  * operands, so no contents of them reach outside.  An infinity or NaN of a
  * key or value changes those queries alone that see it.  fp32 arithmetic;
  * bf16 probabilities are rounded to bf16 for the matrix cores, their sum is
- * not.  No atomics: repeated calls give the same bits.
+ * not.  No atomics: repeated calls give the same bits.  The output shares no
+ * memory with the other operands.
  */
 int sw_window_attention_f32(
     const int32_t *query_offsets, const int32_t *key_offsets,
