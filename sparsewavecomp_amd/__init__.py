@@ -338,16 +338,23 @@ def _workspace(nbytes, like, stream):
     if (like.device.index != torch.cuda.current_device()
             or torch.cuda.is_current_stream_capturing()):
         return None
-    # A new allocation from the driver would invalidate a graph capture that
-    # another thread has under way, unless this thread's interaction mode is
-    # relaxed (2); nothing of this call belongs to that capture.
+    try:
+        return _allocate(nbytes, like)
+    except torch.cuda.OutOfMemoryError:
+        return None
+
+
+def _allocate(nbytes, like):
+    """Bytes of torch's allocator on like's device for the current stream.  A
+    new allocation from the driver would invalidate a graph capture that
+    another thread has under way, unless this thread's interaction mode is
+    relaxed (2); nothing of the call belongs to that capture."""
+    torch = _torch or _load_torch()
     exchange = load_library().hipThreadExchangeStreamCaptureMode
     mode = ctypes.c_int(2)
     exchange(ctypes.byref(mode))
     try:
         return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    except torch.cuda.OutOfMemoryError:
-        return None
     finally:
         exchange(ctypes.byref(mode))
 
@@ -764,8 +771,8 @@ def _scratch(nbytes, like, workspace, stream):
         if not isinstance(stream, torch.cuda.Stream):
             raise ValueError("a stream that is not torch's needs a workspace")
         with torch.cuda.stream(stream):
-            return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+            return _allocate(nbytes, like)
+    return _allocate(nbytes, like)
 
 
 def window_attention_backward(query_offsets, key_offsets, query, key, value,

@@ -2,6 +2,7 @@
 the GPU against float64, element by element within bounds that the arithmetic
 gives (tests/_window_check.py)."""
 import math
+import threading
 
 import pytest
 import torch
@@ -420,3 +421,60 @@ def test_decode_goes_on_from_a_prompt(dev):
             q[n - 1:n], *pages, out, 0.125, window, sinks)
         # both within fp32 sums of the same at most 53 terms of size 1
         assert (out[0] - whole[n - 1]).abs().max() <= 256 * 2.0 ** -24 * 4
+
+
+def test_scratch_while_another_thread_captures(dev):
+    """A backward pass and a step take their scratch memory also when the
+    allocator has to ask the driver for it while another thread captures a
+    graph, and leave that capture alone."""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    t, h, hk, d = 3000, 4, 2, 128
+    off = torch.tensor([0, t], dtype=torch.int32, device=DEV)
+    q, go = (torch.randn(t, h, d, generator=gen, device=DEV) for _ in "qo")
+    k, v = (torch.randn(t, hk, d, generator=gen, device=DEV) for _ in "kv")
+    lse = torch.empty(h, t, device=DEV)
+    out = sw.window_attention(off, off, q, k, v, torch.empty_like(q), lse,
+                              0.1, 100, 4)
+    n = off[1:]
+
+    def calls(b):
+        sw.window_attention_backward(off, off, q, k, v, out, lse, go, *b[:3],
+                                     0.1, 100, 4)
+        sw.window_attention_decode(n, None, q[:1], k[None], v[None], b[3], 0.1,
+                                   2000)
+    want, got = ([torch.zeros_like(x) for x in (q, k, v, q[:1])]
+                 for _ in "ab")
+    lib = sw.load_library()
+    assert lib.sw_window_attention_backward_workspace_bytes(
+        1, t, t, h, hk, d, 100, 4, 4) > 0
+    assert lib.sw_window_attention_decode_workspace_bytes(
+        1, t, 1, h, hk, d, 2000, 0) > 0
+    say("window attention while another thread captures")
+    calls(want)
+    a, b = torch.ones(1000, device=DEV), torch.empty(1000, device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()  # the next scratch memory is a new allocation
+    failed = []
+
+    def other():
+        try:
+            with torch.cuda.stream(side):
+                calls(got)
+        except Exception as e:  # noqa: BLE001 (reported below)
+            failed.append(e)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.mul(a, 3.0, out=b)
+        thread = threading.Thread(target=other)
+        thread.start()
+        thread.join(30)
+    assert not thread.is_alive() and not failed, failed
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    for _ in range(2):
+        b.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((b == 3.0).all())
