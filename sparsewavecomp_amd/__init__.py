@@ -689,10 +689,13 @@ def _heads(dtype, at, *named):
 
 
 def _device_of(stream):
-    """The device that a call on `stream` goes to."""
+    """The device that a call on `stream` goes to; a stream that is not
+    torch's may not name one, and is then taken to be of the current device."""
     torch = _torch or _load_torch()
-    return (torch.cuda.current_device() if stream is None
-            else stream.device.index) if torch.cuda.is_initialized() else -2
+    if not torch.cuda.is_initialized():
+        return -2
+    device = getattr(stream, "device", None)
+    return torch.cuda.current_device() if device is None else device.index
 
 
 def _flat(t, dtype, at, name):

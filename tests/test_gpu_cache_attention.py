@@ -478,3 +478,31 @@ def test_scratch_while_another_thread_captures(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert bool((b == 3.0).all())
+
+
+def test_a_stream_that_is_not_torchs(dev):
+    """Any object with a stream's handle will do where the caller gives the
+    workspace; without one the call is refused."""
+    class Handle:
+        cuda_stream = torch.cuda.Stream().cuda_stream
+
+    say("window attention on a bare handle")
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    k, v = (torch.randn(1, 1100, 2, 64, generator=gen, device=DEV)
+            for _ in "kv")
+    q = torch.randn(1, 4, 64, generator=gen, device=DEV)
+    n = torch.tensor([1100], dtype=torch.int32, device=DEV)
+    want, got = torch.empty_like(q), torch.zeros_like(q)
+    need = sw.load_library().sw_window_attention_decode_workspace_bytes(
+        1, 1100, 1, 4, 2, 64, 1000, 4)
+    assert need > 0
+    space = torch.empty(need, dtype=torch.uint8, device=DEV)
+    sw.window_attention_decode(n, None, q, k, v, want, 0.1, 1000, 4)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="needs a workspace"):
+        sw.window_attention_decode(n, None, q, k, v, got, 0.1, 1000, 4,
+                                   stream=Handle)
+    sw.window_attention_decode(n, None, q, k, v, got, 0.1, 1000, 4,
+                               workspace=space, stream=Handle)
+    torch.cuda.synchronize()
+    assert torch.equal(want, got)
