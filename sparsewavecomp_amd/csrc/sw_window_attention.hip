@@ -484,8 +484,11 @@ struct BackwardArgs {
   // those of the window, for each part and sequence, and of the queries past
   // it, for each chunk of 1 << chunk_shift queries
   float *sink_window, *sink_chunks;
-  float *part_sums; // [parts][key_tokens][key_heads][2][d], of two and more
-  int parts, key_tiles, chunks, chunk_shift;
+  float *part_sums; // [parts][split tiles][128][2][d]
+  // Tiles of keys of all key heads: `whole` of them a workgroup each, the
+  // `split` ones behind them `parts` each.
+  int key_tiles, whole, split, parts;
+  int chunks, chunk_shift;
   int sink_rows; // a multiple of 32
 };
 
@@ -675,8 +678,9 @@ window_query_gradient(BackwardArgs b) {
 // chunk of queries, its waves blocks of 32 queries in turn, each with tiles of
 // its own, and leaves its sums to window_sink_gradient.
 //
-// Where there are few keys, the tiles of their queries are split into `parts`,
-// one workgroup for each, whose sums window_key_join adds up.
+// Where there are few keys, or few behind a last full round of workgroups, the
+// tiles of their queries are split into `parts`, one workgroup for each, whose
+// sums window_key_join adds up.
 //
 // 16,384 tokens, window 1024, 16 bf16 heads of 128 over 4: 307 us, the matrix
 // cores 34 % busy with four products a tile of 32 queries and one barrier (with
@@ -713,7 +717,7 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
   int hk, i, key0, first, last; // keys from key0; queries first .. last
   Sequence s;
   int64_t item;
-  int part = 0;
+  int part = 0, parts = 1;
   if constexpr (SINK) {
     const int sink_blocks = b.sink_rows / 32;
     const int block = (int)(blockIdx.x % sink_blocks);
@@ -733,9 +737,14 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
     const int far = key0 + a.window - (s.nk - s.nq);
     first = far > first ? far : first;
   } else {
-    item = xcd_contiguous(blockIdx.x, gridDim.x);
-    part = (int)(item % b.parts);
-    item /= b.parts;
+    if ((int)blockIdx.x < b.whole) {
+      item = xcd_contiguous(blockIdx.x, b.whole);
+    } else {
+      item = xcd_contiguous(blockIdx.x - b.whole, gridDim.x - b.whole);
+      parts = b.parts;
+      part = (int)(item % parts);
+      item = b.whole + item / parts;
+    }
     const int tile = (int)(item % b.key_tiles);
     hk = (int)(item / b.key_tiles);
     i = sequence_of_tile(a.key_offsets, a.sequences, tile, kRowShift);
@@ -780,10 +789,10 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
   const uint32_t obytes = (uint32_t)(b.go.token * sizeof(T));
   const int tiles = last < first ? 0 : (last - first) / QT + 1;
   // tiles of all heads, and this part's
-  const int begin = SINK ? 0 : (int)((int64_t)tiles * group * part / b.parts);
+  const int begin = SINK ? 0 : (int)((int64_t)tiles * group * part / parts);
   const int count =
       (SINK ? tiles * group
-            : (int)((int64_t)tiles * group * (part + 1) / b.parts)) - begin;
+            : (int)((int64_t)tiles * group * (part + 1) / parts)) - begin;
   typename Tile::FewLane at;
   const uint32_t base =
       lds_address(lds) + (SINK ? wave * F::kParities * 2 * Tile::kBytes : 0);
@@ -977,14 +986,15 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
     return false;
   // A sink's sums wait for those of the queries past the window, and a part's
   // for the other parts'.
-  if (SINK || b.parts > 1 || key < a.sinks) {
+  if (SINK || parts > 1 || key < a.sinks) {
     float *out = SINK || key < a.sinks
                      ? (SINK ? b.sink_chunks : b.sink_window) +
                            (((SINK ? item : (int64_t)part * a.sequences + i) *
                                  a.key_heads + hk) * b.sink_rows + key) *
                                2 * a.d
-                     : b.part_sums + (((int64_t)part * a.key_tokens + s.k0 +
-                                       key) * a.key_heads + hk) * 2 * a.d;
+                     : b.part_sums + (((int64_t)part * b.split + item -
+                                       b.whole) * kRows + key - tile_key) *
+                                         2 * a.d;
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
 #pragma unroll
@@ -1083,7 +1093,10 @@ window_sink_gradient(BackwardArgs b) {
   if (run != 0 || c >= a.d)
     return;
   dk = dv = 0.0f;
-  for (int p = 0; p < b.parts; ++p) {
+  const int tile = (a.key_offsets[i] >> kRowShift) + i + (key >> kRowShift);
+  const int parts =
+      (int64_t)hk * b.key_tiles + tile < b.whole ? 1 : b.parts;
+  for (int p = 0; p < parts; ++p) {
     const float *x = b.sink_window + (((int64_t)p * a.sequences + i) *
                                           a.key_heads + hk) * row + own;
     dk += x[0];
@@ -1109,38 +1122,31 @@ __global__ __launch_bounds__(kThreads) void window_key_join(BackwardArgs b) {
   const WindowArgs &a = b.w;
   const int per_row = a.d / 4;
   const int64_t x = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = x / per_row;
+  const int64_t row = x / per_row; // of the split tiles
   const int c = (int)(x % per_row) * 4;
-  const int token = (int)(row / a.key_heads), hk = (int)(row % a.key_heads);
-  if (token >= a.key_tokens)
-    return;
-  // the sequence of the token: the last that starts at or before it
-  int lo = 0, n = a.sequences;
-  while (n > 1) {
-    const int half = n / 2;
-    if (a.key_offsets[lo + half] <= token) {
-      lo += half;
-      n -= half;
-    } else {
-      n = half;
-    }
-  }
-  const Sequence s = sequence(a, lo);
-  const int key = token - s.k0;
-  if (key < a.sinks || key >= s.nk)
-    return; // (a sink's, or of no sequence)
+  // (a tile has 128 rows of 2 and more threads: whole waves)
+  const int64_t item =
+      b.whole + __builtin_amdgcn_readfirstlane((int)(row >> kRowShift));
+  const int tile = (int)(item % b.key_tiles), hk = (int)(item / b.key_tiles);
+  const int i = sequence_of_tile(a.key_offsets, a.sequences, tile, kRowShift);
+  const Sequence s = sequence(a, i);
+  const int key0 = (tile - (a.key_offsets[i] >> kRowShift) - i) << kRowShift;
+  const int key = key0 + (int)(row & (kRows - 1));
+  if (key0 < 0 || key >= s.nk || key < a.sinks)
+    return; // (none, or a sink's)
+  const int64_t token = s.k0 + key;
   const float *p = b.part_sums + row * 2 * a.d + c;
-  const int64_t step = (int64_t)a.key_tokens * a.key_heads * 2 * a.d;
+  const int64_t step = (int64_t)b.split * kRows * 2 * a.d;
   v4f dk = {}, dv = {};
 #pragma unroll 4
   for (int i = 0; i < b.parts; ++i) {
     dk += ld4(p + i * step);
     dv += ld4(p + i * step + a.d);
   }
-  st4(static_cast<T *>(b.key_gradient) + (int64_t)token * b.gk.token +
+  st4(static_cast<T *>(b.key_gradient) + token * b.gk.token +
           hk * b.gk.head + c, dk[0] * a.alpha, dk[1] * a.alpha,
       dk[2] * a.alpha, dk[3] * a.alpha);
-  st4(static_cast<T *>(b.value_gradient) + (int64_t)token * b.gv.token +
+  st4(static_cast<T *>(b.value_gradient) + token * b.gv.token +
           hk * b.gv.head + c, dv[0], dv[1], dv[2], dv[3]);
 }
 
@@ -1275,7 +1281,7 @@ int forward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
 // queries' numbers, the sinks' sums, the parts' sums.
 struct Scratch {
   int64_t stats, sink_window, sink_chunks, part_sums; // floats of each
-  int64_t chunks;
+  int64_t chunks, whole, split;
   int parts, chunk_shift, sink_rows;
   int64_t bytes() const {
     return 4 * (2 * stats + sink_window + sink_chunks + part_sums);
@@ -1291,21 +1297,31 @@ Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
   // The chip holds 512 workgroups of 128 keys (256 of fp32 rows past 64).
   // Fewer are split until they are as many, as long as each part has eight
   // tiles of queries; a little more than half of them too, where a second part
-  // of at least 32 tiles is worth its sums.  4096 keys, window 1024, bf16 heads
+  // of at least 32 tiles is worth its sums.  So are those behind the last full
+  // round, unless they may be no more than the numbers between the sequences
+  // that hold no keys.  4096 keys, window 1024, bf16 heads
   // of 128, one part / the rule's: 8 heads over 4 (132 workgroups) 164 / 100 us
   // (3 parts; 4: 128 us), 24 over 8 (264) 243 / 200 (2), 12 over 12 (396)
-  // 115 (2 parts: 150).
+  // 115 (2 parts: 150).  The whole backward pass, window 1024 (fp32: 512), the
+  // last round unsplit / split: 17,000 keys, bf16 heads of 128, 16 over 4 (532)
+  // 702 / 573, 20,000 (628) 751 / 658, 16 over 16, 5120 keys (656) 231 / 219,
+  // 4608 (592) 190 / 199; fp32 heads of 64, 16 over 8, 9000 keys (568)
+  // 813 / 707; within the numbers without keys, 8192 (520) 579 / 617.
   const int64_t groups = ((key_tokens >> kRowShift) + sequences) * key_heads;
   const int64_t slots = elem == 4 && d > 64 ? 256 : 512;
+  int64_t tail = groups % slots;
+  if (groups > slots && tail <= sequences * key_heads)
+    tail = 0;
   const int64_t tiles = query_heads / key_heads *
                         (std::min({window, key_tokens, query_tokens}) + kRows) /
                         32;
-  int64_t parts = std::min(slots / std::max<int64_t>(groups, 1), tiles / 8);
-  if (parts == 1 && groups * 8 <= slots * 5 && tiles >= 64)
+  int64_t parts = tail == 0 ? 1 : std::min(slots / tail, tiles / 8);
+  if (parts == 1 && tail * 8 <= slots * 5 && tiles >= 64)
     parts = 2;
   c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(parts, 16));
-  if (c.parts > 1)
-    c.part_sums = c.parts * key_tokens * key_heads * 2 * d;
+  c.split = c.parts > 1 ? tail : 0;
+  c.whole = groups - c.split;
+  c.part_sums = c.split * c.parts * kRows * 2 * d;
   const int64_t s = window >= key_tokens ? 0 : std::min(sinks, key_tokens);
   if (s == 0)
     return c;
@@ -1333,10 +1349,9 @@ int launch_backward(BackwardArgs &b, hipStream_t st) {
   const int streams = choose_streams(a);
   const int64_t rows = (int64_t)a.tiles * a.query_heads;
   const int64_t sinks = (int64_t)b.chunks * a.key_heads * (b.sink_rows / 32);
-  const int64_t keys = (int64_t)b.key_tiles * a.key_heads * b.parts;
-  const int64_t part_rows = sw::ceil_div(
-      b.parts > 1 ? (int64_t)a.key_tokens * a.key_heads * (a.d / 4) : 0,
-      kThreads);
+  const int64_t keys = (int64_t)b.key_tiles * a.key_heads +
+                       (int64_t)b.split * (b.parts - 1);
+  const int64_t part_rows = (int64_t)b.split * kRows * (a.d / 4) / kThreads;
   const int64_t join = (int64_t)a.sequences * a.key_heads * a.sinks;
   if (int rc = sw::check_flat_grid(std::max({rows, sinks, keys, part_rows}),
                                    kThreads, what))
@@ -1437,6 +1452,8 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   b.sink_rows = c.sink_rows;
   b.part_sums = b.sink_chunks + c.sink_chunks;
   b.parts = c.parts;
+  b.whole = (int)c.whole;
+  b.split = (int)c.split;
   b.key_tiles = (int)((key_tokens >> kRowShift) + sequences);
   const hipStream_t st = sw::as_stream(stream);
   return d <= 64 ? launch_backward<T, 64>(b, st)

@@ -319,6 +319,24 @@ def test_backward_parts(dev, dtype, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("sinks", [0, 3])
+def test_backward_parts_of_the_last_tiles(dev, dtype, sinks):
+    """More tiles of keys than run at once: the last ones alone are split,
+    from the middle of a head on."""
+    say(f"window backward parts of the last tiles {dtype} {sinks}")
+    x = inputs(dtype, [1290, 10], [1290, 11], 104, 52, 72, seed=13, lead=2,
+               tail=3)
+    # 624 tiles, of which 512 are whole, 42 heads' and a part of the next's
+    parts, elem = (2, 4) if dtype == "f32" else (3, 2)
+    assert sw.load_library().sw_window_attention_backward_workspace_bytes(
+        2, 1305, 1306, 104, 52, 72, 300, 0, elem) == 4 * (
+            2 * 104 * 1305 + parts * 112 * 128 * 2 * 72)
+    do = output_gradient(x)
+    grads = backward(*x, do, 0.2, 300, sinks)
+    expect_gradients(*x, do, grads, 0.2, 300, sinks, heads=[0, 42, 51])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("h,hk,d", [(1, 1, 8), (3, 3, 24), (6, 2, 64),
                                     (4, 1, 72), (2, 2, 96), (8, 2, 128),
                                     (5, 1, 128), (290, 145, 128)])

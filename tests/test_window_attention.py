@@ -104,12 +104,20 @@ def test_backward_workspace_rule():
         4 * rows * (3 + 78 + 3)
     assert need(3, 99000, 100, 4, 2, 64, 99, 7, 2) == 2 * 4 * 99000 * 4 + \
         4 * rows * (3 + 386 + 3)
-    # parts of few keys: dk and dv of each
+    # parts of few keys: dk and dv of each, in tiles of 128 keys, one more for
+    # each sequence and head than there can be whole ones
+    tiles, row = 33 * 4, 4 * 2 * 128
     one = need(1, 4096, 4096, 8, 4, 128, 4096, 0, 2)
-    assert one == 2 * 4 * 8 * 4096 + 3 * 4 * 4096 * 4 * 2 * 128
+    assert one == 2 * 4 * 8 * 4096 + 3 * tiles * 128 * row
     assert need(1, 4096, 4096, 8, 4, 128, 4096, 0, 4) == \
-        2 * 4 * 8 * 4096 + 2 * 4 * 4096 * 4 * 2 * 128
+        2 * 4 * 8 * 4096 + 2 * tiles * 128 * row
     assert need(1, 4096, 4096, 12, 12, 128, 4096, 0, 2) == 2 * 4 * 12 * 4096
+    # those behind the last 512 tiles, but for the numbers without keys
+    assert need(1, 17000, 17000, 16, 4, 128, 1024, 0, 2) == \
+        2 * 4 * 16 * 17000 + 16 * (133 * 4 - 512) * 128 * row
+    for n in (1, 6):
+        assert need(n, 16384, 16384, 16, 4, 128, 1024, 0, 2) == \
+            2 * 4 * 16 * 16384
     # many sinks: at most the size of bf16 keys apart from a chunk a sequence
     # and the window's
     n = 1 << 20
