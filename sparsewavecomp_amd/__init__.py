@@ -679,11 +679,14 @@ def _heads(dtype, at, *named):
         if last != 1 and t.shape[-1] > 1:
             raise ValueError(f"{name} must have consecutive elements in its "
                              "last dimension")
-        # (the stride of a dimension of one is any number: a packed one)
+        # (the stride of a dimension of one is any number and is not used: one
+        # that the C functions take, whatever the other strides are)
         if t.shape[-2] == 1:
             head = t.shape[-1]
         if t.shape[-3] == 1:
-            row = t.shape[-2] * max(head, t.shape[-1])
+            row = t.shape[-1]
+        if page and t.shape[0] == 1:
+            page = [0]
         strides += [*page, row, head]
     return pointers, (ctypes.c_int64 * len(strides))(*strides)
 

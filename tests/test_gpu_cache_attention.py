@@ -228,6 +228,50 @@ def test_decode_strides(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_one_row_of_buffers_with_far_heads(dev, dtype):
+    """A batch of one whose query and output are a token of buffers with heads
+    before tokens, pages of one key and a prefix of one key laid out alike."""
+    say(f"one row, far heads {dtype}")
+    x = make(dtype, [5], 1, 4, 2, 64, seed=7, prefix=1)
+    t, far = DTYPES[dtype], (1 << 23) // 64 + 10
+
+    def apart(y):
+        """y [1, heads, d] as a token of a buffer [heads, far, d]."""
+        buf = torch.full((y.shape[1], far, 64), 7.0, dtype=t, device=DEV)
+        buf[:, 100:101] = y.transpose(0, 1).to(DEV)
+        return buf, buf[:, 100:101].transpose(0, 1)
+    _, query = apart(x["query"])
+    lengths, table = on_gpu(x, "lengths", "table")
+    caches = on_gpu(x, "key_cache", "value_cache")
+    # (pages, 1, heads, d) of (heads, pages, d)
+    caches = [c.transpose(0, 2).contiguous().transpose(0, 2) for c in caches]
+    buf, out = apart(torch.full((1, 4, 64), 7.0))
+    sw.window_attention_decode(lengths, table, query, *caches, out, 0.125, 3, 1)
+    assert torch.equal(out.cpu(), decode(x, 0.125, 3, 1))
+    assert (buf[:, :100] == 7).all() and (buf[:, 101:] == 7).all()
+    _, pk = apart(x["prefix_key"])
+    _, pv = apart(x["prefix_value"])
+    sw.shared_prefix_attention(lengths, table, query, pk, pv, *caches, out,
+                               0.125)
+    assert torch.equal(out.cpu(), prefixed(x, 0.125))
+    # a prompt of one token, and its gradients into such buffers
+    off = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    want = torch.empty(1, 4, 64, dtype=t, device=DEV)
+    lse = torch.empty(4, 1, device=DEV)
+    q, k, v = on_gpu(x, "query", "prefix_key", "prefix_value")
+    sw.window_attention(off, off, q, k, v, want, None, 0.125, 3, 1)
+    sw.window_attention(off, off, query, pk, pv, out, lse, 0.125, 3, 1)
+    assert torch.equal(out, want)
+    plain = [torch.empty_like(y) for y in (q, k, v)]
+    sw.window_attention_backward(off, off, q, k, v, want, lse, q, *plain,
+                                 0.125, 3, 1)
+    grads = [apart(torch.zeros(y.shape))[1] for y in (q, k, v)]
+    sw.window_attention_backward(off, off, query, pk, pv, out, lse, query,
+                                 *grads, 0.125, 3, 1)
+    assert all(torch.equal(a, b) for a, b in zip(grads, plain))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_decode_past_four_gib(dev, dtype):
     """Rows of a cache whose byte offsets pass 2^32, by a page stride over
     memory that no key lies in."""

@@ -171,3 +171,25 @@ def test_mirror_refuses():
         back(value_gradient=q)
     with pytest.raises(sw.ShapeError, match="log_sum"):
         back(log_sum=torch.zeros(4, 3))
+
+
+def test_strides_of_one_row():
+    """A single token of a buffer whose heads lie far apart: its row stride is
+    not used, and what the mirror passes for it is no reason to refuse."""
+    import torch
+    buf = torch.zeros(4, 1 << 17, 64, dtype=torch.bfloat16)
+    assert buf.stride(0) * 2 > 1 << 23
+    one = buf[:, 7:8].transpose(0, 1)
+    for heads in (4, 1):
+        _, strides = sw._heads(torch.bfloat16, -1, one[:, :heads], "query",
+                               one[:, :2], "key", one[:, :2], "value",
+                               one[:, :heads], "output")
+        rc, message = c_forward(strides, query_tokens=1, key_tokens=1,
+                                query_heads=heads, key_heads=min(heads, 2),
+                                query_offsets=A + 1)
+        # (refused for the offsets alone, behind the checks of all strides)
+        assert rc == -3 and "not aligned" in message
+    page = torch.zeros(3, 8, dtype=torch.bfloat16).as_strided(
+        (1, 2, 1, 8), (5, 8, 8, 1))
+    assert list(sw._heads(torch.bfloat16, -1, page, "key_cache", one,
+                          "query")[1]) == [0, 8, 8, 64, 1 << 23]
