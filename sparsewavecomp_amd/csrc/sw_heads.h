@@ -405,27 +405,34 @@ __device__ __forceinline__ void load_rows(Frag<T> (&f)[STEPS], const T *p,
 }
 
 // ---- packed sequences ----------------------------------------------------------
-// Sequence i of n holds tokens offsets[i] .. offsets[i + 1] - 1, and, cut into
-// tiles of 1 << shift tokens, the tile numbers (offsets[i] >> shift) + i up to
-// that of i + 1: at least as many as it has tiles, without a count of the
-// tiles before it.  Returns the sequence of tile number `tile`, which is
-// wave-uniform, by 64 probes a trip.
-__device__ __forceinline__ int sequence_of_tile(
-    const int32_t *__restrict__ offsets, int n, int tile, int shift) {
+// The last i of 0 .. n - 1 whose value(i) is at most x, 0 where none is; the
+// values do not fall.  x is wave-uniform and so is the result; 64 probes a trip.
+template <typename F>
+__device__ __forceinline__ int last_at_most(int n, int x, F value) {
   const int l = lane_id();
   int from = 0, count = n; // the answer lies in [from, from + count)
   while (count > 1) {
     const int step = (count + kWave - 1) / kWave;
     const int at = from + l * step;
     const bool in = l * (int64_t)step < count;
-    const int32_t first = (offsets[in ? at : from] >> shift) + (in ? at : from);
-    // (probe 0 is at or before the tile: `from` starts there)
-    const uint64_t before = ballot(in && first <= tile);
+    const int first = value(in ? at : from);
+    // (probe 0 is at or before the answer: `from` starts there)
+    const uint64_t before = ballot(in && first <= x);
     const int k = before ? 63 - __builtin_clzll(before) : 0;
     count = count - k * step < step ? count - k * step : step;
     from += k * step;
   }
   return __builtin_amdgcn_readfirstlane(from);
+}
+
+// Sequence i of n holds tokens offsets[i] .. offsets[i + 1] - 1, and, cut into
+// tiles of 1 << shift tokens, the tile numbers (offsets[i] >> shift) + i up to
+// that of i + 1: at least as many as it has tiles, without a count of the
+// tiles before it.  Returns the sequence of tile number `tile`.
+__device__ __forceinline__ int sequence_of_tile(
+    const int32_t *__restrict__ offsets, int n, int tile, int shift) {
+  return last_at_most(n, tile,
+                      [&](int i) { return (offsets[i] >> shift) + i; });
 }
 
 } // namespace swd

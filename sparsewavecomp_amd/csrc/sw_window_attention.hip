@@ -480,17 +480,50 @@ struct BackwardArgs {
   void *query_gradient, *key_gradient, *value_gradient;
   Operand go, gq, gk, gv;
   float *log2_sum, *delta; // [query_heads][query_tokens], of the first kernel
-  // sums of the sinks' gradients in fp32, [..][key_heads][sink_rows][2][d]:
-  // those of the window, for each part and sequence, and of the queries past
-  // it, for each chunk of 1 << chunk_shift queries
+  // Sums of the far sinks' gradients in fp32, [..][key_heads][32][2][d]: those
+  // of the window for each block of 32 keys, and those of the queries past it,
+  // for each block the ones of its sequence's first 1 << chunk_shift queries,
+  // and behind them each later chunk's, sink_blocks of each.
   float *sink_window, *sink_chunks;
   float *part_sums; // [parts][split tiles][128][2][d]
   // Tiles of keys of all key heads: `whole` of them a workgroup each, the
   // `split` ones behind them `parts` each.
   int key_tiles, whole, split, parts;
   int chunks, chunk_shift;
-  int sink_rows; // a multiple of 32
+  int far_blocks, sink_blocks; // blocks of all sequences, and the most of one
+  int far_unit; // 0: far blocks are numbered by sequence; else window + 1
+  bool far_by_key;
+  int join_rows; // workgroups of window_sink_gradient for a block
 };
+
+// A sequence's far sinks, those that a query sees from past its window: its
+// first ones, as its last query stands at place nk - 1.
+__device__ __forceinline__ int far_sinks(const WindowArgs &a,
+                                         const Sequence &s) {
+  const int n = s.nk - a.window < a.sinks ? s.nk - a.window : a.sinks;
+  return n > 0 ? n : 0;
+}
+// The number of the first of a sequence's blocks of 32 far sinks, without a
+// count of those before it.  Its u is its own among the sequences that have
+// far sinks: its number, or, as these hold more than `window` keys each, its
+// first key over window + 1.  A sequence's blocks are those from u sink_blocks
+// on, or, by its first key, those from k0 / 32 + u on: fewer than 1 + f / 32
+// of f far sinks, and k0 + f is at most the next one's first key.
+__device__ __forceinline__ int first_far_block(const BackwardArgs &b, int i,
+                                               int k0) {
+  const int u = b.far_unit ? k0 / b.far_unit : i;
+  return b.far_by_key ? (k0 >> 5) + u : u * b.sink_blocks;
+}
+// The sequence that far block n belongs to, where it belongs to one.
+__device__ __forceinline__ int sequence_of_far_block(const BackwardArgs &b,
+                                                     int n) {
+  if (!b.far_unit && !b.far_by_key)
+    return n / b.sink_blocks;
+  return last_at_most(b.w.sequences, n, [&](int i) {
+    return first_far_block(
+        b, i, clamped(b.w.key_offsets[i], 0, b.w.key_tokens));
+  });
+}
 
 // dq of a tile of rows, and for the second kernel log_sum in powers of two
 // and delta of its rows.  The forward pass's loop with one product more:
@@ -674,7 +707,7 @@ window_query_gradient(BackwardArgs b) {
 // the sums, are more than two waves a SIMD have.
 //
 // The queries past the window that see the sinks are as many as the sequence
-// has, so they are split (SINK): a workgroup of those takes 32 sinks and a
+// has, so they are split (SINK): a workgroup of those takes 32 far sinks and a
 // chunk of queries, its waves blocks of 32 queries in turn, each with tiles of
 // its own, and leaves its sums to window_sink_gradient.
 //
@@ -715,27 +748,41 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
   const int lane = lane_id(), h = lane >> 5, wave = wave_in_group();
   const int group = a.query_heads / a.key_heads;
   int hk, i, key0, first, last; // keys from key0; queries first .. last
+  int far; // the sequence's far sinks
   Sequence s;
   int64_t item;
   int part = 0, parts = 1;
   if constexpr (SINK) {
-    const int sink_blocks = b.sink_rows / 32;
-    const int block = (int)(blockIdx.x % sink_blocks);
-    item = blockIdx.x / sink_blocks;
-    hk = (int)(item % a.key_heads);
-    item /= a.key_heads; // the chunk
-    i = sequence_of_tile(a.query_offsets, a.sequences, (int)item, b.chunk_shift);
-    s = sequence(a, i);
-    const int row0 = ((int)item - (a.query_offsets[i] >> b.chunk_shift) - i)
-                     << b.chunk_shift;
-    key0 = 32 * block;
-    first = row0;
-    last = row0 + (1 << b.chunk_shift) - 1;
-    last = last < s.nq - 1 ? last : s.nq - 1;
-    if (row0 < 0 || last < first || last + s.nk - s.nq < a.window)
-      return false; // (no query, or none past the window: the sum leaves it out)
-    const int far = key0 + a.window - (s.nk - s.nq);
-    first = far > first ? far : first;
+    hk = (int)(blockIdx.x % a.key_heads);
+    item = blockIdx.x / a.key_heads; // the block of sums
+    int chunk = 0, least = 0;        // of the sequence's queries
+    if (item < b.far_blocks) {
+      i = sequence_of_far_block(b, (int)item);
+      s = sequence(a, i);
+      key0 = ((int)item - first_far_block(b, i, s.k0)) * 32;
+    } else {
+      // Later chunks of sequence i have the numbers from q0 >> chunk_shift on:
+      // no more than whole chunks in its queries.
+      const int x = (int)((item - b.far_blocks) / b.sink_blocks);
+      key0 = (int)((item - b.far_blocks) % b.sink_blocks) * 32;
+      i = last_at_most(a.sequences, x, [&](int j) {
+        return clamped(a.query_offsets[j], 0, a.query_tokens) >> b.chunk_shift;
+      });
+      s = sequence(a, i);
+      chunk = x - (s.q0 >> b.chunk_shift) + 1;
+      least = 1;
+    }
+    far = far_sinks(a, s);
+    if (key0 < 0 || key0 >= far || chunk < least ||
+        chunk > (s.nq - 1) >> b.chunk_shift)
+      return false; // (none)
+    first = chunk << b.chunk_shift;
+    last = s.nq - 1 - first < 1 << b.chunk_shift
+               ? s.nq - 1 : first + (1 << b.chunk_shift) - 1;
+    if (last + s.nk - s.nq < a.window)
+      return false; // (no query past the window: the sum leaves it out)
+    const int past = key0 + a.window - (s.nk - s.nq);
+    first = past > first ? past : first;
   } else {
     if ((int)blockIdx.x < b.whole) {
       item = xcd_contiguous(blockIdx.x, b.whole);
@@ -749,6 +796,7 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
     hk = (int)(item / b.key_tiles);
     i = sequence_of_tile(a.key_offsets, a.sequences, tile, kRowShift);
     s = sequence(a, i);
+    far = far_sinks(a, s);
     key0 = (tile - (a.key_offsets[i] >> kRowShift) - i) << kRowShift;
     if (key0 < 0 || key0 >= s.nk)
       return false;
@@ -762,7 +810,7 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
     key0 += 32 * wave;
   const int shift = s.nk - s.nq;
   const int key = key0 + (lane & 31);
-  const bool live = key < s.nk && (!SINK || key < a.sinks);
+  const bool live = key < (SINK ? far : s.nk);
 
   const bool tiny = fabsf(a.alpha) < 0x1p-126f;
   const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
@@ -842,7 +890,7 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
       return; // hidden
     const bool all =
         lo + 31 <= last &&
-        (SINK ? lo + shift - (key0 + 31) >= a.window && key0 + 32 <= a.sinks
+        (SINK ? lo + shift - (key0 + 31) >= a.window && key0 + 32 <= far
               : lo + shift >= key0 + 31 && lo + 31 + shift - key0 < a.window);
     at.fresh();
     v16f p = {}, ds = {};
@@ -984,17 +1032,20 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
   }
   if (!live)
     return false;
-  // A sink's sums wait for those of the queries past the window, and a part's
-  // for the other parts'.
-  if (SINK || parts > 1 || key < a.sinks) {
-    float *out = SINK || key < a.sinks
-                     ? (SINK ? b.sink_chunks : b.sink_window) +
-                           (((SINK ? item : (int64_t)part * a.sequences + i) *
-                                 a.key_heads + hk) * b.sink_rows + key) *
-                               2 * a.d
-                     : b.part_sums + (((int64_t)part * b.split + item -
-                                       b.whole) * kRows + key - tile_key) *
-                                         2 * a.d;
+  // A part's sums wait for the other parts', and a far sink's for those of the
+  // queries past the window.
+  if (SINK || parts > 1 || key < far) {
+    float *out;
+    if (SINK)
+      out = b.sink_chunks +
+            ((item * a.key_heads + hk) * 32 + key - tile_key) * 2 * a.d;
+    else if (parts > 1)
+      out = b.part_sums + (((int64_t)part * b.split + item - b.whole) * kRows +
+                           key - tile_key) * 2 * a.d;
+    else
+      out = b.sink_window +
+            (((int64_t)(first_far_block(b, i, s.k0) + (key >> 5)) *
+                  a.key_heads + hk) * 32 + (key & 31)) * 2 * a.d;
 #pragma unroll
     for (int c = 0; c < F::kBlocks; ++c)
 #pragma unroll
@@ -1049,72 +1100,84 @@ window_key_gradient(BackwardArgs b) {
         &verdict);
 }
 
-// The sinks' gradients: the window's sums and every chunk's, in the same order
-// each time: eight runs of chunks, then the runs.  One workgroup of 128 x 8
-// threads for a sink of one sequence and key head; a launch and its trips to
-// the sums: 64 chunks of 6 sequences, 4 sinks of 4 heads 4.4 us.
+// The far sinks' gradients: the window's sums, or its parts', and every chunk's,
+// in the same order each time: eight runs of chunks, then the runs.  A workgroup
+// of 128 x 8 threads takes a block's far sinks of one key head in turns of
+// join_rows; a launch and its trips to the sums: 64 chunks of 6 sequences, 4
+// sinks of 4 heads 4.4 us.
 constexpr int kSinkRuns = 8;
 template <typename T>
 __global__ __launch_bounds__(128 * kSinkRuns) void
 window_sink_gradient(BackwardArgs b) {
   const WindowArgs &a = b.w;
   __shared__ float sums[2][kSinkRuns][128];
-  const int key = blockIdx.x % a.sinks;
-  const int hk = blockIdx.x / a.sinks % a.key_heads;
-  const int i = blockIdx.x / a.sinks / a.key_heads;
+  const int turn = blockIdx.x % b.join_rows;
+  const int64_t item = blockIdx.x / b.join_rows;
+  const int hk = (int)(item % a.key_heads);
+  const int block = (int)(item / a.key_heads);
+  const int i = sequence_of_far_block(b, block);
   const Sequence s = sequence(a, i);
-  if (key >= s.nk)
+  const int key0 = (block - first_far_block(b, i, s.k0)) * 32;
+  const int far = far_sinks(a, s);
+  if (key0 < 0 || key0 >= far)
     return;
+  const int end = far < key0 + 32 ? far : key0 + 32;
   const int run = threadIdx.x >> 7, c = threadIdx.x & 127;
-  const int64_t row = (int64_t)b.sink_rows * 2 * a.d;
-  const int64_t own = (int64_t)key * 2 * a.d + c;
-  float dk = 0.0f, dv = 0.0f;
-  if (c < a.d) {
-    const int begin = (a.query_offsets[i] >> b.chunk_shift) + i;
-    const int chunks = s.nq == 0 ? 0 : ((s.nq - 1) >> b.chunk_shift) + 1;
-    // chunks that reach past the window: those from the first whose last
-    // query's place is at least a.window
-    const int far = a.window - (s.nk - s.nq); // query of that place
-    int x = far <= 0 ? 0 : far >> b.chunk_shift;
-    if (far > s.nq - 1)
-      x = chunks; // (no query is past the window)
-    for (x += run; x < chunks; x += kSinkRuns) {
-      if (begin + x < 0 || begin + x >= b.chunks)
-        continue; // (offsets outside the operands)
-      const float *y = b.sink_chunks +
-                       ((int64_t)(begin + x) * a.key_heads + hk) * row + own;
-      dk += y[0];
-      dv += y[a.d];
-    }
-  }
-  sums[0][run][c] = dk;
-  sums[1][run][c] = dv;
-  __syncthreads();
-  if (run != 0 || c >= a.d)
-    return;
-  dk = dv = 0.0f;
-  const int tile = (a.key_offsets[i] >> kRowShift) + i + (key >> kRowShift);
-  const int parts =
-      (int64_t)hk * b.key_tiles + tile < b.whole ? 1 : b.parts;
-  for (int p = 0; p < parts; ++p) {
-    const float *x = b.sink_window + (((int64_t)p * a.sequences + i) *
-                                          a.key_heads + hk) * row + own;
-    dk += x[0];
-    dv += x[a.d];
-  }
+  // chunks that reach past the window: those from the first whose last query's
+  // place is at least a.window
+  const int chunks = s.nq == 0 ? 0 : ((s.nq - 1) >> b.chunk_shift) + 1;
+  const int past = a.window - (s.nk - s.nq); // query of that place
+  int begin = past <= 0 ? 0 : past >> b.chunk_shift;
+  if (past > s.nq - 1)
+    begin = chunks; // (no query is past the window)
+  // block of chunk 1's sums (chunk 0's is this one), and from chunk to chunk
+  const int64_t later = b.far_blocks + (key0 >> 5) +
+                        (int64_t)(s.q0 >> b.chunk_shift) * b.sink_blocks;
+  for (int key = key0 + turn; key < end; key += b.join_rows) {
+    const int64_t row = (int64_t)hk * 32 + (key - key0);
+    const int64_t pitch = (int64_t)a.key_heads * 32; // rows of a block
+    float dk = 0.0f, dv = 0.0f;
+    if (c < a.d)
+      for (int x = begin + run; x < chunks; x += kSinkRuns) {
+        const int64_t from =
+            x == 0 ? block : later + (int64_t)(x - 1) * b.sink_blocks;
+        const float *y = b.sink_chunks + (from * pitch + row) * 2 * a.d + c;
+        dk += y[0];
+        dv += y[a.d];
+      }
+    sums[0][run][c] = dk;
+    sums[1][run][c] = dv;
+    __syncthreads();
+    const int tile = (a.key_offsets[i] >> kRowShift) + i + (key >> kRowShift);
+    if (run == 0 && c < a.d && tile >= 0 && tile < b.key_tiles) {
+      // (tiles elsewhere: offsets outside the operands)
+      const int64_t at = (int64_t)hk * b.key_tiles + tile - b.whole;
+      const bool split = at >= 0;
+      const float *x = split ? b.part_sums + (at * kRows + (key & (kRows - 1))) *
+                                                 2 * a.d
+                             : b.sink_window + (block * pitch + row) * 2 * a.d;
+      const int64_t step = (int64_t)b.split * kRows * 2 * a.d;
+      dk = dv = 0.0f;
+      for (int p = 0; p < (split ? b.parts : 1); ++p) {
+        dk += x[p * step + c];
+        dv += x[p * step + a.d + c];
+      }
 #pragma unroll
-  for (int r = 0; r < kSinkRuns; ++r) {
-    dk += sums[0][r][c];
-    dv += sums[1][r][c];
+      for (int r = 0; r < kSinkRuns; ++r) {
+        dk += sums[0][r][c];
+        dv += sums[1][r][c];
+      }
+      const int64_t token = s.k0 + key;
+      stv(static_cast<T *>(b.key_gradient) + token * b.gk.token +
+              hk * b.gk.head + c, dk * a.alpha);
+      stv(static_cast<T *>(b.value_gradient) + token * b.gv.token +
+              hk * b.gv.head + c, dv);
+    }
+    __syncthreads();
   }
-  const int64_t token = s.k0 + key;
-  stv(static_cast<T *>(b.key_gradient) + token * b.gk.token + hk * b.gk.head + c,
-      dk * a.alpha);
-  stv(static_cast<T *>(b.value_gradient) + token * b.gv.token +
-          hk * b.gv.head + c, dv);
 }
 
-// The sums of the parts of the keys that are no sinks, in order: four elements
+// The sums of the parts of the keys that are no far sinks, in order: four elements
 // of a key and head a thread.  A launch and a trip, then memory: 3,001 tokens
 // of 2 heads of 80 in 5 parts 5.5 us.
 template <typename T>
@@ -1132,8 +1195,8 @@ __global__ __launch_bounds__(kThreads) void window_key_join(BackwardArgs b) {
   const Sequence s = sequence(a, i);
   const int key0 = (tile - (a.key_offsets[i] >> kRowShift) - i) << kRowShift;
   const int key = key0 + (int)(row & (kRows - 1));
-  if (key0 < 0 || key >= s.nk || key < a.sinks)
-    return; // (none, or a sink's)
+  if (key0 < 0 || key >= s.nk || key < far_sinks(a, s))
+    return; // (none, or a far sink's)
   const int64_t token = s.k0 + key;
   const float *p = b.part_sums + row * 2 * a.d + c;
   const int64_t step = (int64_t)b.split * kRows * 2 * a.d;
@@ -1281,8 +1344,9 @@ int forward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
 // queries' numbers, the sinks' sums, the parts' sums.
 struct Scratch {
   int64_t stats, sink_window, sink_chunks, part_sums; // floats of each
-  int64_t chunks, whole, split;
-  int parts, chunk_shift, sink_rows;
+  int64_t chunks, whole, split, far_blocks, sink_blocks, far_unit;
+  int parts, chunk_shift, join_rows;
+  bool far_by_key;
   int64_t bytes() const {
     return 4 * (2 * stats + sink_window + sink_chunks + part_sums);
   }
@@ -1322,23 +1386,44 @@ Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
   c.split = c.parts > 1 ? tail : 0;
   c.whole = groups - c.split;
   c.part_sums = c.split * c.parts * kRows * 2 * d;
-  const int64_t s = window >= key_tokens ? 0 : std::min(sinks, key_tokens);
+  // A sequence's far sinks: no more than its keys but `window`.
+  const int64_t s =
+      window >= key_tokens ? 0 : std::min(sinks, key_tokens - window);
   if (s == 0)
     return c;
-  c.sink_rows = (int)sw::ceil_div(s, 32) * 32;
-  // 256 queries a chunk, more where there are more than 64 sinks: the sums
-  // then stay below the size of bf16 keys; fewer, to 64, where that makes
-  // fewer workgroups than the chip has units.
+  // Their blocks by sequence, which needs no search, unless that makes more
+  // rows than there are keys: sequences that are shorter than the sinks are
+  // many, or few hold more than `window` keys.
+  c.sink_blocks = sw::ceil_div(s, 32);
+  c.far_blocks = sequences * c.sink_blocks;
+  if (c.far_blocks * 32 > key_tokens) {
+    const int64_t units = key_tokens / (window + 1);
+    c.far_unit = units < sequences ? window + 1 : 0;
+    const int64_t by_unit = std::min(sequences, units) * c.sink_blocks;
+    const int64_t by_key =
+        (key_tokens - window) / 32 + std::min(sequences, units);
+    c.far_by_key = by_key < by_unit;
+    c.far_blocks = std::min(by_key, by_unit);
+  }
+  // 256 queries a chunk, more where there are more than 64 sinks: the sums of
+  // all but the sequences' first chunks then have at most a row for four
+  // queries, the size of bf16 keys; fewer, to 64, where that makes fewer
+  // workgroups than the chip has units.
   c.chunk_shift = 8;
-  while (((int64_t)64 << (c.chunk_shift - 8)) < s)
+  while (((int64_t)64 << (c.chunk_shift - 8)) < s && c.chunk_shift < 30)
     ++c.chunk_shift;
-  while (c.chunk_shift > 6 && (query_tokens >> c.chunk_shift) * key_heads *
-                                      (c.sink_rows / 32) < 256)
+  while (c.chunk_shift > 6 &&
+         ((query_tokens >> c.chunk_shift) * c.sink_blocks + c.far_blocks) *
+                 key_heads < 256)
     --c.chunk_shift;
-  c.chunks = (query_tokens >> c.chunk_shift) + sequences;
-  const int64_t one = key_heads * c.sink_rows * 2 * d;
-  c.sink_window = c.parts * sequences * one;
-  c.sink_chunks = c.chunks * one;
+  c.chunks = query_tokens >> c.chunk_shift;
+  // one far sink a workgroup of the join, more where there are many
+  c.join_rows = (int)std::min<int64_t>(
+      std::min<int64_t>(s, 32),
+      sw::ceil_div(2048, c.far_blocks * key_heads));
+  const int64_t one = key_heads * 32 * 2 * d;
+  c.sink_window = c.far_blocks * one;
+  c.sink_chunks = (c.far_blocks + c.chunks * c.sink_blocks) * one;
   return c;
 }
 
@@ -1348,11 +1433,12 @@ int launch_backward(BackwardArgs &b, hipStream_t st) {
   const char *what = "window attention's gradient";
   const int streams = choose_streams(a);
   const int64_t rows = (int64_t)a.tiles * a.query_heads;
-  const int64_t sinks = (int64_t)b.chunks * a.key_heads * (b.sink_rows / 32);
+  const int64_t sinks =
+      (b.far_blocks + (int64_t)b.chunks * b.sink_blocks) * a.key_heads;
   const int64_t keys = (int64_t)b.key_tiles * a.key_heads +
                        (int64_t)b.split * (b.parts - 1);
   const int64_t part_rows = (int64_t)b.split * kRows * (a.d / 4) / kThreads;
-  const int64_t join = (int64_t)a.sequences * a.key_heads * a.sinks;
+  const int64_t join = (int64_t)b.far_blocks * a.key_heads * b.join_rows;
   if (int rc = sw::check_flat_grid(std::max({rows, sinks, keys, part_rows}),
                                    kThreads, what))
     return rc;
@@ -1449,7 +1535,11 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   b.sink_chunks = b.sink_window + c.sink_window;
   b.chunks = (int)c.chunks;
   b.chunk_shift = c.chunk_shift;
-  b.sink_rows = c.sink_rows;
+  b.far_blocks = (int)c.far_blocks;
+  b.sink_blocks = (int)c.sink_blocks;
+  b.far_unit = (int)c.far_unit;
+  b.far_by_key = c.far_by_key;
+  b.join_rows = c.join_rows;
   b.part_sums = b.sink_chunks + c.sink_chunks;
   b.parts = c.parts;
   b.whole = (int)c.whole;

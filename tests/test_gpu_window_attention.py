@@ -363,6 +363,61 @@ def test_backward_sinks_over_chunks(dev, dtype, d, window, sinks):
     expect_gradients(*x, do, grads, 1 / math.sqrt(d), window, sinks)
 
 
+SHORT_AND_LONG = [20] * 30 + [200] + [5] * 20 + [300, 170]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,window,sinks,blocks,chunks", [
+    (SHORT_AND_LONG, 64, 40, 42, 21 * 2),        # by long sequence
+    (SHORT_AND_LONG, 64, 2 ** 40, 62, 5 * 42),   # by key and long sequence
+    ([500, 0, 400], 10, 2 ** 40, 31, 10 * 29),   # by key and sequence
+    ([700, 0, 3, 900], 10, 5, 4, 18),            # by sequence
+])
+def test_backward_far_sinks(dev, dtype, lengths, window, sinks, blocks, chunks):
+    """Sinks that some sequences have past their windows and others have not,
+    in each order of the blocks that their sums go to."""
+    say(f"window backward far sinks {dtype} {len(lengths)} {window} {sinks}")
+    queries = [n - n // 4 if n > 300 else n for n in lengths]
+    x = inputs(dtype, queries, lengths, 2, 1, 72, seed=15, lead=3, tail=5)
+    elem, tokens = x[2].element_size(), (len(x[2]), len(x[3]))
+    need = sw.load_library().sw_window_attention_backward_workspace_bytes
+    sizes = [need(len(lengths), *tokens, 2, 1, 72, window, n, elem)
+             for n in (0, sinks)]
+    assert sizes[1] - sizes[0] == 4 * 32 * 2 * 72 * (2 * blocks + chunks)
+    do = output_gradient(x)
+    grads = backward(*x, do, 0.2, window, sinks)
+    expect_gradients(*x, do, grads, 0.2, window, sinks)
+
+
+@pytest.mark.parametrize("n,length,h,hk,d,window,sinks", [
+    (64, 256, 32, 8, 128, 1024, 2 ** 40),
+    (8192, 32, 8, 8, 8, 1024, 64),
+])
+def test_backward_of_more_sinks_than_keys(dev, n, length, h, hk, d, window,
+                                          sinks):
+    """Many short sequences, which see all their keys, and sinks that only one
+    long sequence has: what the forward pass takes the backward pass takes
+    too, in scratch memory of about the gradients' size."""
+    say(f"window backward many sinks {n} {length}")
+    x = inputs("bf16", [length] * n + [1500], [length] * n + [1500], h, hk, d,
+               seed=16)
+    need = sw.load_library().sw_window_attention_backward_workspace_bytes
+    tokens = n * length + 1500
+    one = need(n + 1, tokens, tokens, h, hk, d, window, 0, 2)
+    assert need(n + 1, tokens, tokens, h, hk, d, window, sinks, 2) - one <= \
+        4 * hk * 2 * d * (2 * tokens + tokens // 4 + 8192)
+    do = output_gradient(x)
+    got = backward(*x, do, 0.3, window, sinks)
+    plain = backward(*x, do, 0.3, window, 0)
+    for a, b in zip(got, plain):
+        assert torch.equal(a[:n * length], b[:n * length])
+    a = n * length
+    off = torch.tensor([0, 1500], dtype=torch.int32)
+    expect_gradients(off, off, *(y[a:] for y in x[2:]), do[a:],
+                     [y[a:] for y in got], 0.3, window, sinks,
+                     heads=[0, hk - 1])
+
+
 @pytest.mark.parametrize("alpha", [-0.3, 0.0])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_backward_alpha(dev, dtype, alpha):

@@ -128,6 +128,36 @@ def test_backward_workspace_rule():
     assert need(1, 100, 100, 4, 2, 64, 100, 7, 8) == 0
 
 
+def test_backward_workspace_of_many_sequences():
+    """The sinks' sums are bounded by the keys, however many sequences there
+    are and however many sinks none of them has."""
+    need = sw.load_library().sw_window_attention_backward_workspace_bytes
+
+    def sums(n, tokens, sinks, window=1024):
+        return need(n, tokens, tokens, 32, 8, 128, window, sinks, 2) - \
+            need(n, tokens, tokens, 32, 8, 128, window, 0, 2)
+    keys = 2 * 8 * 128  # bytes of a bf16 key of all heads
+    fp32 = 4 * keys     # of its two sums
+    # the window's and the first chunk's sums, at most a row a key of each, and
+    # one row for four queries of the later chunks' (twice that for fewer sinks
+    # than a block has)
+    for n, tokens in ((1, 65536), (64, 16384), (64, 65536), (4096, 262144),
+                      (8192, 262144), (100, 262144)):
+        for sinks in (1, 4, 32, 64, 65, 1000, 4096, 65536, 2 ** 40):
+            for window in (16, 1024, 16000):
+                bound = fp32 * (2 * (tokens + 32 * min(n, tokens // window)) +
+                                tokens // 4 + 1024)
+                assert 0 < sums(n, tokens, sinks, window) <= bound
+    # blocks of 32 sinks: by sequence,
+    block = 32 * fp32
+    assert sums(6, 16384, 4) == (2 * 6 + 64) * block
+    # by the sequences that may hold more keys than the window, 255 here,
+    assert sums(8192, 262144, 64) == (2 * 255 * 2 + 1024 * 2) * block
+    # and by keys: 15360 / 32 and 15
+    assert sums(64, 16384, 2 ** 40) == 2 * 495 * block
+    assert sums(2, 16384, 2 ** 40) == 2 * 482 * block
+
+
 def test_nothing_to_do():
     assert c_backward(sequences=0, workspace=None)[0] == 0
     assert c_backward(query_tokens=0, key_tokens=0, workspace=None)[0] == 0
