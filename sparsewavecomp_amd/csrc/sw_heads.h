@@ -175,8 +175,12 @@ __device__ __forceinline__ v4u buffer_words(const void *p, uint32_t n) {
 // of LDS at the wave-uniform address.  Written out because the compiler waits
 // for every copy that its builtin has under way before the next LDS read, of
 // whichever tile (which made each tile wait for the next one's copy); this one
-// returns no register, and landed() waits for it.  It sets m0, which nothing
-// else in the kernels that call it uses (LDS instructions do not on gfx9).
+// returns no register, and landed() waits for it.  It sets m0, which the
+// compiler keeps for itself and sets before instructions that read it: the
+// clobber keeps such a value from being carried across, and the warning that
+// this draws (m0 is not preserved) says what is meant.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy_to_lds(v4u buffer, uint32_t at,
                                             uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\t"
@@ -184,7 +188,7 @@ __device__ __forceinline__ void copy_to_lds(v4u buffer, uint32_t at,
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at),
                  "s"(buffer)
-               : "memory");
+               : "memory", "m0");
 }
 
 // The same of 4 bytes a lane, to 256 consecutive bytes.
@@ -195,8 +199,9 @@ __device__ __forceinline__ void copy_words_to_lds(v4u buffer, uint32_t at,
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at),
                  "s"(buffer)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // For N products of this stretch of code, each with one LDS read of its own:
 // four reads first, then a product and a read in turn, so that a product waits

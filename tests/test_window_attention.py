@@ -223,3 +223,21 @@ def test_strides_of_one_row():
         (1, 2, 1, 8), (5, 8, 8, 1))
     assert list(sw._heads(torch.bfloat16, -1, page, "key_cache", one,
                           "query")[1]) == [0, 8, 8, 64, 1 << 23]
+
+
+def test_assembly_names_what_it_changes():
+    """Every written-out statement that sets m0 lists it as changed, so that
+    the compiler carries no value of its own across."""
+    import glob
+    import os
+    import re
+    sources = glob.glob(os.path.join(os.path.dirname(sw.__file__), "csrc", "*"))
+    found = 0
+    for path in sources:
+        with open(path) as f:
+            text = f.read()
+        for m in re.finditer(r"\basm volatile\((.*?)\);", text, re.S):
+            if re.search(r"\bm0,", m[1]):
+                found += 1
+                assert '"m0"' in m[1].rsplit(":", 1)[1], (path, m[0])
+    assert found >= 2
