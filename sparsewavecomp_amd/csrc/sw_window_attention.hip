@@ -210,15 +210,19 @@ template <typename T, int D, int STREAMS> struct Forward {
 };
 
 // Adds up what the shares of the keys left in acc, in the first share's waves,
-// share by share, under their common maximum; true in those.  Every thread must
+// share by share, under their common maximum; true in those waves.  acc and sum
+// are 2^raise times smaller than the row's; they become `room` powers of two
+// smaller still, so that adding keeps within fp32's range.  Every thread must
 // call it, when the tiles' memory is free.
 template <typename T, int D, int STREAMS, int BLOCKS>
 __device__ __forceinline__ bool add_shares(v16f (&acc)[BLOCKS], float &top,
-                                           float &sum, char *lds) {
+                                           float &sum, float &raise, float room,
+                                           char *lds) {
   if constexpr (STREAMS == 1) {
     return true;
   } else {
-    constexpr int kWords = (BLOCKS * 16 + 2) * kWave;
+    constexpr int kRowWords = BLOCKS * 16;
+    constexpr int kWords = (kRowWords + 3) * kWave;
     constexpr int kRowBlocks = 4 / STREAMS;
     static_assert((4 - kRowBlocks) * kWords * 4 <=
                   Forward<T, D, STREAMS>::kBytes, "");
@@ -232,8 +236,9 @@ __device__ __forceinline__ bool add_shares(v16f (&acc)[BLOCKS], float &top,
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           x[(b * 16 + r) * kWave] = acc[b][r];
-      x[BLOCKS * 16 * kWave] = top;
-      x[(BLOCKS * 16 + 1) * kWave] = sum;
+      x[kRowWords * kWave] = top;
+      x[(kRowWords + 1) * kWave] = sum;
+      x[(kRowWords + 2) * kWave] = raise;
     }
     __syncthreads();
     if (wave >= kRowBlocks)
@@ -241,12 +246,18 @@ __device__ __forceinline__ bool add_shares(v16f (&acc)[BLOCKS], float &top,
 #pragma unroll 1
     for (int i = 0; i < STREAMS - 1; ++i) {
       const float *x = words + (wave + i * kRowBlocks) * kWords;
-      const float other = x[BLOCKS * 16 * kWave];
+      const float other = x[kRowWords * kWave];
+      const float other_raise = x[(kRowWords + 2) * kWave];
       const float to = fmaxf(top, other);
-      const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-      const float add = other == to ? 1.0f : __builtin_amdgcn_exp2f(other - to);
+      const float less = fmaxf(raise, other_raise) + room;
+      const float by = (top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to)) *
+                       __builtin_amdgcn_exp2f(raise - less);
+      const float add =
+          (other == to ? 1.0f : __builtin_amdgcn_exp2f(other - to)) *
+          __builtin_amdgcn_exp2f(other_raise - less);
       top = to;
-      sum = fmaf(x[(BLOCKS * 16 + 1) * kWave], add, sum * by);
+      raise = less;
+      sum = fmaf(x[(kRowWords + 1) * kWave], add, sum * by);
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -322,6 +333,7 @@ window_forward(WindowArgs a) {
 
   v16f acc[F::kBlocks];
   float top, sum;
+  float raise = 0.0f; // of this lane's query, in the careful pass
 
   // One tile's products with the wave's queries.  Whole tiles are computed
   // where one of the rows sees a key: blocks of 32 keys apart, so that hidden
@@ -385,6 +397,8 @@ window_forward(WindowArgs a) {
         acc[b] *= by;
     }
     const float less = top == -kInf ? 0.0f : top;
+    // (a factor of its own, so that the exponential keeps its bits)
+    const float lower = __builtin_amdgcn_exp2f(-raise);
     // The wave that has come to its second product goes first: of two waves
     // of a SIMD one then multiplies while the other does its exponentials
     // (65,536 queries, window 4096: 2222 us without, 2167 us with)
@@ -395,6 +409,8 @@ window_forward(WindowArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         p[r] = __builtin_amdgcn_exp2f(fmaf(score[kb][r], scale, -less));
+        if constexpr (decltype(careful)::value)
+          p[r] *= lower;
         sum += p[r];
       }
 #pragma unroll
@@ -443,11 +459,20 @@ window_forward(WindowArgs a) {
   };
   pass(std::false_type{});
   // A finite result has met no infinity or NaN.  Others are computed again
-  // with the keys at the edges of the mask kept apart.
-  if (any_wave(!all_finite<T>(acc), &verdict))
+  // with the keys at the edges of the mask kept apart.  A row that is not finite
+  // may also be a sum past fp32's range of values whose mean lies within: its
+  // probabilities, up to 2^8 of a lagging maximum, then are at most 2^(8 - raise),
+  // so that no sum of them passes the largest value.  (Only in such a row: what
+  // is below 2^(raise - 126) of the largest probability, or such a value, is
+  // lost.)
+  const bool finite = all_finite<T>(acc);
+  if (any_wave(!finite, &verdict)) {
+    if (both_halves_max(finite ? 0.0f : 1.0f) != 0.0f)
+      raise = (float)(8 + 33 - __builtin_clz(keys.count * KT | 1));
     pass(std::true_type{});
+  }
 
-  if (!add_shares<T, D, STREAMS>(acc, top, sum, lds))
+  if (!add_shares<T, D, STREAMS>(acc, top, sum, raise, 2.0f, lds))
     return;
   sum = both_halves_sum(sum);
   const bool empty = place < 0 || s.nk == 0; // a row that sees no key
@@ -468,7 +493,9 @@ window_forward(WindowArgs a) {
       }
     if (a.log_sum && h == 0)
       a.log_sum[(int64_t)head * a.query_tokens + s.q0 + row] =
-          empty ? -kInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+          empty ? -kInf
+                : (top + __builtin_amdgcn_logf(
+                             sum * __builtin_amdgcn_exp2f(raise))) * kLn2;
   }
 }
 
@@ -683,8 +710,9 @@ window_query_gradient(BackwardArgs b) {
   pass(std::false_type{});
   if (any_wave(!all_finite<T>(acc), &verdict))
     pass(std::true_type{});
-  float top = 0.0f, sum = 0.0f; // (the shares' gradients add up as they are)
-  if (!add_shares<T, D, STREAMS>(acc, top, sum, lds))
+  // (the shares' gradients add up as they are)
+  float top = 0.0f, sum = 0.0f, raise = 0.0f;
+  if (!add_shares<T, D, STREAMS>(acc, top, sum, raise, 0.0f, lds))
     return;
   if (live) {
     T *out = static_cast<T *>(b.query_gradient) + token * b.gq.token +

@@ -196,6 +196,30 @@ def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at, heads):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads", [2, 288])
+@pytest.mark.parametrize("alpha,size", [(0.125, 3.0e38), (4.0, 3.0e38),
+                                        (0.0, 3.0e38), (0.0, 8.0e36)])
+def test_forward_of_large_values(dev, dtype, heads, alpha, size):
+    """Values whose weighted mean is finite while a sum of them is not, in one
+    head and sequence; the others keep their bits."""
+    say(f"window forward large values {dtype} {heads} {alpha} {size}")
+    x = list(inputs(dtype, [200, 40], [230, 40], heads, heads, 64, seed=21))
+    clean, clean_lse = forward(*x, alpha, 60, 2)
+    gen = torch.Generator().manual_seed(22)
+    v = x[4].clone()
+    v[:230, 1] = ((0.5 + torch.rand(230, 64, generator=gen) / 2) * size).to(
+        v.dtype)
+    v[:230, 1, 32:] *= -1
+    x[4] = v
+    out, lse = forward(*x, alpha, 60, 2)
+    assert torch.isfinite(out).all()
+    expect(*x, out, lse, alpha, 60, 2, heads=[1])
+    out[:200, 1], clean[:200, 1] = 0, 0
+    lse[1, :200], clean_lse[1, :200] = 0, 0
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_forward_repeats_and_graph(dev, dtype):
     """The same bits again, on another stream, and from a captured graph that
     is replayed with eager work between."""
