@@ -6,7 +6,9 @@
 // head: with G of them a key of d elements takes part in 4 G d operations for
 // 2 d elements read, so memory bounds these kernels.  A sequence's keys are cut
 // into chunks, one workgroup each, and the chunks' (m, l, o) joined:
-//   m = max m_c,  l = sum l_c 2^(m_c - m),  o = sum o_c 2^(m_c - m) / l.
+//   m = max m_c,  w_c = l_c 2^(m_c - m),  l = sum w_c,  o = sum o_c w_c / l,
+// o_c being a chunk's weighted mean: sums of values, which fp32 may not hold
+// where their mean is finite, stay within a chunk, which sees whether they did.
 // The prefix is cut the same way; its rows are the query heads of all
 // sequences together.
 #include "sw_heads.h"
@@ -54,6 +56,8 @@ struct StepArgs {
   // leaves o in [part][rows][dim] and (m, l) in [part][rows][2].
   int chunk, parts, prefix_chunk, prefix_parts;
   int rows, prefix_rows; // of one part: a multiple of 16, of 16 or 128
+  // a power of two: the number of all keys times it is below 1
+  float lower;
   float *sums, *stats, *prefix_sums, *prefix_stats;
   // workgroups of the prefix: by cache_part and by prefix_part
   int64_t prefix_items, wide_items;
@@ -101,10 +105,13 @@ template <typename T, int D> struct CacheParts {
   static constexpr int kWaveBytes =
       Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
   static constexpr int kBytes = 4 * kWaveBytes;
-  static constexpr int kWaves = sizeof(T) * D > 256 ? 1 : 3;
+  // (bf16 rows of up to 64, 64 sequences, window 4096: 114 us with four waves,
+  // 104 with five)
+  static constexpr int kWaves =
+      sizeof(T) * D > 256 ? 1 : sizeof(T) * D > 128 ? 3 : 5;
 };
 struct Totals {
-  float top[4][kRows], sum[4][kRows];
+  float top[4][kRows], sum[4][kRows], raise[4][kRows];
 };
 
 template <typename T, int D>
@@ -239,10 +246,8 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
   };
 
   v4f acc[kBlocks];
-#pragma unroll
-  for (int b = 0; b < kBlocks; ++b)
-    acc[b] = v4f{};
-  float top = -kInf, sum = 0.0f;
+  float top, sum;
+  float lower = 1.0f; // of this lane's row: a factor of the probabilities
   const uint32_t own = lds_address(lds) + wave * kWaveBytes;
   uint32_t across[sizeof(T) == 2 ? 2 * kBlocks : 1]; // (bf16)
   if constexpr (sizeof(T) == 2) {
@@ -256,71 +261,90 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
             (i & 1) * 8;
   }
 
-  bool some = false; // whether a key was there (wave-uniform)
-  int v = v0 + wave * kTile;
-  while (v < v1) {
-    const Data now = fetch(rows_of(v));
-    v4f score[2];
+  bool some; // whether a key was there (wave-uniform)
+  for (;;) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      score[b] = v4f{};
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st)
-        score[b] = mma16(now.k[b][st], q[st], score[b]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if ((now.none >> i) & 1)
-        score[i / 4][i % 4] = -kInf;
-    float big = score[0][0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i)
-      big = fmaxf(big, score[i / 4][i % 4]);
-    big = rows16_max(big) * scale;
-    if (ballot(big > top) != 0) {
-      const float to = fmaxf(top, big);
-      const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-      top = to;
-      sum *= by;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-        acc[b] *= by;
-    }
-    const float less = top == -kInf ? 0.0f : top;
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less));
-      sum += p[i];
-    }
-    // bf16: the probabilities round to the operands' type, as the matrix core
-    // takes them; their sum does not
-    const Frag<T> pf = make_frag<T>(p);
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      lds_write(own + Tile::place(i * kPieceRows + lane / Tile::kChunks,
-                                  lane % Tile::kChunks), now.v[i]);
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      Frag<T> vf;
-      if constexpr (sizeof(T) == 2) {
-        const v2u x = lds_read_across(across[b], 0);
-        const v2u y = lds_read_across(across[kBlocks + b], 0);
-        vf = v4u{x.x, x.y, y.x, y.y};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = 16 * b + (lane & 15);
-          vf[i] = lds_read<float>(
-              own + Tile::place(16 * (i >> 2) + 4 * g + (i & 3), c >> 2) +
-              (c & 3) * 4, 0);
-        }
+    for (int b = 0; b < kBlocks; ++b)
+      acc[b] = v4f{};
+    top = -kInf;
+    sum = 0.0f;
+    some = false;
+    int v = v0 + wave * kTile;
+    while (v < v1) {
+      const Data now = fetch(rows_of(v));
+      v4f score[2];
+  #pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        score[b] = v4f{};
+  #pragma unroll
+        for (int st = 0; st < kSteps; ++st)
+          score[b] = mma16(now.k[b][st], q[st], score[b]);
       }
-      acc[b] = mma16(vf, pf, acc[b]);
+  #pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((now.none >> i) & 1)
+          score[i / 4][i % 4] = -kInf;
+      float big = score[0][0];
+  #pragma unroll
+      for (int i = 1; i < 8; ++i)
+        big = fmaxf(big, score[i / 4][i % 4]);
+      big = rows16_max(big) * scale;
+      if (ballot(big > top) != 0) {
+        const float to = fmaxf(top, big);
+        const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+        top = to;
+        sum *= by;
+  #pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+          acc[b] *= by;
+      }
+      const float less = top == -kInf ? 0.0f : top;
+      float p[8];
+  #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less)) *
+               lower;
+        sum += p[i];
+      }
+      // bf16: the probabilities round to the operands' type, as the matrix core
+      // takes them; their sum does not
+      const Frag<T> pf = make_frag<T>(p);
+  #pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        lds_write(own + Tile::place(i * kPieceRows + lane / Tile::kChunks,
+                                    lane % Tile::kChunks), now.v[i]);
+  #pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        Frag<T> vf;
+        if constexpr (sizeof(T) == 2) {
+          const v2u x = lds_read_across(across[b], 0);
+          const v2u y = lds_read_across(across[kBlocks + b], 0);
+          vf = v4u{x.x, x.y, y.x, y.y};
+        } else {
+  #pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int c = 16 * b + (lane & 15);
+            vf[i] = lds_read<float>(
+                own + Tile::place(16 * (i >> 2) + 4 * g + (i & 3), c >> 2) +
+                (c & 3) * 4, 0);
+          }
+        }
+        acc[b] = mma16(vf, pf, acc[b]);
+      }
+      some |= ballot(((~now.none) & 0xFF) != 0) != 0;
+      v += 4 * kTile;
     }
-    some |= ballot(((~now.none) & 0xFF) != 0) != 0;
-    v += 4 * kTile;
+    // A sum past fp32's range of values whose mean lies within: such rows once
+    // more, under probabilities that are lower by the number of keys.  (Of them
+    // alone, what is below that factor times 2^-126 of the largest probability,
+    // or such a value, is lost.)
+    const bool past = live && !all_finite(acc);
+    if (ballot(past && lower == 1.0f) == 0)
+      break;
+    if (rows16_max(past ? 1.0f : 0.0f) != 0.0f)
+      lower = __builtin_amdgcn_exp2f(-raise_of(v1 - v0));
   }
+  const float raise = lower == 1.0f ? 0.0f : raise_of(v1 - v0);
   if (some && top == -kInf)
     top = kLowest;
 
@@ -329,6 +353,7 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
   if (g == 0) {
     found.top[wave][lane] = top;
     found.sum[wave][lane] = sum;
+    found.raise[wave][lane] = raise;
   }
   // o[row][d] of each wave, in its own part of LDS
 #pragma unroll
@@ -339,16 +364,20 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
     const int r = x / (D / 4), c = x % (D / 4) * 4;
     if (r >= rows)
       break;
-    float m = found.top[0][r];
+    float m = found.top[0][r], most = found.raise[0][r];
 #pragma unroll
-    for (int w = 1; w < 4; ++w)
+    for (int w = 1; w < 4; ++w) {
       m = fmaxf(m, found.top[w][r]);
+      most = fmaxf(most, found.raise[w][r]);
+    }
+    most += 3.0f; // (four sums that are finite have a finite sum)
     float l = 0.0f;
     v4f o = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float by =
+      float by =
           found.top[w][r] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(found.top[w][r] - m);
+      by *= __builtin_amdgcn_exp2f(found.raise[w][r] - most);
       const v4f y =
           lds_read<v4f>(lds_address(lds) + w * kWaveBytes + (r * D + c) * 4, 0);
       l = fmaf(found.sum[w][r], by, l);
@@ -364,10 +393,12 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
             empty ? 0.0f : o[2] * by, empty ? 0.0f : o[3] * by);
       }
     } else {
+      if (l != 0.0f) // (zero: no key, or scores of -inf alone)
+        o *= 1.0f / l;
       *reinterpret_cast<v4f *>(sums + r * D + c) = o;
       if (c == 0) {
         stats[2 * r] = m;
-        stats[2 * r + 1] = l;
+        stats[2 * r + 1] = l * __builtin_amdgcn_exp2f(most);
       }
     }
   }
@@ -390,7 +421,10 @@ template <typename T, int D> struct Prefix {
   static constexpr int kSteps = D / 16;
   static constexpr int kBlocks = D / 32;
   static constexpr int kKeyBlocks = kTile / 32;
-  static constexpr int kWaves = sizeof(T) * D > 256 ? 1 : 2;
+  // (fp32 rows of up to 64, 64 sequences behind 4,096 keys: 65 us with two
+  // waves, 47 with three)
+  static constexpr int kWaves =
+      sizeof(T) * D > 256 ? 1 : sizeof(T) == 4 ? 3 : 2;
   static constexpr int kBytes = std::max(4 * Tile::kBytes,
                                          CacheParts<T, D>::kBytes);
 };
@@ -398,7 +432,7 @@ constexpr int kPrefixRows = 128;
 
 template <typename T, int D>
 __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
-                                            char *lds) {
+                                            char *lds, int *verdict) {
   using F = Prefix<T, D>;
   using Tile = typename F::Tile;
   constexpr int KT = F::kTile;
@@ -442,13 +476,12 @@ __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
   };
 
   v16f acc[F::kBlocks];
-#pragma unroll
-  for (int b = 0; b < F::kBlocks; ++b)
-    acc[b] = v16f{};
-  float top = -kInf, sum = 0.0f;
+  float top, sum;
+  float raise = 0.0f; // as in cache_part
   // (waves without rows only copy)
   const bool work = first_row + 32 * wave < a.sequences * a.group;
-  auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+  auto step = [&](int t, auto parity, auto careful)
+                  __attribute__((always_inline)) {
     landed();
     if (t + 1 < count)
       copy(t + 1);
@@ -490,6 +523,7 @@ __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
         acc[b] *= by;
     }
     const float less = top == -kInf ? 0.0f : top;
+    const float lower = __builtin_amdgcn_exp2f(-raise);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kb = 0; kb < F::kKeyBlocks; ++kb) {
@@ -497,6 +531,8 @@ __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         p[r] = __builtin_amdgcn_exp2f(fmaf(score[kb][r], scale, -less));
+        if constexpr (decltype(careful)::value)
+          p[r] *= lower;
         sum += p[r];
       }
 #pragma unroll
@@ -509,18 +545,39 @@ __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
     }
     __builtin_amdgcn_s_setprio(0);
   };
-  if (count > 0)
-    copy(0);
-  for (int t = 0; t < count; t += 2) {
-    step(t, std::integral_constant<int, 0>{});
-    if (t + 1 < count)
-      step(t + 1, std::integral_constant<int, 1>{});
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < F::kBlocks; ++b)
+      acc[b] = v16f{};
+    top = -kInf;
+    sum = 0.0f;
+    if (count > 0)
+      copy(0);
+    for (int t = 0; t < count; t += 2) {
+      step(t, std::integral_constant<int, 0>{}, careful);
+      if (t + 1 < count)
+        step(t + 1, std::integral_constant<int, 1>{}, careful);
+    }
+  };
+  pass(std::false_type{});
+  // (as in cache_part; the maximum lags by up to 2^8 here)
+  const bool past = live && !all_finite(acc);
+  if (any_wave(past, verdict)) {
+    if (both_halves_max(past ? 1.0f : 0.0f) != 0.0f)
+      raise = 8.0f + raise_of(v1 - v0);
+    pass(std::true_type{});
   }
   sum = both_halves_sum(sum);
   if (!live)
     return;
   if (top == -kInf)
     top = kLowest;
+  if (sum != 0.0f) {
+    const float by = 1.0f / sum;
+#pragma unroll
+    for (int b = 0; b < F::kBlocks; ++b)
+      acc[b] *= by;
+  }
   const int64_t of = ((int64_t)hk * a.prefix_parts + part) * a.prefix_rows + row;
 #pragma unroll
   for (int b = 0; b < F::kBlocks; ++b)
@@ -530,7 +587,7 @@ __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
           acc[b][r + 1], acc[b][r + 2], acc[b][r + 3]);
   if (h == 0) {
     a.prefix_stats[2 * of] = top;
-    a.prefix_stats[2 * of + 1] = sum;
+    a.prefix_stats[2 * of + 1] = sum * __builtin_amdgcn_exp2f(raise);
   }
 }
 
@@ -542,11 +599,12 @@ __global__ __launch_bounds__(kThreads, (Prefix<T, D>::kWaves)) void
 shared_prefix_parts(StepArgs a) {
   __shared__ __align__(1024) char lds[Prefix<T, D>::kBytes];
   __shared__ Totals found;
+  __shared__ int verdict;
   const int64_t all = gridDim.x, prefix = a.wide_items;
   const int64_t before = blockIdx.x * prefix / all;
   if ((blockIdx.x + (int64_t)1) * prefix / all > before)
     // (the row tiles of a chunk next to each other on one XCD)
-    prefix_part<T, D>(a, xcd_contiguous(before, prefix), lds);
+    prefix_part<T, D>(a, xcd_contiguous(before, prefix), lds, &verdict);
   else
     cache_part<T, D>(a, blockIdx.x - before, lds, found);
 }
@@ -579,11 +637,12 @@ __global__ __launch_bounds__(kThreads) void window_cache_join(StepArgs a) {
     const float m = stats[0], to = fmaxf(top, m);
     const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
     const float add = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    const float weight = stats[1] * a.lower * add;
     top = to;
-    l = fmaf(stats[1], add, l * by);
+    l = fmaf(l, by, weight);
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      o[e] = fmaf(sums[e], add, o[e] * by);
+      o[e] = fmaf(sums[e], weight, o[e] * by);
   }
 #pragma unroll
   for (int e = 0; e < N; ++e)
@@ -802,6 +861,9 @@ int step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.prefix_chunk = (int)p.prefix_chunk;
   a.prefix_parts = (int)p.prefix_parts;
   a.prefix_rows = (int)p.prefix_rows;
+  a.lower = std::ldexp(
+      1.0f, -(int)std::ceil(std::log2((double)(p.chunk * p.parts +
+                                               prefix_tokens))) - 1);
   a.sums = static_cast<float *>(workspace);
   a.stats = a.sums + p.sums;
   a.prefix_sums = a.stats + p.stats;

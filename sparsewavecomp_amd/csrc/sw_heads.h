@@ -142,6 +142,35 @@ __device__ __forceinline__ float both_halves_sum(float v) {
   return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// ---- results that are not finite -----------------------------------------------
+// Whether a lane's accumulators all are (V: a vector of fp32).
+template <typename V, int BLOCKS>
+__device__ __forceinline__ bool all_finite(const V (&acc)[BLOCKS]) {
+  float x = 0.0f;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int r = 0; r < (int)(sizeof(V) / 4); ++r)
+      x = fmaf(acc[b][r], 0.0f, x);
+  return x == 0.0f;
+}
+// Whether a wave of the workgroup says so; every thread must call it.
+__device__ __forceinline__ bool any_wave(bool says, int *verdict) {
+  if (threadIdx.x == 0)
+    *verdict = 0;
+  __syncthreads();
+  if (ballot(says) != 0 && lane_id() == 0)
+    *verdict = 1;
+  __syncthreads();
+  return *verdict != 0;
+}
+// For a sum of up to n values (n < 2^31) under weights of at most 1, each
+// rounded: the power of two by which the weights are lowered so that no sum of
+// them passes the largest value.
+__device__ __forceinline__ float raise_of(int n) {
+  return (float)(33 - __builtin_clz(n | 1));
+}
+
 // ---- LDS by address ----------------------------------------------------------
 // Addresses are byte offsets in the workgroup's LDS: a lane's part and a part
 // known when the kernel is built, which becomes the instruction's offset.

@@ -170,27 +170,6 @@ __device__ __forceinline__ v16f mma32_seen(Frag<T> a, Frag<T> b, v16f acc,
   return acc;
 }
 
-template <typename T, int BLOCKS>
-__device__ __forceinline__ bool all_finite(const v16f (&acc)[BLOCKS]) {
-  float x = 0.0f;
-#pragma unroll
-  for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      x = fmaf(acc[b][r], 0.0f, x);
-  return x == 0.0f;
-}
-// Whether a wave of the workgroup says so; every thread must call it.
-__device__ __forceinline__ bool any_wave(bool says, int *verdict) {
-  if (threadIdx.x == 0)
-    *verdict = 0;
-  __syncthreads();
-  if (ballot(says) != 0 && lane_id() == 0)
-    *verdict = 1;
-  __syncthreads();
-  return *verdict != 0;
-}
-
 // ---- forward -------------------------------------------------------------------
 
 // The row kernels: STREAMS shares of the keys, each with tiles of its own that
@@ -465,10 +444,10 @@ window_forward(WindowArgs a) {
   // so that no sum of them passes the largest value.  (Only in such a row: what
   // is below 2^(raise - 126) of the largest probability, or such a value, is
   // lost.)
-  const bool finite = all_finite<T>(acc);
+  const bool finite = all_finite(acc);
   if (any_wave(!finite, &verdict)) {
     if (both_halves_max(finite ? 0.0f : 1.0f) != 0.0f)
-      raise = (float)(8 + 33 - __builtin_clz(keys.count * KT | 1));
+      raise = 8.0f + raise_of(keys.count * KT);
     pass(std::true_type{});
   }
 
@@ -708,7 +687,7 @@ window_query_gradient(BackwardArgs b) {
     }
   };
   pass(std::false_type{});
-  if (any_wave(!all_finite<T>(acc), &verdict))
+  if (any_wave(!all_finite(acc), &verdict))
     pass(std::true_type{});
   // (the shares' gradients add up as they are)
   float top = 0.0f, sum = 0.0f, raise = 0.0f;
@@ -1031,7 +1010,7 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
       }
     }
   }
-  if (!CAREFUL && any_wave(!(all_finite<T>(dk) && all_finite<T>(dv)), verdict))
+  if (!CAREFUL && any_wave(!(all_finite(dk) && all_finite(dv)), verdict))
     return true;
 
   if constexpr (SINK) {

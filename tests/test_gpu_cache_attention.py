@@ -313,6 +313,40 @@ def test_decode_keeps_what_is_masked_apart(dev, dtype, bad):
     assert torch.equal(got, want)
 
 
+def large(y, size, seed):
+    """Values of [.., heads, d] of one sign a column, between size / 2 and
+    size."""
+    gen = torch.Generator().manual_seed(seed)
+    v = (0.5 + torch.rand(y.shape, generator=gen) / 2) * size
+    v[..., y.shape[-1] // 2:] *= -1
+    return v.to(y.dtype)
+
+
+# (what one wave, four waves of a part, and many parts add up passes fp32's
+# range)
+LARGE = [(0.125, 3.0e38), (4.0, 3.0e38), (0.0, 3.0e38), (0.0, 5.0e36),
+         (0.0, 1.5e36)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("alpha,size", LARGE)
+def test_decode_of_large_values(dev, dtype, alpha, size):
+    """Values whose weighted mean is finite while a sum of them is not, in one
+    sequence; the others keep their bits."""
+    say(f"decode large values {dtype} {alpha} {size}")
+    for lengths, window, sinks in (([128, 130], 200, 0), ([2000, 300], 1900, 4),
+                                   ([9000, 8000], 10 ** 6, 0)):
+        x = make(dtype, lengths, 0, 4, 2, 64, seed=31)
+        clean = decode(x, alpha, window, sinks)
+        v = large(x["values"][0], size, 32)
+        x["values"][0] = v
+        x["value_cache"][0, :lengths[0]] = v
+        got = decode(x, alpha, window, sinks)
+        assert torch.isfinite(got).all()
+        expect(x, got, alpha, window, sinks)
+        assert torch.equal(got[1], clean[1])
+
+
 # ---- a shared prefix -------------------------------------------------------------
 
 # lengths, page, prefix, heads, key heads, d: one sequence; no keys of its own;
@@ -350,6 +384,18 @@ def test_prefix_alpha(dev, dtype, alpha):
     for n in (3, 40):
         x = make(dtype, [9] * n, 16, 2, 1, 64, seed=n, prefix=200)
         expect(x, prefixed(x, alpha), alpha)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("alpha,size", LARGE)
+@pytest.mark.parametrize("n", [3, 40])
+def test_prefix_of_large_values(dev, dtype, alpha, size, n):
+    say(f"prefix large values {dtype} {alpha} {size} {n}")
+    x = make(dtype, [9] * n, 16, 4, 2, 64, seed=n, prefix=1000)
+    x["prefix_value"] = large(x["prefix_value"], size, 33)
+    got = prefixed(x, alpha)
+    assert torch.isfinite(got).all()
+    expect(x, got, alpha)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
