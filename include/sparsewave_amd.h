@@ -557,7 +557,8 @@ int sw_window_attention_backward_bf16(
  * Heads, d, types and alignment as in sw_window_attention; `strides` holds, in
  * elements, the token and head stride of query and of output, and the page,
  * token and head stride of key_cache and of value_cache (NULL: as the shapes
- * above).  Offsets into a cache are 64 bits.  No atomics.  The workspace
+ * above).  Offsets into a cache are 64 bits.  bf16 probabilities keep 15 bits.
+ * No atomics.  The workspace
  * (16-byte aligned, of sw_window_attention_decode_workspace_bytes; none where
  * that is 0) belongs to the call until its work on `stream` is done.
  */

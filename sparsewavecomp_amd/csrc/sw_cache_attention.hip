@@ -114,7 +114,7 @@ struct Totals {
   float top[4][kRows], sum[4][kRows], raise[4][kRows];
 };
 
-template <typename T, int D>
+template <typename T, int D, bool SPLIT>
 __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
                                            char *lds, Totals &found) {
   using Tile = RowTile<T, D, kTile, kWave>;
@@ -273,19 +273,19 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
     while (v < v1) {
       const Data now = fetch(rows_of(v));
       v4f score[2];
-  #pragma unroll
+#pragma unroll
       for (int b = 0; b < 2; ++b) {
         score[b] = v4f{};
-  #pragma unroll
+#pragma unroll
         for (int st = 0; st < kSteps; ++st)
           score[b] = mma16(now.k[b][st], q[st], score[b]);
       }
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 8; ++i)
         if ((now.none >> i) & 1)
           score[i / 4][i % 4] = -kInf;
       float big = score[0][0];
-  #pragma unroll
+#pragma unroll
       for (int i = 1; i < 8; ++i)
         big = fmaxf(big, score[i / 4][i % 4]);
       big = rows16_max(big) * scale;
@@ -294,26 +294,34 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
         const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
         top = to;
         sum *= by;
-  #pragma unroll
+#pragma unroll
         for (int b = 0; b < kBlocks; ++b)
           acc[b] *= by;
       }
       const float less = top == -kInf ? 0.0f : top;
       float p[8];
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less)) *
                lower;
         sum += p[i];
       }
-      // bf16: the probabilities round to the operands' type, as the matrix core
-      // takes them; their sum does not
-      const Frag<T> pf = make_frag<T>(p);
-  #pragma unroll
+      // bf16: the matrix core takes the probabilities as two bf16 parts, 15 bits
+      // of them together, for which it has the time (3.6 % busy with one part;
+      // 64 sequences, window 4096: 194.5 us, 192.2 with one; 4 of 65,536 keys:
+      // 179.4, 180.5).  Beside a prefix's products it has not (SPLIT, 128
+      // sequences behind 16,384 keys: 182.8 us, 177.0 with one): they round to
+      // bf16 there, as the prefix's do.  Their sum does not.
+      Frag<T> pf, rest;
+      if constexpr (SPLIT)
+        split_frag(p, pf, rest);
+      else
+        pf = make_frag<T>(p);
+#pragma unroll
       for (int i = 0; i < kPieces; ++i)
         lds_write(own + Tile::place(i * kPieceRows + lane / Tile::kChunks,
                                     lane % Tile::kChunks), now.v[i]);
-  #pragma unroll
+#pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         Frag<T> vf;
         if constexpr (sizeof(T) == 2) {
@@ -321,7 +329,7 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
           const v2u y = lds_read_across(across[kBlocks + b], 0);
           vf = v4u{x.x, x.y, y.x, y.y};
         } else {
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int c = 16 * b + (lane & 15);
             vf[i] = lds_read<float>(
@@ -330,6 +338,8 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
           }
         }
         acc[b] = mma16(vf, pf, acc[b]);
+        if constexpr (SPLIT)
+          acc[b] = mma16(vf, rest, acc[b]);
       }
       some |= ballot(((~now.none) & 0xFF) != 0) != 0;
       v += 4 * kTile;
@@ -409,7 +419,7 @@ __global__ __launch_bounds__(kThreads, (CacheParts<T, D>::kWaves)) void
 window_cache_parts(StepArgs a) {
   __shared__ __align__(1024) char lds[CacheParts<T, D>::kBytes];
   __shared__ Totals found;
-  cache_part<T, D>(a, blockIdx.x, lds, found);
+  cache_part<T, D, sizeof(T) == 2>(a, blockIdx.x, lds, found);
 }
 
 // The prefix against many query rows: 128 rows, 32 a wave, and one chunk of
@@ -606,7 +616,7 @@ shared_prefix_parts(StepArgs a) {
     // (the row tiles of a chunk next to each other on one XCD)
     prefix_part<T, D>(a, xcd_contiguous(before, prefix), lds, &verdict);
   else
-    cache_part<T, D>(a, blockIdx.x - before, lds, found);
+    cache_part<T, D, false>(a, blockIdx.x - before, lds, found);
 }
 
 // Joins the parts of a query head's softmax: one workgroup for each, whose

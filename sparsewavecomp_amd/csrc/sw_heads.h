@@ -65,6 +65,24 @@ template <typename T> __device__ __forceinline__ Frag<T> make_frag(const float *
     return v4u{cvt_pk_bf16(x[0], x[1]), cvt_pk_bf16(x[2], x[3]),
                cvt_pk_bf16(x[4], x[5]), cvt_pk_bf16(x[6], x[7])};
 }
+// Eight fp32 values that are not negative as the sum of two bf16 fragments, to
+// 2^-15 of each: what their upper halves hold, and the rest of it, rounded.  The
+// rest of a value that is not zero is at least 2^-126, so that an infinity times
+// both parts is infinite twice, not NaN where nothing is left.
+__device__ __forceinline__ void split_frag(const float *x, v4u &upper,
+                                           v4u &rest) {
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    r[e] = __builtin_amdgcn_fmed3f(
+        x[e] - __uint_as_float(__float_as_uint(x[e]) & 0xFFFF0000u), 0x1p-126f,
+        x[e]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    upper[e] = __builtin_amdgcn_perm(__float_as_uint(x[2 * e + 1]),
+                                     __float_as_uint(x[2 * e]), 0x07060302u);
+  rest = make_frag<uint16_t>(r);
+}
 template <typename T> __device__ __forceinline__ Frag<T> zero_frag() {
   if constexpr (sizeof(T) == 4)
     return v8f{0, 0, 0, 0, 0, 0, 0, 0};

@@ -313,6 +313,34 @@ def test_decode_keeps_what_is_masked_apart(dev, dtype, bad):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("lengths,page,window", [
+    ([300, 40], 0, 500), ([2000, 1500, 0, 1], 64, 1700)])
+@pytest.mark.parametrize("prefix", [None, 200])
+def test_bf16_probabilities_keep_fifteen_bits(dev, lengths, page, window,
+                                              prefix):
+    """A probability goes into its product as its upper eight bits and as what
+    they leave off, less than 2^-7 of it and rounded by at most 2^-8 of that:
+    off by 2^-15 of itself.  So an output is off by half a step of its own and
+    by 2^-15 of the sum of its terms' sizes, however much of them cancels."""
+    say(f"bf16 probabilities {lengths} {page} {prefix}")
+    t = half_step(torch.bfloat16)
+    x = make("bf16", lengths, page, 4, 2, 64, seed=17, prefix=prefix)
+    out = decode(x, 0.125, window, 0) if prefix is None else prefixed(x, 0.125)
+    for i, n in enumerate(lengths):
+        for h in range(4):
+            k, v = (x[m][i][:, h // 2].double() for m in ("keys", "values"))
+            if prefix is None:
+                k, v = k[-window:], v[-window:]
+            else:
+                k, v = (torch.cat([x[m][:, h // 2].double(), y]) for m, y in (
+                    ("prefix_key", k), ("prefix_value", v)))
+            see = torch.ones(1, len(k), dtype=torch.bool)
+            o, bound, p, *_ = softmax(x["query"][i, h:h + 1].double(), k, v,
+                                      see, 0.125, t)
+            bound += (2.0 ** -15 - t) * (p @ v.abs())
+            check(f"sequence {i}, head {h}", out[i, h:h + 1], o, bound)
+
+
 def large(y, size, seed):
     """Values of [.., heads, d] of one sign a column, between size / 2 and
     size."""
