@@ -166,8 +166,8 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
     return;
   rows = total - first_row < kRows ? total - first_row : kRows;
 
-  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
-  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+  const bool none = a.alpha == 0.0f;
+  const float scale = none ? 1.0f : fabsf(a.alpha) * kLog2e;
   Frag<T> q[kSteps];
   const int my_row = first_row + (lane & 15); // query row of this lane
   const bool live = (lane & 15) < rows;
@@ -180,7 +180,7 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       const int c = 32 * st + 8 * g;
-      q[st] = live && c < a.d && !tiny ? ld_frag(p + c) : zero_frag<T>();
+      q[st] = live && c < a.d && !none ? ld_frag(p + c) : zero_frag<T>();
       if (a.alpha < 0.0f)
         q[st] = negate_frag<T>(q[st]);
     }
@@ -460,15 +460,15 @@ __device__ __forceinline__ void prefix_part(const StepArgs &a, int64_t item,
   const int lane = lane_id(), h = lane >> 5, wave = wave_in_group();
   const int row = first_row + 32 * wave + (lane & 31);
   const bool live = row < a.sequences * a.group;
-  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
-  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+  const bool none = a.alpha == 0.0f;
+  const float scale = none ? 1.0f : fabsf(a.alpha) * kLog2e;
   Frag<T> q[F::kSteps];
   {
     const int r = live ? row : 0;
     const T *p = static_cast<const T *>(a.query) +
                  r / a.group * a.query_token +
                  (hk * a.group + r % a.group) * a.query_head;
-    load_rows<T>(q, p, live && !tiny, a.d, a.alpha < 0.0f);
+    load_rows<T>(q, p, live && !none, a.d, a.alpha < 0.0f);
   }
   const T *keys = static_cast<const T *>(a.prefix.key) + hk * a.prefix.key_head;
   const T *values =

@@ -277,14 +277,14 @@ window_forward(WindowArgs a) {
   const bool live = row < s.nq;
   const int head = w.head, hk = w.key_head;
 
-  // the wave's queries, negated where alpha is negative, and zero for an alpha
-  // too small to scale a masked score of -inf
-  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
+  // the wave's queries, negated where alpha is negative, and zero for an alpha of
+  // zero, which would make a masked score of -inf a NaN
+  const bool none = a.alpha == 0.0f;
   Frag<T> q[F::kSteps];
   load_rows<T>(q, static_cast<const T *>(a.query) +
                       (int64_t)(s.q0 + (live ? row : w.row0)) * a.q.token +
-                      head * a.q.head, live && !tiny, a.d, a.alpha < 0.0f);
-  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+                      head * a.q.head, live && !none, a.d, a.alpha < 0.0f);
+  const float scale = none ? 1.0f : fabsf(a.alpha) * kLog2e;
 
   const KeyTiles<KT> keys(w.row0 + w.shift, w.row0 + w.count - 1 + w.shift,
                           a.window, a.sinks, s.nk);
@@ -560,11 +560,11 @@ window_query_gradient(BackwardArgs b) {
   const int head = w.head, hk = w.key_head;
   const int64_t token = s.q0 + (live ? row : w.row0);
 
-  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
-  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+  const bool none = a.alpha == 0.0f;
+  const float scale = none ? 1.0f : fabsf(a.alpha) * kLog2e;
   Frag<T> q[F::kSteps], go[F::kSteps];
   load_rows<T>(q, static_cast<const T *>(a.query) + token * a.q.token +
-                      head * a.q.head, live && !tiny, a.d, a.alpha < 0.0f);
+                      head * a.q.head, live && !none, a.d, a.alpha < 0.0f);
   load_rows<T>(go, static_cast<const T *>(b.output_gradient) +
                        token * b.go.token + head * b.go.head, live, a.d, false);
   float delta = 0.0f, log2_sum = 0.0f;
@@ -819,15 +819,15 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
   const int key = key0 + (lane & 31);
   const bool live = key < (SINK ? far : s.nk);
 
-  const bool tiny = fabsf(a.alpha) < 0x1p-126f;
-  const float scale = tiny ? 1.0f : fabsf(a.alpha) * kLog2e;
+  const bool none = a.alpha == 0.0f;
+  const float scale = none ? 1.0f : fabsf(a.alpha) * kLog2e;
   const uint32_t vbase =
       lds_address(lds) + F::kBuffers * F::kParities * 2 * Tile::kBytes;
   Frag<T> k[F::kSteps], v[SINK ? F::kSteps : 1];
   {
     const int64_t token = s.k0 + (live ? key : 0);
     load_rows<T>(k, static_cast<const T *>(a.key) + token * a.k.token +
-                        hk * a.k.head, live && !tiny, a.d, a.alpha < 0.0f);
+                        hk * a.k.head, live && !none, a.d, a.alpha < 0.0f);
     const T *values = static_cast<const T *>(a.value) + hk * a.v.head;
     if constexpr (SINK)
       load_rows<T>(v, values + token * a.v.token, live, a.d, false);

@@ -162,6 +162,20 @@ def test_decode_alpha(dev, dtype, alpha):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [2, 70])
+def test_alpha_below_the_normal_numbers(dev, dtype, n):
+    """An alpha of 5e-39 scales scores of 1e37 as any other would."""
+    say(f"decode small alpha {dtype} {n}")
+    x = make(dtype, [40, 700] + [9] * (n - 2), 32, 2, 1, 64, seed=5, prefix=90)
+    x["query"] *= 1e18
+    for name in ("key_cache", "prefix_key"):
+        x[name] *= 1e18
+    x["keys"] = [k * 1e18 for k in x["keys"]]
+    expect(x, decode(x, 5e-39, 500, 2), 5e-39, 500, 2)
+    expect(x, prefixed(x, 5e-39), 5e-39)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("bad", [-1, 10 ** 6, -2 ** 31])
 def test_decode_pages_outside_the_cache(dev, dtype, bad):
     """Their keys are not there; a sequence without any other gets zeros."""

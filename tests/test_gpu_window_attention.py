@@ -452,6 +452,20 @@ def test_backward_alpha(dev, dtype, alpha):
     expect_gradients(*x, do, grads, alpha, 70, 2)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_alpha_below_the_normal_numbers(dev, dtype):
+    """An alpha of 5e-39 scales scores of 1e37 as any other would."""
+    say(f"window small alpha {dtype}")
+    x = list(inputs(dtype, [200, 30], [200, 50], 2, 1, 64, seed=6))
+    x[2], x[3] = x[2] * 1e18, x[3] * 1e18
+    alpha = 5e-39
+    out, lse = forward(*x, alpha, 70, 2)
+    expect(*x, out, lse, alpha, 70, 2)
+    do = output_gradient(x)
+    grads = backward(*x, do, alpha, 70, 2)
+    expect_gradients(*x, do, grads, alpha, 70, 2)
+
+
 def test_backward_against_differences(dev):
     """Directional derivatives of sum(output * do), by central differences in
     fp32: the step 2^-6 leaves a cubic term of about 2^-12 of the derivative,
