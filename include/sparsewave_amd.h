@@ -478,7 +478,7 @@ int sw_attention_tile_floor(const int32_t *row_offsets,
  * holds the token and the head stride, in elements, of query, key, value and
  * output (NULL: as the shapes above); rows start on 16 bytes, a token stride
  * is at least d and at most 2^23 bytes, a head stride of 0 shares one head
- * between all (not in the output).
+ * between all (not in the output).  alpha and alpha log2 e are finite.
  *
  * A query that sees no key (nq > nk) gets zeros and a log_sum of -inf.  Tokens
  * outside every sequence are left as they were.  Offsets are clamped to the

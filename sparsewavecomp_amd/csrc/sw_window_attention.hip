@@ -1239,8 +1239,10 @@ int check_window(int64_t sequences, int64_t query_tokens, int64_t key_tokens,
                     "expected a window of at least 1 and no negative sinks, "
                     "but got %lld and %lld", (long long)window,
                     (long long)sinks);
-  if (!std::isfinite(alpha))
-    return sw::fail(SW_ERR_INVALID_ARGUMENT, "alpha must be finite");
+  // (scores are scaled by alpha log2 e)
+  if (!std::isfinite(alpha * kLog2e))
+    return sw::fail(SW_ERR_INVALID_ARGUMENT,
+                    "alpha must be finite, and alpha log2 e too");
   return SW_OK;
 }
 

@@ -91,6 +91,14 @@ def test_prefix_refused(kw, code, needle):
     assert rc == code and needle in message
 
 
+@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("dt", ["_f32", "_bf16"])
+@pytest.mark.parametrize("alpha", [3.0e38, -2.4e38])
+def test_refuses_an_alpha_that_overflows(dt, prefix, alpha):
+    rc, message = call(prefix, dt, alpha=alpha)
+    assert rc == -3 and "alpha must be finite" in message
+
+
 def test_decode_workspace():
     need = sw.load_library().sw_window_attention_decode_workspace_bytes
     # few keys: one workgroup for each, nothing to join

@@ -158,6 +158,15 @@ def test_backward_workspace_of_many_sequences():
     assert sums(2, 16384, 2 ** 40) == 2 * 482 * block
 
 
+@pytest.mark.parametrize("dt", ["_f32", "_bf16"])
+@pytest.mark.parametrize("alpha", [3.0e38, -2.4e38])
+def test_refuses_an_alpha_that_overflows(dt, alpha):
+    """Scores are scaled by alpha log2 e, which has to be finite itself."""
+    for call in (c_forward, c_backward):
+        rc, message = call(dt=dt, alpha=alpha)
+        assert rc == -3 and "alpha must be finite" in message
+
+
 def test_nothing_to_do():
     assert c_backward(sequences=0, workspace=None)[0] == 0
     assert c_backward(query_tokens=0, key_tokens=0, workspace=None)[0] == 0
