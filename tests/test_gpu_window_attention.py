@@ -196,6 +196,41 @@ def test_forward_keeps_what_is_masked_apart(dev, dtype, bad, at, heads):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("what", ["key", "value"])
+@pytest.mark.parametrize("heads", [2, 288])
+def test_forward_keeps_a_first_key_apart_that_is_no_sink(dev, dtype, bad, what,
+                                                         heads):
+    """The first key without sinks: the rows past the window do not see it, and
+    keep the results of clean operands."""
+    say(f"window forward {bad} at the first key {dtype} {heads} {what}")
+    qo, ko, q, k, v = inputs(dtype, [200], [200], heads, heads, 64, seed=9)
+    clean, clean_lse = forward(qo, ko, q, k, v, 0.125, 50, 0)
+    (v if what == "value" else k)[0, 1, 5] = bad
+    out, lse = forward(qo, ko, q, k, v, 0.125, 50, 0)
+    apart = ~visible(200, 200, 50, 0)[:, 0]
+    assert int(apart.sum()) == 150
+    x, y = out[apart, 1].float(), clean[apart, 1].float()
+    assert torch.isfinite(x).all()
+    # (a repeated pass may add up in another order)
+    assert (x - y).abs().max() <= 4 * half_step(q.dtype) * y.abs().max()
+    x, y = lse[1][apart], clean_lse[1][apart]
+    assert (x - y).abs().max() <= 8 * half_step(torch.float32) * y.abs().max()
+    hit = out[~apart, 1, 5].float()
+    if what == "key" and bad == math.inf:
+        # a score of inf, or of -inf, which leaves the key out: NaN, but for the
+        # rows of a negative element, of which the first sees no other key
+        nan = q[~apart, 1, 5] > 0
+        nan[0] = True
+        assert torch.equal(torch.isnan(hit), nan)
+    else:
+        assert torch.isnan(hit).all() if math.isnan(bad) else \
+            (hit == bad).all()
+    out[:, 1], clean[:, 1], lse[1], clean_lse[1] = 0, 0, 0, 0
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("heads", [2, 288])
 @pytest.mark.parametrize("alpha,size", [(0.125, 3.0e38), (4.0, 3.0e38),
                                         (0.0, 3.0e38), (0.0, 8.0e36)])
