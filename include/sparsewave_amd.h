@@ -559,8 +559,11 @@ int sw_window_attention_backward_bf16(
  * token and head stride of key_cache and of value_cache (NULL: as the shapes
  * above).  Offsets into a cache are 64 bits.  bf16 probabilities keep 15 bits.
  * No atomics.  The workspace
- * (16-byte aligned, of sw_window_attention_decode_workspace_bytes; none where
- * that is 0) belongs to the call until its work on `stream` is done.
+ * (16-byte aligned, of sw_window_attention_decode_workspace_bytes, for a
+ * table_width of 1 without a page_table; none where that is 0) belongs to the
+ * call until its work on `stream` is done.  The keys are split among workgroups
+ * by what a table's row has room for: with much more room than keys a call of
+ * few sequences is several times slower than with a row that fits.
  */
 int64_t sw_window_attention_decode_workspace_bytes(
     int64_t sequences, int64_t page_size, int64_t table_width,
@@ -586,8 +589,10 @@ int sw_window_attention_decode_bf16(
  * One query for each sequence over a prefix that all of them share,
  * prefix_key and prefix_value [prefix_tokens][key_heads][d], and behind it the
  * sequence's own keys, all key_lengths[i] of a cache as above.  The prefix is
- * read once for the whole batch.  `strides` holds four more: the token and
- * head stride of prefix_key and of prefix_value.
+ * read for many query heads at a time, those that share a key head in all
+ * sequences: 128, or 16 where there are no more than 64; the next ones read it
+ * again, most of it from the chip's caches.  `strides` holds four more: the
+ * token and head stride of prefix_key and of prefix_value.
  */
 int64_t sw_shared_prefix_attention_workspace_bytes(
     int64_t sequences, int64_t prefix_tokens, int64_t page_size,

@@ -854,7 +854,9 @@ def window_attention_decode(key_lengths, page_table, query, key_cache,
     page_size, key_heads, d], or, where page_table is None, row j of page i.
     A page number outside the cache means that its keys are not there.
     Lengths are clamped to what a table's row holds; a length of 0 gives
-    zeros.  float32 or bfloat16, any strides of 16 bytes.  The scratch memory
+    zeros.  float32 or bfloat16, any strides of 16 bytes.  The keys are split
+    among workgroups by what a table's row has room for: much more room than
+    keys makes a call of few sequences several times slower.  The scratch memory
     of sw_window_attention_decode_workspace_bytes is taken from torch's
     allocator where `workspace` (uint8) is not given."""
     torch = _torch or _load_torch()
@@ -884,8 +886,9 @@ def shared_prefix_attention(key_lengths, page_table, query, prefix_key,
     """One query for each sequence over a prefix that all share, prefix_key
     and prefix_value [prefix_tokens, key_heads, d], and behind it the sequence's
     own key_lengths[i] keys in a cache laid out as
-    :func:`window_attention_decode` takes it.  The prefix is read once for the
-    whole batch.  Operands, types and workspace as there."""
+    :func:`window_attention_decode` takes it.  The prefix is read for up to 128
+    query heads of all sequences at a time.  Operands, types and workspace as
+    there."""
     torch = _torch or _load_torch()
     shape = _cache_shapes(key_lengths, page_table, query, key_cache,
                           value_cache, output)

@@ -694,6 +694,20 @@ struct Plan {
   }
 };
 
+// Query rows of a key head (of all sequences) past which a prefix goes through
+// tiles of 128 of them instead of 16.  8 key heads, caches of up to 256 keys
+// behind the prefix, parts of 128 / of 16 rows, us:
+//   rows, prefix      bf16, d = 128   bf16, 64      fp32, 64      fp32, 128
+//    32,  1000        12.3 / 12.6     10.1 /  9.8   24.9 / 12.5    41.6 /  19.7
+//    64,  1000        13.0 / 13.2     10.5 / 10.3   25.7 / 13.3    43.6 /  21.4
+//    96,  1000        14.4 / 16.3     11.2 / 12.0   26.7 / 16.6    45.0 /  36.1
+//   256,  1000        25.6 / 28.4     16.3 / 17.7   34.9 / 28.5    78.0 /  68.4
+//    32,  8192        17.4 / 21.5     12.4 / 14.2   29.0 / 21.5    80.8 /  51.9
+//    64,  8192        19.4 / 31.2     14.6 / 19.6   41.8 / 31.7    83.3 /  81.9
+//    96,  8192        22.1 / 39.6     15.6 / 23.8   43.5 / 40.8    86.1 / 108.2
+//   256,  8192        38.8 / 67.7     22.0 / 35.7   55.6 / 71.8   155.7 / 219.4
+// One number for all: bf16 behind a long prefix would gain from 16 rows on, fp32
+// behind a short one only past 256.
 constexpr int64_t kWideRows = 64;
 
 Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
@@ -711,8 +725,16 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
     const int64_t chunk = std::max(least, sw::ceil_div(n, parts));
     return std::min<int64_t>(sw::ceil_div(chunk, step) * step, 1 << 30);
   };
-  // Few keys are one part: a second one and the join of both cost more (one
-  // sequence, 260 keys: 6.1 + 3.5 us in two parts, 6.4 us in one).
+  // Few keys are one part: a second one and the join of both cost more (32 query
+  // heads over 8, bf16 of 128, one part / two, us: 300 keys of one sequence
+  // 11.0 / 11.9, of 32 sequences 11.4 / 16.2; 512 keys 13.7 / 12.1 and
+  // 16.5 / 17.0; 700 keys 17.4 / 12.1 and 20.8 / 20.4; fp32 of 64: 300 keys
+  // 12.2 / 12.2 and 12.7 / 17.4, 512 keys 15.5 / 12.4 and 18.8 / 18.1, 700 keys
+  // 20.4 / 12.5 and 24.9 / 22.2).
+  // The cut is by the keys that there is room for, which the host knows: much
+  // more room than keys makes few and long parts.  64 sequences of 4096 keys take
+  // 194 us with room for 4096 to 131,072; one takes 12.8, and 18.9 with room for
+  // 32,768, 55.9 for 131,072; four 19.7, 56.7 and 100.4.
   p.chunk = visible <= 512
                 ? 512
                 : cut(visible, sequences * key_heads * (p.rows / kRows), 512,

@@ -1085,8 +1085,8 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
 
 // CAREFUL is a function that is called and reads the kernel's arguments where
 // they lie: inlined beside the plain one it takes registers of its loop, and a
-// spilled register read back there waits for every copy under way (16,384
-// tokens, window 1024: 351 us, inlined 370 to 506 us).
+// spilled register read back there waits for every copy under way (a training
+// step of 16,384 tokens, window 1024: 707 us, inlined 752 us).
 template <typename T, int D, bool SINK>
 __device__ __noinline__ void key_gradient_again(const void *args, char *lds,
                                                 float *stats, int *verdict) {
@@ -1304,7 +1304,10 @@ int fill_window(WindowArgs &a, size_t elem, const int32_t *query_offsets,
 // 4096 queries, window 1024, bf16 heads of 128, one share / two: 4 heads (132
 // workgroups) 34.9 / 26.9 us, 8 heads (264) 39.5 / 36.0, 12 heads (396) 45.2 /
 // 51.7, 32 heads (1056) 93.1 / 113.7; 2501 queries of 12 heads (288), window
-// 2000: 63.9 / 72.8.
+// 2000: 63.9 / 72.8.  4, 8 and 12 heads of 64 in bf16 23.9 / 18.7, 24.6 / 21.3,
+// 29.0 / 36.7, in fp32 93 / 52, 95 / 77, 151 / 147; fp32 heads of 128, of which
+// the chip holds 256 workgroups, 167 / 101, 171 / 172, 332 / 257 (one number for
+// all: 12 of these would gain).
 int choose_streams(WindowArgs &a) {
   auto tiles = [&](int streams) {
     return ((int64_t)a.query_tokens >> shared_shift(streams)) + a.sequences;
@@ -1379,7 +1382,10 @@ Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
   // last round unsplit / split: 17,000 keys, bf16 heads of 128, 16 over 4 (532)
   // 702 / 573, 20,000 (628) 751 / 658, 16 over 16, 5120 keys (656) 231 / 219,
   // 4608 (592) 190 / 199; fp32 heads of 64, 16 over 8, 9000 keys (568)
-  // 813 / 707; within the numbers without keys, 8192 (520) 579 / 617.
+  // 813 / 707; within the numbers without keys, 8192 (520) 579 / 617.  Forward
+  // and backward in fp32, window 1024, one part / the rule's: 1000 tokens, 8
+  // heads over 4 of 64 384 / 153 us, of 128 709 / 277; 4096 tokens, 8 over 4 of
+  // 64 516 / 401, of 128 1017 / 1039, 24 over 8 of 64 1106 / 1068.
   const int64_t groups = ((key_tokens >> kRowShift) + sequences) * key_heads;
   const int64_t slots = elem == 4 && d > 64 ? 256 : 512;
   int64_t tail = groups % slots;
