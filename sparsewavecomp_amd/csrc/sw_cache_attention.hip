@@ -98,8 +98,9 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
 // not fetched ahead: the registers hold another wave a SIMD instead, whose
 // fetches go on meanwhile (64 sequences, window 4096: 201 us with two waves
 // and fetches ahead, 195 us with three; four waves' registers spill, 306 us).
-// Memory bounds it: those 64 read 5.6 TB/s, 4 sequences of 65,536 keys take
-// 173 us, 5.2 TB/s; one of 260 keys 6.4 us, a chain of trips.
+// Memory bounds it: those 64 read 5.5 TB/s, 4 sequences of 65,536 keys take
+// 170 us, 5.3 TB/s (a kernel that only reads: 6.5); one of 260 keys 6.8 us, a
+// chain of trips.
 template <typename T, int D> struct CacheParts {
   using Tile = RowTile<T, D, kTile, kWave>;
   static constexpr int kWaveBytes =

@@ -250,9 +250,10 @@ __device__ __forceinline__ bool add_shares(v16f (&acc)[BLOCKS], float &top,
 // o and log_sum of a tile of rows, in one pass over the keys that they see.
 // Matrix cores and the softmax's vector instructions bound it, the two waves
 // of a SIMD taking turns: 65,536 queries, window 4096, 16 bf16 heads of 128
-// take 2113 us, 1012 TFLOP/s (a large matrix product of the library: 1170),
-// the matrix cores half busy at 2.0 GHz; 16,384 queries, window 1024, 32 heads
-// 267 us.  Short calls wait for their chain of trips: 200 queries 7.3 us.
+// take 2100 to 2210 us from card to card, 970 to 1020 TFLOP/s (a large matrix
+// product of the library: 1170), the matrix cores half busy at 2.0 GHz; 16,384
+// queries, window 1024, 32 heads 269 us.  Short calls wait for their chain of
+// trips: 200 queries 7.1 us.
 // A tile's scores computed under the softmax of the one before it, the wave's
 // own turns overlapped, needs 32 registers more than there are: 2623 us.
 template <typename T, int D, int STREAMS>
@@ -534,7 +535,7 @@ __device__ __forceinline__ int sequence_of_far_block(const BackwardArgs &b,
 // dq of a tile of rows, and for the second kernel log_sum in powers of two
 // and delta of its rows.  The forward pass's loop with one product more:
 // ds^T = K Q^T and V dO^T element by element, dq^T += K^T ds^T.  16,384 tokens,
-// window 1024, 16 bf16 heads of 128 over 4: 229 us, the matrix cores 38 % busy
+// window 1024, 16 bf16 heads of 128 over 4: 233 us, the matrix cores 38 % busy
 // (its rows of go leave no registers to read ahead).
 template <typename T, int D, int STREAMS>
 __global__ __launch_bounds__(kThreads, (Forward<T, D, STREAMS>::kWaves)) void
@@ -722,9 +723,11 @@ window_query_gradient(BackwardArgs b) {
 // tiles of their queries are split into `parts`, one workgroup for each, whose
 // sums window_key_join adds up.
 //
-// 16,384 tokens, window 1024, 16 bf16 heads of 128 over 4: 307 us, the matrix
-// cores 34 % busy with four products a tile of 32 queries and one barrier (with
-// K and V both in registers, one wave a SIMD: 603), and the sinks 29 us.
+// 16,384 tokens, window 1024, 16 bf16 heads of 128 over 4: 308 us, the matrix
+// cores 35 % busy with four products a tile of 32 queries and one barrier (with
+// K and V both in registers, one wave a SIMD: 603), and the sinks 31 us, a chain
+// of few tiles: one wave a SIMD, the compiler having spilled 256 registers that
+// its tiles' loop moves about, 4 of a block's 32 keys being sinks.
 template <typename T, int D, bool SINK> struct Backward {
   static constexpr int kTile = 32; // queries
   using Tile = RowTile<T, D, kTile, SINK ? kWave : kThreads>;
