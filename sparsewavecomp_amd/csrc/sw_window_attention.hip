@@ -500,7 +500,6 @@ struct BackwardArgs {
   int far_blocks, sink_blocks; // blocks of all sequences, and the most of one
   int far_unit; // 0: far blocks are numbered by sequence; else window + 1
   bool far_by_key;
-  int join_rows; // workgroups of window_sink_gradient for a block
 };
 
 // A sequence's far sinks, those that a query sees from past its window: its
@@ -763,7 +762,7 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
   int64_t item;
   int part = 0, parts = 1;
   if constexpr (SINK) {
-    hk = (int)(blockIdx.x % a.key_heads);
+    hk = blockIdx.x % a.key_heads;
     item = blockIdx.x / a.key_heads; // the block of sums
     int chunk = 0, least = 0;        // of the sequence's queries
     if (item < b.far_blocks) {
@@ -773,8 +772,8 @@ __device__ __forceinline__ bool key_gradient_rows(const BackwardArgs &b,
     } else {
       // Later chunks of sequence i have the numbers from q0 >> chunk_shift on:
       // no more than whole chunks in its queries.
-      const int x = (int)((item - b.far_blocks) / b.sink_blocks);
-      key0 = (int)((item - b.far_blocks) % b.sink_blocks) * 32;
+      const int x = ((int)item - b.far_blocks) / b.sink_blocks;
+      key0 = ((int)item - b.far_blocks) % b.sink_blocks * 32;
       i = last_at_most(a.sequences, x, [&](int j) {
         return clamped(a.query_offsets[j], 0, a.query_tokens) >> b.chunk_shift;
       });
@@ -1112,79 +1111,79 @@ window_key_gradient(BackwardArgs b) {
 
 // The far sinks' gradients: the window's sums, or its parts', and every chunk's,
 // in the same order each time: eight runs of chunks, then the runs.  A workgroup
-// of 128 x 8 threads takes a block's far sinks of one key head in turns of
-// join_rows; a launch and its trips to the sums: 64 chunks of 6 sequences, 4
-// sinks of 4 heads 4.4 us.
+// of 128 x 8 threads for a far sink of one key head, 1 << shift of them a block; a
+// launch and its trips to the sums: 64 chunks of 6 sequences, 4 sinks of 4 heads
+// 4.2 us; 8 sequences of 64 sinks 10.5 us (with loops over a block's sinks and
+// heads in one workgroup 14).
 constexpr int kSinkRuns = 8;
 template <typename T>
 __global__ __launch_bounds__(128 * kSinkRuns) void
-window_sink_gradient(BackwardArgs b) {
+window_sink_gradient(BackwardArgs b, int shift) {
   const WindowArgs &a = b.w;
   __shared__ float sums[2][kSinkRuns][128];
-  const int turn = blockIdx.x % b.join_rows;
-  const int64_t item = blockIdx.x / b.join_rows;
-  const int hk = (int)(item % a.key_heads);
-  const int block = (int)(item / a.key_heads);
+  const int64_t id = block_id();
+  const uint32_t item = (uint32_t)(id >> shift), heads = a.key_heads;
+  const int hk = (int)(item % heads), block = (int)(item / heads);
+  if (block >= b.far_blocks)
+    return; // (a folded grid's last workgroups)
   const int i = sequence_of_far_block(b, block);
   const Sequence s = sequence(a, i);
   const int key0 = (block - first_far_block(b, i, s.k0)) * 32;
-  const int far = far_sinks(a, s);
-  if (key0 < 0 || key0 >= far)
+  const int row = (int)id & ((1 << shift) - 1), key = key0 + row;
+  if (key0 < 0 || key >= far_sinks(a, s))
     return;
-  const int end = far < key0 + 32 ? far : key0 + 32;
   const int run = threadIdx.x >> 7, c = threadIdx.x & 127;
-  // chunks that reach past the window: those from the first whose last query's
-  // place is at least a.window
-  const int chunks = s.nq == 0 ? 0 : ((s.nq - 1) >> b.chunk_shift) + 1;
-  const int past = a.window - (s.nk - s.nq); // query of that place
-  int begin = past <= 0 ? 0 : past >> b.chunk_shift;
-  if (past > s.nq - 1)
-    begin = chunks; // (no query is past the window)
-  // block of chunk 1's sums (chunk 0's is this one), and from chunk to chunk
-  const int64_t later = b.far_blocks + (key0 >> 5) +
-                        (int64_t)(s.q0 >> b.chunk_shift) * b.sink_blocks;
-  for (int key = key0 + turn; key < end; key += b.join_rows) {
-    const int64_t row = (int64_t)hk * 32 + (key - key0);
-    const int64_t pitch = (int64_t)a.key_heads * 32; // rows of a block
-    float dk = 0.0f, dv = 0.0f;
-    if (c < a.d)
-      for (int x = begin + run; x < chunks; x += kSinkRuns) {
-        const int64_t from =
-            x == 0 ? block : later + (int64_t)(x - 1) * b.sink_blocks;
-        const float *y = b.sink_chunks + (from * pitch + row) * 2 * a.d + c;
-        dk += y[0];
-        dv += y[a.d];
-      }
-    sums[0][run][c] = dk;
-    sums[1][run][c] = dv;
-    __syncthreads();
-    const int tile = (a.key_offsets[i] >> kRowShift) + i + (key >> kRowShift);
-    if (run == 0 && c < a.d && tile >= 0 && tile < b.key_tiles) {
-      // (tiles elsewhere: offsets outside the operands)
-      const int64_t at = (int64_t)hk * b.key_tiles + tile - b.whole;
-      const bool split = at >= 0;
-      const float *x = split ? b.part_sums + (at * kRows + (key & (kRows - 1))) *
-                                                 2 * a.d
-                             : b.sink_window + (block * pitch + row) * 2 * a.d;
-      const int64_t step = (int64_t)b.split * kRows * 2 * a.d;
-      dk = dv = 0.0f;
-      for (int p = 0; p < (split ? b.parts : 1); ++p) {
-        dk += x[p * step + c];
-        dv += x[p * step + a.d + c];
-      }
-#pragma unroll
-      for (int r = 0; r < kSinkRuns; ++r) {
-        dk += sums[0][r][c];
-        dv += sums[1][r][c];
-      }
-      const int64_t token = s.k0 + key;
-      stv(static_cast<T *>(b.key_gradient) + token * b.gk.token +
-              hk * b.gk.head + c, dk * a.alpha);
-      stv(static_cast<T *>(b.value_gradient) + token * b.gv.token +
-              hk * b.gv.head + c, dv);
+  const int64_t size = (int64_t)a.key_heads * 32 * 2 * a.d; // floats of a block
+  const int at = (hk * 32 + row) * 2 * a.d + c;             // in a block
+  float dk = 0.0f, dv = 0.0f;
+  if (c < a.d) {
+    // chunks that reach past the window: those from the first whose last
+    // query's place is at least a.window
+    const int chunks = s.nq == 0 ? 0 : ((s.nq - 1) >> b.chunk_shift) + 1;
+    const int past = a.window - (s.nk - s.nq); // query of that place
+    int x = past <= 0 ? 0 : past >> b.chunk_shift;
+    if (past > s.nq - 1)
+      x = chunks; // (no query is past the window)
+    // the sums of chunk 0 lie in this block, those of chunk x > 0 in
+    // later + x sink_blocks
+    const int64_t later = b.far_blocks + (key0 >> 5) +
+                          ((int64_t)(s.q0 >> b.chunk_shift) - 1) *
+                              b.sink_blocks;
+    for (x += run; x < chunks; x += kSinkRuns) {
+      const float *y =
+          b.sink_chunks +
+          (x == 0 ? block : later + (int64_t)x * b.sink_blocks) * size + at;
+      dk += y[0];
+      dv += y[a.d];
     }
-    __syncthreads();
   }
+  sums[0][run][c] = dk;
+  sums[1][run][c] = dv;
+  __syncthreads();
+  const int tile = (a.key_offsets[i] >> kRowShift) + i + (key >> kRowShift);
+  if (run != 0 || c >= a.d || tile < 0 || tile >= b.key_tiles)
+    return; // (tiles elsewhere: offsets outside the operands)
+  dk = dv = 0.0f;
+  const int64_t split = (int64_t)hk * b.key_tiles + tile - b.whole;
+  const bool whole = split < 0;
+  const float *x =
+      whole ? b.sink_window + block * size + at
+            : b.part_sums + (split * kRows + (key & (kRows - 1))) * 2 * a.d + c;
+  const int64_t step = (int64_t)b.split * kRows * 2 * a.d;
+  for (int p = 0; p < (whole ? 1 : b.parts); ++p) {
+    dk += x[p * step];
+    dv += x[p * step + a.d];
+  }
+#pragma unroll
+  for (int r = 0; r < kSinkRuns; ++r) {
+    dk += sums[0][r][c];
+    dv += sums[1][r][c];
+  }
+  const int64_t token = s.k0 + key;
+  stv(static_cast<T *>(b.key_gradient) + token * b.gk.token + hk * b.gk.head + c,
+      dk * a.alpha);
+  stv(static_cast<T *>(b.value_gradient) + token * b.gv.token +
+          hk * b.gv.head + c, dv);
 }
 
 // The sums of the parts of the keys that are no far sinks, in order: four elements
@@ -1360,7 +1359,7 @@ int forward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
 struct Scratch {
   int64_t stats, sink_window, sink_chunks, part_sums; // floats of each
   int64_t chunks, whole, split, far_blocks, sink_blocks, far_unit;
-  int parts, chunk_shift, join_rows;
+  int parts, chunk_shift, join_shift;
   bool far_by_key;
   int64_t bytes() const {
     return 4 * (2 * stats + sink_window + sink_chunks + part_sums);
@@ -1435,10 +1434,9 @@ Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
                  key_heads < 256)
     --c.chunk_shift;
   c.chunks = query_tokens >> c.chunk_shift;
-  // one far sink a workgroup of the join, more where there are many
-  c.join_rows = (int)std::min<int64_t>(
-      std::min<int64_t>(s, 32),
-      sw::ceil_div(2048, c.far_blocks * key_heads));
+  // places for a block's far sinks in the join's grid
+  while (c.join_shift < 5 && ((int64_t)1 << c.join_shift) < s)
+    ++c.join_shift;
   const int64_t one = key_heads * 32 * 2 * d;
   c.sink_window = c.far_blocks * one;
   c.sink_chunks = (c.far_blocks + c.chunks * c.sink_blocks) * one;
@@ -1446,7 +1444,7 @@ Scratch backward_scratch(int64_t sequences, int64_t query_tokens,
 }
 
 template <typename T, int D>
-int launch_backward(BackwardArgs &b, hipStream_t st) {
+int launch_backward(BackwardArgs &b, int join_shift, hipStream_t st) {
   WindowArgs &a = b.w;
   const char *what = "window attention's gradient";
   const int streams = choose_streams(a);
@@ -1456,11 +1454,11 @@ int launch_backward(BackwardArgs &b, hipStream_t st) {
   const int64_t keys = (int64_t)b.key_tiles * a.key_heads +
                        (int64_t)b.split * (b.parts - 1);
   const int64_t part_rows = (int64_t)b.split * kRows * (a.d / 4) / kThreads;
-  const int64_t join = (int64_t)b.far_blocks * a.key_heads * b.join_rows;
+  const int64_t join = ((int64_t)b.far_blocks * a.key_heads) << join_shift;
   if (int rc = sw::check_flat_grid(std::max({rows, sinks, keys, part_rows}),
                                    kThreads, what))
     return rc;
-  if (int rc = sw::check_flat_grid(join, 128 * kSinkRuns, what))
+  if (int rc = sw::check_grid(join, 128 * kSinkRuns, what))
     return rc;
   if (a.query_tokens > 0) {
     const dim3 g((unsigned)rows);
@@ -1488,9 +1486,9 @@ int launch_backward(BackwardArgs &b, hipStream_t st) {
     if (int rc = sw::launch_check(what))
       return rc;
   }
-  if (join > 0) {
-    window_sink_gradient<T>
-        <<<dim3((unsigned)join), 128 * kSinkRuns, 0, st>>>(b);
+  if (b.far_blocks > 0) {
+    window_sink_gradient<T><<<sw::grid_dim(join, 128 * kSinkRuns),
+                              128 * kSinkRuns, 0, st>>>(b, join_shift);
     return sw::launch_check(what);
   }
   return SW_OK;
@@ -1557,15 +1555,14 @@ int backward_entry(const int32_t *query_offsets, const int32_t *key_offsets,
   b.sink_blocks = (int)c.sink_blocks;
   b.far_unit = (int)c.far_unit;
   b.far_by_key = c.far_by_key;
-  b.join_rows = c.join_rows;
   b.part_sums = b.sink_chunks + c.sink_chunks;
   b.parts = c.parts;
   b.whole = (int)c.whole;
   b.split = (int)c.split;
   b.key_tiles = (int)((key_tokens >> kRowShift) + sequences);
   const hipStream_t st = sw::as_stream(stream);
-  return d <= 64 ? launch_backward<T, 64>(b, st)
-                 : launch_backward<T, 128>(b, st);
+  return d <= 64 ? launch_backward<T, 64>(b, c.join_shift, st)
+                 : launch_backward<T, 128>(b, c.join_shift, st);
 }
 
 } // namespace
