@@ -371,14 +371,15 @@ LARGE = [(0.125, 3.0e38), (4.0, 3.0e38), (0.0, 3.0e38), (0.0, 5.0e36),
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("alpha,size", LARGE)
-def test_decode_of_large_values(dev, dtype, alpha, size):
+def test_decode_of_large_values(dev, dtype, d, alpha, size):
     """Values whose weighted mean is finite while a sum of them is not, in one
     sequence; the others keep their bits."""
-    say(f"decode large values {dtype} {alpha} {size}")
+    say(f"decode large values {dtype} {d} {alpha} {size}")
     for lengths, window, sinks in (([128, 130], 200, 0), ([2000, 300], 1900, 4),
                                    ([9000, 8000], 10 ** 6, 0)):
-        x = make(dtype, lengths, 0, 4, 2, 64, seed=31)
+        x = make(dtype, lengths, 0, 4, 2, d, seed=31)
         clean = decode(x, alpha, window, sinks)
         v = large(x["values"][0], size, 32)
         x["values"][0] = v
@@ -430,10 +431,10 @@ def test_prefix_alpha(dev, dtype, alpha):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("alpha,size", LARGE)
-@pytest.mark.parametrize("n", [3, 40])
-def test_prefix_of_large_values(dev, dtype, alpha, size, n):
-    say(f"prefix large values {dtype} {alpha} {size} {n}")
-    x = make(dtype, [9] * n, 16, 4, 2, 64, seed=n, prefix=1000)
+@pytest.mark.parametrize("n,d", [(3, 64), (40, 64), (3, 128), (40, 128)])
+def test_prefix_of_large_values(dev, dtype, alpha, size, n, d):
+    say(f"prefix large values {dtype} {alpha} {size} {n} {d}")
+    x = make(dtype, [9] * n, 16, 4, 2, d, seed=n, prefix=1000)
     x["prefix_value"] = large(x["prefix_value"], size, 33)
     got = prefixed(x, alpha)
     assert torch.isfinite(got).all()

@@ -231,20 +231,20 @@ def test_forward_keeps_a_first_key_apart_that_is_no_sink(dev, dtype, bad, what,
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("heads", [2, 288])
+@pytest.mark.parametrize("heads,d", [(2, 64), (288, 64), (2, 128), (288, 128)])
 @pytest.mark.parametrize("alpha,size", [(0.125, 3.0e38), (4.0, 3.0e38),
                                         (0.0, 3.0e38), (0.0, 8.0e36)])
-def test_forward_of_large_values(dev, dtype, heads, alpha, size):
+def test_forward_of_large_values(dev, dtype, heads, d, alpha, size):
     """Values whose weighted mean is finite while a sum of them is not, in one
     head and sequence; the others keep their bits."""
-    say(f"window forward large values {dtype} {heads} {alpha} {size}")
-    x = list(inputs(dtype, [200, 40], [230, 40], heads, heads, 64, seed=21))
+    say(f"window forward large values {dtype} {heads} {d} {alpha} {size}")
+    x = list(inputs(dtype, [200, 40], [230, 40], heads, heads, d, seed=21))
     clean, clean_lse = forward(*x, alpha, 60, 2)
     gen = torch.Generator().manual_seed(22)
     v = x[4].clone()
-    v[:230, 1] = ((0.5 + torch.rand(230, 64, generator=gen) / 2) * size).to(
+    v[:230, 1] = ((0.5 + torch.rand(230, d, generator=gen) / 2) * size).to(
         v.dtype)
-    v[:230, 1, 32:] *= -1
+    v[:230, 1, d // 2:] *= -1
     x[4] = v
     out, lse = forward(*x, alpha, 60, 2)
     assert torch.isfinite(out).all()
