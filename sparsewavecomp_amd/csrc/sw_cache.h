@@ -1,0 +1,281 @@
+// What the kernels of single queries against a key-value cache share: which
+// keys a query sees, a part's result and the join of the parts, and the host's
+// checks.
+//
+// A sequence's keys are cut into chunks, one workgroup each, and the chunks'
+// (m, l, o) joined:
+//   m = max m_c,  w_c = l_c 2^(m_c - m),  l = sum w_c,  o = sum o_c w_c / l,
+// o_c being a chunk's weighted mean: sums of values, which fp32 may not hold
+// where their mean is finite, stay within a chunk, which sees whether they did.
+#pragma once
+
+#include "sw_heads.h"
+#include "sw_internal.h"
+
+#include <algorithm>
+#include <cmath>
+
+using namespace swd;
+using sw::Operand;
+using sw::check_operand;
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kInf = __builtin_inff();
+// the maximum of keys whose scores are all -inf: the result is NaN then, where
+// it is zero without a key (a maximum of -inf)
+constexpr float kLowest = -3.402823466e+38f;
+constexpr int kThreads = 256; // four waves
+constexpr int kRows = 16;     // query rows of a workgroup's part
+constexpr int kTile = 32;     // keys a wave takes at a time
+
+// what lanes without a key read
+__device__ const uint32_t kZeros[8] = {};
+
+struct Cache {
+  const void *key, *value;
+  int64_t key_page, key_token, key_head; // strides in elements
+  int64_t value_page, value_token, value_head;
+};
+
+struct StepArgs {
+  const int32_t *lengths, *table; // table may be null: page i is sequence i's
+  const void *query;
+  void *output;
+  Cache cache, prefix; // (the prefix: one page)
+  int64_t query_token, query_head, output_token, output_head;
+  int sequences, pages, page_size, table_width;
+  int query_heads, key_heads, group, d, dim; // dim: d padded to 64 or 128
+  int window, sinks, prefix_tokens;
+  float alpha;
+  // Parts of `chunk` keys: `parts` at most for a sequence, `prefix_parts` of
+  // the prefix, whose query rows are those of all sequences.  A part of rows
+  // leaves o in [part][rows][dim] and (m, l) in [part][rows][2].
+  int chunk, parts, prefix_chunk, prefix_parts;
+  int rows, prefix_rows; // of one part: a multiple of 16, of 16 or 128
+  // a power of two: the number of all keys times it is below 1
+  float lower;
+  float *sums, *stats, *prefix_sums, *prefix_stats;
+  // workgroups of the prefix: by cache_part and by prefix_part
+  int64_t prefix_items, wide_items;
+};
+
+// The keys that sequence i's query sees: the first `lead`, and those from
+// `start` on, `count` in all.
+struct Visible {
+  int lead, start, count;
+  __device__ __forceinline__ Visible(const StepArgs &a, int i) {
+    const int64_t room = (int64_t)a.page_size * a.table_width;
+    int n = a.lengths[i];
+    n = n < 0 ? 0 : n > room ? (int)room : n;
+    start = n > a.window ? n - a.window : 0;
+    lead = a.sinks < start ? a.sinks : start;
+    count = lead + n - start;
+  }
+  __device__ __forceinline__ int key(int v) const {
+    return v < lead ? v : v - lead + start;
+  }
+};
+
+__device__ __forceinline__ float rows16_max(float v) { // over lanes l % 16
+  return both_halves_max(fmaxf(v, swizzle_xor16(v)));
+}
+__device__ __forceinline__ float rows16_sum(float v) {
+  return both_halves_sum(v + swizzle_xor16(v));
+}
+struct Totals {
+  float top[4][kRows], sum[4][kRows], raise[4][kRows];
+};
+
+// The four waves' results of one part of the keys, joined in LDS and written:
+// as the output where the part is the `only` one, else to `sums` and `stats`.
+// acc: o[row][d] of a wave, which it leaves in its own WAVE_BYTES of `lds`.
+template <typename T, int D, int WAVE_BYTES>
+__device__ __forceinline__ void
+store_part(const StepArgs &a, char *lds, Totals &found, float top, float sum,
+           float raise, const v4f (&acc)[D / 16], int rows, bool only, int seq,
+           int hk, int first_row, float *sums, float *stats) {
+  const int lane = lane_id(), g = lane >> 4, wave = wave_in_group();
+  sum = rows16_sum(sum);
+  if (g == 0) {
+    found.top[wave][lane] = top;
+    found.sum[wave][lane] = sum;
+    found.raise[wave][lane] = raise;
+  }
+  // o[row][d] of each wave, in its own part of LDS
+#pragma unroll
+  for (int b = 0; b < D / 16; ++b)
+    lds_write(lds_address(lds) + wave * WAVE_BYTES +
+                  ((lane & 15) * D + 16 * b + 4 * g) * 4, acc[b]);
+  __syncthreads();
+  for (int x = threadIdx.x; x < kRows * D / 4; x += kThreads) {
+    const int r = x / (D / 4), c = x % (D / 4) * 4;
+    if (r >= rows)
+      break;
+    float m = found.top[0][r], most = found.raise[0][r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      m = fmaxf(m, found.top[w][r]);
+      most = fmaxf(most, found.raise[w][r]);
+    }
+    most += 3.0f; // (four sums that are finite have a finite sum)
+    float l = 0.0f;
+    v4f o = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float by =
+          found.top[w][r] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(found.top[w][r] - m);
+      by *= __builtin_amdgcn_exp2f(found.raise[w][r] - most);
+      const v4f y =
+          lds_read<v4f>(lds_address(lds) + w * WAVE_BYTES + (r * D + c) * 4, 0);
+      l = fmaf(found.sum[w][r], by, l);
+      o += y * by;
+    }
+    if (only) {
+      if (c < a.d) {
+        const bool empty = m == -kInf;
+        const float by = 1.0f / l;
+        T *out = static_cast<T *>(a.output) + seq * a.output_token +
+                 (hk * a.group + first_row + r) * a.output_head + c;
+        st4(out, empty ? 0.0f : o[0] * by, empty ? 0.0f : o[1] * by,
+            empty ? 0.0f : o[2] * by, empty ? 0.0f : o[3] * by);
+      }
+    } else {
+      if (l != 0.0f) // (zero: no key, or scores of -inf alone)
+        o *= 1.0f / l;
+      *reinterpret_cast<v4f *>(sums + r * D + c) = o;
+      if (c == 0) {
+        stats[2 * r] = m;
+        stats[2 * r + 1] = l * __builtin_amdgcn_exp2f(most);
+      }
+    }
+  }
+}
+
+// Joins the parts of a query head's softmax: one workgroup for each, whose
+// eight half waves take the parts in turn, DIM / 32 consecutive elements a
+// lane, and are joined in LDS.  A launch and two trips: 16 parts of 4 sequences
+// and 32 heads 4.4 us, 128 sequences' 8.4 us.
+template <typename T, int DIM>
+__global__ __launch_bounds__(kThreads) void window_cache_join(StepArgs a) {
+  constexpr int N = DIM / 32, kHalves = kThreads / 32;
+  __shared__ float outs[kHalves][DIM], tops[kHalves], totals[kHalves];
+  const int seq = (int)(blockIdx.x / a.query_heads);
+  const int head = (int)(blockIdx.x % a.query_heads);
+  const int hk = head / a.group, row = head % a.group;
+  const Visible see(a, seq);
+  const int own = see.count == 0 ? 0 : (see.count - 1) / a.chunk + 1;
+  const int parts = own + a.prefix_parts;
+  const int half = threadIdx.x / 32, c = (threadIdx.x % 32) * N;
+  float top = -kInf, l = 0.0f, o[N] = {};
+#pragma unroll 4
+  for (int i = half; i < parts; i += kHalves) {
+    // row of part i in the buffers of sums and statistics
+    const int64_t r =
+        i < own ? (((int64_t)seq * a.key_heads + hk) * a.parts + i) * a.rows + row
+                : ((int64_t)hk * a.prefix_parts + i - own) * a.prefix_rows +
+                      (int64_t)seq * a.group + row;
+    const float *sums = (i < own ? a.sums : a.prefix_sums) + r * DIM + c;
+    const float *stats = (i < own ? a.stats : a.prefix_stats) + r * 2;
+    const float m = stats[0], to = fmaxf(top, m);
+    const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+    const float add = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    const float weight = stats[1] * a.lower * add;
+    top = to;
+    l = fmaf(l, by, weight);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      o[e] = fmaf(sums[e], weight, o[e] * by);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    outs[half][c + e] = o[e];
+  if (threadIdx.x % 32 == 0) {
+    tops[half] = top;
+    totals[half] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x >= a.d)
+    return;
+  top = tops[0];
+#pragma unroll
+  for (int i = 1; i < kHalves; ++i)
+    top = fmaxf(top, tops[i]);
+  float x = 0.0f;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kHalves; ++i) {
+    const float by =
+        tops[i] == top ? 1.0f : __builtin_amdgcn_exp2f(tops[i] - top);
+    l = fmaf(totals[i], by, l);
+    x = fmaf(outs[i][threadIdx.x], by, x);
+  }
+  stv(static_cast<T *>(a.output) + seq * a.output_token +
+          head * a.output_head + threadIdx.x,
+      top == -kInf ? 0.0f : x * (1.0f / l));
+}
+
+// ---- host ------------------------------------------------------------------------
+
+// The keys that a query sees at most.
+inline int64_t most_visible(int64_t capacity, int64_t window, int64_t sinks) {
+  return window >= capacity || sinks >= capacity - window ? capacity
+                                                          : window + sinks;
+}
+
+// How many keys a part has: n keys for each of `units` workgroups at a time, of
+// which `want` are wanted, in steps, `least` at least.
+inline int64_t part_of(int64_t n, int64_t units, int64_t want, int64_t least,
+                       int64_t step) {
+  const int64_t parts = std::max<int64_t>(1, sw::ceil_div(want, units));
+  const int64_t chunk = std::max(least, sw::ceil_div(n, parts));
+  return std::min<int64_t>(sw::ceil_div(chunk, step) * step, 1 << 30);
+}
+
+int check_sizes(int64_t sequences, int64_t pages, int64_t page_size,
+                int64_t table_width, int64_t query_heads, int64_t key_heads,
+                int64_t d, int64_t window, int64_t sinks,
+                int64_t prefix_tokens, float alpha) {
+  if (sequences < 0 || pages < 0 || page_size < 1 || table_width < 1 ||
+      prefix_tokens < 0 || sequences > (1 << 24) || pages > sw::kMostTokens ||
+      page_size > sw::kMostTokens || prefix_tokens > sw::kMostTokens ||
+      table_width > sw::kMostTokens / page_size)
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "expected up to 2^24 sequences, and pages of a size and a "
+                    "table of a width that hold up to 2^30 keys, but got "
+                    "%lld, %lld, %lld, %lld and a prefix of %lld",
+                    (long long)sequences, (long long)pages,
+                    (long long)page_size, (long long)table_width,
+                    (long long)prefix_tokens);
+  if (int rc = sw::check_heads(query_heads, key_heads, d))
+    return rc;
+  if (window < 1 || sinks < 0)
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "expected a window of at least 1 and no negative sinks, "
+                    "but got %lld and %lld", (long long)window,
+                    (long long)sinks);
+  // (scores are scaled by alpha log2 e)
+  if (!std::isfinite(alpha * kLog2e))
+    return sw::fail(SW_ERR_INVALID_ARGUMENT,
+                    "alpha must be finite, and alpha log2 e too");
+  return SW_OK;
+}
+
+int check_pages(const char *name, const void *p, int64_t page, int64_t token,
+                int64_t head, int64_t d, int64_t elem, int64_t pages,
+                int64_t heads) {
+  if (pages > 0 && (page < 0 || page > sw::kMostStride))
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "%s page stride must be 0 to 2^40, but got %lld", name,
+                    (long long)page);
+  if (int rc = check_operand(name, p, {token, head}, d, elem, false, pages,
+                             heads))
+    return rc;
+  if (pages > 0 && page * elem % 16 != 0)
+    return sw::fail(SW_ERR_INVALID_ARGUMENT,
+                    "%s must be 16-byte aligned, its strides included", name);
+  return SW_OK;
+}
+
+} // namespace
