@@ -616,6 +616,149 @@ int sw_shared_prefix_attention_bf16(
     int64_t workspace_bytes, void *stream);
 
 /*
+ * Rotary positions, an operator without a counterpart in the reference: the
+ * pairs of each head's first 2 * pairs elements turned by an angle,
+ *   (x, y) -> (x cos t - y sin t, x sin t + y cos t),
+ *   t = positions[axis][token] * frequencies[pair],
+ * the other elements copied.  A pair is elements i and i + pairs of a head, or,
+ * interleaved, 2 i and 2 i + 1.  positions[axes][tokens] holds a token's place
+ * on every axis (of a text one, of a clip time, height and width) and
+ * pair_axes[pairs] which of them a pair turns with (NULL: all with axis 0; a
+ * pair whose axis is outside 0 .. axes - 1 is copied).
+ *
+ * query[tokens][query_heads][d] and key[tokens][key_heads][d] (key_heads 0: no
+ * key) and their outputs, d a multiple of 8 up to 128, pairs from 1 to d / 2.
+ * `strides` holds the token and head stride, in elements, of query, key, query
+ * output and key output (NULL: as the shapes), rows and strides 16-byte aligned.
+ * An output may be its own input, with the same strides; otherwise it shares no
+ * memory with an input.  Angles are formed in 64 bits (cosine and sine to
+ * 2^-23 for angles up to 2^31), the rest in fp32, each result rounded once.
+ *
+ * The backward entry points turn the outputs' gradients back, by -t: the
+ * gradients of query and key.  The positions and frequencies have none.
+ */
+int sw_rotary_f32(const int32_t *positions, const float *frequencies,
+                  const int32_t *pair_axes, const float *query,
+                  const float *key, float *query_output, float *key_output,
+                  int64_t tokens, int64_t axes, int64_t query_heads,
+                  int64_t key_heads, int64_t d, int64_t pairs, int interleaved,
+                  const int64_t *strides, void *stream);
+int sw_rotary_bf16(const int32_t *positions, const float *frequencies,
+                   const int32_t *pair_axes, const uint16_t *query,
+                   const uint16_t *key, uint16_t *query_output,
+                   uint16_t *key_output, int64_t tokens, int64_t axes,
+                   int64_t query_heads, int64_t key_heads, int64_t d,
+                   int64_t pairs, int interleaved, const int64_t *strides,
+                   void *stream);
+int sw_rotary_backward_f32(
+    const int32_t *positions, const float *frequencies,
+    const int32_t *pair_axes, const float *query_output_gradient,
+    const float *key_output_gradient, float *query_gradient,
+    float *key_gradient, int64_t tokens, int64_t axes, int64_t query_heads,
+    int64_t key_heads, int64_t d, int64_t pairs, int interleaved,
+    const int64_t *strides, void *stream);
+int sw_rotary_backward_bf16(
+    const int32_t *positions, const float *frequencies,
+    const int32_t *pair_axes, const uint16_t *query_output_gradient,
+    const uint16_t *key_output_gradient, uint16_t *query_gradient,
+    uint16_t *key_gradient, int64_t tokens, int64_t axes, int64_t query_heads,
+    int64_t key_heads, int64_t d, int64_t pairs, int interleaved,
+    const int64_t *strides, void *stream);
+
+/*
+ * A key-value cache of 4-bit codes (no counterpart in the reference).  A row of
+ * d elements, d a multiple of 32 up to 128, is d / 2 bytes of codes, element
+ * 2 j in the low half of byte j, and d / 32 scale bytes, one a block of 32.  A
+ * code is a sign bit over one of the sizes 0, 1/2, 1, 3/2, 2, 3, 4, 6 (E2M1);
+ * the scale byte b stands for 2^(b - 127), 255 for NaN (E8M0).  Writing takes
+ * as a block's scale the smallest power of two from 2^-125 to 2^125 that 7 times
+ * covers its largest size, and rounds each element to the nearest code, ties to
+ * the even one, sizes past 6 to 6.  A block with an infinity or NaN gets 255
+ * and reads as NaN.  Reading gives code times scale, which bf16 and fp32 hold
+ * exactly for scales that were written.
+ *
+ * Codes are [pages][page_size][key_heads][d / 2], scales [..][d / 32], for keys
+ * and for values; place j of sequence i is row j % page_size of page
+ * page_table[i][j / page_size], page_table[sequences][table_width], which may
+ * be NULL: sequence i then has page i to itself.  `strides` holds sixteen: the
+ * token and head stride of key and of value in elements, then in bytes the
+ * page, token and head stride of the key codes, the key scales, the value codes
+ * and the value scales (NULL: as the shapes above).  Rows of codes start on 16
+ * bytes, a token stride is at least a row and at most 2^23 bytes; pages that
+ * hold a head's rows together are read fastest.  What a call writes must not
+ * overlap: strides that let rows share memory are refused.
+ *
+ * sw_fp4_cache_write: sequence i has the packed tokens token_offsets[i] ..
+ * token_offsets[i+1] - 1 of key and value [tokens][key_heads][d], which are the
+ * last of its key_lengths[i] keys.  A token whose place is negative, past the
+ * table's row or on a page outside 0 .. pages - 1 is not written, and neither
+ * is any other byte of the cache.  Two tokens of one place leave either.
+ *
+ * sw_fp4_cache_read: the tokens of sequence i are its places starts[i],
+ * starts[i] + 1, ... (starts NULL: from 0 on), written to key and value.  A
+ * place that is not there (as above) gives zeros.  Tokens of no sequence are
+ * left as they were.
+ */
+int sw_fp4_cache_write_f32(
+    const int32_t *token_offsets, const int32_t *key_lengths,
+    const int32_t *page_table, const float *key, const float *value,
+    uint8_t *key_codes, uint8_t *key_scales, uint8_t *value_codes,
+    uint8_t *value_scales, int64_t sequences, int64_t tokens, int64_t pages,
+    int64_t page_size, int64_t table_width, int64_t key_heads, int64_t d,
+    const int64_t *strides, void *stream);
+int sw_fp4_cache_write_bf16(
+    const int32_t *token_offsets, const int32_t *key_lengths,
+    const int32_t *page_table, const uint16_t *key, const uint16_t *value,
+    uint8_t *key_codes, uint8_t *key_scales, uint8_t *value_codes,
+    uint8_t *value_scales, int64_t sequences, int64_t tokens, int64_t pages,
+    int64_t page_size, int64_t table_width, int64_t key_heads, int64_t d,
+    const int64_t *strides, void *stream);
+int sw_fp4_cache_read_f32(
+    const int32_t *token_offsets, const int32_t *starts,
+    const int32_t *page_table, const uint8_t *key_codes,
+    const uint8_t *key_scales, const uint8_t *value_codes,
+    const uint8_t *value_scales, float *key, float *value, int64_t sequences,
+    int64_t tokens, int64_t pages, int64_t page_size, int64_t table_width,
+    int64_t key_heads, int64_t d, const int64_t *strides, void *stream);
+int sw_fp4_cache_read_bf16(
+    const int32_t *token_offsets, const int32_t *starts,
+    const int32_t *page_table, const uint8_t *key_codes,
+    const uint8_t *key_scales, const uint8_t *value_codes,
+    const uint8_t *value_scales, uint16_t *key, uint16_t *value,
+    int64_t sequences, int64_t tokens, int64_t pages, int64_t page_size,
+    int64_t table_width, int64_t key_heads, int64_t d, const int64_t *strides,
+    void *stream);
+
+/*
+ * sw_window_attention_decode against such a cache: the same keys seen, lengths,
+ * page table, clamps, workspace rules and arithmetic.  A page number outside
+ * the cache means that its keys are not there.  `strides` holds sixteen: the
+ * token and head stride of query and of output in elements, then the cache's as
+ * above.  fp32 queries meet the codes' values without a rounding (three bf16
+ * parts each), and so do their probabilities.
+ */
+int64_t sw_window_attention_decode_fp4_workspace_bytes(
+    int64_t sequences, int64_t page_size, int64_t table_width,
+    int64_t query_heads, int64_t key_heads, int64_t d, int64_t window,
+    int64_t sinks);
+int sw_window_attention_decode_fp4_f32(
+    const int32_t *key_lengths, const int32_t *page_table, const float *query,
+    const uint8_t *key_codes, const uint8_t *key_scales,
+    const uint8_t *value_codes, const uint8_t *value_scales, float *output,
+    int64_t sequences, int64_t pages, int64_t page_size, int64_t table_width,
+    int64_t query_heads, int64_t key_heads, int64_t d, const int64_t *strides,
+    int64_t window, int64_t sinks, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream);
+int sw_window_attention_decode_fp4_bf16(
+    const int32_t *key_lengths, const int32_t *page_table,
+    const uint16_t *query, const uint8_t *key_codes, const uint8_t *key_scales,
+    const uint8_t *value_codes, const uint8_t *value_scales, uint16_t *output,
+    int64_t sequences, int64_t pages, int64_t page_size, int64_t table_width,
+    int64_t query_heads, int64_t key_heads, int64_t d, const int64_t *strides,
+    int64_t window, int64_t sinks, float alpha, void *workspace,
+    int64_t workspace_bytes, void *stream);
+
+/*
  * sparsewave.csr_row_at_position for a batch of positions:
  * out_rows[i] = (first j in [1, rows+1) with row_offsets[j] > positions[i]) - 1,
  * the row search of SparsePositionToSCF.cpp:225-271 that the position

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from typing import Any, NamedTuple
 
 __all__ = [
     "Options", "SparseWaveError", "ShapeError", "library_path",
@@ -22,7 +23,9 @@ __all__ = [
     "spmm", "bsr_spmm", "sddmm", "csr_row_reduce", "csr_rowwise_map",
     "sparse_attention", "window_attention",
     "window_attention_backward", "window_attention_decode",
-    "shared_prefix_attention", "csr_row_at_position",
+    "shared_prefix_attention", "rotary", "rotary_backward", "Fp4Rows",
+    "fp4_cache", "fp4_cache_write", "fp4_cache_read",
+    "window_attention_decode_fp4", "csr_row_at_position",
     "SDDMM_MUL", "SDDMM_AFFINE", "SDDMM_DOT", "MAP_EXP_SUB", "MAP_DIV",
     "MAP_SUB", "MAP_MUL",
 ]
@@ -52,6 +55,12 @@ EXPORTED_SYMBOLS = (
     "sw_shared_prefix_attention_workspace_bytes",
     "sw_shared_prefix_attention_f32", "sw_shared_prefix_attention_bf16",
     "sw_window_attention_backward_f32", "sw_window_attention_backward_bf16",
+    "sw_rotary_f32", "sw_rotary_bf16", "sw_rotary_backward_f32",
+    "sw_rotary_backward_bf16", "sw_fp4_cache_write_f32",
+    "sw_fp4_cache_write_bf16", "sw_fp4_cache_read_f32",
+    "sw_fp4_cache_read_bf16", "sw_window_attention_decode_fp4_workspace_bytes",
+    "sw_window_attention_decode_fp4_f32",
+    "sw_window_attention_decode_fp4_bf16",
     "sw_csr_row_at_position", "sw_attention_tile_floor",
     "sw_host_matrix_free", "sw_host_bsr_free", "sw_matrix_market_read",
     "sw_csr_binary_write", "sw_coo_binary_write", "sw_csr_binary_read",
@@ -190,6 +199,14 @@ def load_library():
             ctypes.c_int, [P] * 6 + [I64] * 7 + [P, I64, I64, F, P, I64, P])
         sig["sw_shared_prefix_attention" + dt] = (
             ctypes.c_int, [P] * 8 + [I64] * 8 + [P, F, P, I64, P])
+        for name in ("sw_rotary", "sw_rotary_backward"):
+            sig[name + dt] = (
+                ctypes.c_int, [P] * 7 + [I64] * 6 + [ctypes.c_int, P, P])
+        for name in ("sw_fp4_cache_write", "sw_fp4_cache_read"):
+            sig[name + dt] = (ctypes.c_int, [P] * 9 + [I64] * 7 + [P, P])
+        sig["sw_window_attention_decode_fp4" + dt] = (
+            ctypes.c_int, [P] * 8 + [I64] * 7 + [P, I64, I64, F, P, I64, P])
+    sig["sw_window_attention_decode_fp4_workspace_bytes"] = (I64, [I64] * 8)
     sig["sw_window_attention_backward_workspace_bytes"] = (
         I64, [I64] * 8 + [ctypes.c_int])
     sig["sw_window_attention_decode_workspace_bytes"] = (I64, [I64] * 8)
@@ -649,14 +666,15 @@ def sparse_attention(row_offsets, column_indices, mask_values, query,
     return output
 
 
-def _heads(dtype, at, *named):
+def _heads(dtype, at, *named, always=False):
     """Addresses and strides of [rows, heads, d] operands, given as tensor and
     name in turn, whose rows of d elements are consecutive, on device `at`:
     a list of addresses, and the (row, head) strides of all as a C array, of
     [pages, rows, heads, d] the page's before them; None where every operand is
-    packed, which is what the C functions take it for."""
+    packed, which is what the C functions take it for.  `always`: a list of the
+    strides instead, of packed operands too."""
     torch = _torch or _load_torch()
-    pointers, packed = [], True
+    pointers, packed = [], not always
     for t, name in zip(named[::2], named[1::2]):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
@@ -688,6 +706,8 @@ def _heads(dtype, at, *named):
         if page and t.shape[0] == 1:
             page = [0]
         strides += [*page, row, head]
+    if always:
+        return pointers, strides
     return pointers, (ctypes.c_int64 * len(strides))(*strides)
 
 
@@ -911,6 +931,214 @@ def shared_prefix_attention(key_lengths, page_table, query, prefix_key,
     _check(_fn("sw_shared_prefix_attention", dt)(
         lengths, table, q, pk, pv, k, v, o, shape[0], prefix_key.shape[0],
         *shape[1:], strides, alpha,
+        None if scratch is None else scratch.data_ptr(), need,
+        _stream(stream)))
+    return output
+
+
+def _rotary(back, positions, frequencies, pair_axes, operands, interleaved,
+            stream):
+    torch = _torch or _load_torch()
+    (query, _), (key, _), (query_to, query_name), (key_to, key_name) = operands
+    _need(query.dim() == 3 and query_to.shape == query.shape,
+          f"expected {operands[0][1]} and {query_name} [tokens, query_heads, "
+          "d]")
+    tokens, heads, d = query.shape
+    _need((key is None) == (key_to is None) and
+          (key is None or key.dim() == 3 and key_to.shape == key.shape and
+           key.shape[::2] == query.shape[::2]),
+          f"expected {operands[1][1]} and {key_name} [tokens, key_heads, d], "
+          "or None for both")
+    _need(positions.dim() == 2 and positions.shape[1] == tokens,
+          "positions must be [axes, tokens]")
+    _need(frequencies.dim() == 1, "frequencies must be [pairs]")
+    _need(pair_axes is None or pair_axes.shape == frequencies.shape,
+          "pair_axes must be [pairs]")
+    dt = _value_dtype(query, operands[0][1])
+    at = _device_of(stream)
+    if key is None:
+        (q, qo), s = _heads(dt, at, *operands[0], *operands[2])
+        k = ko = None
+        if s is not None:
+            s = (ctypes.c_int64 * 8)(s[0], s[1], 0, 0, s[2], s[3], 0, 0)
+    else:
+        (q, k, qo, ko), s = _heads(dt, at, *operands[0], *operands[1],
+                                   *operands[2], *operands[3])
+    _check(_fn("sw_rotary_backward" if back else "sw_rotary", dt)(
+        _flat(positions, torch.int32, at, "positions"),
+        _flat(frequencies, torch.float32, at, "frequencies"),
+        None if pair_axes is None else
+        _flat(pair_axes, torch.int32, at, "pair_axes"), q, k, qo, ko, tokens,
+        positions.shape[0], heads, 0 if key is None else key.shape[1], d,
+        frequencies.shape[0], bool(interleaved), s, _stream(stream)))
+    return query_to, key_to
+
+
+def rotary(positions, frequencies, pair_axes, query, key, query_output,
+           key_output, interleaved=False, stream=None):
+    """Rotary positions of one or several axes (no counterpart in the
+    reference): the pairs of each head of query [tokens, query_heads, d] and
+    key [tokens, key_heads, d] turned by positions[axis, token] *
+    frequencies[pair], (x, y) -> (x cos - y sin, x sin + y cos).
+
+    positions [axes, tokens] int32, frequencies [pairs] float32, pair_axes
+    [pairs] int32, each pair's axis (None: 0 for all).  Pairs are elements i and
+    i + pairs of a head, interleaved 2 i and 2 i + 1; the other elements are
+    copied.  d is a multiple of 8 up to 128.  float32 or bfloat16, any strides
+    of 16 bytes; an output may be its input.  key and key_output may be None."""
+    return _rotary(False, positions, frequencies, pair_axes,
+                   ((query, "query"), (key, "key"),
+                    (query_output, "query_output"),
+                    (key_output, "key_output")), interleaved, stream)
+
+
+def rotary_backward(positions, frequencies, pair_axes, query_output_gradient,
+                    key_output_gradient, query_gradient, key_gradient,
+                    interleaved=False, stream=None):
+    """The gradients of :func:`rotary`'s query and key from those of its
+    outputs: turned back.  A gradient may be written over its input."""
+    return _rotary(True, positions, frequencies, pair_axes,
+                   ((query_output_gradient, "query_output_gradient"),
+                    (key_output_gradient, "key_output_gradient"),
+                    (query_gradient, "query_gradient"),
+                    (key_gradient, "key_gradient")), interleaved, stream)
+
+
+class Fp4Rows(NamedTuple):
+    """Keys or values of a 4-bit cache: codes [pages, page_size, heads, d // 2]
+    and scales [pages, page_size, heads, d // 32], uint8."""
+    codes: Any
+    scales: Any
+
+
+def fp4_cache(pages, page_size, heads, d, device=None):
+    """The keys (or values) of an empty 4-bit cache, :class:`Fp4Rows` of zeros
+    on `device` (None: the current one).  A page holds each head's rows
+    together, which the token step reads fastest."""
+    torch = _torch or _load_torch()
+    _need(d % 32 == 0 and 32 <= d <= 128,
+          "head dimension of a 4-bit cache must be 32, 64, 96 or 128")
+    return Fp4Rows(*(
+        torch.zeros(pages, heads, page_size, width, dtype=torch.uint8,
+                    device="cuda" if device is None else device).transpose(
+                        1, 2) for width in (d // 2, d // 32)))
+
+
+def _fp4_rows(at, d, key_cache, value_cache):
+    """(pages, page_size, heads), addresses and strides of a 4-bit cache."""
+    torch = _torch or _load_torch()
+    (kc, ks), (vc, vs) = key_cache, value_cache
+    shape = kc.shape
+    if len(shape) != 4 or vc.shape != shape or shape[3] * 2 != d or \
+            ks.shape != vs.shape or ks.shape[:3] != shape[:3] or \
+            ks.dim() != 4 or ks.shape[3] * 32 != d:
+        raise ShapeError(
+            "expected key and value caches of codes [pages, page_size, "
+            "key_heads, d / 2] and scales [pages, page_size, key_heads, "
+            "d / 32]")
+    return shape[:3], *_heads(
+        torch.uint8, at, kc, "key_cache codes", ks, "key_cache scales", vc,
+        "value_cache codes", vs, "value_cache scales", always=True)
+
+
+def _table_width(page_table, sequences):
+    if page_table is None:
+        return 1
+    if page_table.dim() != 2 or page_table.shape[0] != sequences:
+        raise ShapeError("page_table must be [sequences, most_pages]")
+    return page_table.shape[1]
+
+
+def _fp4_move(name, token_offsets, per_sequence, page_table, key_cache,
+              value_cache, key, value, stream):
+    torch = _torch or _load_torch()
+    if len(key.shape) != 3 or value.shape != key.shape:
+        raise ShapeError("expected key and value [tokens, key_heads, d]")
+    tokens, heads, d = key.shape
+    sequences = _rows_of(token_offsets, "token_offsets")
+    which = "key_lengths" if name == "sw_fp4_cache_write" else "starts"
+    if per_sequence is not None and per_sequence.shape != (sequences,):
+        raise ShapeError(f"{which} must hold one number a sequence")
+    width = _table_width(page_table, sequences)
+    dt = _value_dtype(key, "key")
+    at = _device_of(stream)
+    (pages, size, of), rows, row_strides = _fp4_rows(at, d, key_cache,
+                                                     value_cache)
+    _need(of == heads, "key and value must have the cache's heads")
+    moved, strides = _heads(dt, at, key, "key", value, "value", always=True)
+    strides = (ctypes.c_int64 * 16)(*strides, *row_strides)
+    pointers = moved + rows if name == "sw_fp4_cache_write" else rows + moved
+    _check(_fn(name, dt)(
+        _flat(token_offsets, torch.int32, at, "token_offsets"),
+        None if per_sequence is None else
+        _flat(per_sequence, torch.int32, at, which),
+        None if page_table is None else
+        _flat(page_table, torch.int32, at, "page_table"), *pointers, sequences,
+        tokens, pages, size, width, heads, d, strides, _stream(stream)))
+
+
+def fp4_cache_write(token_offsets, key_lengths, page_table, key, value,
+                    key_cache, value_cache, stream=None):
+    """Quantise packed keys and values into a 4-bit cache (no counterpart in
+    the reference): sequence i's tokens token_offsets[i] ..
+    token_offsets[i + 1] - 1 of key and value [tokens, key_heads, d] become the
+    last of its key_lengths[i] keys.
+
+    key_cache and value_cache are :class:`Fp4Rows` (or pairs) of codes and
+    scales, any page, row and head strides, codes at steps of 16 bytes; key j of
+    sequence i is row j % page_size of page page_table[i, j // page_size], or of
+    page i where page_table is None.  Blocks of 32 elements share a scale, a
+    power of two; d is a multiple of 32 up to 128.  A place outside the table's
+    row or the cache is not written."""
+    _need(key_lengths is not None, "key_lengths must hold one number a "
+          "sequence")
+    _fp4_move("sw_fp4_cache_write", token_offsets, key_lengths, page_table,
+              key_cache, value_cache, key, value, stream)
+    return key_cache, value_cache
+
+
+def fp4_cache_read(token_offsets, starts, page_table, key_cache, value_cache,
+                   key, value, stream=None):
+    """Read keys and values of a 4-bit cache back, as :func:`window_attention`
+    takes them: the tokens of sequence i are its places starts[i] (None: 0) and
+    on.  Places that are not there give zeros, tokens of no sequence are left as
+    they were.  Operands as in :func:`fp4_cache_write`."""
+    _fp4_move("sw_fp4_cache_read", token_offsets, starts, page_table,
+              key_cache, value_cache, key, value, stream)
+    return key, value
+
+
+def window_attention_decode_fp4(key_lengths, page_table, query, key_cache,
+                                value_cache, output, alpha, window, sinks=0,
+                                workspace=None, stream=None):
+    """:func:`window_attention_decode` against a 4-bit cache: key_cache and
+    value_cache are :class:`Fp4Rows` as :func:`fp4_cache_write` fills them.
+    Everything else as there; the scratch memory is that of
+    sw_window_attention_decode_fp4_workspace_bytes."""
+    torch = _torch or _load_torch()
+    if query.dim() != 3 or output.shape != query.shape:
+        raise ShapeError("expected query and output [sequences, query_heads, "
+                         "d]")
+    sequences, heads, d = query.shape
+    if key_lengths.shape != query.shape[:1]:
+        raise ShapeError("key_lengths must hold one length a sequence")
+    width = _table_width(page_table, sequences)
+    dt = _value_dtype(query, "query")
+    at = _device_of(stream)
+    (pages, size, key_heads), rows, row_strides = _fp4_rows(
+        at, d, key_cache, value_cache)
+    (q, o), strides = _heads(dt, at, query, "query", output, "output",
+                             always=True)
+    strides = (ctypes.c_int64 * 16)(*strides, *row_strides)
+    need = load_library().sw_window_attention_decode_fp4_workspace_bytes(
+        sequences, size, width, heads, key_heads, d, window, sinks)
+    lengths = _flat(key_lengths, torch.int32, at, "key_lengths")
+    table = (None if page_table is None else
+             _flat(page_table, torch.int32, at, "page_table"))
+    scratch = _scratch(need, query, workspace, stream)
+    _check(_fn("sw_window_attention_decode_fp4", dt)(
+        lengths, table, q, *rows, o, sequences, pages, size, width, heads,
+        key_heads, d, strides, window, sinks, alpha,
         None if scratch is None else scratch.data_ptr(), need,
         _stream(stream)))
     return output

@@ -27,6 +27,9 @@ SOURCES = [
     "sw_attention.hip",
     "sw_window_attention.hip",
     "sw_cache_attention.hip",
+    "sw_rotary.hip",
+    "sw_fp4_cache.hip",
+    "sw_fp4_attention.hip",
 ]
 
 # -packed-fp32-ops: keep hipcc from forming v_pk_{add,mul,fma}_f32.

@@ -214,4 +214,112 @@ inline int check_heads(int64_t query_heads, int64_t key_heads, int64_t d) {
   return SW_OK;
 }
 
+// ---- caches of 4-bit codes: [pages][page_size][heads] rows of d / 2 bytes of
+// codes and of d / 32 scales ----
+
+inline int check_fp4_heads(int64_t query_heads, int64_t key_heads, int64_t d) {
+  if (int rc = check_heads(query_heads, key_heads, d))
+    return rc;
+  if (d % 32 != 0)
+    return fail(SW_ERR_INVALID_SHAPE,
+                "head dimension of a 4-bit cache must be a multiple of its "
+                "blocks of 32, but got %lld", (long long)d);
+  return SW_OK;
+}
+
+// Sequences whose packed tokens lie in a cache's pages.
+inline int check_cache_sizes(int64_t sequences, int64_t tokens, int64_t pages,
+                             int64_t page_size, int64_t table_width,
+                             bool table) {
+  if (sequences < 0 || tokens < 0 || pages < 0 || page_size < 1 ||
+      table_width < 1 || sequences > kMostTokens || tokens > kMostTokens ||
+      pages > kMostTokens || page_size > kMostTokens ||
+      table_width > kMostTokens / page_size)
+    return fail(SW_ERR_INVALID_SHAPE,
+                "expected up to 2^30 sequences, tokens and pages, and pages of "
+                "a size and a table of a width that hold up to 2^30 keys, but "
+                "got %lld, %lld, %lld, %lld and %lld", (long long)sequences,
+                (long long)tokens, (long long)pages, (long long)page_size,
+                (long long)table_width);
+  if (!table && pages < sequences)
+    return fail(SW_ERR_INVALID_SHAPE,
+                "without a page table every sequence needs its page, but got "
+                "%lld pages for %lld sequences", (long long)pages,
+                (long long)sequences);
+  return SW_OK;
+}
+
+// Whether rows of `width` at three strides share no memory.
+inline bool rows_apart(int64_t width, std::initializer_list<int64_t> strides,
+                       std::initializer_list<int64_t> counts) {
+  int64_t s[3], n[3], span = width;
+  int dims = 0;
+  for (size_t i = 0; i < strides.size(); ++i)
+    if (counts.begin()[i] > 1) {
+      int at = dims++;
+      for (; at > 0 && s[at - 1] > strides.begin()[i]; --at) {
+        s[at] = s[at - 1];
+        n[at] = n[at - 1];
+      }
+      s[at] = strides.begin()[i];
+      n[at] = counts.begin()[i];
+    }
+  // (spans stay below 2^62: larger ones are no memory)
+  for (int i = 0; i < dims; ++i) {
+    if (s[i] < span || s[i] > ((int64_t)1 << 61) / n[i])
+      return false;
+    span += (n[i] - 1) * s[i];
+  }
+  return true;
+}
+
+// A cache's codes and scales; `s`: page, token and head stride of the codes
+// and of the scales, in bytes.
+inline int check_fp4_cache(const char *name, const uint8_t *codes,
+                           const uint8_t *scales, const int64_t *s, int64_t d,
+                           int64_t pages, int64_t page_size, int64_t heads,
+                           bool written) {
+  if (pages == 0)
+    return SW_OK;
+  if (!codes || !scales)
+    return fail(SW_ERR_INVALID_ARGUMENT, "%s %s pointer is null", name,
+                codes ? "scales" : "codes");
+  for (int i = 0; i < 6; ++i) {
+    const int64_t least = i % 3 == 1 ? (i < 3 ? d / 2 : d / 32) : 0;
+    const int64_t most = i % 3 == 1 ? (int64_t)1 << 23 : kMostStride;
+    if (s[i] < least || s[i] > most)
+      return fail(SW_ERR_INVALID_SHAPE,
+                  "%s %s strides must be 0 to 2^40 (pages and heads) and at "
+                  "least a row and at most 2^23 (tokens) bytes, but got %lld, "
+                  "%lld and %lld", name, i < 3 ? "codes" : "scales",
+                  (long long)s[i / 3 * 3], (long long)s[i / 3 * 3 + 1],
+                  (long long)s[i / 3 * 3 + 2]);
+  }
+  if (!aligned16(codes) || s[0] % 16 != 0 || s[1] % 16 != 0 || s[2] % 16 != 0)
+    return fail(SW_ERR_INVALID_ARGUMENT,
+                "%s codes must be 16-byte aligned, their strides included",
+                name);
+  if (written &&
+      (!rows_apart(d / 2, {s[0], s[1], s[2]}, {pages, page_size, heads}) ||
+       !rows_apart(d / 32, {s[3], s[4], s[5]}, {pages, page_size, heads})))
+    return fail(SW_ERR_INVALID_SHAPE, "%s rows overlap", name);
+  return SW_OK;
+}
+
+// Strides of packed operands: token and head of two [rows][heads][d], then of
+// a key and a value cache.
+inline void fp4_packed_strides(int64_t *s, int64_t heads, int64_t key_heads,
+                               int64_t page_size, int64_t d) {
+  for (int i = 0; i < 2; ++i) {
+    *s++ = heads * d;
+    *s++ = d;
+  }
+  for (int i = 0; i < 4; ++i) {
+    const int64_t width = i % 2 ? d / 32 : d / 2;
+    *s++ = page_size * key_heads * width;
+    *s++ = key_heads * width;
+    *s++ = width;
+  }
+}
+
 } // namespace sw

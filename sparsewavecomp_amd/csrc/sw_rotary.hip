@@ -1,0 +1,336 @@
+// Rotary positions: pairs of each head's elements turned by an angle,
+//   (x, y) -> (x cos t - y sin t, x sin t + y cos t),
+//   t = positions[axis of the pair][token] frequency of the pair,
+// the pairs being elements i and i + pairs of a head, or 2 i and 2 i + 1; the
+// gradients are turned by -t.
+//
+// Each element is read and written once, three operations for it: memory bounds
+// this.  The angles belong to a token and are shared by its heads, so a
+// workgroup computes those of its tokens first.  They are reduced to a quarter
+// turn in 64 bits: a position of 2^17 times a frequency near 1 has lost 2^-8 of
+// a radian in 32.
+#include "sw_heads.h"
+#include "sw_internal.h"
+
+#include <algorithm>
+
+using namespace swd;
+using sw::check_operand;
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Heads {
+  const void *from;
+  void *to;
+  int64_t from_token, from_head, to_token, to_head; // strides in elements
+};
+
+struct RotaryArgs {
+  const int32_t *positions, *axes; // axes may be null: all pairs take axis 0
+  const float *frequencies;
+  Heads query, key;
+  int tokens, axis_count, query_heads, heads, d, pairs;
+  int per; // tokens of a workgroup
+  int turned, units; // units of a head that turn, and all of them
+  Divisor token_units, head_units;
+  bool back;
+};
+
+struct Turn {
+  float cos, sin;
+};
+
+// The cosine and sine of position * frequency.  q = 2/pi of the angle's rest
+// after n quarter turns is found in 64 bits: the product's own rounding and
+// that of 2/pi are added back, so that q is right to 2^-24 of itself for any
+// position and frequencies up to 1, or angles up to 2^31.  The series end past
+// 2^-28 of their sums at pi/4.
+__device__ __forceinline__ Turn turn_of(int position, float frequency) {
+  constexpr double kTwoOverPi = 0.63661977236758134308;
+  constexpr double kRest = -3.9357353350364972e-17; // 2/pi less that double
+  const double p = position, f = frequency;
+  const double t = p * f, t_rest = __builtin_fma(p, f, -t);
+  const double n = __builtin_rint(t * kTwoOverPi);
+  const double q = __builtin_fma(t, kTwoOverPi, -n) +
+                   __builtin_fma(t, kRest, t_rest * kTwoOverPi);
+  const float r = (float)(q * 1.57079632679489661923);
+  const float z = r * r;
+  float s = fmaf(z, 1.0f / 362880, -1.0f / 5040);
+  s = fmaf(z, s, 1.0f / 120);
+  s = fmaf(z, s, -1.0f / 6);
+  s = fmaf(r * z, s, r);
+  float c = fmaf(z, -1.0f / 3628800, 1.0f / 40320);
+  c = fmaf(z, c, -1.0f / 720);
+  c = fmaf(z, c, 1.0f / 24);
+  c = fmaf(z * z, c, fmaf(z, -0.5f, 1.0f));
+  // n modulo 4
+  const int turns = (int)(n - 4.0 * __builtin_floor(n * 0.25));
+  if (turns & 1) {
+    const float x = c;
+    c = -s;
+    s = x;
+  }
+  if (turns & 2) {
+    c = -c;
+    s = -s;
+  }
+  return {c, s};
+}
+
+// 16 bytes of elements as fp32, and back.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+  static constexpr int kCount = 4;
+  float x[4];
+  __device__ __forceinline__ void load(const float *p) {
+    const v4f v = *reinterpret_cast<const v4f *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = v[i];
+  }
+  __device__ __forceinline__ void store(float *p) const {
+    *reinterpret_cast<v4f *>(p) = v4f{x[0], x[1], x[2], x[3]};
+  }
+};
+template <> struct Piece<uint16_t> {
+  static constexpr int kCount = 8;
+  float x[8];
+  __device__ __forceinline__ void load(const uint16_t *p) {
+    const v4u v = *reinterpret_cast<const v4u *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(v[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t *p) const {
+    *reinterpret_cast<v4u *>(p) = make_frag<uint16_t>(x);
+  }
+};
+
+__device__ __forceinline__ void turn(float &x, float &y, const Turn &t) {
+  const float a = x, b = y;
+  x = fmaf(a, t.cos, -(b * t.sin));
+  y = fmaf(a, t.sin, b * t.cos);
+}
+
+// A unit of a head: with VECTOR, two pieces of 16 bytes that turn with each
+// other (neighbours where pairs are) or one that is copied; else a pair, or an
+// element that is copied.
+template <typename T, bool VECTOR, bool NEIGHBOURS>
+__global__ __launch_bounds__(kThreads) void rotary_turn(RotaryArgs a) {
+  extern __shared__ Turn turns[]; // [per][pairs]
+  constexpr int kCount = VECTOR ? Piece<T>::kCount : 1;
+  const int first = blockIdx.x * a.per;
+  const int count = a.tokens - first < a.per ? a.tokens - first : a.per;
+  for (int i = threadIdx.x; i < count * a.pairs; i += kThreads) {
+    const int token = i / a.pairs, pair = i - token * a.pairs;
+    const int axis = a.axes ? a.axes[pair] : 0;
+    Turn t{1.0f, 0.0f}; // (of an axis that is not there)
+    if (axis >= 0 && axis < a.axis_count) {
+      t = turn_of(a.positions[(int64_t)axis * a.tokens + first + token],
+                  a.frequencies[pair]);
+      if (a.back)
+        t.sin = -t.sin;
+    }
+    turns[i] = t;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < count * (int)a.token_units.by; i += kThreads) {
+    const int token = (int)a.token_units.quotient(i);
+    int u = i - token * (int)a.token_units.by;
+    int head = (int)a.head_units.quotient(u);
+    u -= head * (int)a.head_units.by;
+    const bool key = head >= a.query_heads;
+    const Heads &h = key ? a.key : a.query;
+    head -= key ? a.query_heads : 0;
+    const int64_t at = first + token;
+    const T *from = static_cast<const T *>(h.from) + at * h.from_token +
+                    head * h.from_head;
+    T *to = static_cast<T *>(h.to) + at * h.to_token + head * h.to_head;
+    if (u < a.turned) {
+      const Turn *t = turns + token * a.pairs + u * kCount;
+      const int x = NEIGHBOURS ? 2 * u * kCount : u * kCount;
+      const int y = NEIGHBOURS ? x + kCount : x + a.pairs;
+      if constexpr (VECTOR) {
+        Piece<T> p, q;
+        p.load(from + x);
+        q.load(from + y);
+        if constexpr (NEIGHBOURS) {
+#pragma unroll
+          for (int e = 0; e < kCount; e += 2) {
+            turn(p.x[e], p.x[e + 1], t[e / 2]);
+            turn(q.x[e], q.x[e + 1], t[(kCount + e) / 2]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kCount; ++e)
+            turn(p.x[e], q.x[e], t[e]);
+        }
+        p.store(to + x);
+        q.store(to + y);
+      } else {
+        float p = ldv(from + x), q = ldv(from + y);
+        turn(p, q, *t);
+        stv(to + x, p);
+        stv(to + y, q);
+      }
+    } else {
+      const int x = 2 * a.pairs + (u - a.turned) * kCount;
+      if constexpr (VECTOR)
+        *reinterpret_cast<v4u *>(to + x) =
+            *reinterpret_cast<const v4u *>(from + x);
+      else
+        to[x] = from[x];
+    }
+  }
+}
+
+template <typename T>
+int rotary_entry(const int32_t *positions, const float *frequencies,
+                 const int32_t *pair_axes, const T *query, const T *key,
+                 T *query_output, T *key_output, int64_t tokens, int64_t axes,
+                 int64_t query_heads, int64_t key_heads, int64_t d,
+                 int64_t pairs, int interleaved, const int64_t *strides,
+                 bool back, void *stream) {
+  const char *what = back ? "rotary backward" : "rotary";
+  sw::clear_error();
+  if (tokens < 0 || tokens > sw::kMostTokens || axes < 1 || axes > 65536)
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "expected up to 2^30 tokens and 1 to 65536 axes, but got "
+                    "%lld and %lld", (long long)tokens, (long long)axes);
+  if (query_heads < 1 || query_heads > 65536 || key_heads < 0 ||
+      key_heads > 65536)
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "expected 1 to 65536 query heads and 0 to 65536 key heads, "
+                    "but got %lld and %lld", (long long)query_heads,
+                    (long long)key_heads);
+  if (d < 8 || d > 128 || d % 8 != 0)
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "head dimension must be a multiple of 8 up to 128, but "
+                    "got %lld", (long long)d);
+  if (pairs < 1 || pairs > d / 2)
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "pairs must be 1 to half of the head dimension, but got "
+                    "%lld", (long long)pairs);
+  if (tokens > 0 && (!positions || !frequencies))
+    return sw::fail(SW_ERR_INVALID_ARGUMENT, "%s pointer is null",
+                    positions ? "frequencies" : "positions");
+  if (int rc = sw::check_value_alignment(4, {positions, frequencies,
+                                             pair_axes}))
+    return rc;
+  const int64_t qs = query_heads * d, ks = key_heads * d;
+  const int64_t packed[8] = {qs, d, ks, d, qs, d, ks, d};
+  const int64_t *s = strides ? strides : packed;
+  const char *names[4] = {"query", "key",
+                          back ? "query gradient" : "query output",
+                          back ? "key gradient" : "key output"};
+  const T *rows[4] = {query, key, query_output, key_output};
+  for (int i = 0; i < 4; ++i)
+    if (i % 2 == 0 || key_heads > 0)
+      if (int rc = check_operand(names[i], rows[i], {s[2 * i], s[2 * i + 1]}, d,
+                                 sizeof(T), i >= 2, tokens,
+                                 i % 2 ? key_heads : query_heads))
+        return rc;
+  for (int i = 0; i < 2; ++i)
+    if (rows[i] && rows[i] == rows[i + 2] && tokens > 0 &&
+        (i == 0 || key_heads > 0) &&
+        ((tokens > 1 && s[2 * i] != s[2 * i + 4]) ||
+         ((i ? key_heads : query_heads) > 1 && s[2 * i + 1] != s[2 * i + 5])))
+      return sw::fail(SW_ERR_INVALID_ARGUMENT,
+                      "%s in place needs its input's strides", names[i]);
+  if (tokens == 0)
+    return SW_OK;
+  RotaryArgs a{};
+  a.positions = positions;
+  a.axes = pair_axes;
+  a.frequencies = frequencies;
+  a.query = {query, query_output, s[0], s[1], s[4], s[5]};
+  a.key = {key, key_output, s[2], s[3], s[6], s[7]};
+  a.tokens = (int)tokens;
+  a.axis_count = (int)axes;
+  a.query_heads = (int)query_heads;
+  a.heads = (int)(query_heads + key_heads);
+  a.d = (int)d;
+  a.pairs = (int)pairs;
+  a.back = back;
+  const int64_t count = 16 / (int64_t)sizeof(T);
+  // (neighbours: two pieces hold `count` pairs)
+  const bool vector = pairs % count == 0;
+  a.turned = (int)(vector ? pairs / count : pairs);
+  a.units = a.turned + (int)((d - 2 * pairs) / (vector ? count : 1));
+  a.head_units = Divisor((uint32_t)a.units);
+  a.token_units = Divisor((uint32_t)(a.units * a.heads));
+  a.per = (int)std::clamp<int64_t>(2 * kThreads / (a.units * a.heads), 1, 16);
+  const int64_t grid = sw::ceil_div(tokens, a.per);
+  if (int rc = sw::check_flat_grid(grid, kThreads, what))
+    return rc;
+  const hipStream_t st = sw::as_stream(stream);
+  const dim3 g((unsigned)grid);
+  const size_t lds = a.per * a.pairs * sizeof(Turn);
+  if (vector && interleaved)
+    rotary_turn<T, true, true><<<g, kThreads, lds, st>>>(a);
+  else if (vector)
+    rotary_turn<T, true, false><<<g, kThreads, lds, st>>>(a);
+  else if (interleaved)
+    rotary_turn<T, false, true><<<g, kThreads, lds, st>>>(a);
+  else
+    rotary_turn<T, false, false><<<g, kThreads, lds, st>>>(a);
+  return sw::launch_check(what);
+}
+
+} // namespace
+
+extern "C" int sw_rotary_f32(
+    const int32_t *positions, const float *frequencies,
+    const int32_t *pair_axes, const float *query, const float *key,
+    float *query_output, float *key_output, int64_t tokens, int64_t axes,
+    int64_t query_heads, int64_t key_heads, int64_t d, int64_t pairs,
+    int interleaved, const int64_t *strides, void *stream) {
+  return rotary_entry<float>(positions, frequencies, pair_axes, query, key,
+                             query_output, key_output, tokens, axes,
+                             query_heads, key_heads, d, pairs, interleaved,
+                             strides, false, stream);
+}
+
+extern "C" int sw_rotary_bf16(
+    const int32_t *positions, const float *frequencies,
+    const int32_t *pair_axes, const uint16_t *query, const uint16_t *key,
+    uint16_t *query_output, uint16_t *key_output, int64_t tokens, int64_t axes,
+    int64_t query_heads, int64_t key_heads, int64_t d, int64_t pairs,
+    int interleaved, const int64_t *strides, void *stream) {
+  return rotary_entry<uint16_t>(positions, frequencies, pair_axes, query, key,
+                                query_output, key_output, tokens, axes,
+                                query_heads, key_heads, d, pairs, interleaved,
+                                strides, false, stream);
+}
+
+extern "C" int sw_rotary_backward_f32(
+    const int32_t *positions, const float *frequencies,
+    const int32_t *pair_axes, const float *query_output_gradient,
+    const float *key_output_gradient, float *query_gradient,
+    float *key_gradient, int64_t tokens, int64_t axes, int64_t query_heads,
+    int64_t key_heads, int64_t d, int64_t pairs, int interleaved,
+    const int64_t *strides, void *stream) {
+  return rotary_entry<float>(positions, frequencies, pair_axes,
+                             query_output_gradient, key_output_gradient,
+                             query_gradient, key_gradient, tokens, axes,
+                             query_heads, key_heads, d, pairs, interleaved,
+                             strides, true, stream);
+}
+
+extern "C" int sw_rotary_backward_bf16(
+    const int32_t *positions, const float *frequencies,
+    const int32_t *pair_axes, const uint16_t *query_output_gradient,
+    const uint16_t *key_output_gradient, uint16_t *query_gradient,
+    uint16_t *key_gradient, int64_t tokens, int64_t axes, int64_t query_heads,
+    int64_t key_heads, int64_t d, int64_t pairs, int interleaved,
+    const int64_t *strides, void *stream) {
+  return rotary_entry<uint16_t>(positions, frequencies, pair_axes,
+                                query_output_gradient, key_output_gradient,
+                                query_gradient, key_gradient, tokens, axes,
+                                query_heads, key_heads, d, pairs, interleaved,
+                                strides, true, stream);
+}
