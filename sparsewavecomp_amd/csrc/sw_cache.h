@@ -54,6 +54,7 @@ struct StepArgs {
   // leaves o in [part][rows][dim] and (m, l) in [part][rows][2].
   int chunk, parts, prefix_chunk, prefix_parts;
   int rows, prefix_rows; // of one part: a multiple of 16, of 16 or 128
+  bool by_tiles; // parts are cut at multiples of 32 keys, see Visible::tiles
   // a power of two: the number of all keys times it is below 1
   float lower;
   float *sums, *stats, *prefix_sums, *prefix_stats;
@@ -76,6 +77,30 @@ struct Visible {
   __device__ __forceinline__ int key(int v) const {
     return v < lead ? v : v - lead + start;
   }
+  __device__ __forceinline__ int end() const { return start + count - lead; }
+  __device__ __forceinline__ bool sees(int j) const {
+    return (j < lead || j >= start) && j < end();
+  }
+  // The tiles of kTile keys from multiples of it on that hold those keys: the
+  // sinks' that lie before the window's first one, and the window's.
+  __device__ __forceinline__ int lead_tiles() const {
+    const int sinks = (lead + kTile - 1) / kTile, first = start / kTile;
+    return sinks < first ? sinks : first;
+  }
+  __device__ __forceinline__ int tiles() const {
+    return count == 0 ? 0
+                      : lead_tiles() + (end() + kTile - 1) / kTile -
+                            start / kTile;
+  }
+  __device__ __forceinline__ int tile_key(int tile) const {
+    const int sinks = lead_tiles();
+    return kTile * (tile < sinks ? tile : tile - sinks + start / kTile);
+  }
+  // How many parts of a.chunk keys they are.
+  __device__ __forceinline__ int parts(const StepArgs &a) const {
+    return a.by_tiles ? (tiles() * kTile + a.chunk - 1) / a.chunk
+           : count == 0 ? 0 : (count - 1) / a.chunk + 1;
+  }
 };
 
 __device__ __forceinline__ float rows16_max(float v) { // over lanes l % 16
@@ -90,14 +115,14 @@ struct Totals {
 
 // The four waves' results of one part of the keys, joined in LDS and written:
 // as the output where the part is the `only` one, else to `sums` and `stats`.
-// acc: o[row][d] of a wave, which it leaves in its own WAVE_BYTES of `lds`.
+// acc: o[row][d] of a wave, which it leaves in its own WAVE_BYTES of `lds`;
+// top, sum and raise: of row l % 16.
 template <typename T, int D, int WAVE_BYTES>
 __device__ __forceinline__ void
 store_part(const StepArgs &a, char *lds, Totals &found, float top, float sum,
            float raise, const v4f (&acc)[D / 16], int rows, bool only, int seq,
            int hk, int first_row, float *sums, float *stats) {
   const int lane = lane_id(), g = lane >> 4, wave = wave_in_group();
-  sum = rows16_sum(sum);
   if (g == 0) {
     found.top[wave][lane] = top;
     found.sum[wave][lane] = sum;
@@ -165,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void window_cache_join(StepArgs a) {
   const int head = (int)(blockIdx.x % a.query_heads);
   const int hk = head / a.group, row = head % a.group;
   const Visible see(a, seq);
-  const int own = see.count == 0 ? 0 : (see.count - 1) / a.chunk + 1;
+  const int own = see.parts(a);
   const int parts = own + a.prefix_parts;
   const int half = threadIdx.x / 32, c = (threadIdx.x % 32) * N;
   float top = -kInf, l = 0.0f, o[N] = {};

@@ -281,8 +281,8 @@ __device__ __forceinline__ void cache_part(const StepArgs &a, int64_t item,
   if (some && top == -kInf)
     top = kLowest;
 
-  store_part<T, D, kWaveBytes>(a, lds, found, top, sum, raise, acc, rows, only,
-                               seq, hk, first_row, sums, stats);
+  store_part<T, D, kWaveBytes>(a, lds, found, top, rows16_sum(sum), raise, acc,
+                               rows, only, seq, hk, first_row, sums, stats);
 }
 
 template <typename T, int D>

@@ -81,6 +81,12 @@ __device__ __forceinline__ void weight_parts(const float *x, v4u (&part)[3]) {
 // one load for d = 128; quarter g of step st is elements D / 4 g + 8 st + i of
 // the products' K index, in the queries too.  Values go through LDS as bf16, to
 // be read across their rows.
+//
+// Tiles start at multiples of 32 keys, so that a half of 16 lies in one page
+// wherever a page holds a multiple of 16: its addresses are then scalar ones
+// plus a lane's constant offset.  Halves that cross a page's end take each
+// lane's own.  The pages of a wave's next 32 tiles are found at once, a half by
+// each lane; the next tile is on its way while one is multiplied.
 template <typename T, int D> struct Fp4Parts {
   using Tile = RowTile<uint16_t, D, kTile, kWave>;
   static constexpr int kWaveBytes =
@@ -110,12 +116,13 @@ fp4_cache_parts(Fp4StepArgs args) {
   const int hk = (int)(item % a.key_heads);
   const int seq = (int)(item / a.key_heads);
   const Visible see(a, seq);
-  const int v0 = part * a.chunk;
-  const int v1 = see.count < v0 + a.chunk ? see.count : v0 + a.chunk;
+  const int t0 = part * (a.chunk / kTile);
+  const int t1 = see.tiles() < t0 + a.chunk / kTile ? see.tiles()
+                                                    : t0 + a.chunk / kTile;
   const int64_t of =
       (((int64_t)seq * a.key_heads + hk) * a.parts + part) * a.rows + first_row;
   const bool only = a.parts == 1;
-  if (v1 <= v0 && !only)
+  if (t1 <= t0 && !only)
     return;
   const int rows = a.group - first_row < kRows ? a.group - first_row : kRows;
 
@@ -141,158 +148,234 @@ fp4_cache_parts(Fp4StepArgs args) {
     }
   }
 
-  // this lane's quarter of a row: codes, and the scale of its block
-  const int code_at = D / 8 * g, scale_at = D * g / 128;
-  const bool inside = code_at * 2 < a.d;
-  const uint8_t *zeros = reinterpret_cast<const uint8_t *>(kZeros);
-  const uint8_t *key_codes = static_cast<const uint8_t *>(a.cache.key) +
-                             hk * a.cache.key_head + code_at;
-  const uint8_t *value_codes = static_cast<const uint8_t *>(a.cache.value) +
-                               hk * a.cache.value_head + code_at;
-  const uint8_t *key_scales =
-      args.scales.key + hk * args.scales.key_head + scale_at;
-  const uint8_t *value_scales =
-      args.scales.value + hk * args.scales.value_head + scale_at;
+  // This lane's quarter of a row: codes, and the scale of its block.  Quarters
+  // past d read the row's first one; the queries are zero there, and so is the
+  // scale.
+  const bool inside = D / 4 * g < a.d;
+  const int code_at = inside ? D / 8 * g : 0, scale_at = inside ? D * g / 128 : 0;
+  const int row_of = lane & 15;
+  const Scales &sc = args.scales;
+  const uint8_t *key_codes =
+      static_cast<const uint8_t *>(a.cache.key) + hk * a.cache.key_head;
+  const uint8_t *value_codes =
+      static_cast<const uint8_t *>(a.cache.value) + hk * a.cache.value_head;
+  const uint8_t *key_scales = sc.key + hk * sc.key_head;
+  const uint8_t *value_scales = sc.value + hk * sc.value_head;
+  // (a token stride is at most 2^23)
+  const uint32_t key_off = row_of * (uint32_t)a.cache.key_token + code_at;
+  const uint32_t value_off = row_of * (uint32_t)a.cache.value_token + code_at;
+  const uint32_t key_scale_off = row_of * (uint32_t)sc.key_token + scale_at;
+  const uint32_t value_scale_off = row_of * (uint32_t)sc.value_token + scale_at;
+
   typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
   struct Data {
     Words key[2], value[2];
     uint32_t key_scale[2], value_scale[2];
-    uint32_t none; // bit i: key i of this lane's scores is none
+    uint32_t has; // bit i: key i of the tile is seen (wave-uniform)
   };
-  auto fetch = [&](int v) __attribute__((always_inline)) {
-    Data x;
-    uint64_t has[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int at = v + 16 * b + (lane & 15);
-      int page = -1, slot = 0;
-      if (at < v1) {
-        slot = see.key(at);
-        page = seq;
-        if (a.table) {
-          const int n = (int)args.page_size.quotient(slot);
-          slot -= n * a.page_size;
-          page = a.table[(int64_t)seq * a.table_width + n];
-        }
-      }
-      const bool there = page >= 0 && page < a.pages;
-      has[b] = ballot(there);
-      const bool reads = there && inside;
-      x.key[b] = *reinterpret_cast<const Words *>(
-          reads ? key_codes + page * a.cache.key_page +
-                      slot * a.cache.key_token : zeros);
-      x.value[b] = *reinterpret_cast<const Words *>(
-          reads ? value_codes + page * a.cache.value_page +
-                      slot * a.cache.value_token : zeros);
-      x.key_scale[b] = *(reads ? key_scales + page * args.scales.key_page +
-                                     slot * args.scales.key_token : zeros);
-      x.value_scale[b] = *(reads ? value_scales + page * args.scales.value_page +
-                                       slot * args.scales.value_token : zeros);
+  struct Halves { // of the wave's next tiles: lane l has half l % 2 of l / 2
+    int page, slot; // of its first key; page -1: it is not there
+  };
+  auto page_of = [&](int key, int &slot) __attribute__((always_inline)) {
+    int page = seq;
+    slot = key;
+    if (a.table) {
+      const int n = (int)args.page_size.quotient(key);
+      slot -= n * a.page_size;
+      page = a.table[(int64_t)seq * a.table_width + n];
     }
-    x.none = 0;
+    return page >= 0 && page < a.pages ? page : -1;
+  };
+  auto locate = [&](int first) __attribute__((always_inline)) {
+    const int tile = first + 4 * (lane >> 1);
+    const int key = see.tile_key(tile) + 16 * (lane & 1);
+    Halves h{-1, 0};
+    if (tile < t1 && key < see.end())
+      h.page = page_of(key, h.slot);
+    return h;
+  };
+  auto load = [&](Data &x, int b, int64_t kc, int64_t vc, int64_t ks,
+                  int64_t vs) __attribute__((always_inline)) {
+    x.key[b] = *reinterpret_cast<const Words *>(key_codes + kc);
+    x.value[b] = *reinterpret_cast<const Words *>(value_codes + vc);
+    x.key_scale[b] = key_scales[ks];
+    x.value_scale[b] = value_scales[vs];
+  };
+  // tile k of `h`, whose first key is `key`
+  auto fetch = [&](const Halves &h, int k, int key)
+                   __attribute__((always_inline)) {
+    Data x;
+    x.has = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x.none |= (uint32_t)(~(has[i / 4] >> (4 * g + i % 4)) & 1) << i;
+    for (int b = 0; b < 2; ++b, key += 16) {
+      const int64_t page = __builtin_amdgcn_readlane(h.page, 2 * k + b);
+      const int64_t slot = __builtin_amdgcn_readlane(h.slot, 2 * k + b);
+      x.key[b] = x.value[b] = Words{};
+      x.key_scale[b] = x.value_scale[b] = 0;
+      if (slot + 16 <= a.page_size) {
+        if (page < 0)
+          continue;
+        const uint8_t *kc = key_codes + (page * a.cache.key_page +
+                                         slot * a.cache.key_token);
+        const uint8_t *vc = value_codes + (page * a.cache.value_page +
+                                           slot * a.cache.value_token);
+        const uint8_t *ks =
+            key_scales + (page * sc.key_page + slot * sc.key_token);
+        const uint8_t *vs =
+            value_scales + (page * sc.value_page + slot * sc.value_token);
+        x.key[b] = *reinterpret_cast<const Words *>(kc + key_off);
+        x.value[b] = *reinterpret_cast<const Words *>(vc + value_off);
+        x.key_scale[b] = ks[key_scale_off];
+        x.value_scale[b] = vs[value_scale_off];
+        const bool all = (key + 16 <= see.lead || key >= see.start) &&
+                         key + 16 <= see.end();
+        x.has |= (all ? 0xFFFFu
+                      : (uint32_t)ballot(see.sees(key + row_of)) & 0xFFFFu)
+                 << (16 * b);
+      } else {
+        int s = 0, p = -1;
+        if (see.sees(key + row_of))
+          p = page_of(key + row_of, s);
+        if (p >= 0)
+          load(x, b, p * a.cache.key_page + s * a.cache.key_token + code_at,
+               p * a.cache.value_page + s * a.cache.value_token + code_at,
+               p * sc.key_page + s * sc.key_token + scale_at,
+               p * sc.value_page + s * sc.value_token + scale_at);
+        x.has |= ((uint32_t)ballot(p >= 0) & 0xFFFFu) << (16 * b);
+      }
+    }
     return x;
   };
 
-  v4f acc[kBlocks];
-  float top, sum;
+  v4f acc[kBlocks], total; // total: the probabilities' sums, in all four
+  float top;
   float lower = 1.0f; // of this lane's row: a factor of the probabilities
+  bool again = false; // whether a row has such a factor (wave-uniform)
   const uint32_t own = lds_address(lds) + wave * kWaveBytes;
-  uint32_t across[2 * kBlocks];
+  // of a read across rows 4 g + .. and of a write: chunks differ by what the
+  // swizzle leaves alone, rows 16 apart have the same
+  uint32_t across = own +
+                    Tile::place(4 * g + (row_of >> 2), (lane & 3) >> 1) +
+                    (lane & 1) * 8;
+  uint32_t along = own + Tile::place(row_of, kWords * g);
+  const v4u ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+
+  auto compute = [&](Data &x) __attribute__((always_inline)) {
+    // (keeps the compiler from holding every address in a register)
+    asm volatile("" : "+v"(across), "+v"(along));
+    v4f score[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+    for (int b = 0; b < 2; ++b) {
+      score[b] = v4f{};
+      const float by = fp4_scale(inside ? x.key_scale[b] : 0u);
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-      across[e * kBlocks + b] =
-          own +
-          Tile::place(16 * e + 4 * g + ((lane & 15) >> 2),
-                      2 * b + ((lane & 3) >> 1)) + (lane & 1) * 8;
+      for (int st = 0; st < kSteps; ++st) {
+        const v4u k = fp4_values(x.key[b][st], by);
+#pragma unroll
+        for (int i = kQueryParts<T> - 1; i >= 0; --i)
+          score[b] = mma16(k, q[i][st], score[b]);
+      }
+    }
+    if (x.has != 0xFFFFFFFFu) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!((x.has >> (16 * (i / 4) + 4 * g + i % 4)) & 1))
+          score[i / 4][i % 4] = -kInf;
+      // (what lies at a place that is not seen may be NaN)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        if (!((x.has >> (16 * b + row_of)) & 1))
+          x.value_scale[b] = 0;
+    }
+    float big = score[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+      big = fmaxf(big, score[i / 4][i % 4]);
+    big = rows16_max(big) * scale;
+    if (ballot(big > top) != 0) {
+      const float to = fmaxf(top, big);
+      const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      total *= by;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        acc[b] *= by;
+    }
+    const float less = top == -kInf ? 0.0f : top;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less));
+    if (again) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        p[i] *= lower;
+    }
+    v4u weight[kWeightParts<T>];
+    weight_parts(p, weight);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float by = fp4_scale(x.value_scale[b]);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        lds_write((along ^ (w << 4)) + 16 * b * Tile::kPitch,
+                  fp4_values(x.value[b][w], by));
+    }
+#pragma unroll
+    for (int i = 0; i < kWeightParts<T>; ++i)
+      total = mma16(ones, weight[i], total);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const v2u lo = lds_read_across(across ^ (b << 5), 0);
+      const v2u hi = lds_read_across(across ^ (b << 5), 16 * Tile::kPitch);
+      const v4u vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int i = 0; i < kWeightParts<T>; ++i)
+        acc[b] = mma16(vf, weight[i], acc[b]);
+    }
+  };
 
   bool some; // whether a key was there (wave-uniform)
+  const int mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;
   for (;;) {
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
       acc[b] = v4f{};
+    total = v4f{};
     top = -kInf;
-    sum = 0.0f;
     some = false;
-    for (int v = v0 + wave * kTile; v < v1; v += 4 * kTile) {
-      const Data now = fetch(v);
-      v4f score[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        score[b] = v4f{};
-        const float by = fp4_scale(now.key_scale[b]);
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const v4u k = fp4_values(now.key[b][st], by);
-#pragma unroll
-          for (int i = kQueryParts<T> - 1; i >= 0; --i)
-            score[b] = mma16(k, q[i][st], score[b]);
+    for (int done = 0; done < mine; done += kWave / 2) {
+      const int first = t0 + wave + 4 * done;
+      const int n = mine - done < kWave / 2 ? mine - done : kWave / 2;
+      const Halves h = locate(first);
+      Data x = fetch(h, 0, see.tile_key(first)), y;
+      for (int k = 0; k < n; k += 2) {
+        if (k + 1 < n)
+          y = fetch(h, k + 1, see.tile_key(first + 4 * k + 4));
+        some |= x.has != 0;
+        compute(x);
+        if (k + 1 < n) {
+          if (k + 2 < n)
+            x = fetch(h, k + 2, see.tile_key(first + 4 * k + 8));
+          some |= y.has != 0;
+          compute(y);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if ((now.none >> i) & 1)
-          score[i / 4][i % 4] = -kInf;
-      float big = score[0][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i)
-        big = fmaxf(big, score[i / 4][i % 4]);
-      big = rows16_max(big) * scale;
-      if (ballot(big > top) != 0) {
-        const float to = fmaxf(top, big);
-        const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-        top = to;
-        sum *= by;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-          acc[b] *= by;
-      }
-      const float less = top == -kInf ? 0.0f : top;
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less)) *
-               lower;
-        sum += p[i];
-      }
-      v4u weight[kWeightParts<T>];
-      weight_parts(p, weight);
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float by = fp4_scale(now.value_scale[b]);
-#pragma unroll
-        for (int w = 0; w < kWords; ++w)
-          lds_write(own + Tile::place(16 * b + (lane & 15), kWords * g + w),
-                    fp4_values(now.value[b][w], by));
-      }
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const v2u x = lds_read_across(across[b], 0);
-        const v2u y = lds_read_across(across[kBlocks + b], 0);
-        const v4u vf = {x.x, x.y, y.x, y.y};
-#pragma unroll
-        for (int i = 0; i < kWeightParts<T>; ++i)
-          acc[b] = mma16(vf, weight[i], acc[b]);
-      }
-      some |= ballot(((~now.none) & 0xFF) != 0) != 0;
     }
     // (a sum past fp32's range of values whose mean lies within: such rows once
     // more under lower probabilities, as in the attention of bf16 caches)
     const bool past = live && !all_finite(acc);
-    if (ballot(past && lower == 1.0f) == 0)
+    if (again || ballot(past) == 0)
       break;
+    again = true;
     if (rows16_max(past ? 1.0f : 0.0f) != 0.0f)
-      lower = __builtin_amdgcn_exp2f(-raise_of(v1 - v0));
+      lower = __builtin_amdgcn_exp2f(-raise_of((t1 - t0) * kTile));
   }
-  const float raise = lower == 1.0f ? 0.0f : raise_of(v1 - v0);
+  const float raise = lower == 1.0f ? 0.0f : raise_of((t1 - t0) * kTile);
   if (some && top == -kInf)
     top = kLowest;
-  store_part<T, D, kWaveBytes>(a, lds, found, top, sum, raise, acc, rows, only,
-                               seq, hk, first_row, a.sums + of * a.dim,
+  store_part<T, D, kWaveBytes>(a, lds, found, top, total[0], raise, acc, rows,
+                               only, seq, hk, first_row, a.sums + of * a.dim,
                                a.stats + of * 2);
 }
 
@@ -308,11 +391,15 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
   Plan p{};
   p.rows = sw::ceil_div(query_heads / key_heads, kRows) * kRows;
   const int64_t visible = most_visible(capacity, window, sinks);
+  // Tiles of 32 keys hold less than they might at both ends of the window and
+  // behind the sinks.
+  const int64_t tiled =
+      std::min(visible + 3 * (kTile - 1), sw::ceil_div(capacity, kTile) * kTile);
   p.chunk = visible <= 512
-                ? 512
-                : part_of(visible, sequences * key_heads * (p.rows / kRows),
+                ? 640
+                : part_of(tiled, sequences * key_heads * (p.rows / kRows),
                           512, 256, 128);
-  p.parts = std::max<int64_t>(1, sw::ceil_div(visible, p.chunk));
+  p.parts = std::max<int64_t>(1, sw::ceil_div(tiled, p.chunk));
   if (p.parts > 1) {
     const int64_t all = sequences * key_heads * p.parts * p.rows;
     p.sums = all * (d <= 64 ? 64 : 128);
@@ -407,6 +494,7 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.chunk = (int)p.chunk;
   a.parts = (int)p.parts;
   a.rows = (int)p.rows;
+  a.by_tiles = true;
   a.lower = std::ldexp(
       1.0f, -(int)std::ceil(std::log2((double)(p.chunk * p.parts))) - 1);
   a.sums = static_cast<float *>(workspace);
