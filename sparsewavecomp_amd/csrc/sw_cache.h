@@ -54,7 +54,6 @@ struct StepArgs {
   // leaves o in [part][rows][dim] and (m, l) in [part][rows][2].
   int chunk, parts, prefix_chunk, prefix_parts;
   int rows, prefix_rows; // of one part: a multiple of 16, of 16 or 128
-  bool by_tiles; // parts are cut at multiples of 32 keys, see Visible::tiles
   // a power of two: the number of all keys times it is below 1
   float lower;
   float *sums, *stats, *prefix_sums, *prefix_stats;
@@ -76,30 +75,6 @@ struct Visible {
   }
   __device__ __forceinline__ int key(int v) const {
     return v < lead ? v : v - lead + start;
-  }
-  __device__ __forceinline__ int end() const { return start + count - lead; }
-  __device__ __forceinline__ bool sees(int j) const {
-    return (j < lead || j >= start) && j < end();
-  }
-  // The tiles of kTile keys from multiples of it on that hold those keys: the
-  // sinks' that lie before the window's first one, and the window's.
-  __device__ __forceinline__ int lead_tiles() const {
-    const int sinks = (lead + kTile - 1) / kTile, first = start / kTile;
-    return sinks < first ? sinks : first;
-  }
-  __device__ __forceinline__ int tiles() const {
-    return count == 0 ? 0
-                      : lead_tiles() + (end() + kTile - 1) / kTile -
-                            start / kTile;
-  }
-  __device__ __forceinline__ int tile_key(int tile) const {
-    const int sinks = lead_tiles();
-    return kTile * (tile < sinks ? tile : tile - sinks + start / kTile);
-  }
-  // How many parts of a.chunk keys they are.
-  __device__ __forceinline__ int parts(const StepArgs &a) const {
-    return a.by_tiles ? (tiles() * kTile + a.chunk - 1) / a.chunk
-           : count == 0 ? 0 : (count - 1) / a.chunk + 1;
   }
 };
 
@@ -178,35 +153,27 @@ store_part(const StepArgs &a, char *lds, Totals &found, float top, float sum,
   }
 }
 
-// Joins the parts of a query head's softmax: one workgroup for each, whose
-// eight half waves take the parts in turn, DIM / 32 consecutive elements a
-// lane, and are joined in LDS.  A launch and two trips: 16 parts of 4 sequences
-// and 32 heads 4.4 us, 128 sequences' 8.4 us.
-template <typename T, int DIM>
-__global__ __launch_bounds__(kThreads) void window_cache_join(StepArgs a) {
+// Joins the parts of a query head's softmax, 0 .. parts - 1, in a workgroup
+// whose eight half waves take them in turn, DIM / 32 consecutive elements a lane,
+// and are joined in LDS.  `row`: of part i, its o and its (m, l).
+struct PartRow {
+  const float *sums, *stats;
+};
+template <typename T, int DIM, typename F>
+__device__ __forceinline__ void join_parts(const StepArgs &a, int seq, int head,
+                                           int parts, F row) {
   constexpr int N = DIM / 32, kHalves = kThreads / 32;
   __shared__ float outs[kHalves][DIM], tops[kHalves], totals[kHalves];
-  const int seq = (int)(blockIdx.x / a.query_heads);
-  const int head = (int)(blockIdx.x % a.query_heads);
-  const int hk = head / a.group, row = head % a.group;
-  const Visible see(a, seq);
-  const int own = see.parts(a);
-  const int parts = own + a.prefix_parts;
   const int half = threadIdx.x / 32, c = (threadIdx.x % 32) * N;
   float top = -kInf, l = 0.0f, o[N] = {};
 #pragma unroll 4
   for (int i = half; i < parts; i += kHalves) {
-    // row of part i in the buffers of sums and statistics
-    const int64_t r =
-        i < own ? (((int64_t)seq * a.key_heads + hk) * a.parts + i) * a.rows + row
-                : ((int64_t)hk * a.prefix_parts + i - own) * a.prefix_rows +
-                      (int64_t)seq * a.group + row;
-    const float *sums = (i < own ? a.sums : a.prefix_sums) + r * DIM + c;
-    const float *stats = (i < own ? a.stats : a.prefix_stats) + r * 2;
-    const float m = stats[0], to = fmaxf(top, m);
+    const PartRow r = row(i);
+    const float *sums = r.sums + c;
+    const float m = r.stats[0], to = fmaxf(top, m);
     const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
     const float add = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-    const float weight = stats[1] * a.lower * add;
+    const float weight = r.stats[1] * a.lower * add;
     top = to;
     l = fmaf(l, by, weight);
 #pragma unroll

@@ -12,6 +12,9 @@
 
 namespace {
 
+// how many powers of two a part's maximum may lag
+constexpr float kLag = 8.0f;
+
 struct Scales {
   const uint8_t *key, *value;
   int64_t key_page, key_token, key_head; // strides in bytes
@@ -22,7 +25,98 @@ struct Fp4StepArgs {
   StepArgs s; // (its cache: the codes, strides in bytes)
   Scales scales;
   Divisor page_size;
+  // A unit is 16 query rows of a key head, for all sequences; `shares` workgroups
+  // split a unit's tiles evenly, each taking `least` at least.  0 shares: a
+  // workgroup for each sequence of a unit.
+  int units, shares, least;
 };
+
+// The tiles of kTile keys, from multiples of it on, that hold the keys that a
+// sequence's query sees: the sinks' that lie before the window's first one, and
+// the window's.
+struct Tiles : Visible {
+  using Visible::Visible;
+  __device__ __forceinline__ int end() const { return start + count - lead; }
+  __device__ __forceinline__ bool sees(int j) const {
+    return (j < lead || j >= start) && j < end();
+  }
+  __device__ __forceinline__ int sink_tiles() const {
+    const int sinks = (lead + kTile - 1) / kTile, first = start / kTile;
+    return sinks < first ? sinks : first;
+  }
+  __device__ __forceinline__ int tiles() const {
+    return count == 0 ? 0
+                      : sink_tiles() + (end() + kTile - 1) / kTile -
+                            start / kTile;
+  }
+  __device__ __forceinline__ int first_key(int tile) const {
+    const int sinks = sink_tiles();
+    return kTile * (tile < sinks ? tile : tile - sinks + start / kTile);
+  }
+};
+__device__ __forceinline__ int tiles_of(const StepArgs &a, int sequence) {
+  return Tiles(a, sequence).tiles();
+}
+
+// The same of a sequence that is wave-uniform, in scalar registers.
+__device__ __forceinline__ Tiles uniform_tiles(const StepArgs &a,
+                                               int sequence) {
+  Tiles see(a, sequence);
+  see.lead = __builtin_amdgcn_readfirstlane(see.lead);
+  see.start = __builtin_amdgcn_readfirstlane(see.start);
+  see.count = __builtin_amdgcn_readfirstlane(see.count);
+  return see;
+}
+
+// The sum over this lane and those before it.
+__device__ __forceinline__ int sum_to_lane(int v) {
+  const int l = lane_id();
+#pragma unroll
+  for (int step = 1; step < kWave; step <<= 1) {
+    const int x = __builtin_amdgcn_ds_bpermute((l - step) * 4, v);
+    v += l >= step ? x : 0;
+  }
+  return v;
+}
+
+// A workgroup's share of a unit's tiles: `share` tiles from `from` on, of which
+// sequence `seq` has those from `offset` on.  Up to 4096 sequences: a lane of a
+// wave sums those of up to 64, the sums are added up over the lanes, and then
+// those of one lane.
+struct Share {
+  int from, to, seq, offset;
+};
+__device__ __forceinline__ int share_of(const Fp4StepArgs &args, int total) {
+  const int even = (total + args.shares - 1) / args.shares;
+  return even < args.least ? args.least : even;
+}
+__device__ __forceinline__ Share find_share(const Fp4StepArgs &args, int p) {
+  const StepArgs &a = args.s;
+  const int l = lane_id(), each = (a.sequences + kWave - 1) / kWave;
+  int own = 0;
+  for (int i = 0; i < each; ++i)
+    if (l * each + i < a.sequences)
+      own += tiles_of(a, l * each + i);
+  int sum = sum_to_lane(own);
+  const int total = __builtin_amdgcn_readlane(sum, kWave - 1);
+  const int share = share_of(args, total);
+  Share s{0, 0, 0, 0};
+  if (total == 0 || p > (total - 1) / share)
+    return s; // (nothing is left)
+  s.from = p * share;
+  s.to = total - s.from < share ? total : s.from + share;
+  int at = __builtin_popcountll(ballot(sum <= s.from));
+  s.seq = at * each;
+  s.offset = __builtin_amdgcn_readlane(sum - own, at);
+  if (each > 1) {
+    own = l < each && s.seq + l < a.sequences ? tiles_of(a, s.seq + l) : 0;
+    sum = s.offset + sum_to_lane(own);
+    at = __builtin_popcountll(ballot(l < each && sum <= s.from));
+    s.seq += at;
+    s.offset = __builtin_amdgcn_readlane(sum - own, at);
+  }
+  return s;
+}
 
 // bf16 parts of a query's elements and of a probability: of fp32 operands all 24
 // bits.  bf16 probabilities keep 15 bits, as in the attention of bf16 caches.
@@ -92,7 +186,7 @@ template <typename T, int D> struct Fp4Parts {
   static constexpr int kWaveBytes =
       Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
   static constexpr int kBytes = 4 * kWaveBytes;
-  static constexpr int kWaves = sizeof(T) == 4 ? 2 : D > 64 ? 3 : 4;
+  static constexpr int kWaves = sizeof(T) == 4 && D > 64 ? 3 : 4;
 };
 
 template <typename T, int D>
@@ -104,49 +198,28 @@ fp4_cache_parts(Fp4StepArgs args) {
   constexpr int kWords = D / 32;  // words of codes of a lane's quarter row
   constexpr int kWaveBytes = Fp4Parts<T, D>::kWaveBytes;
   __shared__ __align__(1024) char lds[Fp4Parts<T, D>::kBytes];
+  // the queries' fragments, [part][step][lane], which all waves read
+  __shared__ v4u queries[kQueryParts<T> * kSteps * kWave];
   __shared__ Totals found;
   const StepArgs &a = args.s;
 
   const int lane = lane_id(), g = lane >> 4, wave = wave_in_group();
-  int64_t item = blockIdx.x;
-  const int part = (int)(item % a.parts);
-  item /= a.parts;
-  const int first_row = (int)(item % (a.rows / kRows)) * kRows;
-  item /= a.rows / kRows;
-  const int hk = (int)(item % a.key_heads);
-  const int seq = (int)(item / a.key_heads);
-  const Visible see(a, seq);
-  const int t0 = part * (a.chunk / kTile);
-  const int t1 = see.tiles() < t0 + a.chunk / kTile ? see.tiles()
-                                                    : t0 + a.chunk / kTile;
-  const int64_t of =
-      (((int64_t)seq * a.key_heads + hk) * a.parts + part) * a.rows + first_row;
-  const bool only = a.parts == 1;
-  if (t1 <= t0 && !only)
-    return;
+  const int unit = (int)(blockIdx.x % args.units);
+  const int number = (int)(blockIdx.x / args.units);
+  const int hk = unit / (a.rows / kRows);
+  const int first_row = (unit - hk * (a.rows / kRows)) * kRows;
   const int rows = a.group - first_row < kRows ? a.group - first_row : kRows;
-
-  const bool none = a.alpha == 0.0f;
-  const float scale = none ? 1.0f : fabsf(a.alpha) * kLog2e;
-  const bool live = (lane & 15) < rows;
-  v4u q[kQueryParts<T>][kSteps];
-  {
-    const int row = first_row + (live ? lane & 15 : 0);
-    const T *p = static_cast<const T *>(a.query) + seq * a.query_token +
-                 (hk * a.group + row) * a.query_head;
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const int c = D / 4 * g + 8 * st;
-      Frag<T> x = live && c < a.d && !none ? ld_frag(p + c) : zero_frag<T>();
-      if (a.alpha < 0.0f)
-        x = negate_frag<T>(x);
-      v4u cut[kQueryParts<T>];
-      query_parts(x, cut);
-#pragma unroll
-      for (int i = 0; i < kQueryParts<T>; ++i)
-        q[i][st] = cut[i];
-    }
+  Share my{0, 0, number, 0};
+  bool begun = false; // whether a part of the share is done
+  if (args.shares != 0) {
+    my = find_share(args, number);
+    if (my.from == my.to)
+      return;
   }
+  const bool none = a.alpha == 0.0f;
+  const float scale = __uint_as_float(__builtin_amdgcn_readfirstlane(
+      __float_as_uint(none ? 1.0f : fabsf(a.alpha) * kLog2e)));
+  const bool live = (lane & 15) < rows;
 
   // This lane's quarter of a row: codes, and the scale of its block.  Quarters
   // past d read the row's first one; the queries are zero there, and so is the
@@ -162,19 +235,25 @@ fp4_cache_parts(Fp4StepArgs args) {
   const uint8_t *key_scales = sc.key + hk * sc.key_head;
   const uint8_t *value_scales = sc.value + hk * sc.value_head;
   // (a token stride is at most 2^23)
-  const uint32_t key_off = row_of * (uint32_t)a.cache.key_token + code_at;
-  const uint32_t value_off = row_of * (uint32_t)a.cache.value_token + code_at;
-  const uint32_t key_scale_off = row_of * (uint32_t)sc.key_token + scale_at;
-  const uint32_t value_scale_off = row_of * (uint32_t)sc.value_token + scale_at;
+  uint32_t key_off = row_of * (uint32_t)a.cache.key_token + code_at;
+  uint32_t value_off = row_of * (uint32_t)a.cache.value_token + code_at;
+  uint32_t key_scale_off = row_of * (uint32_t)sc.key_token + scale_at;
+  uint32_t value_scale_off = row_of * (uint32_t)sc.value_token + scale_at;
 
   typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
+  // (of the sequence at hand, set below)
+  int seq = my.seq, t0, t1;
+  Tiles see = uniform_tiles(a, seq);
   struct Data {
     Words key[2], value[2];
     uint32_t key_scale[2], value_scale[2];
     uint32_t has; // bit i: key i of the tile is seen (wave-uniform)
   };
-  struct Halves { // of the wave's next tiles: lane l has half l % 2 of l / 2
-    int page, slot; // of its first key; page -1: it is not there
+  // Of the wave's next tiles: lane l has half l % 2 of l / 2.
+  enum { kNone, kWhole, kCut };
+  struct Halves {
+    int state; // whether it lies in one page, crosses a page's end, or neither
+    int64_t key, value, key_scale, value_scale; // where its rows start
   };
   auto page_of = [&](int key, int &slot) __attribute__((always_inline)) {
     int page = seq;
@@ -188,43 +267,50 @@ fp4_cache_parts(Fp4StepArgs args) {
   };
   auto locate = [&](int first) __attribute__((always_inline)) {
     const int tile = first + 4 * (lane >> 1);
-    const int key = see.tile_key(tile) + 16 * (lane & 1);
-    Halves h{-1, 0};
-    if (tile < t1 && key < see.end())
-      h.page = page_of(key, h.slot);
+    const int key = see.first_key(tile) + 16 * (lane & 1);
+    Halves h{kNone, 0, 0, 0, 0};
+    if (tile < t1 && key < see.end()) {
+      int slot;
+      const int64_t page = page_of(key, slot);
+      h.state = slot + 16 > a.page_size ? kCut : page < 0 ? kNone : kWhole;
+      h.key = page * a.cache.key_page + slot * a.cache.key_token;
+      h.value = page * a.cache.value_page + slot * a.cache.value_token;
+      h.key_scale = page * sc.key_page + slot * sc.key_token;
+      h.value_scale = page * sc.value_page + slot * sc.value_token;
+    }
     return h;
   };
-  auto load = [&](Data &x, int b, int64_t kc, int64_t vc, int64_t ks,
-                  int64_t vs) __attribute__((always_inline)) {
-    x.key[b] = *reinterpret_cast<const Words *>(key_codes + kc);
-    x.value[b] = *reinterpret_cast<const Words *>(value_codes + vc);
-    x.key_scale[b] = key_scales[ks];
-    x.value_scale[b] = value_scales[vs];
+  // An address in scalar registers, to which a load adds a lane's offset.
+  typedef const __attribute__((address_space(1))) uint8_t *Global;
+  typedef const __attribute__((address_space(1))) Words *GlobalWords;
+  auto scalar = [&](const uint8_t *p) __attribute__((always_inline)) {
+    uint64_t at = (uint64_t)p;
+    asm("" : "+s"(at));
+    return (Global)at;
+  };
+  auto uniform = [&](int64_t v, int from) __attribute__((always_inline)) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, from);
+    const int hi = __builtin_amdgcn_readlane((int)(v >> 32), from);
+    return (int64_t)hi << 32 | lo;
   };
   // tile k of `h`, whose first key is `key`
-  auto fetch = [&](const Halves &h, int k, int key)
+  auto fetch = [&](Data &x, const Halves &h, int k, int key)
                    __attribute__((always_inline)) {
-    Data x;
+    // (32 bits, which the loads extend)
+    asm volatile("" : "+v"(key_off), "+v"(value_off), "+v"(key_scale_off),
+                 "+v"(value_scale_off));
     x.has = 0;
 #pragma unroll
     for (int b = 0; b < 2; ++b, key += 16) {
-      const int64_t page = __builtin_amdgcn_readlane(h.page, 2 * k + b);
-      const int64_t slot = __builtin_amdgcn_readlane(h.slot, 2 * k + b);
-      x.key[b] = x.value[b] = Words{};
-      x.key_scale[b] = x.value_scale[b] = 0;
-      if (slot + 16 <= a.page_size) {
-        if (page < 0)
-          continue;
-        const uint8_t *kc = key_codes + (page * a.cache.key_page +
-                                         slot * a.cache.key_token);
-        const uint8_t *vc = value_codes + (page * a.cache.value_page +
-                                           slot * a.cache.value_token);
-        const uint8_t *ks =
-            key_scales + (page * sc.key_page + slot * sc.key_token);
-        const uint8_t *vs =
-            value_scales + (page * sc.value_page + slot * sc.value_token);
-        x.key[b] = *reinterpret_cast<const Words *>(kc + key_off);
-        x.value[b] = *reinterpret_cast<const Words *>(vc + value_off);
+      const int from = 2 * k + b;
+      const int state = __builtin_amdgcn_readlane(h.state, from);
+      if (state == kWhole) {
+        const Global kc = scalar(key_codes + uniform(h.key, from));
+        const Global vc = scalar(value_codes + uniform(h.value, from));
+        const Global ks = scalar(key_scales + uniform(h.key_scale, from));
+        const Global vs = scalar(value_scales + uniform(h.value_scale, from));
+        x.key[b] = *(GlobalWords)(kc + key_off);
+        x.value[b] = *(GlobalWords)(vc + value_off);
         x.key_scale[b] = ks[key_scale_off];
         x.value_scale[b] = vs[value_scale_off];
         const bool all = (key + 16 <= see.lead || key >= see.start) &&
@@ -233,24 +319,36 @@ fp4_cache_parts(Fp4StepArgs args) {
                       : (uint32_t)ballot(see.sees(key + row_of)) & 0xFFFFu)
                  << (16 * b);
       } else {
-        int s = 0, p = -1;
-        if (see.sees(key + row_of))
-          p = page_of(key + row_of, s);
-        if (p >= 0)
-          load(x, b, p * a.cache.key_page + s * a.cache.key_token + code_at,
-               p * a.cache.value_page + s * a.cache.value_token + code_at,
-               p * sc.key_page + s * sc.key_token + scale_at,
-               p * sc.value_page + s * sc.value_token + scale_at);
-        x.has |= ((uint32_t)ballot(p >= 0) & 0xFFFFu) << (16 * b);
+        x.key[b] = x.value[b] = Words{};
+        x.key_scale[b] = x.value_scale[b] = 0;
+        if (state == kCut) {
+          int slot = 0, lane_row = row_of, code = code_at, block = scale_at;
+          // (what this path needs is not held for it)
+          asm volatile("" : "+v"(lane_row), "+v"(code), "+v"(block));
+          int64_t page = -1;
+          if (see.sees(key + lane_row))
+            page = page_of(key + lane_row, slot);
+          if (page >= 0) {
+            x.key[b] = *reinterpret_cast<const Words *>(
+                key_codes + page * a.cache.key_page +
+                slot * a.cache.key_token + code);
+            x.value[b] = *reinterpret_cast<const Words *>(
+                value_codes + page * a.cache.value_page +
+                slot * a.cache.value_token + code);
+            x.key_scale[b] =
+                key_scales[page * sc.key_page + slot * sc.key_token + block];
+            x.value_scale[b] = value_scales[page * sc.value_page +
+                                            slot * sc.value_token + block];
+          }
+          x.has |= ((uint32_t)ballot(page >= 0) & 0xFFFFu) << (16 * b);
+        }
       }
     }
-    return x;
   };
 
   v4f acc[kBlocks], total; // total: the probabilities' sums, in all four
   float top;
   float lower = 1.0f; // of this lane's row: a factor of the probabilities
-  bool again = false; // whether a row has such a factor (wave-uniform)
   const uint32_t own = lds_address(lds) + wave * kWaveBytes;
   // of a read across rows 4 g + .. and of a write: chunks differ by what the
   // swizzle leaves alone, rows 16 apart have the same
@@ -258,61 +356,44 @@ fp4_cache_parts(Fp4StepArgs args) {
                     Tile::place(4 * g + (row_of >> 2), (lane & 3) >> 1) +
                     (lane & 1) * 8;
   uint32_t along = own + Tile::place(row_of, kWords * g);
+  const uint32_t query_at = lds_address(queries) + lane * 16;
   const v4u ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 
-  auto compute = [&](Data &x) __attribute__((always_inline)) {
+  auto compute = [&](Data &x, auto careful) __attribute__((always_inline)) {
     // (keeps the compiler from holding every address in a register)
     asm volatile("" : "+v"(across), "+v"(along));
-    v4f score[2];
+    v4f score[2] = {};
+    float by[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      score[b] = v4f{};
-      const float by = fp4_scale(inside ? x.key_scale[b] : 0u);
+    for (int b = 0; b < 2; ++b)
+      by[b] = fp4_scale(inside ? x.key_scale[b] : 0u);
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        const v4u k = fp4_values(x.key[b][st], by);
+    for (int st = 0; st < kSteps; ++st) {
+      v4u q[kQueryParts<T>];
+#pragma unroll
+      for (int i = 0; i < kQueryParts<T>; ++i)
+        q[i] = lds_read<v4u>(query_at, (i * kSteps + st) * kWave * 16);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const v4u k = fp4_values(x.key[b][st], by[b]);
 #pragma unroll
         for (int i = kQueryParts<T> - 1; i >= 0; --i)
-          score[b] = mma16(k, q[i][st], score[b]);
+          score[b] = mma16(k, q[i], score[b]);
       }
     }
     if (x.has != 0xFFFFFFFFu) {
+      const uint32_t seen = x.has >> (4 * g);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (!((x.has >> (16 * (i / 4) + 4 * g + i % 4)) & 1))
+        if (!(seen & (1u << (16 * (i / 4) + i % 4))))
           score[i / 4][i % 4] = -kInf;
       // (what lies at a place that is not seen may be NaN)
+      const uint32_t own_key = x.has >> row_of;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        if (!((x.has >> (16 * b + row_of)) & 1))
+        if (!(own_key & (1u << (16 * b))))
           x.value_scale[b] = 0;
     }
-    float big = score[0][0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i)
-      big = fmaxf(big, score[i / 4][i % 4]);
-    big = rows16_max(big) * scale;
-    if (ballot(big > top) != 0) {
-      const float to = fmaxf(top, big);
-      const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-      top = to;
-      total *= by;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-        acc[b] *= by;
-    }
-    const float less = top == -kInf ? 0.0f : top;
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less));
-    if (again) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        p[i] *= lower;
-    }
-    v4u weight[kWeightParts<T>];
-    weight_parts(p, weight);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float by = fp4_scale(x.value_scale[b]);
@@ -321,23 +402,91 @@ fp4_cache_parts(Fp4StepArgs args) {
         lds_write((along ^ (w << 4)) + 16 * b * Tile::kPitch,
                   fp4_values(x.value[b][w], by));
     }
+    float big = score[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+      big = fmaxf(big, score[i / 4][i % 4]);
+    big *= scale;
+    // The maximum lags by up to 2^8: fewer sums are scaled anew, and a row's
+    // four lanes only then compare theirs.
+    if (ballot(big > top + kLag) != 0) {
+      const float to = fmaxf(top, rows16_max(big));
+      const float by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      total *= by;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        acc[b] *= by;
+    }
+    // Reads of kAhead pairs of blocks across the values' rows are on their way
+    // before the probabilities are formed, then one for each pair that is
+    // multiplied (the compiler, left to itself, waits for every read).
+    constexpr int kAhead = 2 < kBlocks / 2 ? 2 : kBlocks / 2;
+    v4u vf[kBlocks];
+    auto read = [&](int pair) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 2 * pair; b < 2 * pair + 2; ++b) {
+        const v2u lo = lds_read_across(across ^ (b << 5), 0);
+        const v2u hi = lds_read_across(across ^ (b << 5), 16 * Tile::kPitch);
+        vf[b] = v4u{lo.x, lo.y, hi.x, hi.y};
+      }
+    };
+#pragma unroll
+    for (int pair = 0; pair < kAhead; ++pair)
+      read(pair);
+    __builtin_amdgcn_sched_barrier(0);
+    const float less = top == -kInf ? 0.0f : top;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less));
+    if constexpr (decltype(careful)::value) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        p[i] *= lower;
+    }
+    v4u weight[kWeightParts<T>];
+    weight_parts(p, weight);
 #pragma unroll
     for (int i = 0; i < kWeightParts<T>; ++i)
       total = mma16(ones, weight[i], total);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      const v2u lo = lds_read_across(across ^ (b << 5), 0);
-      const v2u hi = lds_read_across(across ^ (b << 5), 16 * Tile::kPitch);
-      const v4u vf = {lo.x, lo.y, hi.x, hi.y};
+    for (int pair = 0; pair < kBlocks / 2; ++pair) {
 #pragma unroll
       for (int i = 0; i < kWeightParts<T>; ++i)
-        acc[b] = mma16(vf, weight[i], acc[b]);
+#pragma unroll
+        for (int b = 2 * pair; b < 2 * pair + 2; ++b)
+          acc[b] = mma16(vf[b], weight[i], acc[b]);
+      if (pair + kAhead < kBlocks / 2)
+        read(pair + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
+  for (;;) {
+  const int all = see.tiles();
+  t0 = my.from - my.offset;
+  t1 = args.shares == 0 || my.to - my.offset > all ? all : my.to - my.offset;
+  for (int st = wave; st < kSteps; st += kThreads / kWave) {
+    const int row = first_row + (live ? lane & 15 : 0);
+    const int c = D / 4 * g + 8 * st;
+    const T *p = static_cast<const T *>(a.query) + seq * a.query_token +
+                 (hk * a.group + row) * a.query_head + c;
+    Frag<T> x = live && c < a.d && !none ? ld_frag(p) : zero_frag<T>();
+    if (a.alpha < 0.0f)
+      x = negate_frag<T>(x);
+    v4u cut[kQueryParts<T>];
+    query_parts(x, cut);
+#pragma unroll
+    for (int i = 0; i < kQueryParts<T>; ++i)
+      queries[(i * kSteps + st) * kWave + lane] = cut[i];
+  }
+  __syncthreads();
+  lower = 1.0f;
   bool some; // whether a key was there (wave-uniform)
   const int mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;
-  for (;;) {
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
       acc[b] = v4f{};
@@ -348,63 +497,119 @@ fp4_cache_parts(Fp4StepArgs args) {
       const int first = t0 + wave + 4 * done;
       const int n = mine - done < kWave / 2 ? mine - done : kWave / 2;
       const Halves h = locate(first);
-      Data x = fetch(h, 0, see.tile_key(first)), y;
-      for (int k = 0; k < n; k += 2) {
-        if (k + 1 < n)
-          y = fetch(h, k + 1, see.tile_key(first + 4 * k + 4));
+      for (int k = 0; k < n; ++k) {
+        Data x;
+        fetch(x, h, k, see.first_key(first + 4 * k));
         some |= x.has != 0;
-        compute(x);
-        if (k + 1 < n) {
-          if (k + 2 < n)
-            x = fetch(h, k + 2, see.tile_key(first + 4 * k + 8));
-          some |= y.has != 0;
-          compute(y);
-        }
+        compute(x, careful);
       }
     }
-    // (a sum past fp32's range of values whose mean lies within: such rows once
-    // more under lower probabilities, as in the attention of bf16 caches)
-    const bool past = live && !all_finite(acc);
-    if (again || ballot(past) == 0)
-      break;
-    again = true;
+  };
+  pass(std::false_type{});
+  // (a sum past fp32's range of values whose mean lies within: such rows once
+  // more under lower probabilities, as in the attention of bf16 caches)
+  const bool past = live && !all_finite(acc);
+  if (ballot(past) != 0) {
     if (rows16_max(past ? 1.0f : 0.0f) != 0.0f)
-      lower = __builtin_amdgcn_exp2f(-raise_of((t1 - t0) * kTile));
+      lower = __builtin_amdgcn_exp2f(-kLag - raise_of((t1 - t0) * kTile));
+    pass(std::true_type{});
   }
-  const float raise = lower == 1.0f ? 0.0f : raise_of((t1 - t0) * kTile);
+  const float raise =
+      lower == 1.0f ? 0.0f : kLag + raise_of((t1 - t0) * kTile);
   if (some && top == -kInf)
     top = kLowest;
+  // (a share's first part may go on from the one before: slot 0)
+  const int64_t of =
+      (((int64_t)unit * args.shares + number) * 2 +
+       (begun ? 1 : 0)) * kRows;
   store_part<T, D, kWaveBytes>(a, lds, found, top, total[0], raise, acc, rows,
-                               only, seq, hk, first_row, a.sums + of * a.dim,
-                               a.stats + of * 2);
+                               t0 == 0 && t1 == all, seq, hk, first_row,
+                               a.sums + of * D, a.stats + of * 2);
+  begun = true;
+  my.offset += all;
+  my.from = my.offset;
+  if (args.shares == 0 || my.from >= my.to)
+    return;
+  do {
+    if (++seq >= a.sequences) // (only if lengths change under the call)
+      return;
+    see = uniform_tiles(a, seq);
+  } while (see.count == 0);
+  __syncthreads(); // (LDS of the part before is free)
+  }
+}
+
+// The parts of a query head whose sequence's tiles several shares hold; zeros for
+// one without a key.
+template <typename T, int DIM>
+__global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
+  const StepArgs &a = args.s;
+  __shared__ int sums[2][kThreads / kWave];
+  const int seq = (int)(blockIdx.x / a.query_heads);
+  const int head = (int)(blockIdx.x % a.query_heads);
+  const int hk = head / a.group, row = head % a.group;
+  int before = 0, total = 0;
+  for (int i = threadIdx.x; i < a.sequences; i += kThreads) {
+    const int n = tiles_of(a, i);
+    total += n;
+    before += i < seq ? n : 0;
+  }
+  before = sum_to_lane(before);
+  total = sum_to_lane(total);
+  if (lane_id() == kWave - 1) {
+    sums[0][wave_in_group()] = before;
+    sums[1][wave_in_group()] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; ++w) {
+    before += sums[0][w];
+    total += sums[1][w];
+  }
+  const int own = tiles_of(a, seq);
+  int first = 0, parts = 0, share = 1;
+  if (own > 0) {
+    share = share_of(args, total);
+    first = before / share;
+    parts = (before + own - 1) / share - first + 1;
+    if (parts == 1)
+      return; // (it is written)
+  }
+  const int64_t unit = hk * (a.rows / kRows) + row / kRows;
+  join_parts<T, DIM>(a, seq, head, parts, [&](int i) {
+    const int64_t r =
+        ((unit * args.shares + first + i) * 2 +
+         (i == 0 && before != first * share ? 1 : 0)) * kRows + row % kRows;
+    return PartRow{a.sums + r * DIM, a.stats + r * 2};
+  });
 }
 
 // ---- host ------------------------------------------------------------------------
 
 struct Plan {
-  int64_t chunk, parts, rows, sums, stats; // sums, stats: floats
+  int64_t rows, units, shares, sums, stats; // sums, stats: floats
   int64_t bytes() const { return 4 * (sums + stats); }
 };
 
+// Compute units, and the fewest tiles that a workgroup is made for.
+constexpr int64_t kUnits = 256, kLeast = 16;
+
+// Few keys, or more sequences than a share can be found among, are not split.
 Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
-          int64_t key_heads, int64_t d, int64_t window, int64_t sinks) {
+          int64_t key_heads, int64_t d, int64_t window, int64_t sinks,
+          int64_t waves) {
   Plan p{};
   p.rows = sw::ceil_div(query_heads / key_heads, kRows) * kRows;
+  p.units = key_heads * (p.rows / kRows);
   const int64_t visible = most_visible(capacity, window, sinks);
-  // Tiles of 32 keys hold less than they might at both ends of the window and
-  // behind the sinks.
-  const int64_t tiled =
-      std::min(visible + 3 * (kTile - 1), sw::ceil_div(capacity, kTile) * kTile);
-  p.chunk = visible <= 512
-                ? 640
-                : part_of(tiled, sequences * key_heads * (p.rows / kRows),
-                          512, 256, 128);
-  p.parts = std::max<int64_t>(1, sw::ceil_div(tiled, p.chunk));
-  if (p.parts > 1) {
-    const int64_t all = sequences * key_heads * p.parts * p.rows;
-    p.sums = all * (d <= 64 ? 64 : 128);
-    p.stats = all * 2;
-  }
+  if (visible <= 512 || sequences > 4096 ||
+      sequences * sw::ceil_div(capacity, kTile) > sw::kMostTokens)
+    return p;
+  p.shares = std::max<int64_t>(1, kUnits * waves / p.units);
+  const int64_t all = p.units * p.shares * 2 * kRows;
+  p.sums = all * (d <= 64 ? 64 : 128);
+  p.stats = all * 2;
   return p;
 }
 
@@ -459,7 +664,9 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   if (sequences == 0)
     return SW_OK;
   const Plan p = plan(sequences, page_size * table_width, query_heads,
-                      key_heads, d, window, sinks);
+                      key_heads, d, window, sinks,
+                      d <= 64 ? Fp4Parts<T, 64>::kWaves
+                              : Fp4Parts<T, 128>::kWaves);
   if (p.bytes() > 0 && (!workspace || !sw::aligned16(workspace) ||
                         workspace_bytes < p.bytes()))
     return sw::fail(SW_ERR_INVALID_ARGUMENT,
@@ -491,15 +698,16 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.window = (int)std::min<int64_t>(window, sw::kMostTokens);
   a.sinks = (int)std::min<int64_t>(sinks, sw::kMostTokens);
   a.alpha = alpha;
-  a.chunk = (int)p.chunk;
-  a.parts = (int)p.parts;
   a.rows = (int)p.rows;
-  a.by_tiles = true;
+  args.units = (int)p.units;
+  args.shares = (int)p.shares;
+  args.least = (int)kLeast;
   a.lower = std::ldexp(
-      1.0f, -(int)std::ceil(std::log2((double)(p.chunk * p.parts))) - 1);
+      1.0f, -(int)std::ceil(std::log2((double)(page_size * table_width + kTile))) -
+                1 - (int)kLag);
   a.sums = static_cast<float *>(workspace);
   a.stats = a.sums + p.sums;
-  const int64_t grid = sequences * key_heads * (p.rows / kRows) * p.parts;
+  const int64_t grid = p.units * (p.shares ? p.shares : sequences);
   const int64_t join = sequences * query_heads;
   if (int rc = sw::check_flat_grid(std::max(grid, join), kThreads, what))
     return rc;
@@ -511,12 +719,12 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
     fp4_cache_parts<T, 128><<<g, kThreads, 0, st>>>(args);
   if (int rc = sw::launch_check(what))
     return rc;
-  if (p.parts == 1)
+  if (p.shares == 0)
     return SW_OK;
   if (d <= 64)
-    window_cache_join<T, 64><<<dim3((unsigned)join), kThreads, 0, st>>>(a);
+    fp4_cache_join<T, 64><<<dim3((unsigned)join), kThreads, 0, st>>>(args);
   else
-    window_cache_join<T, 128><<<dim3((unsigned)join), kThreads, 0, st>>>(a);
+    fp4_cache_join<T, 128><<<dim3((unsigned)join), kThreads, 0, st>>>(args);
   return sw::launch_check(what);
 }
 
@@ -531,7 +739,7 @@ extern "C" int64_t sw_window_attention_decode_fp4_workspace_bytes(
                 window, sinks, 0.0f) != SW_OK)
     return 0;
   return plan(sequences, page_size * table_width, query_heads, key_heads, d,
-              window, sinks).bytes();
+              window, sinks, 4).bytes();
 }
 
 extern "C" int sw_window_attention_decode_fp4_f32(
