@@ -90,9 +90,10 @@ struct Totals {
 
 // The four waves' results of one part of the keys, joined in LDS and written:
 // as the output where the part is the `only` one, else to `sums` and `stats`.
-// acc: o[row][d] of a wave, which it leaves in its own WAVE_BYTES of `lds`;
-// top, sum and raise: of row l % 16.
-template <typename T, int D, int WAVE_BYTES>
+// acc: o[column][d] of a wave, which it leaves in its own WAVE_BYTES of `lds`;
+// top, sum and raise: of column l % 16.  Columns ROWS apart are one row's, of
+// different keys.
+template <typename T, int D, int WAVE_BYTES, int ROWS = kRows>
 __device__ __forceinline__ void
 store_part(const StepArgs &a, char *lds, Totals &found, float top, float sum,
            float raise, const v4f (&acc)[D / 16], int rows, bool only, int seq,
@@ -103,33 +104,37 @@ store_part(const StepArgs &a, char *lds, Totals &found, float top, float sum,
     found.sum[wave][lane] = sum;
     found.raise[wave][lane] = raise;
   }
-  // o[row][d] of each wave, in its own part of LDS
+  // o[column][d] of each wave, in its own part of LDS
 #pragma unroll
   for (int b = 0; b < D / 16; ++b)
     lds_write(lds_address(lds) + wave * WAVE_BYTES +
                   ((lane & 15) * D + 16 * b + 4 * g) * 4, acc[b]);
   __syncthreads();
-  for (int x = threadIdx.x; x < kRows * D / 4; x += kThreads) {
+  constexpr int kParts = 4 * (kRows / ROWS); // of a row: wave i % 4, column r + ..
+  for (int x = threadIdx.x; x < ROWS * D / 4; x += kThreads) {
     const int r = x / (D / 4), c = x % (D / 4) * 4;
     if (r >= rows)
       break;
     float m = found.top[0][r], most = found.raise[0][r];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      m = fmaxf(m, found.top[w][r]);
-      most = fmaxf(most, found.raise[w][r]);
+    for (int i = 1; i < kParts; ++i) {
+      m = fmaxf(m, found.top[i % 4][r + i / 4 * ROWS]);
+      most = fmaxf(most, found.raise[i % 4][r + i / 4 * ROWS]);
     }
-    most += 3.0f; // (four sums that are finite have a finite sum)
+    // (as many sums that are finite have a finite sum)
+    most += kRows / ROWS == 1 ? 3.0f : 5.0f;
     float l = 0.0f;
     v4f o = {};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float by =
-          found.top[w][r] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(found.top[w][r] - m);
-      by *= __builtin_amdgcn_exp2f(found.raise[w][r] - most);
-      const v4f y =
-          lds_read<v4f>(lds_address(lds) + w * WAVE_BYTES + (r * D + c) * 4, 0);
-      l = fmaf(found.sum[w][r], by, l);
+    for (int i = 0; i < kParts; ++i) {
+      const int w = i % 4, column = r + i / 4 * ROWS;
+      float by = found.top[w][column] == -kInf
+                     ? 0.0f
+                     : __builtin_amdgcn_exp2f(found.top[w][column] - m);
+      by *= __builtin_amdgcn_exp2f(found.raise[w][column] - most);
+      const v4f y = lds_read<v4f>(
+          lds_address(lds) + w * WAVE_BYTES + (column * D + c) * 4, 0);
+      l = fmaf(found.sum[w][column], by, l);
       o += y * by;
     }
     if (only) {

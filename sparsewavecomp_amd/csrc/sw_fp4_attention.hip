@@ -25,10 +25,11 @@ struct Fp4StepArgs {
   StepArgs s; // (its cache: the codes, strides in bytes)
   Scales scales;
   Divisor page_size;
-  // A unit is 16 query rows of a key head, for all sequences; `shares` workgroups
+  // A unit is `block` query rows (8 or 16) of a key head, for all sequences;
+  // `shares` workgroups
   // split a unit's tiles evenly, each taking `least` at least.  0 shares: a
   // workgroup for each sequence of a unit.
-  int units, shares, least;
+  int units, shares, least, block;
 };
 
 // The tiles of kTile keys, from multiples of it on, that hold the keys that a
@@ -151,64 +152,98 @@ __device__ __forceinline__ void query_parts(v8f x, v4u (&part)[3]) {
   }
 }
 
-// Eight probabilities as two fragments to 2^-15, or three to 2^-23 of each (as
-// split_frag: what is left of one is at least 2^-126).
-__device__ __forceinline__ void weight_parts(const float *x, v4u (&part)[2]) {
-  split_frag(x, part[0], part[1]);
-}
-__device__ __forceinline__ void weight_parts(const float *x, v4u (&part)[3]) {
-  float r[8];
+// Four probabilities as the sum of two bf16 parts, to 2^-15 of each, or of three,
+// to 2^-23: what their upper halves hold, and the rest of it, at the end rounded.
+// The rest of one that is not zero is at least 2^-126, so that an infinity of a
+// value meets no zero.
+template <int N>
+__device__ __forceinline__ void weight_parts(const float *x, v2u (&part)[N]) {
+  float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    r[e] = __builtin_amdgcn_fmed3f(
-        x[e] - __uint_as_float(__float_as_uint(x[e]) & 0xFFFF0000u), 0x1p-126f,
-        x[e]);
+  for (int i = 0; i < N - 1; ++i) {
+    part[i] = v2u{__builtin_amdgcn_perm(__float_as_uint(r[1]),
+                                        __float_as_uint(r[0]), 0x07060302u),
+                  __builtin_amdgcn_perm(__float_as_uint(r[3]),
+                                        __float_as_uint(r[2]), 0x07060302u)};
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    part[0][e] = __builtin_amdgcn_perm(__float_as_uint(x[2 * e + 1]),
-                                       __float_as_uint(x[2 * e]), 0x07060302u);
-  split_frag(r, part[1], part[2]);
+    for (int e = 0; e < 4; ++e)
+      r[e] = __builtin_amdgcn_fmed3f(
+          r[e] - __uint_as_float(__float_as_uint(r[e]) & 0xFFFF0000u), 0x1p-126f,
+          r[e]);
+  }
+  part[N - 1] = v2u{cvt_pk_bf16(r[0], r[1]), cvt_pk_bf16(r[2], r[3])};
 }
 
-// One chunk of keys against up to 16 query rows, 32 keys a wave at a time: lane
-// l holds a quarter (l / 16) of the keys l % 16 and 16 + l % 16, whose codes are
-// one load for d = 128; quarter g of step st is elements D / 4 g + 8 st + i of
-// the products' K index, in the queries too.  Values go through LDS as bf16, to
-// be read across their rows.
+// Rows of 16-bit values of a wave's LDS, in chunks of 16 bytes; chunk c of row r
+// lies at place c ^ swizzle(r).  Free of bank conflicts: a write of one chunk of
+// eight consecutive rows (32 banks of 4 bytes; with the swizzle of RowTile such
+// writes took twice as long), and half a wave's transposing load, two chunks of
+// eight rows (64 banks).
+template <int D> struct ValueTile {
+  static constexpr int kPitch = 2 * D;
+  static constexpr int kBytes = 32 * kPitch;
+  __device__ static __forceinline__ int place(int row, int chunk) {
+    const int swizzle =
+        D > 64 ? (row & 4) << 1 | (row & 1) << 2 | (row & 2) | (row >> 2 & 1)
+               : (row & 2) << 1 | (row >> 1 & 2) | (row & 1);
+    return row * kPitch + ((chunk ^ swizzle) << 4);
+  }
+};
+
+// One share of a unit's tiles, a tile a wave at a time, part by part (a part:
+// the share's tiles of one sequence).  Lane l holds a quarter (l / 16) of key
+// l % 16 of each of the tile's runs of 16 keys, whose codes are one load for
+// d = 128; quarter g of step st is elements D / 4 g + 8 st + i of the products'
+// K index, in the queries too.  Values go through LDS as bf16, to be read across
+// their rows.
 //
-// Tiles start at multiples of 32 keys, so that a half of 16 lies in one page
-// wherever a page holds a multiple of 16: its addresses are then scalar ones
-// plus a lane's constant offset.  Halves that cross a page's end take each
-// lane's own.  The pages of a wave's next 32 tiles are found at once, a half by
-// each lane; the next tile is on its way while one is multiplied.
+// A run of 16 keys lies in one page wherever a page holds a multiple of 16: its
+// addresses are then scalar ones plus a lane's constant offset.  Runs that cross
+// a page's end take each lane's own.  The pages of a wave's next runs are found
+// 64 at once, one by each lane.
+//
+// Up to 8 query rows (ROWS) have the 16 columns of a product twice, each half for
+// the scores of one of the tile's two runs, so that a lane has 4 scores instead of
+// 8, half of them of rows that are not there.  A half's probabilities are masked
+// out where the other run's values are multiplied; each column keeps a maximum and
+// sums of its own, joined like a part's at the end.
+//
+// STREAM: the codes pass by the caches, where no other workgroup reads them.
 template <typename T, int D> struct Fp4Parts {
-  using Tile = RowTile<uint16_t, D, kTile, kWave>;
+  using Tile = ValueTile<D>;
   static constexpr int kWaveBytes =
       Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
   static constexpr int kBytes = 4 * kWaveBytes;
-  static constexpr int kWaves = sizeof(T) == 4 && D > 64 ? 3 : 4;
+  static constexpr int kWaves = D > 64 ? 3 : 4;
 };
 
-template <typename T, int D>
+template <typename T, int D, int ROWS, bool STREAM>
 __global__ __launch_bounds__(kThreads, (Fp4Parts<T, D>::kWaves)) void
 fp4_cache_parts(Fp4StepArgs args) {
-  using Tile = typename Fp4Parts<T, D>::Tile;
+  using F = Fp4Parts<T, D>;
+  using Tile = typename F::Tile;
   constexpr int kSteps = D / 32;  // products along d
   constexpr int kBlocks = D / 16; // output rows of 16
   constexpr int kWords = D / 32;  // words of codes of a lane's quarter row
-  constexpr int kWaveBytes = Fp4Parts<T, D>::kWaveBytes;
-  __shared__ __align__(1024) char lds[Fp4Parts<T, D>::kBytes];
+  constexpr bool kHalves = ROWS == 8;
+  constexpr int kSets = kHalves ? 1 : 2; // of 4 scores a lane
+  __shared__ __align__(1024) char lds[F::kBytes];
   // the queries' fragments, [part][step][lane], which all waves read
   __shared__ v4u queries[kQueryParts<T> * kSteps * kWave];
   __shared__ Totals found;
   const StepArgs &a = args.s;
 
   const int lane = lane_id(), g = lane >> 4, wave = wave_in_group();
-  const int unit = (int)(blockIdx.x % args.units);
+  const int row_of = lane & 15; // key of a run, column of a product
+  // (neighbours take the units in turn, starting with another one each time: an
+  // XCD, which gets every eighth workgroup, does not keep to one head's rows)
   const int number = (int)(blockIdx.x / args.units);
-  const int hk = unit / (a.rows / kRows);
-  const int first_row = (unit - hk * (a.rows / kRows)) * kRows;
-  const int rows = a.group - first_row < kRows ? a.group - first_row : kRows;
+  const int unit = (int)((blockIdx.x + number) % args.units);
+  const int blocks = (a.group + ROWS - 1) / ROWS; // of rows, of a key head
+  const int hk = unit / blocks;
+  const int first_row = (unit - hk * blocks) * ROWS;
+  const int rows = a.group - first_row < ROWS ? a.group - first_row : ROWS;
+  const bool live = row_of % ROWS < rows;
   Share my{0, 0, number, 0};
   bool begun = false; // whether a part of the share is done
   if (args.shares != 0) {
@@ -219,14 +254,12 @@ fp4_cache_parts(Fp4StepArgs args) {
   const bool none = a.alpha == 0.0f;
   const float scale = __uint_as_float(__builtin_amdgcn_readfirstlane(
       __float_as_uint(none ? 1.0f : fabsf(a.alpha) * kLog2e)));
-  const bool live = (lane & 15) < rows;
 
   // This lane's quarter of a row: codes, and the scale of its block.  Quarters
   // past d read the row's first one; the queries are zero there, and so is the
   // scale.
   const bool inside = D / 4 * g < a.d;
   const int code_at = inside ? D / 8 * g : 0, scale_at = inside ? D * g / 128 : 0;
-  const int row_of = lane & 15;
   const Scales &sc = args.scales;
   const uint8_t *key_codes =
       static_cast<const uint8_t *>(a.cache.key) + hk * a.cache.key_head;
@@ -240,18 +273,18 @@ fp4_cache_parts(Fp4StepArgs args) {
   uint32_t key_scale_off = row_of * (uint32_t)sc.key_token + scale_at;
   uint32_t value_scale_off = row_of * (uint32_t)sc.value_token + scale_at;
 
-  typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
   // (of the sequence at hand, set below)
   int seq = my.seq, t0, t1;
   Tiles see = uniform_tiles(a, seq);
+  typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
   struct Data {
     Words key[2], value[2];
     uint32_t key_scale[2], value_scale[2];
-    uint32_t has; // bit i: key i of the tile is seen (wave-uniform)
+    uint32_t has[2]; // bit i: key i of the run is seen (wave-uniform)
   };
-  // Of the wave's next tiles: lane l has half l % 2 of l / 2.
+  // Of the wave's next tiles: lane l has run l % 2 of tile l / 2.
   enum { kNone, kWhole, kCut };
-  struct Halves {
+  struct Runs {
     int state; // whether it lies in one page, crosses a page's end, or neither
     int64_t key, value, key_scale, value_scale; // where its rows start
   };
@@ -266,58 +299,61 @@ fp4_cache_parts(Fp4StepArgs args) {
     return page >= 0 && page < a.pages ? page : -1;
   };
   auto locate = [&](int first) __attribute__((always_inline)) {
-    const int tile = first + 4 * (lane >> 1);
-    const int key = see.first_key(tile) + 16 * (lane & 1);
-    Halves h{kNone, 0, 0, 0, 0};
+    const int tile = first + 4 * (lane / 2);
+    const int key = see.first_key(tile) + 16 * (lane % 2);
+    Runs r{kNone, 0, 0, 0, 0};
     if (tile < t1 && key < see.end()) {
       int slot;
       const int64_t page = page_of(key, slot);
-      h.state = slot + 16 > a.page_size ? kCut : page < 0 ? kNone : kWhole;
-      h.key = page * a.cache.key_page + slot * a.cache.key_token;
-      h.value = page * a.cache.value_page + slot * a.cache.value_token;
-      h.key_scale = page * sc.key_page + slot * sc.key_token;
-      h.value_scale = page * sc.value_page + slot * sc.value_token;
+      r.state = slot + 16 > a.page_size ? kCut : page < 0 ? kNone : kWhole;
+      r.key = page * a.cache.key_page + slot * a.cache.key_token;
+      r.value = page * a.cache.value_page + slot * a.cache.value_token;
+      r.key_scale = page * sc.key_page + slot * sc.key_token;
+      r.value_scale = page * sc.value_page + slot * sc.value_token;
     }
-    return h;
+    return r;
   };
   // An address in scalar registers, to which a load adds a lane's offset.
   typedef const __attribute__((address_space(1))) uint8_t *Global;
   typedef const __attribute__((address_space(1))) Words *GlobalWords;
-  auto scalar = [&](const uint8_t *p) __attribute__((always_inline)) {
-    uint64_t at = (uint64_t)p;
-    asm("" : "+s"(at));
-    return (Global)at;
+  auto scalar = [&](const uint8_t *p, int64_t at, int from)
+                    __attribute__((always_inline)) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)at, from);
+    const int hi = __builtin_amdgcn_readlane((int)(at >> 32), from);
+    uint64_t address = (uint64_t)p + ((uint64_t)(uint32_t)hi << 32 | lo);
+    asm("" : "+s"(address));
+    return (Global)address;
   };
-  auto uniform = [&](int64_t v, int from) __attribute__((always_inline)) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)v, from);
-    const int hi = __builtin_amdgcn_readlane((int)(v >> 32), from);
-    return (int64_t)hi << 32 | lo;
+  auto codes = [](GlobalWords p) __attribute__((always_inline)) {
+    if constexpr (STREAM)
+      return __builtin_nontemporal_load(p);
+    else
+      return *p;
   };
-  // tile k of `h`, whose first key is `key`
-  auto fetch = [&](Data &x, const Halves &h, int k, int key)
+  // tile k of those located, whose first key is `key`
+  auto fetch = [&](Data &x, const Runs &r, int k, int key)
                    __attribute__((always_inline)) {
     // (32 bits, which the loads extend)
     asm volatile("" : "+v"(key_off), "+v"(value_off), "+v"(key_scale_off),
                  "+v"(value_scale_off));
-    x.has = 0;
 #pragma unroll
     for (int b = 0; b < 2; ++b, key += 16) {
       const int from = 2 * k + b;
-      const int state = __builtin_amdgcn_readlane(h.state, from);
+      const int state = __builtin_amdgcn_readlane(r.state, from);
+      x.has[b] = 0;
       if (state == kWhole) {
-        const Global kc = scalar(key_codes + uniform(h.key, from));
-        const Global vc = scalar(value_codes + uniform(h.value, from));
-        const Global ks = scalar(key_scales + uniform(h.key_scale, from));
-        const Global vs = scalar(value_scales + uniform(h.value_scale, from));
-        x.key[b] = *(GlobalWords)(kc + key_off);
-        x.value[b] = *(GlobalWords)(vc + value_off);
+        const Global kc = scalar(key_codes, r.key, from);
+        const Global vc = scalar(value_codes, r.value, from);
+        const Global ks = scalar(key_scales, r.key_scale, from);
+        const Global vs = scalar(value_scales, r.value_scale, from);
+        x.key[b] = codes((GlobalWords)(kc + key_off));
         x.key_scale[b] = ks[key_scale_off];
+        x.value[b] = codes((GlobalWords)(vc + value_off));
         x.value_scale[b] = vs[value_scale_off];
         const bool all = (key + 16 <= see.lead || key >= see.start) &&
                          key + 16 <= see.end();
-        x.has |= (all ? 0xFFFFu
-                      : (uint32_t)ballot(see.sees(key + row_of)) & 0xFFFFu)
-                 << (16 * b);
+        x.has[b] = all ? 0xFFFFu
+                       : (uint32_t)ballot(see.sees(key + row_of)) & 0xFFFFu;
       } else {
         x.key[b] = x.value[b] = Words{};
         x.key_scale[b] = x.value_scale[b] = 0;
@@ -340,7 +376,7 @@ fp4_cache_parts(Fp4StepArgs args) {
             x.value_scale[b] = value_scales[page * sc.value_page +
                                             slot * sc.value_token + block];
           }
-          x.has |= ((uint32_t)ballot(page >= 0) & 0xFFFFu) << (16 * b);
+          x.has[b] = (uint32_t)ballot(page >= 0) & 0xFFFFu;
         }
       }
     }
@@ -348,12 +384,11 @@ fp4_cache_parts(Fp4StepArgs args) {
 
   v4f acc[kBlocks], total; // total: the probabilities' sums, in all four
   float top;
-  float lower = 1.0f; // of this lane's row: a factor of the probabilities
-  const uint32_t own = lds_address(lds) + wave * kWaveBytes;
+  float lower = 1.0f; // of this lane's column: a factor of the probabilities
+  const uint32_t own = lds_address(lds) + wave * F::kWaveBytes;
   // of a read across rows 4 g + .. and of a write: chunks differ by what the
   // swizzle leaves alone, rows 16 apart have the same
-  uint32_t across = own +
-                    Tile::place(4 * g + (row_of >> 2), (lane & 3) >> 1) +
+  uint32_t across = own + Tile::place(4 * g + (row_of >> 2), (lane & 3) >> 1) +
                     (lane & 1) * 8;
   uint32_t along = own + Tile::place(row_of, kWords * g);
   const uint32_t query_at = lds_address(queries) + lane * 16;
@@ -362,52 +397,60 @@ fp4_cache_parts(Fp4StepArgs args) {
   auto compute = [&](Data &x, auto careful) __attribute__((always_inline)) {
     // (keeps the compiler from holding every address in a register)
     asm volatile("" : "+v"(across), "+v"(along));
-    v4f score[2] = {};
-    float by[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-      by[b] = fp4_scale(inside ? x.key_scale[b] : 0u);
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      v4u q[kQueryParts<T>];
-#pragma unroll
-      for (int i = 0; i < kQueryParts<T>; ++i)
-        q[i] = lds_read<v4u>(query_at, (i * kSteps + st) * kWave * 16);
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const v4u k = fp4_values(x.key[b][st], by[b]);
-#pragma unroll
-        for (int i = kQueryParts<T> - 1; i >= 0; --i)
-          score[b] = mma16(k, q[i], score[b]);
-      }
-    }
-    if (x.has != 0xFFFFFFFFu) {
-      const uint32_t seen = x.has >> (4 * g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!(seen & (1u << (16 * (i / 4) + i % 4))))
-          score[i / 4][i % 4] = -kInf;
-      // (what lies at a place that is not seen may be NaN)
-      const uint32_t own_key = x.has >> row_of;
+    // element i of set s: of key 4 g + i of run s, or with halves of this
+    // column's run
+    v4f score[kSets];
+    {
+      v4f product[2] = {};
+      float by[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        if (!(own_key & (1u << (16 * b))))
-          x.value_scale[b] = 0;
+        by[b] = fp4_scale(inside ? x.key_scale[b] : 0u);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        v4u q[kQueryParts<T>];
+#pragma unroll
+        for (int i = 0; i < kQueryParts<T>; ++i)
+          q[i] = lds_read<v4u>(query_at, (i * kSteps + st) * kWave * 16);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const v4u k = fp4_values(x.key[b][st], by[b]);
+#pragma unroll
+          for (int i = kQueryParts<T> - 1; i >= 0; --i)
+            product[b] = mma16(k, q[i], product[b]);
+        }
+      }
+      if constexpr (kHalves) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          score[0][i] = row_of < ROWS ? product[0][i] : product[1][i];
+      } else {
+        score[0] = product[0];
+        score[1] = product[1];
+      }
     }
+    if ((x.has[0] & x.has[1]) != 0xFFFFu) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const float by = fp4_scale(x.value_scale[b]);
+      for (int s = 0; s < kSets; ++s) {
+        const uint32_t seen =
+            (kHalves && row_of >= ROWS ? x.has[1] : x.has[s]) >> (4 * g);
 #pragma unroll
-      for (int w = 0; w < kWords; ++w)
-        lds_write((along ^ (w << 4)) + 16 * b * Tile::kPitch,
-                  fp4_values(x.value[b][w], by));
+        for (int i = 0; i < 4; ++i)
+          if (!(seen & (1u << i)))
+            score[s][i] = -kInf;
+      }
+      // (what lies at a place that is not seen may be NaN)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        if (!(x.has[b] >> row_of & 1))
+          x.value_scale[b] = 0;
     }
     float big = score[0][0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i)
+    for (int i = 1; i < 4 * kSets; ++i)
       big = fmaxf(big, score[i / 4][i % 4]);
     big *= scale;
-    // The maximum lags by up to 2^8: fewer sums are scaled anew, and a row's
+    // The maximum lags by up to 2^8: fewer sums are scaled anew, and a column's
     // four lanes only then compare theirs.
     if (ballot(big > top + kLag) != 0) {
       const float to = fmaxf(top, rows16_max(big));
@@ -418,10 +461,30 @@ fp4_cache_parts(Fp4StepArgs args) {
       for (int b = 0; b < kBlocks; ++b)
         acc[b] *= by;
     }
-    // Reads of kAhead pairs of blocks across the values' rows are on their way
-    // before the probabilities are formed, then one for each pair that is
-    // multiplied (the compiler, left to itself, waits for every read).
-    constexpr int kAhead = 2 < kBlocks / 2 ? 2 : kBlocks / 2;
+    const float less = top == -kInf ? 0.0f : top;
+    float p[4 * kSets];
+#pragma unroll
+    for (int i = 0; i < 4 * kSets; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less));
+      if constexpr (decltype(careful)::value)
+        p[i] *= lower;
+    }
+    v2u weight[kSets][kWeightParts<T>];
+#pragma unroll
+    for (int s = 0; s < kSets; ++s)
+      weight_parts(p + 4 * s, weight[s]);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float by = fp4_scale(x.value_scale[b]);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        lds_write((along ^ (w << 4)) + 16 * b * Tile::kPitch,
+                  fp4_values(x.value[b][w], by));
+    }
+    // Reads of two pairs of blocks across the values' rows are on their way before
+    // the products, then one for each pair that is multiplied (the compiler, left
+    // to itself, waits for every read).
+    constexpr int kPairs = kBlocks / 2, kAhead = 2 < kPairs ? 2 : kPairs;
     v4u vf[kBlocks];
     auto read = [&](int pair) __attribute__((always_inline)) {
 #pragma unroll
@@ -435,107 +498,113 @@ fp4_cache_parts(Fp4StepArgs args) {
     for (int pair = 0; pair < kAhead; ++pair)
       read(pair);
     __builtin_amdgcn_sched_barrier(0);
-    const float less = top == -kInf ? 0.0f : top;
-    float p[8];
+    v4u by[kWeightParts<T>];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      p[i] = __builtin_amdgcn_exp2f(fmaf(score[i / 4][i % 4], scale, -less));
-    if constexpr (decltype(careful)::value) {
+    for (int i = 0; i < kWeightParts<T>; ++i) {
+      v2u run[2] = {weight[0][i], weight[kSets - 1][i]};
+      if constexpr (kHalves) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        p[i] *= lower;
+        for (int e = 0; e < 2; ++e) {
+          run[0][e] = row_of < ROWS ? run[0][e] : 0u;
+          run[1][e] = row_of < ROWS ? 0u : run[1][e];
+        }
+      }
+      by[i] = v4u{run[0].x, run[0].y, run[1].x, run[1].y};
+      total = mma16(ones, by[i], total);
     }
-    v4u weight[kWeightParts<T>];
-    weight_parts(p, weight);
-#pragma unroll
-    for (int i = 0; i < kWeightParts<T>; ++i)
-      total = mma16(ones, weight[i], total);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int pair = 0; pair < kBlocks / 2; ++pair) {
+    for (int pair = 0; pair < kPairs; ++pair) {
 #pragma unroll
       for (int i = 0; i < kWeightParts<T>; ++i)
 #pragma unroll
         for (int b = 2 * pair; b < 2 * pair + 2; ++b)
-          acc[b] = mma16(vf[b], weight[i], acc[b]);
-      if (pair + kAhead < kBlocks / 2)
+          acc[b] = mma16(vf[b], by[i], acc[b]);
+      if (pair + kAhead < kPairs)
         read(pair + kAhead);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
   for (;;) {
-  const int all = see.tiles();
-  t0 = my.from - my.offset;
-  t1 = args.shares == 0 || my.to - my.offset > all ? all : my.to - my.offset;
-  for (int st = wave; st < kSteps; st += kThreads / kWave) {
-    const int row = first_row + (live ? lane & 15 : 0);
-    const int c = D / 4 * g + 8 * st;
-    const T *p = static_cast<const T *>(a.query) + seq * a.query_token +
-                 (hk * a.group + row) * a.query_head + c;
-    Frag<T> x = live && c < a.d && !none ? ld_frag(p) : zero_frag<T>();
-    if (a.alpha < 0.0f)
-      x = negate_frag<T>(x);
-    v4u cut[kQueryParts<T>];
-    query_parts(x, cut);
+    const int all = see.tiles();
+    t0 = my.from - my.offset;
+    t1 = args.shares == 0 || my.to - my.offset > all ? all : my.to - my.offset;
+    static_assert(kSteps <= kThreads / kWave, ""); // (a step of queries a wave)
+    if (wave < kSteps) {
+      const int c = D / 4 * g + 8 * wave;
+      const T *p = static_cast<const T *>(a.query) + seq * a.query_token +
+                   (hk * a.group + first_row + row_of % ROWS) * a.query_head + c;
+      Frag<T> x = live && c < a.d && !none ? ld_frag(p) : zero_frag<T>();
+      if (a.alpha < 0.0f)
+        x = negate_frag<T>(x);
+      v4u cut[kQueryParts<T>];
+      query_parts(x, cut);
 #pragma unroll
-    for (int i = 0; i < kQueryParts<T>; ++i)
-      queries[(i * kSteps + st) * kWave + lane] = cut[i];
-  }
-  __syncthreads();
-  lower = 1.0f;
-  bool some; // whether a key was there (wave-uniform)
-  const int mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;
-  auto pass = [&](auto careful) __attribute__((always_inline)) {
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-      acc[b] = v4f{};
-    total = v4f{};
-    top = -kInf;
-    some = false;
-    for (int done = 0; done < mine; done += kWave / 2) {
-      const int first = t0 + wave + 4 * done;
-      const int n = mine - done < kWave / 2 ? mine - done : kWave / 2;
-      const Halves h = locate(first);
-      for (int k = 0; k < n; ++k) {
-        Data x;
-        fetch(x, h, k, see.first_key(first + 4 * k));
-        some |= x.has != 0;
-        compute(x, careful);
-      }
+      for (int i = 0; i < kQueryParts<T>; ++i)
+        queries[(i * kSteps + wave) * kWave + lane] = cut[i];
     }
-  };
-  pass(std::false_type{});
-  // (a sum past fp32's range of values whose mean lies within: such rows once
-  // more under lower probabilities, as in the attention of bf16 caches)
-  const bool past = live && !all_finite(acc);
-  if (ballot(past) != 0) {
-    if (rows16_max(past ? 1.0f : 0.0f) != 0.0f)
-      lower = __builtin_amdgcn_exp2f(-kLag - raise_of((t1 - t0) * kTile));
-    pass(std::true_type{});
-  }
-  const float raise =
-      lower == 1.0f ? 0.0f : kLag + raise_of((t1 - t0) * kTile);
-  if (some && top == -kInf)
-    top = kLowest;
-  // (a share's first part may go on from the one before: slot 0)
-  const int64_t of =
-      (((int64_t)unit * args.shares + number) * 2 +
-       (begun ? 1 : 0)) * kRows;
-  store_part<T, D, kWaveBytes>(a, lds, found, top, total[0], raise, acc, rows,
-                               t0 == 0 && t1 == all, seq, hk, first_row,
-                               a.sums + of * D, a.stats + of * 2);
-  begun = true;
-  my.offset += all;
-  my.from = my.offset;
-  if (args.shares == 0 || my.from >= my.to)
-    return;
-  do {
-    if (++seq >= a.sequences) // (only if lengths change under the call)
+    __syncthreads();
+    lower = 1.0f;
+    bool some; // whether a key was there (wave-uniform)
+    const int mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;
+    auto pass = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        acc[b] = v4f{};
+      total = v4f{};
+      top = -kInf;
+      some = false;
+      for (int done = 0; done < mine; done += kWave / 2) {
+        const int first = t0 + wave + 4 * done;
+        const int n = mine - done < kWave / 2 ? mine - done : kWave / 2;
+        const Runs runs = locate(first);
+        Data x, y;
+        fetch(x, runs, 0, see.first_key(first));
+        for (int k = 0; k < n; k += 2) {
+          if (k + 1 < n)
+            fetch(y, runs, k + 1, see.first_key(first + 4 * k + 4));
+          some |= (x.has[0] | x.has[1]) != 0;
+          compute(x, careful);
+          if (k + 1 < n) {
+            if (k + 2 < n)
+              fetch(x, runs, k + 2, see.first_key(first + 4 * k + 8));
+            some |= (y.has[0] | y.has[1]) != 0;
+            compute(y, careful);
+          }
+        }
+      }
+    };
+    pass(std::false_type{});
+    // (a sum past fp32's range of values whose mean lies within: such columns
+    // once more under lower probabilities, as in the attention of bf16 caches)
+    const bool past = live && !all_finite(acc);
+    if (ballot(past) != 0) {
+      if (rows16_max(past ? 1.0f : 0.0f) != 0.0f)
+        lower = __builtin_amdgcn_exp2f(-kLag - raise_of((t1 - t0) * kTile));
+      pass(std::true_type{});
+    }
+    const float raise =
+        lower == 1.0f ? 0.0f : kLag + raise_of((t1 - t0) * kTile);
+    if (some && top == -kInf)
+      top = kLowest;
+    // (a share's first part may go on from the one before: slot 0)
+    const int64_t of =
+        (((int64_t)unit * args.shares + number) * 2 + (begun ? 1 : 0)) * ROWS;
+    store_part<T, D, F::kWaveBytes, ROWS>(
+        a, lds, found, top, total[0], raise, acc, rows, t0 == 0 && t1 == all,
+        seq, hk, first_row, a.sums + of * D, a.stats + of * 2);
+    begun = true;
+    my.offset += all;
+    my.from = my.offset;
+    if (args.shares == 0 || my.from >= my.to)
       return;
-    see = uniform_tiles(a, seq);
-  } while (see.count == 0);
-  __syncthreads(); // (LDS of the part before is free)
+    do {
+      if (++seq >= a.sequences) // (only if lengths change under the call)
+        return;
+      see = uniform_tiles(a, seq);
+    } while (see.count == 0);
+    __syncthreads(); // (LDS of the part before is free)
   }
 }
 
@@ -576,11 +645,13 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
     if (parts == 1)
       return; // (it is written)
   }
-  const int64_t unit = hk * (a.rows / kRows) + row / kRows;
+  const int64_t unit = hk * ((a.group + args.block - 1) / args.block) +
+                       row / args.block;
   join_parts<T, DIM>(a, seq, head, parts, [&](int i) {
     const int64_t r =
         ((unit * args.shares + first + i) * 2 +
-         (i == 0 && before != first * share ? 1 : 0)) * kRows + row % kRows;
+         (i == 0 && before != first * share ? 1 : 0)) * args.block +
+        row % args.block;
     return PartRow{a.sums + r * DIM, a.stats + r * 2};
   });
 }
@@ -588,26 +659,28 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
 // ---- host ------------------------------------------------------------------------
 
 struct Plan {
-  int64_t rows, units, shares, sums, stats; // sums, stats: floats
+  int64_t block, units, shares, sums, stats; // sums, stats: floats
   int64_t bytes() const { return 4 * (sums + stats); }
 };
 
 // Compute units, and the fewest tiles that a workgroup is made for.
 constexpr int64_t kUnits = 256, kLeast = 16;
 
-// Few keys, or more sequences than a share can be found among, are not split.
+// `waves`: workgroups of a compute unit.  Few keys, or more sequences than a
+// share can be found among, are not split.
 Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
           int64_t key_heads, int64_t d, int64_t window, int64_t sinks,
           int64_t waves) {
   Plan p{};
-  p.rows = sw::ceil_div(query_heads / key_heads, kRows) * kRows;
-  p.units = key_heads * (p.rows / kRows);
+  const int64_t group = query_heads / key_heads;
+  p.block = group <= 8 ? 8 : kRows;
+  p.units = key_heads * sw::ceil_div(group, p.block);
   const int64_t visible = most_visible(capacity, window, sinks);
   if (visible <= 512 || sequences > 4096 ||
-      sequences * sw::ceil_div(capacity, kTile) > sw::kMostTokens)
+      sequences * sw::ceil_div(capacity, 32) > sw::kMostTokens)
     return p;
   p.shares = std::max<int64_t>(1, kUnits * waves / p.units);
-  const int64_t all = p.units * p.shares * 2 * kRows;
+  const int64_t all = p.units * p.shares * 2 * p.block;
   p.sums = all * (d <= 64 ? 64 : 128);
   p.stats = all * 2;
   return p;
@@ -698,12 +771,12 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.window = (int)std::min<int64_t>(window, sw::kMostTokens);
   a.sinks = (int)std::min<int64_t>(sinks, sw::kMostTokens);
   a.alpha = alpha;
-  a.rows = (int)p.rows;
+  args.block = (int)p.block;
   args.units = (int)p.units;
   args.shares = (int)p.shares;
   args.least = (int)kLeast;
   a.lower = std::ldexp(
-      1.0f, -(int)std::ceil(std::log2((double)(page_size * table_width + kTile))) -
+      1.0f, -(int)std::ceil(std::log2((double)(page_size * table_width + 64))) -
                 1 - (int)kLag);
   a.sums = static_cast<float *>(workspace);
   a.stats = a.sums + p.sums;
@@ -713,10 +786,19 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
     return rc;
   const hipStream_t st = sw::as_stream(stream);
   const dim3 g((unsigned)grid);
+  auto launch = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    if (a.group <= 8)
+      fp4_cache_parts<T, D, 8, true><<<g, kThreads, 0, st>>>(args);
+    else if (a.group <= kRows)
+      fp4_cache_parts<T, D, kRows, true><<<g, kThreads, 0, st>>>(args);
+    else
+      fp4_cache_parts<T, D, kRows, false><<<g, kThreads, 0, st>>>(args);
+  };
   if (d <= 64)
-    fp4_cache_parts<T, 64><<<g, kThreads, 0, st>>>(args);
+    launch(std::integral_constant<int, 64>{});
   else
-    fp4_cache_parts<T, 128><<<g, kThreads, 0, st>>>(args);
+    launch(std::integral_constant<int, 128>{});
   if (int rc = sw::launch_check(what))
     return rc;
   if (p.shares == 0)
