@@ -71,12 +71,13 @@ __device__ __forceinline__ Tiles uniform_tiles(const StepArgs &a,
 
 // The sum over this lane and those before it.
 __device__ __forceinline__ int sum_to_lane(int v) {
-  const int l = lane_id();
-#pragma unroll
-  for (int step = 1; step < kWave; step <<= 1) {
-    const int x = __builtin_amdgcn_ds_bpermute((l - step) * 4, v);
-    v += l >= step ? x : 0;
-  }
+  v += dpp_i<kRowShr1>(0, v);
+  v += dpp_i<kRowShr2>(0, v);
+  v += dpp_i<kRowShr4>(0, v);
+  v += dpp_i<kRowShr8>(0, v);
+  // (the last lane of rows 0 and 2 into rows 1 and 3, then of row 1 into both)
+  v += dpp_i<kRowBcast15, 0xA>(0, v);
+  v += dpp_i<kRowBcast31, 0xC>(0, v);
   return v;
 }
 
@@ -617,6 +618,7 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
   const int seq = (int)(blockIdx.x / a.query_heads);
   const int head = (int)(blockIdx.x % a.query_heads);
   const int hk = head / a.group, row = head % a.group;
+  const int own = tiles_of(a, seq);
   int before = 0, total = 0;
   for (int i = threadIdx.x; i < a.sequences; i += kThreads) {
     const int n = tiles_of(a, i);
@@ -636,7 +638,6 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
     before += sums[0][w];
     total += sums[1][w];
   }
-  const int own = tiles_of(a, seq);
   int first = 0, parts = 0, share = 1;
   if (own > 0) {
     share = share_of(args, total);
