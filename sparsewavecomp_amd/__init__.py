@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Any, NamedTuple
 
 __all__ = [
@@ -936,41 +937,91 @@ def shared_prefix_attention(key_lengths, page_table, query, prefix_key,
     return output
 
 
-def _rotary(back, positions, frequencies, pair_axes, operands, interleaved,
-            stream):
+_PACK8, _PACK16 = struct.Struct("8q").pack, struct.Struct("16q").pack
+
+
+def _place(stream):
+    """(device, stream handle) of a call, as :func:`_device_of` and
+    :func:`_stream` say, in one go where the stream is torch's current one (0.5
+    us instead of 1.2)."""
     torch = _torch or _load_torch()
-    (query, _), (key, _), (query_to, query_name), (key_to, key_name) = operands
-    _need(query.dim() == 3 and query_to.shape == query.shape,
-          f"expected {operands[0][1]} and {query_name} [tokens, query_heads, "
-          "d]")
-    tokens, heads, d = query.shape
-    _need((key is None) == (key_to is None) and
-          (key is None or key.dim() == 3 and key_to.shape == key.shape and
-           key.shape[::2] == query.shape[::2]),
-          f"expected {operands[1][1]} and {key_name} [tokens, key_heads, d], "
-          "or None for both")
-    _need(positions.dim() == 2 and positions.shape[1] == tokens,
-          "positions must be [axes, tokens]")
-    _need(frequencies.dim() == 1, "frequencies must be [pairs]")
-    _need(pair_axes is None or pair_axes.shape == frequencies.shape,
-          "pair_axes must be [pairs]")
-    dt = _value_dtype(query, operands[0][1])
+    if stream is None and torch.cuda.is_initialized():
+        at = torch._C._cuda_getDevice()
+        return at, torch._C._cuda_getCurrentRawStream(at)
     at = _device_of(stream)
-    if key is None:
-        (q, qo), s = _heads(dt, at, *operands[0], *operands[2])
-        k = ko = None
-        if s is not None:
-            s = (ctypes.c_int64 * 8)(s[0], s[1], 0, 0, s[2], s[3], 0, 0)
+    return at, None if at < 0 else _stream(stream)
+
+
+def _operands(dtype, at, shape, *named):
+    """Addresses and strides of operands of one shape (or of two, of which one
+    has a 1 where the other has), as :func:`_heads` gives them with `always`;
+    this way takes a third of its time on operands that are as they should be
+    (four of a cache 1.9 us instead of 5)."""
+    pointers, strides = [], []
+    if 1 not in shape:
+        tensor = _torch.Tensor
+        for t in named[::2]:
+            if type(t) is not tensor or t.dtype is not dtype or \
+                    t.get_device() != at:
+                break
+            s = t.stride()
+            if s[-1] != 1:
+                break
+            strides += s[:-1]
+            pointers.append(t.data_ptr())
+        else:
+            return pointers, strides
+    return _heads(dtype, at, *named, always=True)
+
+
+def _array(t, dtype, at, name):
+    """:func:`_flat` of an operand that may be None."""
+    if t is None:
+        return None
+    if type(t) is _torch.Tensor and t.dtype is dtype and t.get_device() == at and t.is_contiguous():
+        return t.data_ptr()
+    return _flat(t, dtype, at, name)
+
+
+def _rotary(back, positions, frequencies, pair_axes, query, key, query_to,
+            key_to, names, interleaved, stream):
+    torch = _torch or _load_torch()
+    shape = query.shape
+    if len(shape) != 3 or query_to.shape != shape:
+        raise ShapeError(f"expected {names[0]} and {names[2]} [tokens, "
+                         "query_heads, d]")
+    tokens, heads, d = shape
+    if key is None and key_to is None:
+        key_shape = (tokens, 0, d)
+    elif key is None or key_to is None or key.dim() != 3 or \
+            key_to.shape != key.shape or key.shape[0] != tokens or \
+            key.shape[2] != d:
+        raise ShapeError(f"expected {names[1]} and {names[3]} [tokens, "
+                         "key_heads, d], or None for both")
     else:
-        (q, k, qo, ko), s = _heads(dt, at, *operands[0], *operands[1],
-                                   *operands[2], *operands[3])
+        key_shape = key.shape
+    if positions.dim() != 2 or positions.shape[1] != tokens:
+        raise ShapeError("positions must be [axes, tokens]")
+    if frequencies.dim() != 1:
+        raise ShapeError("frequencies must be [pairs]")
+    if pair_axes is not None and pair_axes.shape != frequencies.shape:
+        raise ShapeError("pair_axes must be [pairs]")
+    dt = _value_dtype(query, names[0])
+    at, handle = _place(stream)
+    (q, qo), s = _operands(dt, at, shape, query, names[0], query_to, names[2])
+    if key is None:
+        k = ko = None
+        ks = (0, 0, 0, 0)
+    else:
+        (k, ko), ks = _operands(dt, at, key_shape, key, names[1], key_to,
+                                names[3])
+    strides = _PACK8(s[0], s[1], ks[0], ks[1], s[2], s[3], ks[2], ks[3])
     _check(_fn("sw_rotary_backward" if back else "sw_rotary", dt)(
-        _flat(positions, torch.int32, at, "positions"),
-        _flat(frequencies, torch.float32, at, "frequencies"),
-        None if pair_axes is None else
-        _flat(pair_axes, torch.int32, at, "pair_axes"), q, k, qo, ko, tokens,
-        positions.shape[0], heads, 0 if key is None else key.shape[1], d,
-        frequencies.shape[0], bool(interleaved), s, _stream(stream)))
+        _array(positions, torch.int32, at, "positions"),
+        _array(frequencies, torch.float32, at, "frequencies"),
+        _array(pair_axes, torch.int32, at, "pair_axes"), q, k, qo, ko, tokens,
+        positions.shape[0], heads, key_shape[1], d, frequencies.shape[0],
+        bool(interleaved), strides, handle))
     return query_to, key_to
 
 
@@ -986,10 +1037,10 @@ def rotary(positions, frequencies, pair_axes, query, key, query_output,
     i + pairs of a head, interleaved 2 i and 2 i + 1; the other elements are
     copied.  d is a multiple of 8 up to 128.  float32 or bfloat16, any strides
     of 16 bytes; an output may be its input.  key and key_output may be None."""
-    return _rotary(False, positions, frequencies, pair_axes,
-                   ((query, "query"), (key, "key"),
-                    (query_output, "query_output"),
-                    (key_output, "key_output")), interleaved, stream)
+    return _rotary(False, positions, frequencies, pair_axes, query, key,
+                   query_output, key_output,
+                   ("query", "key", "query_output", "key_output"), interleaved,
+                   stream)
 
 
 def rotary_backward(positions, frequencies, pair_axes, query_output_gradient,
@@ -998,10 +1049,10 @@ def rotary_backward(positions, frequencies, pair_axes, query_output_gradient,
     """The gradients of :func:`rotary`'s query and key from those of its
     outputs: turned back.  A gradient may be written over its input."""
     return _rotary(True, positions, frequencies, pair_axes,
-                   ((query_output_gradient, "query_output_gradient"),
-                    (key_output_gradient, "key_output_gradient"),
-                    (query_gradient, "query_gradient"),
-                    (key_gradient, "key_gradient")), interleaved, stream)
+                   query_output_gradient, key_output_gradient, query_gradient,
+                   key_gradient,
+                   ("query_output_gradient", "key_output_gradient",
+                    "query_gradient", "key_gradient"), interleaved, stream)
 
 
 class Fp4Rows(NamedTuple):
@@ -1026,19 +1077,18 @@ def fp4_cache(pages, page_size, heads, d, device=None):
 
 def _fp4_rows(at, d, key_cache, value_cache):
     """(pages, page_size, heads), addresses and strides of a 4-bit cache."""
-    torch = _torch or _load_torch()
     (kc, ks), (vc, vs) = key_cache, value_cache
-    shape = kc.shape
-    if len(shape) != 4 or vc.shape != shape or shape[3] * 2 != d or \
-            ks.shape != vs.shape or ks.shape[:3] != shape[:3] or \
-            ks.dim() != 4 or ks.shape[3] * 32 != d:
+    shape, scales = kc.shape, ks.shape
+    if len(shape) != 4 or len(scales) != 4 or vc.shape != shape or \
+            vs.shape != scales or shape[:3] != scales[:3] or \
+            shape[3] * 2 != d or scales[3] * 32 != d:
         raise ShapeError(
             "expected key and value caches of codes [pages, page_size, "
             "key_heads, d / 2] and scales [pages, page_size, key_heads, "
             "d / 32]")
-    return shape[:3], *_heads(
-        torch.uint8, at, kc, "key_cache codes", ks, "key_cache scales", vc,
-        "value_cache codes", vs, "value_cache scales", always=True)
+    return shape[:3], *_operands(
+        _torch.uint8, at, shape[:3], kc, "key_cache codes", ks,
+        "key_cache scales", vc, "value_cache codes", vs, "value_cache scales")
 
 
 def _table_width(page_table, sequences):
@@ -1061,20 +1111,18 @@ def _fp4_move(name, token_offsets, per_sequence, page_table, key_cache,
         raise ShapeError(f"{which} must hold one number a sequence")
     width = _table_width(page_table, sequences)
     dt = _value_dtype(key, "key")
-    at = _device_of(stream)
+    at, handle = _place(stream)
     (pages, size, of), rows, row_strides = _fp4_rows(at, d, key_cache,
                                                      value_cache)
     _need(of == heads, "key and value must have the cache's heads")
-    moved, strides = _heads(dt, at, key, "key", value, "value", always=True)
-    strides = (ctypes.c_int64 * 16)(*strides, *row_strides)
+    moved, strides = _operands(dt, at, key.shape, key, "key", value, "value")
     pointers = moved + rows if name == "sw_fp4_cache_write" else rows + moved
     _check(_fn(name, dt)(
-        _flat(token_offsets, torch.int32, at, "token_offsets"),
-        None if per_sequence is None else
-        _flat(per_sequence, torch.int32, at, which),
-        None if page_table is None else
-        _flat(page_table, torch.int32, at, "page_table"), *pointers, sequences,
-        tokens, pages, size, width, heads, d, strides, _stream(stream)))
+        _array(token_offsets, torch.int32, at, "token_offsets"),
+        _array(per_sequence, torch.int32, at, which),
+        _array(page_table, torch.int32, at, "page_table"), *pointers, sequences,
+        tokens, pages, size, width, heads, d,
+        _PACK16(*strides, *row_strides), handle))
 
 
 def fp4_cache_write(token_offsets, key_lengths, page_table, key, value,
@@ -1124,23 +1172,20 @@ def window_attention_decode_fp4(key_lengths, page_table, query, key_cache,
         raise ShapeError("key_lengths must hold one length a sequence")
     width = _table_width(page_table, sequences)
     dt = _value_dtype(query, "query")
-    at = _device_of(stream)
+    at, handle = _place(stream)
     (pages, size, key_heads), rows, row_strides = _fp4_rows(
         at, d, key_cache, value_cache)
-    (q, o), strides = _heads(dt, at, query, "query", output, "output",
-                             always=True)
-    strides = (ctypes.c_int64 * 16)(*strides, *row_strides)
+    (q, o), strides = _operands(dt, at, query.shape, query, "query", output,
+                                "output")
     need = load_library().sw_window_attention_decode_fp4_workspace_bytes(
         sequences, size, width, heads, key_heads, d, window, sinks)
-    lengths = _flat(key_lengths, torch.int32, at, "key_lengths")
-    table = (None if page_table is None else
-             _flat(page_table, torch.int32, at, "page_table"))
+    lengths = _array(key_lengths, torch.int32, at, "key_lengths")
+    table = _array(page_table, torch.int32, at, "page_table")
     scratch = _scratch(need, query, workspace, stream)
     _check(_fn("sw_window_attention_decode_fp4", dt)(
         lengths, table, q, *rows, o, sequences, pages, size, width, heads,
-        key_heads, d, strides, window, sinks, alpha,
-        None if scratch is None else scratch.data_ptr(), need,
-        _stream(stream)))
+        key_heads, d, _PACK16(*strides, *row_strides), window, sinks, alpha,
+        None if scratch is None else scratch.data_ptr(), need, handle))
     return output
 
 
