@@ -32,20 +32,11 @@ __device__ __forceinline__ v4u fp4_values(uint32_t codes, float scale) {
                                        codes, scale, 3))};
 }
 
-// The largest size of eight values, as its bits: above 0x7F800000 for a NaN.
-__device__ __forceinline__ uint32_t top_bits(v4u x) { // bf16
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    top = max(top, max(x[i] & 0x7FFF0000u, x[i] << 16 & 0x7FFF0000u));
-  return top;
-}
-__device__ __forceinline__ uint32_t top_bits(v8f x) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  return top;
+// The four values of two bytes of codes, as fp32.
+__device__ __forceinline__ v4u fp4_values_f32(uint32_t codes, float scale) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0);
+  const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
+  return __builtin_bit_cast(v4u, v4f{a[0], a[1], b[0], b[1]});
 }
 
 // The scale byte of a block whose largest size has these bits: the smallest
@@ -60,7 +51,7 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t top) {
   return top >= 0x7F800000u ? 255u : byte < 4 ? 2u : byte > 254 ? 252u : byte - 2;
 }
 
-// The codes of eight values, each rounded to nearest, ties to the even code and
+// The codes of eight bf16 or four fp32 values, each rounded to nearest, ties to the even code and
 // sizes past 6 to 6, as the conversion instructions do.
 __device__ __forceinline__ uint32_t fp4_codes(v4u x, float scale) {
   uint32_t c = 0;
@@ -73,12 +64,10 @@ __device__ __forceinline__ uint32_t fp4_codes(v4u x, float scale) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(
       c, __builtin_bit_cast(bf16x2, (uint32_t)x[3]), scale, 3);
 }
-__device__ __forceinline__ uint32_t fp4_codes(v8f x, float scale) {
-  uint32_t c = 0;
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], scale, 0);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], scale, 2);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
+__device__ __forceinline__ uint32_t fp4_codes(v4f x, float scale) {
+  const uint32_t c =
+      __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, x[0], x[1], scale, 0);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
 }
 
 } // namespace swd

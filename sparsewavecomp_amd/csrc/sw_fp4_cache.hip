@@ -8,7 +8,7 @@
 #include "sw_fp4.h"
 #include "sw_internal.h"
 
-#include <algorithm>
+#include <type_traits>
 
 using namespace swd;
 using sw::check_operand;
@@ -16,7 +16,8 @@ using sw::check_operand;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnit = 8; // elements of a thread: four threads hold a block
+// elements of a lane, 16 bytes of them: a block lies in 32 / kUnit lanes
+template <typename T> constexpr int kUnit = 16 / (int)sizeof(T);
 
 struct Rows {
   uint8_t *codes, *scales;
@@ -31,10 +32,10 @@ struct MoveArgs {
   void *key, *value;
   int64_t key_token, key_head, value_token, value_head;
   Rows keys, values;
-  int sequences, tokens, pages, table_width, units;
+  int sequences, tokens, pages, table_width, heads;
   int64_t room; // places of a sequence
-  int team; // log2 of the threads that share a token
-  Divisor page_size, row_units;
+  int at_once; // tokens that a wave moves at once, 64 / lanes
+  Divisor page_size, lanes, rows; // lanes of a token; rows: 2 heads
 };
 
 constexpr int kNoPage = -1, kNoSequence = -2;
@@ -90,133 +91,165 @@ __device__ __forceinline__ Place place_of(const MoveArgs &a, int first,
   return p;
 }
 
-// Which elements a thread takes of a token: unit `u` of those of its keys and
-// then of its values.
-struct Unit {
-  bool value;
-  int head, piece;
-  __device__ __forceinline__ Unit(const MoveArgs &a, int u) {
-    value = 2 * u >= a.units;
-    u -= value ? a.units / 2 : 0;
-    head = (int)a.row_units.quotient(u);
-    piece = u - head * (int)a.row_units.by;
+// What a wave moves: the keys or the values of one head, of PASSES times
+// `at_once` consecutive tokens.  Their codes lie next to each other in a page that
+// holds a head's rows together, their scales too, so that lines are written whole;
+// of the tokens' side 16 bytes a lane are whole lines in any case.  (A token's keys
+// and values of all heads in a workgroup: 134 MB written 54.8 us, read 53; 600 MB
+// read 216.)
+template <typename T> struct Wave {
+  bool value, any;
+  int first, token, piece; // the wave's first token; this lane's of a pass
+  int64_t token_stride, at; // of a lane's elements
+  const Rows &rows;
+  int64_t codes, scales;
+  __device__ __forceinline__ Wave(const MoveArgs &a, int passes, int number,
+                                  int tile)
+      : value(number - tile * (int)a.rows.by >= a.heads),
+        rows(value ? a.values : a.keys) {
+    const int head = number - tile * (int)a.rows.by - (value ? a.heads : 0);
+    first = tile * passes * a.at_once;
+    any = first < a.tokens;
+    token = (int)a.lanes.quotient(lane_id());
+    piece = lane_id() - token * (int)a.lanes.by;
+    token_stride = value ? a.value_token : a.key_token;
+    at = head * (value ? a.value_head : a.key_head) + piece * kUnit<T>;
+    codes = head * rows.codes_head + piece * (kUnit<T> / 2);
+    scales = head * rows.scales_head + piece * kUnit<T> / 32;
   }
-  __device__ __forceinline__ int64_t element(const MoveArgs &a,
-                                             int token) const {
-    return token * (value ? a.value_token : a.key_token) +
-           head * (value ? a.value_head : a.key_head) + piece * kUnit;
+};
+template <typename T>
+__device__ __forceinline__ Wave<T> wave_of(const MoveArgs &a, int passes) {
+  const int number = (int)blockIdx.x * (kThreads / kWave) + wave_in_group();
+  return {a, passes, number, (int)a.rows.quotient(number)};
+}
+
+// Units pass by the caches.  Reads of the tokens' side: written 32,768 tokens of
+// 8 heads of 128, bf16, 38.1 us, 44 with plain loads.  Writes of it: read back
+// 28.8 us with them, 38.9 plain; 262,144 tokens at most of 4 sequences 133 and 145;
+// in fp32 53 and 83.  A kernel that reads 67 to 134 MB of them right away finds
+// less in the caches (sum of both: 72 us against 68, 39 and 36), of smaller and
+// larger ones or in fp32 the sum is smaller too (13 and 13.6, 291 and 299, 150 and
+// 164).
+__device__ __forceinline__ v4u load_unit(const void *p) {
+  return __builtin_nontemporal_load(static_cast<const v4u *>(p));
+}
+__device__ __forceinline__ void store_unit(void *p, v4u x) {
+  __builtin_nontemporal_store(x, static_cast<v4u *>(p));
+}
+
+// Of the block that a lane's unit lies in, the largest size's bits.
+__device__ __forceinline__ uint32_t block_top(v4u x, uint16_t) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    top = max(top, max(x[i] & 0x7FFF0000u, x[i] << 16 & 0x7FFF0000u));
+  top = max(top, (uint32_t)dpp_i<kQuadXor1>(0, (int)top));
+  return max(top, (uint32_t)dpp_i<kQuadXor2>(0, (int)top));
+}
+__device__ __forceinline__ uint32_t block_top(v4u x, float) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    top = max(top, x[i] & 0x7FFFFFFFu);
+  top = max(top, (uint32_t)dpp_i<kQuadXor1>(0, (int)top));
+  top = max(top, (uint32_t)dpp_i<kQuadXor2>(0, (int)top));
+  return max(top, (uint32_t)dpp_i<kRowHalfMirror>(0, (int)top));
+}
+
+// The codes of a unit: four bytes of bf16 values, two of fp32 ones.
+template <typename T> struct Codes;
+template <> struct Codes<uint16_t> {
+  using Word = uint32_t;
+  __device__ static __forceinline__ Word of(v4u x, float scale) {
+    return fp4_codes(x, scale);
   }
-  __device__ __forceinline__ uint32_t *codes(const MoveArgs &a,
-                                             const Place &p) const {
-    const Rows &r = value ? a.values : a.keys;
-    return reinterpret_cast<uint32_t *>(
-        r.codes + p.page * r.codes_page + p.slot * r.codes_token +
-        head * r.codes_head + piece * 4);
+  __device__ static __forceinline__ v4u values(Word codes, float scale) {
+    return fp4_values(codes, scale);
   }
-  __device__ __forceinline__ uint8_t *scale(const MoveArgs &a,
-                                            const Place &p) const {
-    const Rows &r = value ? a.values : a.keys;
-    return r.scales + p.page * r.scales_page + p.slot * r.scales_token +
-           head * r.scales_head + piece / 4;
+};
+template <> struct Codes<float> {
+  using Word = uint16_t;
+  __device__ static __forceinline__ Word of(v4u x, float scale) {
+    return (Word)fp4_codes(__builtin_bit_cast(v4f, x), scale);
+  }
+  __device__ static __forceinline__ v4u values(Word codes, float scale) {
+    return fp4_values_f32(codes, scale);
   }
 };
 
-// A workgroup takes PER tokens for each of its teams of 2^team threads, team t
-// the tokens t, t + teams, ...; a wave finds the places of them all, one a lane.
-template <typename T, int PER>
+template <typename T, int PASSES>
 __global__ __launch_bounds__(kThreads) void fp4_cache_write(MoveArgs a) {
-  const int team = threadIdx.x >> a.team, teams = kThreads >> a.team;
-  const int first = blockIdx.x * teams * PER;
-  int u = threadIdx.x & ((1 << a.team) - 1);
-  Frag<T> x[PER];
-  auto load = [&]() __attribute__((always_inline)) {
-    const Unit unit(a, u);
-    const T *from = static_cast<const T *>(unit.value ? a.value : a.key);
+  using C = Codes<T>;
+  const Wave<T> w = wave_of<T>(a, PASSES);
+  if (!w.any)
+    return;
+  const T *from = static_cast<const T *>(w.value ? a.value : a.key) + w.at;
+  const bool lane = w.token < a.at_once; // (some are left over of rows of 96)
+  v4u x[PASSES];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int token = first + i * teams + team;
-      x[i] = token < a.tokens ? ld_frag(from + unit.element(a, token))
-                              : zero_frag<T>();
-    }
-  };
-  if (u < a.units)
-    load();
-  const Place all = place_of<true>(
-      a, first, lane_id() < teams * PER && first + lane_id() < a.tokens);
-  Place p[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int from = (i * teams + team) * 4;
-    p[i].page = __builtin_amdgcn_ds_bpermute(from, all.page);
-    p[i].slot = __builtin_amdgcn_ds_bpermute(from, all.slot);
+  for (int i = 0; i < PASSES; ++i) {
+    const int token = w.first + i * a.at_once + w.token;
+    x[i] = v4u{};
+    if (lane && token < a.tokens)
+      x[i] = load_unit(from + token * w.token_stride);
   }
-  while (u < a.units) {
-    const Unit unit(a, u);
+  const Place all = place_of<true>(a, w.first,
+                                   lane_id() < PASSES * a.at_once &&
+                                       w.first + lane_id() < a.tokens);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      // (a block lies in four neighbours, all of one team)
-      int top = (int)top_bits(x[i]);
-      top = max(top, dpp_i<kQuadXor1>(0, top));
-      top = max(top, dpp_i<kQuadXor2>(0, top));
-      const uint32_t byte = fp4_scale_byte((uint32_t)top);
-      const uint32_t codes =
-          byte == 255 ? 0u : fp4_codes(x[i], fp4_scale(byte));
-      if (p[i].page >= 0) {
-        *unit.codes(a, p[i]) = codes;
-        if (unit.piece % 4 == 0)
-          *unit.scale(a, p[i]) = (uint8_t)byte;
-      }
+  for (int i = 0; i < PASSES; ++i) {
+    const int of = (i * a.at_once + w.token) * 4;
+    const int page = __builtin_amdgcn_ds_bpermute(of, all.page);
+    const int slot = __builtin_amdgcn_ds_bpermute(of, all.slot);
+    const uint32_t byte = fp4_scale_byte(block_top(x[i], T{}));
+    const typename C::Word codes =
+        byte == 255 ? 0u : C::of(x[i], fp4_scale(byte));
+    if (lane && page >= 0) {
+      *reinterpret_cast<typename C::Word *>(
+          w.rows.codes + page * w.rows.codes_page + slot * w.rows.codes_token +
+          w.codes) = codes;
+      if (w.piece % (32 / kUnit<T>) == 0)
+        w.rows.scales[page * w.rows.scales_page + slot * w.rows.scales_token +
+                      w.scales] = (uint8_t)byte;
     }
-    u += 1 << a.team;
-    if (u < a.units)
-      load();
   }
 }
 
-__device__ __forceinline__ void store_values(uint16_t *p, uint32_t codes,
-                                             float scale) {
-  *reinterpret_cast<v4u *>(p) = fp4_values(codes, scale);
-}
-__device__ __forceinline__ void store_values(float *p, uint32_t codes,
-                                             float scale) {
-  const v4u x = fp4_values(codes, scale);
-#pragma unroll
-  for (int i = 0; i < 4; i += 2)
-    *reinterpret_cast<v4f *>(p + 2 * i) =
-        v4f{__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xFFFF0000u),
-            __uint_as_float(x[i + 1] << 16),
-            __uint_as_float(x[i + 1] & 0xFFFF0000u)};
-}
-
-template <typename T, int PER>
+template <typename T, int PASSES>
 __global__ __launch_bounds__(kThreads) void fp4_cache_read(MoveArgs a) {
-  const int team = threadIdx.x >> a.team, teams = kThreads >> a.team;
-  const int first = blockIdx.x * teams * PER;
-  const Place all = place_of<false>(
-      a, first, lane_id() < teams * PER && first + lane_id() < a.tokens);
-  Place p[PER];
+  using C = Codes<T>;
+  const Wave<T> w = wave_of<T>(a, PASSES);
+  if (!w.any)
+    return;
+  const bool lane = w.token < a.at_once;
+  const Place all = place_of<false>(a, w.first,
+                                    lane_id() < PASSES * a.at_once &&
+                                        w.first + lane_id() < a.tokens);
+  int page[PASSES];
+  typename C::Word codes[PASSES];
+  uint8_t bytes[PASSES];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int from = (i * teams + team) * 4;
-    p[i].page = __builtin_amdgcn_ds_bpermute(from, all.page);
-    p[i].slot = __builtin_amdgcn_ds_bpermute(from, all.slot);
-  }
-  for (int u = threadIdx.x & ((1 << a.team) - 1); u < a.units;
-       u += 1 << a.team) {
-    const Unit unit(a, u);
-    T *to = static_cast<T *>(unit.value ? a.value : a.key);
-    uint32_t codes[PER], bytes[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      codes[i] = p[i].page >= 0 ? *unit.codes(a, p[i]) : 0u;
-      bytes[i] = p[i].page >= 0 ? *unit.scale(a, p[i]) : 0u;
+  for (int i = 0; i < PASSES; ++i) {
+    const int of = (i * a.at_once + w.token) * 4;
+    page[i] = __builtin_amdgcn_ds_bpermute(of, all.page);
+    const int slot = __builtin_amdgcn_ds_bpermute(of, all.slot);
+    codes[i] = 0;
+    bytes[i] = 0;
+    if (lane && page[i] >= 0) {
+      codes[i] = *reinterpret_cast<const typename C::Word *>(
+          w.rows.codes + page[i] * w.rows.codes_page +
+          slot * w.rows.codes_token + w.codes);
+      bytes[i] = w.rows.scales[page[i] * w.rows.scales_page +
+                               slot * w.rows.scales_token + w.scales];
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (p[i].page != kNoSequence)
-        store_values(to + unit.element(a, first + i * teams + team), codes[i],
-                     fp4_scale(bytes[i]));
   }
+  T *to = static_cast<T *>(w.value ? a.value : a.key) + w.at;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+    if (lane && page[i] != kNoSequence)
+      store_unit(to + (w.first + i * a.at_once + w.token) * w.token_stride,
+                 C::values(codes[i], fp4_scale(bytes[i])));
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -282,26 +315,44 @@ int move_entry(const int32_t *token_offsets, const int32_t *from,
   a.table_width = (int)table_width;
   a.room = page_size * table_width;
   a.page_size = Divisor((uint32_t)page_size);
-  a.row_units = Divisor((uint32_t)(d / kUnit));
-  a.units = (int)(2 * key_heads * (d / kUnit));
-  a.team = 2;
-  while (a.team < 8 && 1 << a.team < a.units)
-    ++a.team;
-  const int64_t teams = kThreads >> a.team;
-  const int64_t per = tokens >= 4096 * teams && teams <= 16 ? 4 : 1;
-  const int64_t grid = sw::ceil_div(tokens, teams * per);
+  a.heads = (int)key_heads;
+  a.lanes = Divisor((uint32_t)(d / kUnit<T>));
+  a.rows = Divisor((uint32_t)(2 * key_heads));
+  a.at_once = (int)(kWave / (d / kUnit<T>));
+  const int64_t bytes = 2 * tokens * key_heads * d * (int64_t)sizeof(T);
+  // Passes of a wave, us (keys and values in bytes; write, read back):
+  //            0.26 MB     4.2 MB      6.9 MB (fp32)  16.8 MB     67 MB        134 MB       600 MB
+  //   1        3.5, 3.3    4.2, 4.0    6.7, 5.5       10.5, 8.8   31.0, 25.3   57.0, 46.3   -, 265
+  //   4        4.5, 4.2    4.8, 4.5    5.7, 4.9        8.6, 6.9   23.0, 16.5   39.9, 27.8   -, 162
+  //   8        5.7, 5.4    6.1, 5.6    6.7, 6.0        8.9, 7.1   21.4, 16.4   37.8, 28.7   -, 132
+  // (and 64 tokens at most, whose places a wave finds at once)
+  int64_t passes = bytes < (6 << 20) ? 1 : bytes < (48 << 20) ? 4 : 8;
+  if (passes * a.at_once > kWave)
+    passes = 4;
+  const int64_t waves =
+      sw::ceil_div(tokens, a.at_once * passes) * 2 * key_heads;
+  const int64_t grid = sw::ceil_div(waves, kThreads / kWave);
+  if (waves > INT32_MAX)
+    return sw::fail(SW_ERR_INVALID_SHAPE, "%s of %lld tokens and %lld heads is "
+                    "more than one launch holds", what, (long long)tokens,
+                    (long long)key_heads);
   if (int rc = sw::check_flat_grid(grid, kThreads, what))
     return rc;
   const hipStream_t st = sw::as_stream(stream);
   const dim3 g((unsigned)grid);
-  if (WRITE && per == 4)
-    fp4_cache_write<T, 4><<<g, kThreads, 0, st>>>(a);
-  else if (WRITE)
-    fp4_cache_write<T, 1><<<g, kThreads, 0, st>>>(a);
-  else if (per == 4)
-    fp4_cache_read<T, 4><<<g, kThreads, 0, st>>>(a);
+  auto launch = [&](auto count) {
+    constexpr int N = decltype(count)::value;
+    if constexpr (WRITE)
+      fp4_cache_write<T, N><<<g, kThreads, 0, st>>>(a);
+    else
+      fp4_cache_read<T, N><<<g, kThreads, 0, st>>>(a);
+  };
+  if (passes == 1)
+    launch(std::integral_constant<int, 1>{});
+  else if (passes == 4)
+    launch(std::integral_constant<int, 4>{});
   else
-    fp4_cache_read<T, 1><<<g, kThreads, 0, st>>>(a);
+    launch(std::integral_constant<int, 8>{});
   return sw::launch_check(what);
 }
 
