@@ -13,6 +13,7 @@
 #include "sw_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace swd;
 using sw::check_operand;
@@ -79,34 +80,45 @@ __device__ __forceinline__ Turn turn_of(int position, float frequency) {
   return {c, s};
 }
 
-// 16 bytes of elements as fp32, and back.
-template <typename T> struct Piece;
-template <> struct Piece<float> {
-  static constexpr int kCount = 4;
-  float x[4];
-  __device__ __forceinline__ void load(const float *p) {
-    const v4f v = *reinterpret_cast<const v4f *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[i] = v[i];
+// W consecutive elements, aligned to their size, as fp32 and back.  Pieces of 16
+// bytes are written past the caches (32,760 tokens of 40 bf16 heads of 128: 110 us,
+// 115 with plain stores; 16,384 of 20: 27.1 and 32.8; with loads past them too 107
+// and 30.5).
+template <typename T, int W> struct Piece {
+  typedef T Raw __attribute__((ext_vector_type(W)));
+  float x[W];
+  __device__ __forceinline__ static Raw read(const T *p) {
+    return *reinterpret_cast<const Raw *>(p);
   }
-  __device__ __forceinline__ void store(float *p) const {
-    *reinterpret_cast<v4f *>(p) = v4f{x[0], x[1], x[2], x[3]};
+  __device__ __forceinline__ static void write(T *p, Raw v) {
+    if constexpr (W * sizeof(T) == 16)
+      __builtin_nontemporal_store(v, reinterpret_cast<Raw *>(p));
+    else
+      *reinterpret_cast<Raw *>(p) = v;
   }
-};
-template <> struct Piece<uint16_t> {
-  static constexpr int kCount = 8;
-  float x[8];
-  __device__ __forceinline__ void load(const uint16_t *p) {
-    const v4u v = *reinterpret_cast<const v4u *>(p);
+  __device__ __forceinline__ void load(const T *p) {
+    const Raw v = read(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(v[i] << 16);
-      x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    for (int i = 0; i < W; ++i)
+      x[i] = tof((T)v[i]);
+  }
+  __device__ __forceinline__ void store(T *p) const {
+    if constexpr (sizeof(T) == 2 && W % 2 == 0) {
+      typedef uint32_t Words __attribute__((ext_vector_type(W / 2)));
+      Words v;
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i)
+        v[i] = cvt_pk_bf16(x[2 * i], x[2 * i + 1]);
+      write(p, __builtin_bit_cast(Raw, v));
+    } else if constexpr (sizeof(T) == 2) {
+      write(p, Raw{f32_to_bf16(x[0])});
+    } else {
+      Raw v;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        v[i] = x[i];
+      write(p, v);
     }
-  }
-  __device__ __forceinline__ void store(uint16_t *p) const {
-    *reinterpret_cast<v4u *>(p) = make_frag<uint16_t>(x);
   }
 };
 
@@ -116,13 +128,12 @@ __device__ __forceinline__ void turn(float &x, float &y, const Turn &t) {
   y = fmaf(a, t.sin, b * t.cos);
 }
 
-// A unit of a head: with VECTOR, two pieces of 16 bytes that turn with each
-// other (neighbours where pairs are) or one that is copied; else a pair, or an
-// element that is copied.
-template <typename T, bool VECTOR, bool NEIGHBOURS>
+// A unit of a head: two pieces of W elements that turn with each other, or with
+// NEIGHBOURS one that holds its pairs; or one that is copied.
+template <typename T, int W, bool NEIGHBOURS>
 __global__ __launch_bounds__(kThreads) void rotary_turn(RotaryArgs a) {
   extern __shared__ Turn turns[]; // [per][pairs]
-  constexpr int kCount = VECTOR ? Piece<T>::kCount : 1;
+  using P = Piece<T, W>;
   const int first = blockIdx.x * a.per;
   const int count = a.tokens - first < a.per ? a.tokens - first : a.per;
   for (int i = threadIdx.x; i < count * a.pairs; i += kThreads) {
@@ -150,40 +161,27 @@ __global__ __launch_bounds__(kThreads) void rotary_turn(RotaryArgs a) {
     const T *from = static_cast<const T *>(h.from) + at * h.from_token +
                     head * h.from_head;
     T *to = static_cast<T *>(h.to) + at * h.to_token + head * h.to_head;
-    if (u < a.turned) {
-      const Turn *t = turns + token * a.pairs + u * kCount;
-      const int x = NEIGHBOURS ? 2 * u * kCount : u * kCount;
-      const int y = NEIGHBOURS ? x + kCount : x + a.pairs;
-      if constexpr (VECTOR) {
-        Piece<T> p, q;
-        p.load(from + x);
-        q.load(from + y);
-        if constexpr (NEIGHBOURS) {
+    if (u >= a.turned) {
+      const int x = 2 * a.pairs + (u - a.turned) * W;
+      P::write(to + x, P::read(from + x));
+    } else if constexpr (NEIGHBOURS) {
+      const Turn *t = turns + token * a.pairs + u * (W / 2);
+      P p;
+      p.load(from + u * W);
 #pragma unroll
-          for (int e = 0; e < kCount; e += 2) {
-            turn(p.x[e], p.x[e + 1], t[e / 2]);
-            turn(q.x[e], q.x[e + 1], t[(kCount + e) / 2]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < kCount; ++e)
-            turn(p.x[e], q.x[e], t[e]);
-        }
-        p.store(to + x);
-        q.store(to + y);
-      } else {
-        float p = ldv(from + x), q = ldv(from + y);
-        turn(p, q, *t);
-        stv(to + x, p);
-        stv(to + y, q);
-      }
+      for (int e = 0; e < W; e += 2)
+        turn(p.x[e], p.x[e + 1], t[e / 2]);
+      p.store(to + u * W);
     } else {
-      const int x = 2 * a.pairs + (u - a.turned) * kCount;
-      if constexpr (VECTOR)
-        *reinterpret_cast<v4u *>(to + x) =
-            *reinterpret_cast<const v4u *>(from + x);
-      else
-        to[x] = from[x];
+      const Turn *t = turns + token * a.pairs + u * W;
+      P p, q;
+      p.load(from + u * W);
+      q.load(from + u * W + a.pairs);
+#pragma unroll
+      for (int e = 0; e < W; ++e)
+        turn(p.x[e], q.x[e], t[e]);
+      p.store(to + u * W);
+      q.store(to + u * W + a.pairs);
     }
   }
 }
@@ -256,13 +254,16 @@ int rotary_entry(const int32_t *positions, const float *frequencies,
   a.d = (int)d;
   a.pairs = (int)pairs;
   a.back = back;
-  const int64_t count = 16 / (int64_t)sizeof(T);
-  // (neighbours: two pieces hold `count` pairs)
-  const bool vector = pairs % count == 0;
-  a.turned = (int)(vector ? pairs / count : pairs);
-  a.units = a.turned + (int)((d - 2 * pairs) / (vector ? count : 1));
+  // the widest pieces that the pairs are made of, up to 16 bytes
+  const int64_t run = interleaved ? 2 * pairs : pairs;
+  int64_t width = 16 / (int64_t)sizeof(T);
+  while (run % width != 0)
+    width /= 2;
+  a.turned = (int)(run / width);
+  a.units = a.turned + (int)((d - 2 * pairs) / width);
   a.head_units = Divisor((uint32_t)a.units);
   a.token_units = Divisor((uint32_t)(a.units * a.heads));
+  // (two units a thread; with four 16,384 and 32,760 tokens take 4 to 10 % longer)
   a.per = (int)std::clamp<int64_t>(2 * kThreads / (a.units * a.heads), 1, 16);
   const int64_t grid = sw::ceil_div(tokens, a.per);
   if (int rc = sw::check_flat_grid(grid, kThreads, what))
@@ -270,14 +271,24 @@ int rotary_entry(const int32_t *positions, const float *frequencies,
   const hipStream_t st = sw::as_stream(stream);
   const dim3 g((unsigned)grid);
   const size_t lds = a.per * a.pairs * sizeof(Turn);
-  if (vector && interleaved)
-    rotary_turn<T, true, true><<<g, kThreads, lds, st>>>(a);
-  else if (vector)
-    rotary_turn<T, true, false><<<g, kThreads, lds, st>>>(a);
-  else if (interleaved)
-    rotary_turn<T, false, true><<<g, kThreads, lds, st>>>(a);
-  else
-    rotary_turn<T, false, false><<<g, kThreads, lds, st>>>(a);
+  auto launch = [&](auto w) {
+    constexpr int W = decltype(w)::value;
+    if constexpr (W > 1)
+      if (interleaved) {
+        rotary_turn<T, W, true><<<g, kThreads, lds, st>>>(a);
+        return;
+      }
+    rotary_turn<T, W, false><<<g, kThreads, lds, st>>>(a);
+  };
+  if constexpr (sizeof(T) == 2)
+    if (width == 8)
+      launch(std::integral_constant<int, 8>{});
+  if (width == 4)
+    launch(std::integral_constant<int, 4>{});
+  else if (width == 2)
+    launch(std::integral_constant<int, 2>{});
+  else if (width == 1)
+    launch(std::integral_constant<int, 1>{});
   return sw::launch_check(what);
 }
 
