@@ -153,6 +153,54 @@ def test_decode_long(dev, dtype):
     expect(x, decode(x, 0.125, 15000, 7), 0.125, 15000, 7)
 
 
+def ragged(n, most, seed):
+    """Lengths from 0 to `most`, a fifth of them 0."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randint(0, most + 1, (n,), generator=gen)
+    x[torch.rand(n, generator=gen) < 0.2] = 0
+    x[n // 2] = most
+    return x.tolist()
+
+
+# sequences, most keys, page, window, sinks, heads, key heads: more sequences than
+# a wave has lanes, none in front or behind; windows and sinks whose tiles overlap;
+# shares of less than a sequence and of many; more key heads than workgroups that
+# run at once
+SHARES = [
+    (65, 700, 16, 10 ** 6, 0, 2, 1),
+    (150, 900, 16, 600, 40, 4, 2),
+    (300, 520, 0, 515, 3, 1, 1),
+    (3, 6000, 64, 10 ** 6, 0, 12, 1),
+    (7, 3000, 24, 1000, 2000, 20, 1),
+    (2, 1500, 16, 10 ** 6, 0, 1100, 1100),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(SHARES)))
+def test_shares_of_many_sequences(dev, dtype, case):
+    n, most, page, window, sinks, h, hk = SHARES[case]
+    say(f"fp4 shares {dtype} {SHARES[case]}")
+    lengths = ragged(n, most, case)
+    if case == 1:
+        lengths[0] = lengths[-1] = 0
+    x = make(dtype, lengths, page, h, hk, 32, seed=case, capacity=most)
+    expect(x, decode(x, 0.2, window, sinks), 0.2, window, sinks)
+    x["lengths"][:] = 0  # nothing is left to share
+    got = decode(x, 0.2, window, sinks)
+    assert torch.equal(got, torch.zeros_like(got))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_sequences_than_are_shared(dev, dtype):
+    """Past 4096 each has a workgroup to itself, whatever room it has."""
+    say(f"fp4 4,200 sequences {dtype}")
+    lengths = ragged(4200, 40, 5)
+    lengths[17] = 800
+    x = make(dtype, lengths, 16, 1, 1, 32, seed=7)
+    expect(x, decode(x, 0.2, 10 ** 6, 0), 0.2, 10 ** 6, 0)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_one_key_comes_back(dev, dtype):
     """One key's output is its value: bf16 its bits.  In fp32 the probability p

@@ -367,6 +367,37 @@ def test_past_four_gib(dev, dtype):
             assert torch.equal(y.cpu().double(), z)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_past_four_gib_of_one_page(dev, dtype):
+    """The last keys of a page of 2^20 rows that lie 8 KiB apart, codes and
+    scales: written, read back and attended to."""
+    say(f"fp4 far rows {dtype}")
+    gen = torch.Generator().manual_seed(8)
+    n, new, h, hk, d = 2 ** 20 - 3, 20, 4, 2, 64
+    x = [values(gen, "f32", new, hk, d).clamp(-4, 4).to(DTYPES[dtype])
+         for _ in "kv"]
+    q = torch.randn(1, h, d, generator=gen).to(DTYPES[dtype])
+    rows = []
+    for _ in "kv":
+        store = torch.empty(2 ** 33, dtype=torch.uint8, device=DEV)
+        rows.append(sw.Fp4Rows(
+            store.as_strided((1, 2 ** 20, hk, 32), (0, 8192, 32, 1)),
+            store.as_strided((1, 2 ** 20, hk, 2), (0, 8192, 2, 1), 4096)))
+    a = on_gpu(i32(0, new), i32(n), q, *x)
+    sw.fp4_cache_write(a[0], a[1], None, *a[3:], *rows)
+    out = [torch.empty_like(y) for y in a[3:]]
+    sw.fp4_cache_read(a[0], a[1] - new, None, *rows, *out)
+    held = [dequantise(*quantise(y)) for y in x]
+    for y, z in zip(out, held):
+        assert torch.equal(y.cpu().double(), z)
+    got = torch.empty_like(a[2])
+    sw.window_attention_decode_fp4(a[1], None, a[2], *rows, got, 0.125, new)
+    for i in range(h):
+        o, bound = attend(q[:, i].double(), held[0][:, i // 2],
+                          held[1][:, i // 2], 0.125, DTYPES[dtype])
+        check(f"head {i}", got[:, i], o, bound)
+
+
 def test_repeats_streams_and_graphs(dev):
     """The same bytes on another stream and from a captured graph whose
     lengths grow."""

@@ -110,6 +110,21 @@ def test_rotary(dev, dtype, interleaved, case):
     check("key in place", kg, *turned(k, p, f, ax, interleaved))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,pairs", [(80, 10), (96, 35), (64, 6), (128, 52),
+                                     (128, 2), (8, 2), (104, 52), (120, 59)])
+def test_pieces_of_every_width(dev, dtype, interleaved, d, pairs):
+    """Pairs that make whole pieces of 16, 8, 4 and 2 bytes."""
+    say(f"rotary pieces {dtype} {interleaved} {d} {pairs}")
+    p, f, ax, q, k = make(dtype, 45, 2, 3, 2, d, pairs, seed=d + pairs)
+    pg, fg, ag, qg, kg = on_gpu(p, f, ax, q, k)
+    qo, ko = torch.full_like(qg, 7.0), torch.full_like(kg, 7.0)
+    sw.rotary(pg, fg, ag, qg, kg, qo, ko, interleaved)
+    check("query", qo, *turned(q, p, f, ax, interleaved))
+    check("key", ko, *turned(k, p, f, ax, interleaved))
+
+
 @pytest.mark.parametrize("far", [2 ** 20, 2 ** 31 - 1])
 def test_far_positions(dev, far):
     """Whole turns by the million: the rest of the angle is right all the
