@@ -25,10 +25,9 @@ struct Fp4StepArgs {
   StepArgs s; // (its cache: the codes, strides in bytes)
   Scales scales;
   Divisor page_size;
-  // A unit is `block` query rows (8 or 16) of a key head, for all sequences;
-  // `shares` workgroups
-  // split a unit's tiles evenly, each taking `least` at least.  0 shares: a
-  // workgroup for each sequence of a unit.
+  // A unit is `block` query rows (8 or 16) of a key head, for all sequences.  Its
+  // tiles are split evenly among `shares` workgroups, each taking `least` at
+  // least.  0 shares: a workgroup for each sequence of a unit.
   int units, shares, least, block;
 };
 
@@ -81,41 +80,87 @@ __device__ __forceinline__ int sum_to_lane(int v) {
   return v;
 }
 
-// A workgroup's share of a unit's tiles: `share` tiles from `from` on, of which
-// sequence `seq` has those from `offset` on.  Up to 4096 sequences: a lane of a
-// wave sums those of up to 64, the sums are added up over the lanes, and then
-// those of one lane.
+// How a unit's tiles are split: `most` for a workgroup, and whether none takes
+// those of two sequences (`whole`: a sequence's tiles divided by `most`, rounded
+// up, are its shares, one more for each sequence at most).  A second sequence
+// costs a workgroup about as much as 8 tiles (4 sequences of up to 8,192 keys 21.6
+// us, whole 18.6; 32 of up to 2,048 25.7 and 23.3; 64 of up to 20,000, over four
+// key heads of 64, 61.4 and 68.5).
+struct Split {
+  int most;
+  bool whole;
+  __device__ __forceinline__ Split(const Fp4StepArgs &args, int total) {
+    constexpr int kSecond = 8;
+    const int apart = args.shares - args.s.sequences;
+    const int even = (total + args.shares - 1) / args.shares;
+    most = even < args.least ? args.least : even;
+    whole = false;
+    if (apart > 0) {
+      const int more = (total + apart - 1) / apart;
+      whole = more <= most + kSecond;
+      if (whole && more > most)
+        most = more;
+    }
+  }
+  __device__ __forceinline__ int shares(int tiles) const {
+    return (tiles + most - 1) / most;
+  }
+};
+
+// A workgroup's share of a unit's tiles: those from `from` on, of which sequence
+// `seq` has the ones from `offset` on.  Up to 4096 sequences: a lane of a wave
+// sums up to 64 of them, the sums are added up over the lanes, and then those of
+// one lane.  What is summed are tiles, or where sequences stay whole their shares.
 struct Share {
   int from, to, seq, offset;
 };
-__device__ __forceinline__ int share_of(const Fp4StepArgs &args, int total) {
-  const int even = (total + args.shares - 1) / args.shares;
-  return even < args.least ? args.least : even;
-}
 __device__ __forceinline__ Share find_share(const Fp4StepArgs &args, int p) {
   const StepArgs &a = args.s;
   const int l = lane_id(), each = (a.sequences + kWave - 1) / kWave;
-  int own = 0;
-  for (int i = 0; i < each; ++i)
-    if (l * each + i < a.sequences)
-      own += tiles_of(a, l * each + i);
+  auto tiles = [&](int i) __attribute__((always_inline)) {
+    return i < a.sequences ? tiles_of(a, i) : 0;
+  };
+  int held = tiles(l * each), own = held; // (the lane's first one's, and all)
+  for (int i = 1; i < each; ++i)
+    own += tiles(l * each + i);
   int sum = sum_to_lane(own);
   const int total = __builtin_amdgcn_readlane(sum, kWave - 1);
-  const int share = share_of(args, total);
+  const Split split(args, total);
   Share s{0, 0, 0, 0};
-  if (total == 0 || p > (total - 1) / share)
+  int first = p, end = total; // what is looked for, and of how many
+  if (split.whole) {
+    own = split.shares(held);
+    for (int i = 1; i < each; ++i)
+      own += split.shares(tiles(l * each + i));
+    sum = sum_to_lane(own);
+    end = __builtin_amdgcn_readlane(sum, kWave - 1);
+  } else if (p > total / split.most) {
     return s; // (nothing is left)
-  s.from = p * share;
-  s.to = total - s.from < share ? total : s.from + share;
-  int at = __builtin_popcountll(ballot(sum <= s.from));
+  } else {
+    first = p * split.most;
+  }
+  if (first >= end)
+    return s;
+  int at = __builtin_popcountll(ballot(sum <= first));
   s.seq = at * each;
-  s.offset = __builtin_amdgcn_readlane(sum - own, at);
+  int offset = __builtin_amdgcn_readlane(sum - own, at);
   if (each > 1) {
-    own = l < each && s.seq + l < a.sequences ? tiles_of(a, s.seq + l) : 0;
-    sum = s.offset + sum_to_lane(own);
-    at = __builtin_popcountll(ballot(l < each && sum <= s.from));
+    held = l < each ? tiles(s.seq + l) : 0;
+    own = split.whole ? split.shares(held) : held;
+    sum = offset + sum_to_lane(own);
+    at = __builtin_popcountll(ballot(l < each && sum <= first));
     s.seq += at;
-    s.offset = __builtin_amdgcn_readlane(sum - own, at);
+    offset = __builtin_amdgcn_readlane(sum - own, at);
+  }
+  if (split.whole) {
+    const int all = __builtin_amdgcn_readlane(held, at);
+    const int shares = split.shares(all), even = (all + shares - 1) / shares;
+    s.from = (p - offset) * even;
+    s.to = all - s.from < even ? all : s.from + even;
+  } else {
+    s.from = first;
+    s.to = total - first < split.most ? total : first + split.most;
+    s.offset = offset;
   }
   return s;
 }
@@ -413,13 +458,14 @@ fp4_cache_parts(Fp4StepArgs args) {
 #pragma unroll
         for (int i = 0; i < kQueryParts<T>; ++i)
           q[i] = lds_read<v4u>(query_at, (i * kSteps + st) * kWave * 16);
+        const v4u k[2] = {fp4_values(x.key[0][st], by[0]),
+                          fp4_values(x.key[1][st], by[1])};
+        // (the runs in turn: a product waits for the one before of its run)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const v4u k = fp4_values(x.key[b][st], by[b]);
+        for (int i = kQueryParts<T> - 1; i >= 0; --i)
 #pragma unroll
-          for (int i = kQueryParts<T> - 1; i >= 0; --i)
-            product[b] = mma16(k, q[i], product[b]);
-        }
+          for (int b = 0; b < 2; ++b)
+            product[b] = mma16(k[b], q[i], product[b]);
       }
       if constexpr (kHalves) {
 #pragma unroll
@@ -511,7 +557,6 @@ fp4_cache_parts(Fp4StepArgs args) {
         }
       }
       by[i] = v4u{run[0].x, run[0].y, run[1].x, run[1].y};
-      total = mma16(ones, by[i], total);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -521,6 +566,9 @@ fp4_cache_parts(Fp4StepArgs args) {
 #pragma unroll
         for (int b = 2 * pair; b < 2 * pair + 2; ++b)
           acc[b] = mma16(vf[b], by[i], acc[b]);
+#pragma unroll
+      for (int i = pair; i < kWeightParts<T>; i += kPairs)
+        total = mma16(ones, by[i], total);
       if (pair + kAhead < kPairs)
         read(pair + kAhead);
       __builtin_amdgcn_sched_barrier(0);
@@ -614,35 +662,30 @@ fp4_cache_parts(Fp4StepArgs args) {
 template <typename T, int DIM>
 __global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
   const StepArgs &a = args.s;
-  __shared__ int sums[2][kThreads / kWave];
   const int seq = (int)(blockIdx.x / a.query_heads);
   const int head = (int)(blockIdx.x % a.query_heads);
   const int hk = head / a.group, row = head % a.group;
+  // of the sequences, or of those before this one (each wave for itself)
+  auto sum = [&](int end, auto value) __attribute__((always_inline)) {
+    int x = 0;
+    for (int i = lane_id(); i < end; i += kWave)
+      x += value(tiles_of(a, i));
+    return __builtin_amdgcn_readlane(sum_to_lane(x), kWave - 1);
+  };
   const int own = tiles_of(a, seq);
-  int before = 0, total = 0;
-  for (int i = threadIdx.x; i < a.sequences; i += kThreads) {
-    const int n = tiles_of(a, i);
-    total += n;
-    before += i < seq ? n : 0;
-  }
-  before = sum_to_lane(before);
-  total = sum_to_lane(total);
-  if (lane_id() == kWave - 1) {
-    sums[0][wave_in_group()] = before;
-    sums[1][wave_in_group()] = total;
-  }
-  __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w) {
-    before += sums[0][w];
-    total += sums[1][w];
-  }
-  int first = 0, parts = 0, share = 1;
+  const int total = sum(a.sequences, [](int n) { return n; });
+  int first = 0, parts = 0, slot = 0;
   if (own > 0) {
-    share = share_of(args, total);
-    first = before / share;
-    parts = (before + own - 1) / share - first + 1;
+    const Split split(args, total);
+    if (split.whole) {
+      first = sum(seq, [&](int n) { return split.shares(n); });
+      parts = split.shares(own);
+    } else {
+      const int before = sum(seq, [](int n) { return n; });
+      first = before / split.most;
+      parts = (before + own - 1) / split.most - first + 1;
+      slot = before != first * split.most ? 1 : 0; // (of the first one)
+    }
     if (parts == 1)
       return; // (it is written)
   }
@@ -650,8 +693,8 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
                        row / args.block;
   join_parts<T, DIM>(a, seq, head, parts, [&](int i) {
     const int64_t r =
-        ((unit * args.shares + first + i) * 2 +
-         (i == 0 && before != first * share ? 1 : 0)) * args.block +
+        ((unit * args.shares + first + i) * 2 + (i == 0 ? slot : 0)) *
+            args.block +
         row % args.block;
     return PartRow{a.sums + r * DIM, a.stats + r * 2};
   });
