@@ -38,15 +38,16 @@ struct MoveArgs {
   Divisor page_size, lanes, rows; // lanes of a token; rows: 2 heads
 };
 
-constexpr int kNoPage = -1, kNoSequence = -2;
+constexpr int kNoPage = -1, kNoSequence = -2; // in the place of `codes`
 struct Place {
-  int page, slot;
+  int64_t codes, scales; // where a head's row starts, from its first row on
 };
 
-// Lane l: the place of token first + l (first is wave-uniform).
+// Lane l: the place of token first + l (first is wave-uniform) in a cache's keys
+// or values.
 template <bool WRITE>
-__device__ __forceinline__ Place place_of(const MoveArgs &a, int first,
-                                          bool live) {
+__device__ __forceinline__ Place place_of(const MoveArgs &a, const Rows &rows,
+                                          int first, bool live) {
   const int l = lane_id(), token = first + l, n = a.sequences;
   const int32_t *offsets = a.offsets;
   const int base =
@@ -78,17 +79,24 @@ __device__ __forceinline__ Place place_of(const MoveArgs &a, int first,
     return p;
   const int64_t place = WRITE ? a.from[i] - (end - token)
                               : (a.from ? a.from[i] : 0) + (token - begin);
-  p.page = kNoPage;
+  p.codes = kNoPage;
   if (place < 0 || place >= a.room)
     return p;
   const int number = (int)a.page_size.quotient((uint32_t)place);
-  const int page =
+  const int64_t page =
       a.table ? a.table[(int64_t)i * a.table_width + number] : i;
   if (page < 0 || page >= a.pages)
     return p;
-  p.page = page;
-  p.slot = (int)place - number * (int)a.page_size.by;
+  const int64_t slot = (int)place - number * (int)a.page_size.by;
+  p.codes = page * rows.codes_page + slot * rows.codes_token;
+  p.scales = page * rows.scales_page + slot * rows.scales_token;
   return p;
+}
+// What `lane` holds in v.
+__device__ __forceinline__ int64_t of_lane(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, (int)v);
+  const int hi = __builtin_amdgcn_ds_bpermute(lane * 4, (int)(v >> 32));
+  return (int64_t)hi << 32 | lo;
 }
 
 // What a wave moves: the keys or the values of one head, of PASSES times
@@ -102,7 +110,7 @@ template <typename T> struct Wave {
   int first, token, piece; // the wave's first token; this lane's of a pass
   int64_t token_stride, at; // of a lane's elements
   const Rows &rows;
-  int64_t codes, scales;
+  uint8_t *codes, *scales; // of this lane in the head's first row
   __device__ __forceinline__ Wave(const MoveArgs &a, int passes, int number,
                                   int tile)
       : value(number - tile * (int)a.rows.by >= a.heads),
@@ -114,8 +122,8 @@ template <typename T> struct Wave {
     piece = lane_id() - token * (int)a.lanes.by;
     token_stride = value ? a.value_token : a.key_token;
     at = head * (value ? a.value_head : a.key_head) + piece * kUnit<T>;
-    codes = head * rows.codes_head + piece * (kUnit<T> / 2);
-    scales = head * rows.scales_head + piece * kUnit<T> / 32;
+    codes = rows.codes + head * rows.codes_head + piece * (kUnit<T> / 2);
+    scales = rows.scales + head * rows.scales_head + piece * kUnit<T> / 32;
   }
 };
 template <typename T>
@@ -194,24 +202,20 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_write(MoveArgs a) {
     if (lane && token < a.tokens)
       x[i] = load_unit(from + token * w.token_stride);
   }
-  const Place all = place_of<true>(a, w.first,
+  const Place all = place_of<true>(a, w.rows, w.first,
                                    lane_id() < PASSES * a.at_once &&
                                        w.first + lane_id() < a.tokens);
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int of = (i * a.at_once + w.token) * 4;
-    const int page = __builtin_amdgcn_ds_bpermute(of, all.page);
-    const int slot = __builtin_amdgcn_ds_bpermute(of, all.slot);
+    const int of = i * a.at_once + w.token;
+    const int64_t at = of_lane(all.codes, of), scale = of_lane(all.scales, of);
     const uint32_t byte = fp4_scale_byte(block_top(x[i], T{}));
     const typename C::Word codes =
         byte == 255 ? 0u : C::of(x[i], fp4_scale(byte));
-    if (lane && page >= 0) {
-      *reinterpret_cast<typename C::Word *>(
-          w.rows.codes + page * w.rows.codes_page + slot * w.rows.codes_token +
-          w.codes) = codes;
+    if (lane && at >= 0) {
+      *reinterpret_cast<typename C::Word *>(w.codes + at) = codes;
       if (w.piece % (32 / kUnit<T>) == 0)
-        w.rows.scales[page * w.rows.scales_page + slot * w.rows.scales_token +
-                      w.scales] = (uint8_t)byte;
+        w.scales[scale] = (uint8_t)byte;
     }
   }
 }
@@ -223,31 +227,28 @@ __global__ __launch_bounds__(kThreads) void fp4_cache_read(MoveArgs a) {
   if (!w.any)
     return;
   const bool lane = w.token < a.at_once;
-  const Place all = place_of<false>(a, w.first,
+  const Place all = place_of<false>(a, w.rows, w.first,
                                     lane_id() < PASSES * a.at_once &&
                                         w.first + lane_id() < a.tokens);
-  int page[PASSES];
+  int state[PASSES];
   typename C::Word codes[PASSES];
   uint8_t bytes[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int of = (i * a.at_once + w.token) * 4;
-    page[i] = __builtin_amdgcn_ds_bpermute(of, all.page);
-    const int slot = __builtin_amdgcn_ds_bpermute(of, all.slot);
+    const int of = i * a.at_once + w.token;
+    const int64_t at = of_lane(all.codes, of), scale = of_lane(all.scales, of);
+    state[i] = (int)(at >> 32) < 0 ? (int)at : 0;
     codes[i] = 0;
     bytes[i] = 0;
-    if (lane && page[i] >= 0) {
-      codes[i] = *reinterpret_cast<const typename C::Word *>(
-          w.rows.codes + page[i] * w.rows.codes_page +
-          slot * w.rows.codes_token + w.codes);
-      bytes[i] = w.rows.scales[page[i] * w.rows.scales_page +
-                               slot * w.rows.scales_token + w.scales];
+    if (lane && at >= 0) {
+      codes[i] = *reinterpret_cast<const typename C::Word *>(w.codes + at);
+      bytes[i] = w.scales[scale];
     }
   }
   T *to = static_cast<T *>(w.value ? a.value : a.key) + w.at;
 #pragma unroll
   for (int i = 0; i < PASSES; ++i)
-    if (lane && page[i] != kNoSequence)
+    if (lane && state[i] != kNoSequence)
       store_unit(to + (w.first + i * a.at_once + w.token) * w.token_stride,
                  C::values(codes[i], fp4_scale(bytes[i])));
 }
