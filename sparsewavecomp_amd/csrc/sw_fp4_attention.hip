@@ -80,30 +80,98 @@ __device__ __forceinline__ int sum_to_lane(int v) {
   return v;
 }
 
+// The tiles of up to 4096 sequences: lane l of a wave has those of number
+// l each to l each + each - 1, the first HELD of them in registers (1, where that
+// is all, or 8: for one sequence the 8 would cost 1.5 us).
+template <int HELD> struct AllTiles {
+  const StepArgs &a;
+  int each, held[HELD];
+  __device__ __forceinline__ explicit AllTiles(const StepArgs &args)
+      : a(args), each(HELD == 1 ? 1 : (args.sequences + kWave - 1) / kWave) {
+    load(held, 0);
+  }
+  __device__ __forceinline__ int of(int sequence, bool there = true) const {
+    const int last = a.sequences - 1;
+    const int tiles = tiles_of(a, sequence < last ? sequence : last);
+    return there && sequence <= last ? tiles : 0;
+  }
+  // (their loads are on their way together)
+  __device__ __forceinline__ void load(int (&n)[HELD], int from) const {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      n[i] = of(lane_id() * each + from + i, from + i < each);
+  }
+  // The sum of value(tiles) over this lane's first `end` ones; value(0) is 0.
+  template <typename F>
+  __device__ __forceinline__ int sum(int end, F value) const {
+    int x = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      x += i < end ? value(held[i]) : 0;
+    for (int from = HELD; from < end; from += HELD) {
+      int n[HELD];
+      load(n, from);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        x += from + i < end ? value(n[i]) : 0;
+    }
+    return x;
+  }
+  template <typename F> __device__ __forceinline__ int sum(F value) const {
+    return sum(each, value);
+  }
+};
+
 // How a unit's tiles are split: `most` for a workgroup, and whether none takes
-// those of two sequences (`whole`: a sequence's tiles divided by `most`, rounded
-// up, are its shares, one more for each sequence at most).  A second sequence
-// costs a workgroup about as much as 8 tiles (4 sequences of up to 8,192 keys 21.6
-// us, whole 18.6; 32 of up to 2,048 25.7 and 23.3; 64 of up to 20,000, over four
-// key heads of 64, 61.4 and 68.5).
+// those of two sequences (`whole`: a sequence's tiles are divided among its
+// shares).  A second sequence costs a workgroup about as much as 8 tiles (4
+// sequences of up to 8,192 keys 21.6 us, whole 18.6; 32 of up to 2,048 25.7 and
+// 23.3; 64 of up to 20,000, over four key heads of 64, 61.4 and 68.5), so that
+// shares may be longer by as much to keep them whole: by as little as does, where
+// a wave has all sequences' tiles in registers.
 struct Split {
   int most;
   bool whole;
-  __device__ __forceinline__ Split(const Fp4StepArgs &args, int total) {
+  float by; // 1 / most
+  template <int HELD>
+  __device__ __forceinline__ Split(const Fp4StepArgs &args, int total,
+                                   const AllTiles<HELD> &all) {
     constexpr int kSecond = 8;
-    const int apart = args.shares - args.s.sequences;
     const int even = (total + args.shares - 1) / args.shares;
-    most = even < args.least ? args.least : even;
-    whole = false;
-    if (apart > 0) {
-      const int more = (total + apart - 1) / apart;
-      whole = more <= most + kSecond;
-      if (whole && more > most)
-        most = more;
+    const int fewest = even < args.least ? args.least : even;
+    if (all.each <= HELD) {
+      auto fits = [&](int n) __attribute__((always_inline)) {
+        set(n);
+        const int own = all.sum([&](int t) { return shares(t); });
+        return __builtin_amdgcn_readlane(sum_to_lane(own), kWave - 1) <=
+               args.shares;
+      };
+      int n = fewest + kSecond;
+      whole = args.s.sequences < args.shares && fits(n);
+      if (whole) {
+        if (fits(fewest))
+          n = fewest;
+        else
+          for (int step = kSecond / 2; step > 0; step /= 2)
+            n -= fits(n - step) ? step : 0;
+      }
+      set(whole ? n : fewest);
+    } else {
+      const int apart = args.shares - args.s.sequences;
+      const int more = apart > 0 ? (total + apart - 1) / apart : INT32_MAX;
+      whole = more <= fewest + kSecond;
+      set(whole && more > fewest ? more : fewest);
     }
   }
+  __device__ __forceinline__ void set(int n) {
+    most = n;
+    by = __builtin_amdgcn_rcpf((float)n);
+  }
+  // Of a whole sequence: about tiles / most rounded up (in 32 bits, the same in
+  // each wave that asks; at least 1 of a tile, and up to 4096 sequences no more in
+  // all than exact ones could be).
   __device__ __forceinline__ int shares(int tiles) const {
-    return (tiles + most - 1) / most;
+    return (int)ceilf((float)tiles * by);
   }
 };
 
@@ -114,24 +182,19 @@ struct Split {
 struct Share {
   int from, to, seq, offset;
 };
+template <int HELD>
 __device__ __forceinline__ Share find_share(const Fp4StepArgs &args, int p) {
-  const StepArgs &a = args.s;
-  const int l = lane_id(), each = (a.sequences + kWave - 1) / kWave;
-  auto tiles = [&](int i) __attribute__((always_inline)) {
-    return i < a.sequences ? tiles_of(a, i) : 0;
-  };
-  int held = tiles(l * each), own = held; // (the lane's first one's, and all)
-  for (int i = 1; i < each; ++i)
-    own += tiles(l * each + i);
+  const AllTiles<HELD> all(args.s);
+  auto tiles = [](int n) { return n; };
+  int own = all.sum(tiles);
   int sum = sum_to_lane(own);
   const int total = __builtin_amdgcn_readlane(sum, kWave - 1);
-  const Split split(args, total);
+  const Split split(args, total, all);
+  auto shares = [&](int n) { return split.shares(n); };
   Share s{0, 0, 0, 0};
   int first = p, end = total; // what is looked for, and of how many
   if (split.whole) {
-    own = split.shares(held);
-    for (int i = 1; i < each; ++i)
-      own += split.shares(tiles(l * each + i));
+    own = all.sum(shares);
     sum = sum_to_lane(own);
     end = __builtin_amdgcn_readlane(sum, kWave - 1);
   } else if (p > total / split.most) {
@@ -142,21 +205,23 @@ __device__ __forceinline__ Share find_share(const Fp4StepArgs &args, int p) {
   if (first >= end)
     return s;
   int at = __builtin_popcountll(ballot(sum <= first));
-  s.seq = at * each;
+  s.seq = at * all.each;
   int offset = __builtin_amdgcn_readlane(sum - own, at);
-  if (each > 1) {
-    held = l < each ? tiles(s.seq + l) : 0;
-    own = split.whole ? split.shares(held) : held;
+  int held = all.held[0];
+  if (all.each > 1) {
+    held = lane_id() < all.each ? all.of(s.seq + lane_id()) : 0;
+    own = split.whole ? shares(held) : held;
     sum = offset + sum_to_lane(own);
-    at = __builtin_popcountll(ballot(l < each && sum <= first));
+    at = __builtin_popcountll(ballot(lane_id() < all.each && sum <= first));
     s.seq += at;
     offset = __builtin_amdgcn_readlane(sum - own, at);
   }
   if (split.whole) {
-    const int all = __builtin_amdgcn_readlane(held, at);
-    const int shares = split.shares(all), even = (all + shares - 1) / shares;
-    s.from = (p - offset) * even;
-    s.to = all - s.from < even ? all : s.from + even;
+    const int n = __builtin_amdgcn_readlane(held, at);
+    const int parts = shares(n), i = p - offset;
+    const int even = n / parts, longer = n - even * parts;
+    s.from = i * even + (i < longer ? i : longer);
+    s.to = s.from + even + (i < longer ? 1 : 0);
   } else {
     s.from = first;
     s.to = total - first < split.most ? total : first + split.most;
@@ -293,7 +358,8 @@ fp4_cache_parts(Fp4StepArgs args) {
   Share my{0, 0, number, 0};
   bool begun = false; // whether a part of the share is done
   if (args.shares != 0) {
-    my = find_share(args, number);
+    my = a.sequences <= kWave ? find_share<1>(args, number)
+                              : find_share<8>(args, number);
     if (my.from == my.to)
       return;
   }
@@ -657,47 +723,164 @@ fp4_cache_parts(Fp4StepArgs args) {
   }
 }
 
-// The parts of a query head whose sequence's tiles several shares hold; zeros for
-// one without a key.
-template <typename T, int DIM>
-__global__ __launch_bounds__(kThreads) void fp4_cache_join(Fp4StepArgs args) {
-  const StepArgs &a = args.s;
-  const int seq = (int)(blockIdx.x / a.query_heads);
-  const int head = (int)(blockIdx.x % a.query_heads);
-  const int hk = head / a.group, row = head % a.group;
-  // of the sequences, or of those before this one (each wave for itself)
-  auto sum = [&](int end, auto value) __attribute__((always_inline)) {
-    int x = 0;
-    for (int i = lane_id(); i < end; i += kWave)
-      x += value(tiles_of(a, i));
-    return __builtin_amdgcn_readlane(sum_to_lane(x), kWave - 1);
+// The parts of a sequence's tiles in the shares of a unit: the first of these,
+// how many, and their slot in the first one.
+struct Parts {
+  int first, count, slot;
+};
+template <int HELD>
+__device__ __forceinline__ Parts parts_of(const Fp4StepArgs &args, int seq) {
+  const int own = tiles_of(args.s, seq);
+  const AllTiles<HELD> all(args.s);
+  auto tiles = [](int n) { return n; };
+  const int total = __builtin_amdgcn_readlane(sum_to_lane(all.sum(tiles)),
+                                              kWave - 1);
+  const Split split(args, total, all);
+  // the sum over the sequences before this one
+  const int lane = seq / all.each, within = seq - lane * all.each;
+  auto before = [&](auto value) __attribute__((always_inline)) {
+    const int sum = all.sum(value);
+    return __builtin_amdgcn_readlane(
+        sum_to_lane(sum) - sum + all.sum(within, value), lane);
   };
-  const int own = tiles_of(a, seq);
-  const int total = sum(a.sequences, [](int n) { return n; });
-  int first = 0, parts = 0, slot = 0;
-  if (own > 0) {
-    const Split split(args, total);
-    if (split.whole) {
-      first = sum(seq, [&](int n) { return split.shares(n); });
-      parts = split.shares(own);
-    } else {
-      const int before = sum(seq, [](int n) { return n; });
-      first = before / split.most;
-      parts = (before + own - 1) / split.most - first + 1;
-      slot = before != first * split.most ? 1 : 0; // (of the first one)
-    }
-    if (parts == 1)
-      return; // (it is written)
+  if (own == 0)
+    return {0, 0, 0};
+  if (split.whole) {
+    auto shares = [&](int n) { return split.shares(n); };
+    return {before(shares), shares(own), 0};
   }
-  const int64_t unit = hk * ((a.group + args.block - 1) / args.block) +
-                       row / args.block;
-  join_parts<T, DIM>(a, seq, head, parts, [&](int i) {
-    const int64_t r =
-        ((unit * args.shares + first + i) * 2 + (i == 0 ? slot : 0)) *
-            args.block +
-        row % args.block;
+  const int n = before(tiles), first = n / split.most;
+  return {first, (n + own - 1) / split.most - first + 1,
+          n != first * split.most ? 1 : 0};
+}
+
+// Parts of a query head, joined: DIM / 32 consecutive elements a lane.
+template <int N> struct Joined {
+  float top = -kInf, l = 0.0f, o[N] = {};
+  __device__ __forceinline__ void scale(float to) {
+    const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+    top = to;
+    l *= by;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      o[e] *= by;
+  }
+  // AT_ONCE of `count` parts, `step` apart: their loads are on their way together.
+  template <int AT_ONCE, typename F>
+  __device__ __forceinline__ void add(int from, int step, int count, float lower,
+                                      F row) {
+    typedef float Sums __attribute__((ext_vector_type(N)));
+    const int c = lane_id() % 32 * N;
+    Sums sums[AT_ONCE];
+    float m[AT_ONCE], weight[AT_ONCE], to = top;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int part = from + i * step;
+      const PartRow r = row(part < count ? part : 0);
+      sums[i] = *reinterpret_cast<const Sums *>(r.sums + c);
+      m[i] = r.stats[0];
+      weight[i] = r.stats[1];
+      if (part >= count) {
+        sums[i] = Sums{};
+        m[i] = -kInf;
+        weight[i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+      to = fmaxf(to, m[i]);
+    scale(to);
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      weight[i] *= lower * (m[i] == to ? 1.0f
+                                       : __builtin_amdgcn_exp2f(m[i] - to));
+      l += weight[i];
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        o[e] = fmaf(sums[i][e], weight[i], o[e]);
+    }
+  }
+};
+
+// The parts of the query heads of a sequence whose tiles several shares hold; zeros
+// for one without a key.  THREADS / 256 is 1, a head a wave; or 4, one head, whose
+// parts the half waves take in turn.
+template <typename T, int DIM, int THREADS>
+__global__ __launch_bounds__(THREADS) void fp4_cache_join(Fp4StepArgs args) {
+  constexpr int N = DIM / 32, kHalves = THREADS / 32;
+  constexpr int kHeads = THREADS == kThreads ? THREADS / kWave : 1;
+  const StepArgs &a = args.s;
+  const int of = (a.query_heads + kHeads - 1) / kHeads; // a sequence's workgroups
+  const int seq = (int)(blockIdx.x / of);
+  const int head = (int)(blockIdx.x - seq * of) * kHeads +
+                   (kHeads > 1 ? wave_in_group() : 0);
+  // (each wave for itself)
+  const Parts parts = a.sequences <= kWave ? parts_of<1>(args, seq)
+                                           : parts_of<8>(args, seq);
+  if (parts.count == 1 || head >= a.query_heads)
+    return; // (it is written)
+  const int hk = head / a.group, in_group = head - hk * a.group;
+  const int block = in_group / args.block;
+  const int64_t unit = hk * ((a.group + args.block - 1) / args.block) + block;
+  const int64_t first =
+      (unit * args.shares + parts.first) * 2 * args.block +
+      (in_group - block * args.block);
+  auto row = [&](int i) __attribute__((always_inline)) {
+    const int64_t r = first + (2 * i + (i == 0 ? parts.slot : 0)) * args.block;
     return PartRow{a.sums + r * DIM, a.stats + r * 2};
-  });
+  };
+  T *out = static_cast<T *>(a.output) + seq * a.output_token +
+           head * a.output_head;
+  const int half = (int)threadIdx.x % (kHeads > 1 ? kWave : THREADS) / 32;
+  constexpr int kStep = kHalves / kHeads;
+  Joined<N> x;
+  int from = half;
+  if constexpr (kHeads > 1) // (8 at once for many parts in a wave)
+    for (; from + 4 * kStep < parts.count; from += 8 * kStep)
+      x.template add<8>(from, kStep, parts.count, a.lower, row);
+  for (; from < parts.count; from += 4 * kStep)
+    x.template add<4>(from, kStep, parts.count, a.lower, row);
+  // both halves of a wave
+  x.scale(fmaxf(x.top, shfl_xor32(x.top)));
+  x.l += shfl_xor32(x.l);
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    x.o[e] += shfl_xor32(x.o[e]);
+  const int c = lane_id() % 32 * N;
+  if constexpr (kHeads > 1) {
+    if (lane_id() < 32 && c < a.d) {
+      const float by = 1.0f / x.l;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        stv(out + c + e, x.top == -kInf ? 0.0f : x.o[e] * by);
+    }
+  } else {
+    constexpr int kWaves = THREADS / kWave;
+    __shared__ float outs[kWaves][DIM], tops[kWaves], totals[kWaves];
+    const int wave = wave_in_group();
+    if (lane_id() < 32) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        outs[wave][c + e] = x.o[e];
+      tops[wave] = x.top;
+      totals[wave] = x.l;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x >= a.d)
+      return;
+    float top = tops[0], l = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i)
+      top = fmaxf(top, tops[i]);
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const float by =
+          tops[i] == top ? 1.0f : __builtin_amdgcn_exp2f(tops[i] - top);
+      l = fmaf(totals[i], by, l);
+      o = fmaf(outs[i][threadIdx.x], by, o);
+    }
+    stv(out + threadIdx.x, top == -kInf ? 0.0f : o * (1.0f / l));
+  }
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -707,11 +890,21 @@ struct Plan {
   int64_t bytes() const { return 4 * (sums + stats); }
 };
 
-// Compute units, and the fewest tiles that a workgroup is made for.
-constexpr int64_t kUnits = 256, kLeast = 16;
+// Compute units, and the fewest tiles that a workgroup is made for (bf16, 32 heads
+// over 8 of 128, us with 4, 8 and 16: one sequence of 1,024 keys 10.6, 11.5 and
+// 13.5, eight of up to 1,024 12.9, 12.3 and 14.6, one of 32,768 19.8, 19.7 and
+// 19.1, eight of up to 8,192 19.7, 19.7 and 18.2).
+constexpr int64_t kUnits = 256, kLeast = 8;
 
-// `waves`: workgroups of a compute unit.  Few keys, or more sequences than a
-// share can be found among, are not split.
+// `waves`: workgroups of a compute unit.  Not split, a workgroup for each sequence
+// and no join, are sequences of few keys, of not many where there are half as many
+// of them as shares, and more of them than a share can be found among.  (us of
+// sequences of up to so many keys, 32 heads over 8 of 128, bf16, split and not: 1 of
+// 1,024 11.5 and 13.1, 8 of 1,024 12.3 and 14.7, 8 of 544 11.3 and 10.6, 32 of 2,048
+// 21.8 and 25.4, 64 of 1,024 22 and 18.7, 64 of 2,048 33 and 30.6, 256 of 2,048 89
+// and 84, 256 of 4,096 145.5 and 146.6; fp32: 64 of 1,024 26 and 23, 64 of 2,048
+// 38.3 and 37.2, 256 of 4,096 170 and 172.  400 of 2,048, 16 heads over one: 38.5 and
+// 31.)
 Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
           int64_t key_heads, int64_t d, int64_t window, int64_t sinks,
           int64_t waves) {
@@ -720,10 +913,12 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
   p.block = group <= 8 ? 8 : kRows;
   p.units = key_heads * sw::ceil_div(group, p.block);
   const int64_t visible = most_visible(capacity, window, sinks);
-  if (visible <= 512 || sequences > 4096 ||
+  const int64_t shares = std::max<int64_t>(1, kUnits * waves / p.units);
+  if (visible <= std::max<int64_t>(512, std::min<int64_t>(2048, 4096 * sequences / shares)) ||
+      sequences > 4096 ||
       sequences * sw::ceil_div(capacity, 32) > sw::kMostTokens)
     return p;
-  p.shares = std::max<int64_t>(1, kUnits * waves / p.units);
+  p.shares = shares;
   const int64_t all = p.units * p.shares * 2 * p.block;
   p.sums = all * (d <= 64 ? 64 : 128);
   p.stats = all * 2;
@@ -825,8 +1020,14 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.sums = static_cast<float *>(workspace);
   a.stats = a.sums + p.sums;
   const int64_t grid = p.units * (p.shares ? p.shares : sequences);
-  const int64_t join = sequences * query_heads;
-  if (int rc = sw::check_flat_grid(std::max(grid, join), kThreads, what))
+  // Few rows take a workgroup of 1024 each (4 sequences of up to 100,000 keys, 12
+  // heads: 33.9 us of both kernels, 36 with 256); one of four rows else (256
+  // sequences, 32 heads: the join 19.8 us with one of 256 for each row).
+  const bool few = sequences * query_heads <= 512;
+  const int64_t join =
+      sequences * (few ? query_heads
+                       : sw::ceil_div(query_heads, kThreads / kWave));
+  if (int rc = sw::check_flat_grid(std::max(grid, join), 4 * kThreads, what))
     return rc;
   const hipStream_t st = sw::as_stream(stream);
   const dim3 g((unsigned)grid);
@@ -847,10 +1048,18 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
     return rc;
   if (p.shares == 0)
     return SW_OK;
+  const dim3 j((unsigned)join);
+  auto launch_join = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    if (few)
+      fp4_cache_join<T, D, 4 * kThreads><<<j, 4 * kThreads, 0, st>>>(args);
+    else
+      fp4_cache_join<T, D, kThreads><<<j, kThreads, 0, st>>>(args);
+  };
   if (d <= 64)
-    fp4_cache_join<T, 64><<<dim3((unsigned)join), kThreads, 0, st>>>(args);
+    launch_join(std::integral_constant<int, 64>{});
   else
-    fp4_cache_join<T, 128><<<dim3((unsigned)join), kThreads, 0, st>>>(args);
+    launch_join(std::integral_constant<int, 128>{});
   return sw::launch_check(what);
 }
 

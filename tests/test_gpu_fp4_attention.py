@@ -191,6 +191,32 @@ def test_shares_of_many_sequences(dev, dtype, case):
     assert torch.equal(got, torch.zeros_like(got))
 
 
+# sequences, their most keys, one's, room, heads, key heads: rows joined by a wave
+# and by a workgroup, of a part or two and of more than either takes at once, some
+# behind the last full workgroup; more sequences than a wave's registers hold
+JOINS = [
+    (80, 300, 9000, 9100, 16, 2),
+    (600, 60, 2500, 2600, 1, 1),
+    (600, 300, 2500, 2600, 1, 1),
+    (200, 500, 3000, 3000, 2, 1),
+    (40, 700, 700, 5000, 17, 1),
+    (1, 40000, 40000, 40000, 3, 1),
+    (30, 9, 33000, 33000, 18, 1),
+    (260, 1000, 1000, 4000, 3, 3),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(JOINS)))
+def test_joins(dev, dtype, case):
+    n, most, one, room, h, hk = JOINS[case]
+    say(f"fp4 joins {dtype} {JOINS[case]}")
+    lengths = ragged(n, most, case)
+    lengths[n // 2] = one
+    x = make(dtype, lengths, 0, h, hk, 32, seed=case, capacity=room)
+    expect(x, decode(x, 0.2, 10 ** 6, 0), 0.2, 10 ** 6)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_more_sequences_than_are_shared(dev, dtype):
     """Past 4096 each has a workgroup to itself, whatever room it has."""
