@@ -686,7 +686,8 @@ int sw_rotary_backward_bf16(
  * and the value scales (NULL: as the shapes above).  Rows of codes start on 16
  * bytes, a token stride is at least a row and at most 2^23 bytes; pages that
  * hold a head's rows together are read fastest.  What a call writes must not
- * overlap: strides that let rows share memory are refused.
+ * overlap: strides that let rows share memory are refused, and the four arrays of
+ * a cache share no memory.
  *
  * sw_fp4_cache_write: sequence i has the packed tokens token_offsets[i] ..
  * token_offsets[i+1] - 1 of key and value [tokens][key_heads][d], which are the
@@ -735,7 +736,9 @@ int sw_fp4_cache_read_bf16(
  * the cache means that its keys are not there.  `strides` holds sixteen: the
  * token and head stride of query and of output in elements, then the cache's as
  * above.  fp32 queries meet the codes' values without a rounding (three bf16
- * parts each), and so do their probabilities.
+ * parts each), and so do their probabilities.  A byte of 254 that no write leaves
+ * can give infinities.  How a sequence's keys are split, and so the order of its
+ * sums, follows all lengths of the call and the table's width.
  */
 int64_t sw_window_attention_decode_fp4_workspace_bytes(
     int64_t sequences, int64_t page_size, int64_t table_width,

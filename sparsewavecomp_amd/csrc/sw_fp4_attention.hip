@@ -7,6 +7,15 @@
 // probabilities lose nothing either.  A key and its value take 17/16 d bytes for
 // 4 G d operations of the G query heads that share them: 3.75 times fewer bytes
 // than in bf16, for the same products, exponentials and conversions besides.
+//
+// Memory bounds long batches: 64 sequences of up to 20,000 keys, 32 query heads
+// over 8 of 128, bf16, 887 MB, take 149 us in the kernel and 4 in the join, 5.7
+// TB/s with both; the same loads alone, streamed, take 134.  The matrix cores are
+// busy for 23 % of it, vector instructions for 42 %.  In fp32 (5 sequences, windows
+// of 65,544 keys, 12 heads over 4 of 96, 104 MB: 37 and 4.5 us) three parts of
+// queries and of probabilities are three times the products, which a wave's loads
+// of one tile ahead do not hide.  A short call is its chain of trips (length, page,
+// key) and the join's.
 #include "sw_cache.h"
 #include "sw_fp4.h"
 
@@ -311,15 +320,21 @@ template <int D> struct ValueTile {
 // A run of 16 keys lies in one page wherever a page holds a multiple of 16: its
 // addresses are then scalar ones plus a lane's constant offset.  Runs that cross
 // a page's end take each lane's own.  The pages of a wave's next runs are found
-// 64 at once, one by each lane.
+// 64 at once, one by each lane.  (The batch above: 413 us with each lane's
+// addresses for each key, 310 so, 185 with even shares and the queries' fragments
+// in LDS instead of registers, 167 with the next tile's loads under way.  The next
+// tile's scores before this one's values: 339.)
 //
 // Up to 8 query rows (ROWS) have the 16 columns of a product twice, each half for
 // the scores of one of the tile's two runs, so that a lane has 4 scores instead of
 // 8, half of them of rows that are not there.  A half's probabilities are masked
 // out where the other run's values are multiplied; each column keeps a maximum and
-// sums of its own, joined like a part's at the end.
+// sums of its own, joined like a part's at the end.  (171 us for 175; 8 heads a key
+// head 156 for 157.)
 //
-// STREAM: the codes pass by the caches, where no other workgroup reads them.
+// STREAM: the codes pass by the caches, where no other workgroup reads them: up to
+// 16 rows (166 us, 174 through them; 16 heads a key head 91 and 99); with 32, whose
+// two workgroups read the same keys, 168 past them and 156 through them.
 template <typename T, int D> struct Fp4Parts {
   using Tile = ValueTile<D>;
   static constexpr int kWaveBytes =
@@ -1027,7 +1042,7 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   const int64_t join =
       sequences * (few ? query_heads
                        : sw::ceil_div(query_heads, kThreads / kWave));
-  if (int rc = sw::check_flat_grid(std::max(grid, join), 4 * kThreads, what))
+  if (int rc = sw::check_flat_grid(std::max(grid, join), kThreads, what))
     return rc;
   const hipStream_t st = sw::as_stream(stream);
   const dim3 g((unsigned)grid);
