@@ -223,11 +223,13 @@ __device__ __forceinline__ Share find_share(const Fp4StepArgs &args, int p) {
     sum = offset + sum_to_lane(own);
     at = __builtin_popcountll(ballot(lane_id() < all.each && sum <= first));
     s.seq += at;
+    if (s.seq >= args.s.sequences) // (only if lengths change under the call)
+      return s;
     offset = __builtin_amdgcn_readlane(sum - own, at);
   }
   if (split.whole) {
     const int n = __builtin_amdgcn_readlane(held, at);
-    const int parts = shares(n), i = p - offset;
+    const int parts = n > 0 ? shares(n) : 1, i = p - offset;
     const int even = n / parts, longer = n - even * parts;
     s.from = i * even + (i < longer ? i : longer);
     s.to = s.from + even + (i < longer ? 1 : 0);
@@ -758,15 +760,24 @@ __device__ __forceinline__ Parts parts_of(const Fp4StepArgs &args, int seq) {
     return __builtin_amdgcn_readlane(
         sum_to_lane(sum) - sum + all.sum(within, value), lane);
   };
+  Parts p{0, 0, 0};
   if (own == 0)
-    return {0, 0, 0};
+    return p;
   if (split.whole) {
     auto shares = [&](int n) { return split.shares(n); };
-    return {before(shares), shares(own), 0};
+    p.first = before(shares);
+    p.count = shares(own);
+  } else {
+    const int n = before(tiles);
+    p.first = n / split.most;
+    p.count = (n + own - 1) / split.most - p.first + 1;
+    p.slot = n != p.first * split.most ? 1 : 0;
   }
-  const int n = before(tiles), first = n / split.most;
-  return {first, (n + own - 1) / split.most - first + 1,
-          n != first * split.most ? 1 : 0};
+  // (more only if lengths change under the call)
+  const int left = args.shares - p.first;
+  if (p.count > left)
+    p.count = left > 0 ? left : 0;
+  return p;
 }
 
 // Parts of a query head, joined: DIM / 32 consecutive elements a lane.
