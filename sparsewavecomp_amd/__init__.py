@@ -957,10 +957,15 @@ def _two(dtype, at, shape, a, a_name, b, b_name):
     operands of one shape: as :func:`_heads`, in less time (0.7 us instead of
     1.6) where they are as they should be."""
     if type(a) is type(b) is _torch.Tensor and a.dtype is b.dtype is dtype and \
-            a.get_device() == b.get_device() == at and 1 not in shape:
+            a.get_device() == b.get_device() == at:
         row, head, last = a.stride()
         other_row, other_head, other_last = b.stride()
         if last == other_last == 1:
+            rows, heads, d = shape
+            if rows == 1:
+                row = other_row = d
+            if heads == 1:
+                head = other_head = d
             return (a.data_ptr(), b.data_ptr()), (row, head, other_row,
                                                   other_head)
     return _heads(dtype, at, a, a_name, b, b_name, always=True)
@@ -1083,12 +1088,18 @@ def _fp4_rows(at, d, key_cache, value_cache):
     if type(kc) is type(ks) is type(vc) is type(vs) is tensor and \
             kc.dtype is ks.dtype is vc.dtype is vs.dtype is byte and \
             kc.get_device() == ks.get_device() == vc.get_device() == \
-            vs.get_device() == at and pages != 1 and size != 1 and heads != 1:
+            vs.get_device() == at:
         a, b, c, e = kc.stride(), ks.stride(), vc.stride(), vs.stride()
         if a[3] == b[3] == c[3] == e[3] == 1:
-            return (pages, size, heads), (
-                kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()), (
-                    *a[:3], *b[:3], *c[:3], *e[:3])
+            strides = (*a[:3], *b[:3], *c[:3], *e[:3])
+            if pages == 1 or size == 1 or heads == 1:
+                blocks = d // 32
+                strides = tuple(
+                    y if n != 1 else z for n, y, z in zip(
+                        (pages, size, heads) * 4, strides,
+                        (0, width, width, 0, blocks, blocks) * 2))
+            return (pages, size, heads), (kc.data_ptr(), ks.data_ptr(),
+                                          vc.data_ptr(), vs.data_ptr()), strides
     return (pages, size, heads), *_heads(
         byte, at, kc, "key_cache codes", ks, "key_cache scales", vc,
         "value_cache codes", vs, "value_cache scales", always=True)
