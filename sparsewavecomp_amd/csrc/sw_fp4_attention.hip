@@ -36,7 +36,8 @@ struct Fp4StepArgs {
   Divisor page_size;
   // A unit is `block` query rows (8 or 16) of a key head, for all sequences.  Its
   // tiles are split evenly among `shares` workgroups, each taking `least` at
-  // least.  0 shares: a workgroup for each sequence of a unit.
+  // least.  0 shares: a workgroup for each sequence of a unit, which has `least`
+  // tiles at most.
   int units, shares, least, block;
 };
 
@@ -312,6 +313,22 @@ template <int D> struct ValueTile {
   }
 };
 
+// Of a SIMD's waves the one with most left to do goes first.  Left to themselves
+// the oldest does: the three workgroups of a compute unit, which have the same to
+// do, ended after 111, 124 and 142 us and left it half idle (124, 132 and 141 so,
+// and in all 169 us -> 163; heads of 64 60.4 -> 57.2).  Later thresholds and quarters
+// balance less.
+__device__ __forceinline__ void go_first(int all, int left) {
+  if (left > all / 2)
+    __builtin_amdgcn_s_setprio(3);
+  else if (left > all / 4)
+    __builtin_amdgcn_s_setprio(2);
+  else if (left > all / 8)
+    __builtin_amdgcn_s_setprio(1);
+  else
+    __builtin_amdgcn_s_setprio(0);
+}
+
 // One share of a unit's tiles, a tile a wave at a time, part by part (a part:
 // the share's tiles of one sequence).  Lane l holds a quarter (l / 16) of key
 // l % 16 of each of the tile's runs of 16 keys, whose codes are one load for
@@ -373,12 +390,14 @@ fp4_cache_parts(Fp4StepArgs args) {
   const int rows = a.group - first_row < ROWS ? a.group - first_row : ROWS;
   const bool live = row_of % ROWS < rows;
   Share my{0, 0, number, 0};
+  int extent = args.least; // the share's tiles
   bool begun = false; // whether a part of the share is done
   if (args.shares != 0) {
     my = a.sequences <= kWave ? find_share<1>(args, number)
                               : find_share<8>(args, number);
     if (my.from == my.to)
       return;
+    extent = my.to - my.from;
   }
   const bool none = a.alpha == 0.0f;
   const float scale = __uint_as_float(__builtin_amdgcn_readfirstlane(
@@ -661,7 +680,8 @@ fp4_cache_parts(Fp4StepArgs args) {
   for (;;) {
     const int all = see.tiles();
     t0 = my.from - my.offset;
-    t1 = args.shares == 0 || my.to - my.offset > all ? all : my.to - my.offset;
+    const int end = args.shares == 0 ? all : my.to - my.offset; // the share's
+    t1 = end > all ? all : end;
     static_assert(kSteps <= kThreads / kWave, ""); // (a step of queries a wave)
     if (wave < kSteps) {
       const int c = D / 4 * g + 8 * wave;
@@ -694,6 +714,7 @@ fp4_cache_parts(Fp4StepArgs args) {
         Data x, y;
         fetch(x, runs, 0, see.first_key(first));
         for (int k = 0; k < n; k += 2) {
+          go_first(extent, end - (first + 4 * k));
           if (k + 1 < n)
             fetch(y, runs, k + 1, see.first_key(first + 4 * k + 4));
           some |= (x.has[0] | x.has[1]) != 0;
@@ -1040,6 +1061,9 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   args.units = (int)p.units;
   args.shares = (int)p.shares;
   args.least = (int)kLeast;
+  if (p.shares == 0)
+    args.least = (int)sw::ceil_div(
+        most_visible(page_size * table_width, window, sinks), kTile);
   a.lower = std::ldexp(
       1.0f, -(int)std::ceil(std::log2((double)(page_size * table_width + 64))) -
                 1 - (int)kLag);
