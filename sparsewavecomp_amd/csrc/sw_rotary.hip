@@ -36,8 +36,8 @@ struct RotaryArgs {
   Heads query, key;
   int tokens, axis_count, query_heads, heads, d, pairs;
   int per; // tokens of a workgroup
-  int turned, units; // units of a head that turn, and all of them
-  Divisor token_units, head_units;
+  int turned; // pieces of a head that turn
+  Divisor token_pieces, head_pieces; // (of all of them)
   bool back;
 };
 
@@ -82,12 +82,12 @@ __device__ __forceinline__ Turn turn_of(int position, float frequency) {
   return {c, s};
 }
 
-// W consecutive elements, aligned to their size, as fp32 and back.  Pieces of 16
+// W consecutive elements, aligned to one of them, as fp32 and back.  Pieces of 16
 // bytes are written past the caches (32,760 tokens of 40 bf16 heads of 128: 110 us,
 // 115 with plain stores; 16,384 of 20: 27.1 and 32.8; with loads past them too 107
 // and 30.5).
 template <typename T, int W> struct Piece {
-  typedef T Raw __attribute__((ext_vector_type(W)));
+  typedef T Raw __attribute__((ext_vector_type(W), aligned(sizeof(T))));
   float x[W];
   __device__ __forceinline__ static Raw read(const T *p) {
     return *reinterpret_cast<const Raw *>(p);
@@ -98,28 +98,29 @@ template <typename T, int W> struct Piece {
     else
       *reinterpret_cast<Raw *>(p) = v;
   }
-  __device__ __forceinline__ void load(const T *p) {
-    const Raw v = read(p);
+  __device__ __forceinline__ void take(Raw v) {
 #pragma unroll
     for (int i = 0; i < W; ++i)
       x[i] = tof((T)v[i]);
   }
-  __device__ __forceinline__ void store(T *p) const {
+  __device__ __forceinline__ void load(const T *p) { take(read(p)); }
+  __device__ __forceinline__ void store(T *p) const { write(p, raw()); }
+  __device__ __forceinline__ Raw raw() const {
     if constexpr (sizeof(T) == 2 && W % 2 == 0) {
       typedef uint32_t Words __attribute__((ext_vector_type(W / 2)));
       Words v;
 #pragma unroll
       for (int i = 0; i < W / 2; ++i)
         v[i] = cvt_pk_bf16(x[2 * i], x[2 * i + 1]);
-      write(p, __builtin_bit_cast(Raw, v));
+      return __builtin_bit_cast(Raw, v);
     } else if constexpr (sizeof(T) == 2) {
-      write(p, Raw{f32_to_bf16(x[0])});
+      return Raw{f32_to_bf16(x[0])};
     } else {
       Raw v;
 #pragma unroll
       for (int i = 0; i < W; ++i)
         v[i] = x[i];
-      write(p, v);
+      return v;
     }
   }
 };
@@ -130,12 +131,15 @@ __device__ __forceinline__ void turn(float &x, float &y, const Turn &t) {
   y = fmaf(a, t.sin, b * t.cos);
 }
 
-// A unit of a head: two pieces of W elements that turn with each other, or with
-// NEIGHBOURS one that holds its pairs; or one that is copied.
+// A head is cut into pieces of W elements.  Of neighbours one holds its pairs, the
+// last one maybe with elements that are copied; else two turn with each other, and
+// those of the second half start anywhere, as do those that are copied; what is left
+// over of either goes in pieces of half the size, a quarter and so on.  (45,248
+// tokens of 9 bf16 heads of 96, 25 pairs of neighbours: 26.2 us, in pieces of one
+// pair 85.)
 template <typename T, int W, bool NEIGHBOURS>
 __global__ __launch_bounds__(kThreads) void rotary_turn(RotaryArgs a) {
   extern __shared__ Turn turns[]; // [per][pairs]
-  using P = Piece<T, W>;
   const int first = blockIdx.x * a.per;
   const int count = a.tokens - first < a.per ? a.tokens - first : a.per;
   for (int i = threadIdx.x; i < count * a.pairs; i += kThreads) {
@@ -151,11 +155,11 @@ __global__ __launch_bounds__(kThreads) void rotary_turn(RotaryArgs a) {
     turns[i] = t;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < count * (int)a.token_units.by; i += kThreads) {
-    const int token = (int)a.token_units.quotient(i);
-    int u = i - token * (int)a.token_units.by;
-    int head = (int)a.head_units.quotient(u);
-    u -= head * (int)a.head_units.by;
+  for (int n = threadIdx.x; n < count * (int)a.token_pieces.by; n += kThreads) {
+    const int token = (int)a.token_pieces.quotient(n);
+    int u = n - token * (int)a.token_pieces.by;
+    int head = (int)a.head_pieces.quotient(u);
+    u -= head * (int)a.head_pieces.by;
     const bool key = head >= a.query_heads;
     const Heads &h = key ? a.key : a.query;
     head -= key ? a.query_heads : 0;
@@ -163,27 +167,62 @@ __global__ __launch_bounds__(kThreads) void rotary_turn(RotaryArgs a) {
     const T *from = static_cast<const T *>(h.from) + at * h.from_token +
                     head * h.from_head;
     T *to = static_cast<T *>(h.to) + at * h.to_token + head * h.to_head;
-    if (u >= a.turned) {
-      const int x = 2 * a.pairs + (u - a.turned) * W;
-      P::write(to + x, P::read(from + x));
-    } else if constexpr (NEIGHBOURS) {
-      const Turn *t = turns + token * a.pairs + u * (W / 2);
-      P p;
-      p.load(from + u * W);
+    const Turn *t = turns + token * a.pairs;
+    const bool copy = u >= a.turned;
+    if constexpr (NEIGHBOURS) {
+      using P = Piece<T, W>;
+      const auto raw = P::read(from + u * W);
+      auto out = raw;
+      if (!copy) {
+        const int some = a.pairs - u * (W / 2); // its pairs
+        P p;
+        p.take(raw);
 #pragma unroll
-      for (int e = 0; e < W; e += 2)
-        turn(p.x[e], p.x[e + 1], t[e / 2]);
-      p.store(to + u * W);
+        for (int e = 0; e < W; e += 2)
+          turn(p.x[e], p.x[e + 1],
+               t[u * (W / 2) + (e / 2 < some ? e / 2 : 0)]);
+        out = p.raw();
+        if (some < W / 2)
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            out[e] = e / 2 < some ? out[e] : raw[e];
+      }
+      P::write(to + u * W, out);
     } else {
-      const Turn *t = turns + token * a.pairs + u * W;
-      P p, q;
-      p.load(from + u * W);
-      q.load(from + u * W + a.pairs);
+      // N elements of either half, or N that are copied
+      auto piece = [&](auto width, int i) __attribute__((always_inline)) {
+        constexpr int N = decltype(width)::value;
+        Piece<T, N> p, q;
+        if (copy) {
+          p.write(to + i, p.read(from + i));
+          return;
+        }
+        p.load(from + i);
+        q.load(from + i + a.pairs);
 #pragma unroll
-      for (int e = 0; e < W; ++e)
-        turn(p.x[e], q.x[e], t[e]);
-      p.store(to + u * W);
-      q.store(to + u * W + a.pairs);
+        for (int e = 0; e < N; ++e)
+          turn(p.x[e], q.x[e], t[i + e]);
+        p.store(to + i);
+        q.store(to + i + a.pairs);
+      };
+      int i = copy ? 2 * a.pairs + (u - a.turned) * W : u * W;
+      const int left = (copy ? a.d : a.pairs) - i;
+      if (left >= W) {
+        piece(std::integral_constant<int, W>{}, i);
+        continue;
+      }
+      if constexpr (W > 4)
+        if (left & 4) {
+          piece(std::integral_constant<int, 4>{}, i);
+          i += 4;
+        }
+      if constexpr (W > 2)
+        if (left & 2) {
+          piece(std::integral_constant<int, 2>{}, i);
+          i += 2;
+        }
+      if (left & 1)
+        piece(std::integral_constant<int, 1>{}, i);
     }
   }
 }
@@ -256,41 +295,40 @@ int rotary_entry(const int32_t *positions, const float *frequencies,
   a.d = (int)d;
   a.pairs = (int)pairs;
   a.back = back;
-  // the widest pieces that the pairs are made of, up to 16 bytes
-  const int64_t run = interleaved ? 2 * pairs : pairs;
-  int64_t width = 16 / (int64_t)sizeof(T);
-  while (run % width != 0)
-    width /= 2;
-  a.turned = (int)(run / width);
-  a.units = a.turned + (int)((d - 2 * pairs) / width);
-  a.head_units = Divisor((uint32_t)a.units);
-  a.token_units = Divisor((uint32_t)(a.units * a.heads));
-  // (two units a thread; with four 16,384 and 32,760 tokens take 4 to 10 % longer)
-  a.per = (int)std::clamp<int64_t>(2 * kThreads / (a.units * a.heads), 1, 16);
+  // Pieces of 16 bytes, or of 8 where that makes for less work: the pieces, times
+  // the rounds of a wave that holds some of what is left over (1, and each smaller
+  // size that there is).  (bf16, heads of 40: 59,464 tokens of 5, 20 pairs, 13.9 us
+  // and 12.5; 46,588 of 4, 5 pairs, 13.3, with single elements 26; of 80: 16,384 of
+  // 20, 10 pairs, 30.7, in twos 37.)
+  constexpr int kWide = 16 / sizeof(T);
+  const int64_t copied = d - 2 * pairs;
+  auto pieces = [&](int64_t w) {
+    return sw::ceil_div(pairs, w) + sw::ceil_div(copied, w);
+  };
+  auto work = [&](int64_t w) {
+    const int64_t rest = pairs % w | copied % w;
+    return pieces(w) * (1 + (rest & 1) + (rest >> 1 & 1) + (rest >> 2));
+  };
+  const bool narrow = !interleaved && work(kWide / 2) < work(kWide);
+  const int64_t width = narrow ? kWide / 2 : kWide;
+  const int64_t all = interleaved ? d / width : pieces(width);
+  a.turned = (int)sw::ceil_div((interleaved ? 2 : 1) * pairs, width);
+  a.head_pieces = Divisor((uint32_t)all);
+  a.token_pieces = Divisor((uint32_t)(all * a.heads));
+  // (two pieces a thread; with four 16,384 and 32,760 tokens take 4 to 10 % longer)
+  a.per = (int)std::clamp<int64_t>(2 * kThreads / (all * a.heads), 1, 16);
   const int64_t grid = sw::ceil_div(tokens, a.per);
   if (int rc = sw::check_flat_grid(grid, kThreads, what))
     return rc;
   const hipStream_t st = sw::as_stream(stream);
   const dim3 g((unsigned)grid);
   const size_t lds = a.per * a.pairs * sizeof(Turn);
-  auto launch = [&](auto w) {
-    constexpr int W = decltype(w)::value;
-    if constexpr (W > 1)
-      if (interleaved) {
-        rotary_turn<T, W, true><<<g, kThreads, lds, st>>>(a);
-        return;
-      }
-    rotary_turn<T, W, false><<<g, kThreads, lds, st>>>(a);
-  };
-  if constexpr (sizeof(T) == 2)
-    if (width == 8)
-      launch(std::integral_constant<int, 8>{});
-  if (width == 4)
-    launch(std::integral_constant<int, 4>{});
-  else if (width == 2)
-    launch(std::integral_constant<int, 2>{});
-  else if (width == 1)
-    launch(std::integral_constant<int, 1>{});
+  if (interleaved)
+    rotary_turn<T, kWide, true><<<g, kThreads, lds, st>>>(a);
+  else if (narrow)
+    rotary_turn<T, kWide / 2, false><<<g, kThreads, lds, st>>>(a);
+  else
+    rotary_turn<T, kWide, false><<<g, kThreads, lds, st>>>(a);
   return sw::launch_check(what);
 }
 

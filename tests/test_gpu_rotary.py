@@ -5,6 +5,8 @@ a quarter turn rounds once, u pi / 4 of it at most, then about two roundings of
 the series of sizes up to 1), a result (x, y) by 4 u (|x| + |y|) for both and
 another u for its product and sum each, and half a step of its type.
 """
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -123,6 +125,37 @@ def test_pieces_of_every_width(dev, dtype, interleaved, d, pairs):
     sw.rotary(pg, fg, ag, qg, kg, qo, ko, interleaved)
     check("query", qo, *turned(q, p, f, ax, interleaved))
     check("key", ko, *turned(k, p, f, ax, interleaved))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,pairs", [(40, 5), (40, 20), (96, 25), (128, 1),
+                                     (8, 3), (16, 7), (72, 33), (128, 63)])
+def test_pieces_that_leave_some_over(dev, dtype, interleaved, d, pairs):
+    """What whole pieces leave over of the pairs and of what is copied, within
+    rows of more than the heads, in place too; copied elements keep their bits."""
+    say(f"rotary rest {dtype} {interleaved} {d} {pairs}")
+    p, f, ax, q, k = make(dtype, 333, 3, 3, 1, d, pairs, seed=d + pairs)
+    word = torch.int16 if dtype == "bf16" else torch.int32
+    odd = torch.tensor([-0.0, math.nan, math.inf, -math.inf], dtype=q.dtype)
+    for x in (q, k):
+        n = min(4, d - 2 * pairs)
+        x[5::7, :, 2 * pairs:2 * pairs + n] = odd[:n]
+    pg, fg, ag, qg, kg = on_gpu(p, f, ax, q, k)
+    wide = torch.full((333, 4, d + 8), 7.0, dtype=q.dtype, device=qg.device)
+    qo, ko = wide[:, :3, :d], torch.full_like(kg, 7.0)
+    sw.rotary(pg, fg, ag, qg, kg, qo, ko, interleaved)
+    for name, x, y in (("query", q, qo), ("key", k, ko)):
+        some = slice(0, 2 * pairs)
+        want, bound = turned(x.clone().nan_to_num(0.0, 0.0, 0.0), p, f, ax,
+                             interleaved)
+        check(name, y[..., some], want[..., some], bound[..., some])
+        assert torch.equal(y[..., 2 * pairs:].cpu().contiguous().view(word),
+                           x[..., 2 * pairs:].contiguous().view(word))
+    assert (wide[:, 3] == 7.0).all() and (wide[..., d:] == 7.0).all()
+    sw.rotary(pg, fg, ag, qg, kg, qg, kg, interleaved)
+    assert torch.equal(qg.view(word), qo.contiguous().view(word))
+    assert torch.equal(kg.view(word), ko.view(word))
 
 
 @pytest.mark.parametrize("far", [2 ** 20, 2 ** 31 - 1])
