@@ -307,8 +307,9 @@ template <int D> struct ValueTile {
   static constexpr int kBytes = 32 * kPitch;
   __device__ static __forceinline__ int place(int row, int chunk) {
     const int swizzle =
-        D > 64 ? (row & 4) << 1 | (row & 1) << 2 | (row & 2) | (row >> 2 & 1)
-               : (row & 2) << 1 | (row >> 1 & 2) | (row & 1);
+        D > 64   ? (row & 4) << 1 | (row & 1) << 2 | (row & 2) | (row >> 2 & 1)
+        : D > 32 ? (row & 2) << 1 | (row >> 1 & 2) | (row & 1)
+                 : row >> 1 & 3;
     return row * kPitch + ((chunk ^ swizzle) << 4);
   }
 };
@@ -359,7 +360,11 @@ template <typename T, int D> struct Fp4Parts {
   static constexpr int kWaveBytes =
       Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
   static constexpr int kBytes = 4 * kWaveBytes;
-  static constexpr int kWaves = D > 64 ? 3 : 4;
+  // waves of a SIMD (heads of 32: 46 sequences of up to 28,000 keys, 24 over 8, bf16
+  // 129 us with 5, 145 with 4, and 142 as heads of 64; fp32 spills with 5)
+  static constexpr int kWaves = D > 64                        ? 3
+                                : D > 32 || sizeof(T) == 4 ? 4
+                                                              : 5;
 };
 
 template <typename T, int D, int ROWS, bool STREAM>
@@ -967,7 +972,7 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
     return p;
   p.shares = shares;
   const int64_t all = p.units * p.shares * 2 * p.block;
-  p.sums = all * (d <= 64 ? 64 : 128);
+  p.sums = all * (d <= 32 ? 32 : d <= 64 ? 64 : 128);
   p.stats = all * 2;
   return p;
 }
@@ -1024,8 +1029,9 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
     return SW_OK;
   const Plan p = plan(sequences, page_size * table_width, query_heads,
                       key_heads, d, window, sinks,
-                      d <= 64 ? Fp4Parts<T, 64>::kWaves
-                              : Fp4Parts<T, 128>::kWaves);
+                      d <= 32   ? Fp4Parts<T, 32>::kWaves
+                      : d <= 64 ? Fp4Parts<T, 64>::kWaves
+                                : Fp4Parts<T, 128>::kWaves);
   if (p.bytes() > 0 && (!workspace || !sw::aligned16(workspace) ||
                         workspace_bytes < p.bytes()))
     return sw::fail(SW_ERR_INVALID_ARGUMENT,
@@ -1090,7 +1096,9 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
     else
       fp4_cache_parts<T, D, kRows, false><<<g, kThreads, 0, st>>>(args);
   };
-  if (d <= 64)
+  if (d <= 32)
+    launch(std::integral_constant<int, 32>{});
+  else if (d <= 64)
     launch(std::integral_constant<int, 64>{});
   else
     launch(std::integral_constant<int, 128>{});
@@ -1106,7 +1114,9 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
     else
       fp4_cache_join<T, D, kThreads><<<j, kThreads, 0, st>>>(args);
   };
-  if (d <= 64)
+  if (d <= 32)
+    launch_join(std::integral_constant<int, 32>{});
+  else if (d <= 64)
     launch_join(std::integral_constant<int, 64>{});
   else
     launch_join(std::integral_constant<int, 128>{});
@@ -1124,7 +1134,7 @@ extern "C" int64_t sw_window_attention_decode_fp4_workspace_bytes(
                 window, sinks, 0.0f) != SW_OK)
     return 0;
   return plan(sequences, page_size * table_width, query_heads, key_heads, d,
-              window, sinks, 4).bytes();
+              window, sinks, d <= 32 ? 5 : 4).bytes(); // (the most of any type)
 }
 
 extern "C" int sw_window_attention_decode_fp4_f32(
