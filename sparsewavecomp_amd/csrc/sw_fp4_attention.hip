@@ -92,7 +92,8 @@ __device__ __forceinline__ int sum_to_lane(int v) {
 
 // The tiles of up to 4096 sequences: lane l of a wave has those of number
 // l each to l each + each - 1, the first HELD of them in registers (1, where that
-// is all, or 8: for one sequence the 8 would cost 1.5 us).
+// is all, or 4: with 8 for one sequence a call took 1.5 us longer, for 122 of up to
+// 1,495 keys 21.8 us for 19.8).
 template <int HELD> struct AllTiles {
   const StepArgs &a;
   int each, held[HELD];
@@ -398,8 +399,19 @@ fp4_cache_parts(Fp4StepArgs args) {
   int extent = args.least; // the share's tiles
   bool begun = false; // whether a part of the share is done
   if (args.shares != 0) {
-    my = a.sequences <= kWave ? find_share<1>(args, number)
-                              : find_share<8>(args, number);
+    // (one wave for all: 122 sequences of up to 1,495 keys 21.8 us, 28.5 with each)
+    __shared__ Share share;
+    if (wave == 0) {
+      my = a.sequences <= kWave ? find_share<1>(args, number)
+                                : find_share<4>(args, number);
+      if (lane == 0)
+        share = my;
+    }
+    __syncthreads();
+    my.from = __builtin_amdgcn_readfirstlane(share.from);
+    my.to = __builtin_amdgcn_readfirstlane(share.to);
+    my.seq = __builtin_amdgcn_readfirstlane(share.seq);
+    my.offset = __builtin_amdgcn_readfirstlane(share.offset);
     if (my.from == my.to)
       return;
     extent = my.to - my.from;
@@ -866,9 +878,17 @@ __global__ __launch_bounds__(THREADS) void fp4_cache_join(Fp4StepArgs args) {
   const int seq = (int)(blockIdx.x / of);
   const int head = (int)(blockIdx.x - seq * of) * kHeads +
                    (kHeads > 1 ? wave_in_group() : 0);
-  // (each wave for itself)
-  const Parts parts = a.sequences <= kWave ? parts_of<1>(args, seq)
-                                           : parts_of<8>(args, seq);
+  __shared__ Parts found; // (by one wave for all)
+  if (wave_in_group() == 0) {
+    const Parts p = a.sequences <= kWave ? parts_of<1>(args, seq)
+                                         : parts_of<4>(args, seq);
+    if (lane_id() == 0)
+      found = p;
+  }
+  __syncthreads();
+  const Parts parts{__builtin_amdgcn_readfirstlane(found.first),
+                    __builtin_amdgcn_readfirstlane(found.count),
+                    __builtin_amdgcn_readfirstlane(found.slot)};
   if (parts.count == 1 || head >= a.query_heads)
     return; // (it is written)
   const int hk = head / a.group, in_group = head - hk * a.group;
