@@ -9,13 +9,14 @@
 // than in bf16, for the same products, exponentials and conversions besides.
 //
 // Memory bounds long batches: 64 sequences of up to 20,000 keys, 32 query heads
-// over 8 of 128, bf16, 887 MB, take 149 us in the kernel and 4 in the join, 5.7
+// over 8 of 128, bf16, 887 MB, take 145 us in the kernel and 4 in the join, 5.8
 // TB/s with both; the same loads alone, streamed, take 134.  The matrix cores are
-// busy for 23 % of it, vector instructions for 42 %.  In fp32 (5 sequences, windows
-// of 65,544 keys, 12 heads over 4 of 96, 104 MB: 37 and 4.5 us) three parts of
-// queries and of probabilities are three times the products, which a wave's loads
-// of one tile ahead do not hide.  A short call is its chain of trips (length, page,
-// key) and the join's.
+// busy for 25 % of it, vector instructions for 44 %.  Heads of 64 and 32 are bound
+// by the instructions of a tile, which are not many fewer for its fewer bytes: 64
+// sequences of up to 20,000, 16 heads over 4 of 64, 58 us, 3.9 TB/s.  In fp32 (5
+// sequences, windows of 65,544 keys, 12 heads over 4 of 96, 104 MB: 35 and 4.5 us)
+// three parts of queries and of probabilities are three times the products.  A
+// short call is its chain of trips (length, page, key) and the join's.
 #include "sw_cache.h"
 #include "sw_fp4.h"
 

@@ -6,7 +6,7 @@
 // tokens the chain of reads that leads to a token's page (offsets, length,
 // table).  32,768 tokens of 8 heads of 128, bf16: written in 36 us, 4.7 TB/s, read
 // back in 28, 6 TB/s; a large copy reaches 6.3.  One token of each of 64 sequences:
-// 4.1 and 3.7 us.
+// 3.8 and 3.6 us.
 #include "sw_fp4.h"
 #include "sw_internal.h"
 

@@ -5,8 +5,8 @@
 // gradients are turned by -t.
 //
 // Each element is read and written once, three operations for it: memory bounds
-// this (32,760 tokens of 40 heads of 128, bf16, three axes, 671 MB: 109 us, 6.1
-// TB/s; 16,384 of 20, 168 MB: 26, 6.5; a large copy reaches 6.3; 64 tokens: 3.8).
+// this (32,760 tokens of 40 heads of 128, bf16, three axes, 671 MB: 107 us, 6.2
+// TB/s; 16,384 of 20, 168 MB: 26, 6.5; a large copy reaches 6.3; 64 tokens: 3.1).
 // The angles belong to a token and are shared by its heads, so a
 // workgroup computes those of its tokens first.  They are reduced to a quarter
 // turn in 64 bits: a position of 2^17 times a frequency near 1 has lost 2^-8 of
