@@ -736,8 +736,9 @@ int sw_fp4_cache_read_bf16(
  * the cache means that its keys are not there.  `strides` holds sixteen: the
  * token and head stride of query and of output in elements, then the cache's as
  * above.  fp32 queries meet the codes' values without a rounding (three bf16
- * parts each), and so do their probabilities.  A byte of 254 that no write leaves
- * can give infinities.  How a sequence's keys are split, and so the order of its
+ * parts each), and so do their probabilities.  Under scale bytes of 253 and 254,
+ * which no write leaves, sizes past the types' range are infinite, and so is the sum
+ * of what is seen of them.  How a sequence's keys are split, and so the order of its
  * sums, follows all lengths of the call and the table's width.
  */
 int64_t sw_window_attention_decode_fp4_workspace_bytes(

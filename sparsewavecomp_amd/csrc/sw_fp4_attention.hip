@@ -280,7 +280,7 @@ __device__ __forceinline__ void query_parts(v8f x, v4u (&part)[3]) {
 // Four probabilities as the sum of two bf16 parts, to 2^-15 of each, or of three,
 // to 2^-23: what their upper halves hold, and the rest of it, at the end rounded.
 // The rest of one that is not zero is at least 2^-126, so that an infinity of a
-// value meets no zero.
+// value meets no zero that stands for it.
 template <int N>
 __device__ __forceinline__ void weight_parts(const float *x, v2u (&part)[N]) {
   float r[4] = {x[0], x[1], x[2], x[3]};
@@ -352,7 +352,8 @@ __device__ __forceinline__ void go_first(int all, int left) {
 // 8, half of them of rows that are not there.  A half's probabilities are masked
 // out where the other run's values are multiplied; each column keeps a maximum and
 // sums of its own, joined like a part's at the end.  (171 us for 175; 8 heads a key
-// head 156 for 157.)
+// head 156 for 157.)  Where that leaves sums that are not finite (a zero of these
+// masks times an infinity may be why) each run is multiplied by itself.
 //
 // STREAM: the codes pass by the caches, where no other workgroup reads them: up to
 // 16 rows (166 us, 174 through them; 16 heads a key head 91 and 99); with 32, whose
@@ -561,6 +562,9 @@ fp4_cache_parts(Fp4StepArgs args) {
   const v4u ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 
   auto compute = [&](Data &x, auto careful) __attribute__((always_inline)) {
+    // whether a column's zeros for the other run meet none of its values, which
+    // may be infinite
+    constexpr bool kApart = kHalves && decltype(careful)::value;
     // (keeps the compiler from holding every address in a register)
     asm volatile("" : "+v"(across), "+v"(along));
     // element i of set s: of key 4 g + i of run s, or with halves of this
@@ -684,8 +688,15 @@ fp4_cache_parts(Fp4StepArgs args) {
 #pragma unroll
       for (int i = 0; i < kWeightParts<T>; ++i)
 #pragma unroll
-        for (int b = 2 * pair; b < 2 * pair + 2; ++b)
-          acc[b] = mma16(vf[b], by[i], acc[b]);
+        for (int b = 2 * pair; b < 2 * pair + 2; ++b) {
+          if constexpr (kApart) {
+            const v4f first = mma16(v4u{vf[b].x, vf[b].y, 0, 0}, by[i], acc[b]);
+            const v4f second = mma16(v4u{0, 0, vf[b].z, vf[b].w}, by[i], acc[b]);
+            acc[b] = row_of < ROWS ? first : second;
+          } else {
+            acc[b] = mma16(vf[b], by[i], acc[b]);
+          }
+        }
 #pragma unroll
       for (int i = pair; i < kWeightParts<T>; i += kPairs)
         total = mma16(ones, by[i], total);
@@ -731,6 +742,18 @@ fp4_cache_parts(Fp4StepArgs args) {
         const Runs runs = locate(first);
         Data x, y;
         fetch(x, runs, 0, see.first_key(first));
+        if constexpr (kHalves && decltype(careful)::value) {
+          // (the next tile's loads under way would need registers that the
+          // products of single runs take)
+          for (int k = 0;;) {
+            some |= (x.has[0] | x.has[1]) != 0;
+            compute(x, careful);
+            if (++k == n)
+              break;
+            fetch(x, runs, k, see.first_key(first + 4 * k));
+          }
+          continue;
+        }
         for (int k = 0; k < n; k += 2) {
           go_first(extent, end - (first + 4 * k));
           if (k + 1 < n)
@@ -748,7 +771,8 @@ fp4_cache_parts(Fp4StepArgs args) {
     };
     pass(std::false_type{});
     // (a sum past fp32's range of values whose mean lies within: such columns
-    // once more under lower probabilities, as in the attention of bf16 caches)
+    // once more under lower probabilities, as in the attention of bf16 caches; or
+    // a value that is infinite)
     const bool past = live && !all_finite(acc);
     if (ballot(past) != 0) {
       if (rows16_max(past ? 1.0f : 0.0f) != 0.0f)
