@@ -7,6 +7,8 @@
 // measured no slower: the values of the position and COO SpMV kernels.
 #pragma once
 
+#include "sw_divisor.h"
+
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,26 +44,6 @@ __device__ __forceinline__ int64_t grid_blocks() {
 __device__ __forceinline__ int wave_in_group() {
   return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 }
-
-// Division of numbers below 2^31 by one that the host knows: n m / 2^(31 + s),
-// m = 2^(31 + s) / d rounded up and s the logarithm of d rounded up.  m d passes
-// 2^(31 + s) by less than d <= 2^s, which moves no quotient of such n.
-struct Divisor {
-  uint32_t by, factor, shift;
-  Divisor() : by(1), factor(0), shift(0) {}
-  explicit Divisor(uint32_t d) : by(d), factor(0), shift(0) {
-    uint32_t s = 0;
-    while (((uint64_t)1 << s) < d)
-      ++s;
-    if (s > 0) {
-      factor = (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d);
-      shift = s - 1;
-    }
-  }
-  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
-    return by == 1 ? n : __umulhi(n, factor) >> shift;
-  }
-};
 
 // ---- DPP --------------------------------------------------------------
 // DPP control codes (GFX9 encoding).
