@@ -946,8 +946,12 @@ def _place(stream):
     us instead of 0.8)."""
     torch = _torch or _load_torch()
     if stream is None and torch.cuda.is_initialized():
-        at = torch._C._cuda_getDevice()
-        return at, torch._C._cuda_getCurrentRawStream(at)
+        # (neither name is promised by torch)
+        device = getattr(torch._C, "_cuda_getDevice", None)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if device is not None and raw is not None:
+            at = device()
+            return at, raw(at)
     at = _device_of(stream)
     return at, None if at < 0 else _stream(stream)
 
