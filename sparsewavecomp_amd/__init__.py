@@ -938,6 +938,9 @@ def shared_prefix_attention(key_lengths, page_table, query, prefix_key,
 
 
 _PACK8, _PACK16 = struct.Struct("8q").pack, struct.Struct("16q").pack
+# The library splits no sequence of which so few keys are seen, and asks for no
+# workspace then (its plan in csrc/sw_fp4_attention.hip).
+_FP4_WHOLE = 512
 
 
 def _place(stream):
@@ -1198,7 +1201,7 @@ def window_attention_decode_fp4(key_lengths, page_table, query, key_cache,
         at, d, key_cache, value_cache)
     (q, o), strides = _two(dt, at, shape, query, "query", output, "output")
     need = 0
-    if size * width > 512 < window + sinks:  # (else the answer is 0)
+    if size * width > _FP4_WHOLE < window + sinks:  # (else the answer is 0)
         need = load_library().sw_window_attention_decode_fp4_workspace_bytes(
             sequences, size, width, heads, key_heads, d, window, sinks)
     lengths = _array(key_lengths, torch.int32, at, "key_lengths")

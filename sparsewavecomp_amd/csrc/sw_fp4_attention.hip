@@ -1011,8 +1011,10 @@ Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
   p.units = key_heads * sw::ceil_div(group, p.block);
   const int64_t visible = most_visible(capacity, window, sinks);
   const int64_t shares = std::max<int64_t>(1, kUnits * waves / p.units);
-  if (visible <= std::max<int64_t>(512, std::min<int64_t>(2048, 4096 * sequences / shares)) ||
-      sequences > 4096 ||
+  // (kWhole is _FP4_WHOLE of ../__init__.py)
+  constexpr int64_t kWhole = 512;
+  const int64_t few = std::min<int64_t>(2048, 4096 * sequences / shares);
+  if (visible <= std::max(kWhole, few) || sequences > 4096 ||
       sequences * sw::ceil_div(capacity, 32) > sw::kMostTokens)
     return p;
   p.shares = shares;
