@@ -1,12 +1,12 @@
-// What the kernels of single queries against a key-value cache share: which
-// keys a query sees, a part's result and the join of the parts, and the host's
-// checks.
+// What the kernels of single queries against a key-value cache share, of bf16 and
+// fp32 values and of 4-bit codes: which keys a query sees, what a workgroup
+// leaves of the keys it took, and the host's checks.
 //
-// A sequence's keys are cut into chunks, one workgroup each, and the chunks'
-// (m, l, o) joined:
-//   m = max m_c,  w_c = l_c 2^(m_c - m),  l = sum w_c,  o = sum o_c w_c / l,
-// o_c being a chunk's weighted mean: sums of values, which fp32 may not hold
-// where their mean is finite, stay within a chunk, which sees whether they did.
+// Where several workgroups take a sequence's keys each leaves, of its part c of
+// them, the maximum m_c, the sum l_c and the mean o_c, and they are joined:
+//   m = max m_c,  w_c = l_c 2^(m_c - m),  l = sum w_c,  o = sum o_c w_c / l.
+// Means and not sums of values, which fp32 may not hold where their mean is
+// finite: those stay within a part, which sees whether they did.
 #pragma once
 
 #include "sw_heads.h"
@@ -30,15 +30,14 @@ constexpr int kThreads = 256; // four waves
 constexpr int kRows = 16;     // query rows of a workgroup's part
 constexpr int kTile = 32;     // keys a wave takes at a time
 
-// what lanes without a key read
-__device__ const uint32_t kZeros[8] = {};
-
 struct Cache {
   const void *key, *value;
   int64_t key_page, key_token, key_head; // strides in elements
   int64_t value_page, value_token, value_head;
 };
 
+// (The prefix, `dim` and the parts' numbers and rows are sw_cache_attention.hip's
+// alone.)
 struct StepArgs {
   const int32_t *lengths, *table; // table may be null: page i is sequence i's
   const void *query;
@@ -80,9 +79,6 @@ struct Visible {
 
 __device__ __forceinline__ float rows16_max(float v) { // over lanes l % 16
   return both_halves_max(fmaxf(v, swizzle_xor16(v)));
-}
-__device__ __forceinline__ float rows16_sum(float v) {
-  return both_halves_sum(v + swizzle_xor16(v));
 }
 struct Totals {
   float top[4][kRows], sum[4][kRows], raise[4][kRows];
@@ -158,60 +154,10 @@ store_part(const StepArgs &a, char *lds, Totals &found, float top, float sum,
   }
 }
 
-// Joins the parts of a query head's softmax, 0 .. parts - 1, in a workgroup
-// whose eight half waves take them in turn, DIM / 32 consecutive elements a lane,
-// and are joined in LDS.  `row`: of part i, its o and its (m, l).
+// A row of a part.
 struct PartRow {
   const float *sums, *stats;
 };
-template <typename T, int DIM, typename F>
-__device__ __forceinline__ void join_parts(const StepArgs &a, int seq, int head,
-                                           int parts, F row) {
-  constexpr int N = DIM / 32, kHalves = kThreads / 32;
-  __shared__ float outs[kHalves][DIM], tops[kHalves], totals[kHalves];
-  const int half = threadIdx.x / 32, c = (threadIdx.x % 32) * N;
-  float top = -kInf, l = 0.0f, o[N] = {};
-#pragma unroll 4
-  for (int i = half; i < parts; i += kHalves) {
-    const PartRow r = row(i);
-    const float *sums = r.sums + c;
-    const float m = r.stats[0], to = fmaxf(top, m);
-    const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-    const float add = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-    const float weight = r.stats[1] * a.lower * add;
-    top = to;
-    l = fmaf(l, by, weight);
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      o[e] = fmaf(sums[e], weight, o[e] * by);
-  }
-#pragma unroll
-  for (int e = 0; e < N; ++e)
-    outs[half][c + e] = o[e];
-  if (threadIdx.x % 32 == 0) {
-    tops[half] = top;
-    totals[half] = l;
-  }
-  __syncthreads();
-  if (threadIdx.x >= a.d)
-    return;
-  top = tops[0];
-#pragma unroll
-  for (int i = 1; i < kHalves; ++i)
-    top = fmaxf(top, tops[i]);
-  float x = 0.0f;
-  l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kHalves; ++i) {
-    const float by =
-        tops[i] == top ? 1.0f : __builtin_amdgcn_exp2f(tops[i] - top);
-    l = fmaf(totals[i], by, l);
-    x = fmaf(outs[i][threadIdx.x], by, x);
-  }
-  stv(static_cast<T *>(a.output) + seq * a.output_token +
-          head * a.output_head + threadIdx.x,
-      top == -kInf ? 0.0f : x * (1.0f / l));
-}
 
 // ---- host ------------------------------------------------------------------------
 
@@ -219,15 +165,6 @@ __device__ __forceinline__ void join_parts(const StepArgs &a, int seq, int head,
 inline int64_t most_visible(int64_t capacity, int64_t window, int64_t sinks) {
   return window >= capacity || sinks >= capacity - window ? capacity
                                                           : window + sinks;
-}
-
-// How many keys a part has: n keys for each of `units` workgroups at a time, of
-// which `want` are wanted, in steps, `least` at least.
-inline int64_t part_of(int64_t n, int64_t units, int64_t want, int64_t least,
-                       int64_t step) {
-  const int64_t parts = std::max<int64_t>(1, sw::ceil_div(want, units));
-  const int64_t chunk = std::max(least, sw::ceil_div(n, parts));
-  return std::min<int64_t>(sw::ceil_div(chunk, step) * step, 1 << 30);
 }
 
 int check_sizes(int64_t sequences, int64_t pages, int64_t page_size,
@@ -256,22 +193,6 @@ int check_sizes(int64_t sequences, int64_t pages, int64_t page_size,
   if (!std::isfinite(alpha * kLog2e))
     return sw::fail(SW_ERR_INVALID_ARGUMENT,
                     "alpha must be finite, and alpha log2 e too");
-  return SW_OK;
-}
-
-int check_pages(const char *name, const void *p, int64_t page, int64_t token,
-                int64_t head, int64_t d, int64_t elem, int64_t pages,
-                int64_t heads) {
-  if (pages > 0 && (page < 0 || page > sw::kMostStride))
-    return sw::fail(SW_ERR_INVALID_SHAPE,
-                    "%s page stride must be 0 to 2^40, but got %lld", name,
-                    (long long)page);
-  if (int rc = check_operand(name, p, {token, head}, d, elem, false, pages,
-                             heads))
-    return rc;
-  if (pages > 0 && page * elem % 16 != 0)
-    return sw::fail(SW_ERR_INVALID_ARGUMENT,
-                    "%s must be 16-byte aligned, its strides included", name);
   return SW_OK;
 }
 

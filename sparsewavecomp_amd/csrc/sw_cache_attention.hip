@@ -11,6 +11,12 @@
 
 namespace {
 
+// what lanes without a key read
+__device__ const uint32_t kZeros[8] = {};
+
+__device__ __forceinline__ float rows16_sum(float v) {
+  return both_halves_sum(v + swizzle_xor16(v));
+}
 __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
   const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, (int)v);
   const int hi = __builtin_amdgcn_ds_bpermute(lane * 4, (int)(v >> 32));
@@ -490,6 +496,58 @@ shared_prefix_parts(StepArgs a) {
     cache_part<T, D, false>(a, blockIdx.x - before, lds, found);
 }
 
+// Joins the parts of a query head's softmax, 0 .. parts - 1, in a workgroup
+// whose eight half waves take them in turn, DIM / 32 consecutive elements a lane,
+// and are joined in LDS.  `row`: of part i, its o and its (m, l).
+template <typename T, int DIM, typename F>
+__device__ __forceinline__ void join_parts(const StepArgs &a, int seq, int head,
+                                           int parts, F row) {
+  constexpr int N = DIM / 32, kHalves = kThreads / 32;
+  __shared__ float outs[kHalves][DIM], tops[kHalves], totals[kHalves];
+  const int half = threadIdx.x / 32, c = (threadIdx.x % 32) * N;
+  float top = -kInf, l = 0.0f, o[N] = {};
+#pragma unroll 4
+  for (int i = half; i < parts; i += kHalves) {
+    const PartRow r = row(i);
+    const float *sums = r.sums + c;
+    const float m = r.stats[0], to = fmaxf(top, m);
+    const float by = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+    const float add = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    const float weight = r.stats[1] * a.lower * add;
+    top = to;
+    l = fmaf(l, by, weight);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      o[e] = fmaf(sums[e], weight, o[e] * by);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    outs[half][c + e] = o[e];
+  if (threadIdx.x % 32 == 0) {
+    tops[half] = top;
+    totals[half] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x >= a.d)
+    return;
+  top = tops[0];
+#pragma unroll
+  for (int i = 1; i < kHalves; ++i)
+    top = fmaxf(top, tops[i]);
+  float x = 0.0f;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kHalves; ++i) {
+    const float by =
+        tops[i] == top ? 1.0f : __builtin_amdgcn_exp2f(tops[i] - top);
+    l = fmaf(totals[i], by, l);
+    x = fmaf(outs[i][threadIdx.x], by, x);
+  }
+  stv(static_cast<T *>(a.output) + seq * a.output_token +
+          head * a.output_head + threadIdx.x,
+      top == -kInf ? 0.0f : x * (1.0f / l));
+}
+
 // The parts of a query head: a launch and two trips.  16 parts of 4 sequences and
 // 32 heads 4.4 us, 128 sequences' 8.4 us.
 template <typename T, int DIM>
@@ -511,6 +569,31 @@ __global__ __launch_bounds__(kThreads) void window_cache_join(StepArgs a) {
 }
 
 // ---- host ------------------------------------------------------------------------
+
+// How many keys a part has: n keys for each of `units` workgroups at a time, of
+// which `want` are wanted, in steps, `least` at least.
+inline int64_t part_of(int64_t n, int64_t units, int64_t want, int64_t least,
+                       int64_t step) {
+  const int64_t parts = std::max<int64_t>(1, sw::ceil_div(want, units));
+  const int64_t chunk = std::max(least, sw::ceil_div(n, parts));
+  return std::min<int64_t>(sw::ceil_div(chunk, step) * step, 1 << 30);
+}
+
+int check_pages(const char *name, const void *p, int64_t page, int64_t token,
+                int64_t head, int64_t d, int64_t elem, int64_t pages,
+                int64_t heads) {
+  if (pages > 0 && (page < 0 || page > sw::kMostStride))
+    return sw::fail(SW_ERR_INVALID_SHAPE,
+                    "%s page stride must be 0 to 2^40, but got %lld", name,
+                    (long long)page);
+  if (int rc = check_operand(name, p, {token, head}, d, elem, false, pages,
+                             heads))
+    return rc;
+  if (pages > 0 && page * elem % 16 != 0)
+    return sw::fail(SW_ERR_INVALID_ARGUMENT,
+                    "%s must be 16-byte aligned, its strides included", name);
+  return SW_OK;
+}
 
 // How a call is cut into parts.
 struct Plan {

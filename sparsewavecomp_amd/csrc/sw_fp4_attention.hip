@@ -1106,7 +1106,6 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.key_heads = (int)key_heads;
   a.group = (int)(query_heads / key_heads);
   a.d = (int)d;
-  a.dim = d <= 64 ? 64 : 128;
   a.window = (int)std::min<int64_t>(window, sw::kMostTokens);
   a.sinks = (int)std::min<int64_t>(sinks, sw::kMostTokens);
   a.alpha = alpha;
