@@ -734,8 +734,8 @@ int sw_fp4_cache_read_bf16(
  * sw_window_attention_decode against such a cache: the same keys seen, lengths,
  * page table, clamps, workspace rules and arithmetic.  A page number outside
  * the cache means that its keys are not there.  `strides` holds sixteen: the
- * token and head stride of query and of output in elements, then the cache's as
- * above.  fp32 queries meet the codes' values without a rounding (three bf16
+ * token and head stride of query and of output in elements (not those of a write's
+ * keys and values), then the cache's as above.  fp32 queries meet the codes' values without a rounding (three bf16
  * parts each), and so do their probabilities.  Under scale bytes of 253 and 254,
  * which no write leaves, sizes past the types' range are infinite, and so is the sum
  * of what is seen of them.  How a sequence's keys are split, and so the order of its
