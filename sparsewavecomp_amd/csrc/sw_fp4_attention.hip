@@ -9,14 +9,16 @@
 // than in bf16, for the same products, exponentials and conversions besides.
 //
 // Memory bounds long batches: 64 sequences of up to 20,000 keys, 32 query heads
-// over 8 of 128, bf16, 887 MB, take 145 us in the kernel and 4 in the join, 5.8
-// TB/s with both; the same loads alone, streamed, take 134.  The matrix cores are
-// busy for 25 % of it, vector instructions for 44 %.  Heads of 64 and 32 are bound
-// by the instructions of a tile, which are not many fewer for its fewer bytes: 64
-// sequences of up to 20,000, 16 heads over 4 of 64, 58 us, 3.9 TB/s.  In fp32 (5
-// sequences, windows of 65,544 keys, 12 heads over 4 of 96, 104 MB: 35 and 4.5 us)
-// three parts of queries and of probabilities are three times the products.  A
-// short call is its chain of trips (length, page, key) and the join's.
+// over 8 of 128, bf16, 887 MB, take 154 us in the kernel and 5 in the join (the
+// medians of 22; at best 144 and 4), 5.6 TB/s with both; the same loads alone,
+// streamed, take 134.  The matrix cores are busy for 25 % of it, vector instructions
+// for 44 %.  Heads of 64 and 32 are bound by the instructions of a tile, which are
+// not many fewer for its fewer bytes: 64 sequences of up to 20,000, 16 heads over 4
+// of 64, 57 us, 3.9 TB/s.  In fp32 (5 sequences, windows of 65,544 keys, 12 heads
+// over 4 of 96, 104 MB: 36 and 5 us) three parts of queries and of probabilities
+// are three times the products.  A short call is its chain of trips (length, page,
+// key) and the join's, and so is each sequence's part of a batch of short ones: 64
+// of up to 1,024 keys, 32 heads over 8 of 128, take 19 us, their bytes 6.5.
 #include "sw_cache.h"
 #include "sw_fp4.h"
 
@@ -137,8 +139,8 @@ template <int HELD> struct AllTiles {
 // How a unit's tiles are split: `most` for a workgroup, and whether none takes
 // those of two sequences (`whole`: a sequence's tiles are divided among its
 // shares).  A second sequence costs a workgroup about as much as 8 tiles (4
-// sequences of up to 8,192 keys 21.6 us, whole 18.6; 32 of up to 2,048 25.7 and
-// 23.3; 64 of up to 20,000, over four key heads of 64, 61.4 and 68.5), so that
+// sequences of up to 8,192 keys 21.4 us, whole 19.2; 32 of up to 2,048 23.3 and
+// 21.0; 64 of up to 20,000, over four key heads of 64, 56.5 and 58.2), so that
 // shares may be longer by as much to keep them whole: by as little as does, where
 // a wave has all sequences' tiles in registers.
 struct Split {
@@ -319,7 +321,7 @@ template <int D> struct ValueTile {
 // Of a SIMD's waves the one with most left to do goes first.  Left to themselves
 // the oldest does: the three workgroups of a compute unit, which have the same to
 // do, ended after 111, 124 and 142 us and left it half idle (124, 132 and 141 so,
-// and in all 169 us -> 163; heads of 64 60.4 -> 57.2).  Later thresholds and quarters
+// and in all 166.6 us -> 163.1; heads of 64 59.7 -> 57.1).  Later thresholds and quarters
 // balance less.
 __device__ __forceinline__ void go_first(int all, int left) {
   if (left > all / 2)
@@ -364,7 +366,7 @@ template <typename T, int D> struct Fp4Parts {
       Tile::kBytes > kRows * D * 4 ? Tile::kBytes : kRows * D * 4;
   static constexpr int kBytes = 4 * kWaveBytes;
   // waves of a SIMD (heads of 32: 46 sequences of up to 28,000 keys, 24 over 8, bf16
-  // 129 us with 5, 145 with 4, and 142 as heads of 64; fp32 spills with 5)
+  // 88 us with 5, 98 with 4, and 92 as heads of 64; fp32 spills with 5)
   static constexpr int kWaves = D > 64                        ? 3
                                 : D > 32 || sizeof(T) == 4 ? 4
                                                               : 5;
@@ -1001,7 +1003,8 @@ constexpr int64_t kUnits = 256, kLeast = 8;
 // 21.8 and 25.4, 64 of 1,024 22 and 18.7, 64 of 2,048 33 and 30.6, 256 of 2,048 89
 // and 84, 256 of 4,096 145.5 and 146.6; fp32: 64 of 1,024 26 and 23, 64 of 2,048
 // 38.3 and 37.2, 256 of 4,096 170 and 172.  400 of 2,048, 16 heads over one: 38.5 and
-// 31.)
+// 31.)  Either way such batches are far from their bytes' time: 32 of 2,048 6.7, 64 of
+// 1,024 6.5, of 2,048 14, 256 of 1,024 28 (50 here), of 2,048 55.
 Plan plan(int64_t sequences, int64_t capacity, int64_t query_heads,
           int64_t key_heads, int64_t d, int64_t window, int64_t sinks,
           int64_t waves) {
@@ -1123,8 +1126,9 @@ int fp4_step_entry(const int32_t *key_lengths, const int32_t *page_table,
   a.stats = a.sums + p.sums;
   const int64_t grid = p.units * (p.shares ? p.shares : sequences);
   // Few rows take a workgroup of 1024 each (4 sequences of up to 100,000 keys, 12
-  // heads: 33.9 us of both kernels, 36 with 256); one of four rows else (256
-  // sequences, 32 heads: the join 19.8 us with one of 256 for each row).
+  // heads over 4 of 128, bf16: 32.5 us of both kernels, 37.3 with a wave each; up to
+  // 25,000 18.9 and 23.5); one of four rows else (256 sequences, 32 heads: the join
+  // 19.8 us with one of 256 for each row).
   const bool few = sequences * query_heads <= 512;
   const int64_t join =
       sequences * (few ? query_heads

@@ -5,8 +5,8 @@
 // and 17/32 on the other, and compute little: memory bounds them, and for few
 // tokens the chain of reads that leads to a token's page (offsets, length,
 // table).  32,768 tokens of 8 heads of 128, bf16: written in 36 us, 4.7 TB/s, read
-// back in 28, 6 TB/s; a large copy reaches 6.3.  One token of each of 64 sequences:
-// 3.8 and 3.6 us.
+// back in 29, 5.9 TB/s; a large copy reaches 6.3.  One token of each of 64 sequences:
+// 4.4 and 4.0 us.
 #include "sw_fp4.h"
 #include "sw_internal.h"
 

@@ -5,8 +5,8 @@
 // gradients are turned by -t.
 //
 // Each element is read and written once, three operations for it: memory bounds
-// this (32,760 tokens of 40 heads of 128, bf16, three axes, 671 MB: 107 us, 6.2
-// TB/s; 16,384 of 20, 168 MB: 26, 6.5; a large copy reaches 6.3; 64 tokens: 3.1).
+// this (32,760 tokens of 40 heads of 128, bf16, three axes, 671 MB: 109 us, 6.1
+// TB/s; 16,384 of 20, 168 MB: 26, 6.5; a large copy reaches 6.3; 64 tokens: 3.5).
 // The angles belong to a token and are shared by its heads, so a
 // workgroup computes those of its tokens first.  They are reduced to a quarter
 // turn in 64 bits: a position of 2^17 times a frequency near 1 has lost 2^-8 of
@@ -299,7 +299,8 @@ int rotary_entry(const int32_t *positions, const float *frequencies,
   // the rounds of a wave that holds some of what is left over (1, and each smaller
   // size that there is).  (bf16, heads of 40: 59,464 tokens of 5, 20 pairs, 13.9 us
   // and 12.5; 46,588 of 4, 5 pairs, 13.3, with single elements 26; of 80: 16,384 of
-  // 20, 10 pairs, 30.7, in twos 37.)
+  // 20, 10 pairs, 30.6, in twos 37, where the bytes take 16.6: pairs that are no
+  // whole pieces, whose second halves start off their alignment, cost that much.)
   constexpr int kWide = 16 / sizeof(T);
   const int64_t copied = d - 2 * pairs;
   auto pieces = [&](int64_t w) {
