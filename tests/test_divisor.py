@@ -11,7 +11,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
-DRIVER = r'''
+PROGRAM = r'''
 #include "sw_divisor.h"
 #include <cstdio>
 int main() {
@@ -31,7 +31,7 @@ def divide(tmp_path_factory):
         pytest.skip("g++ and the HIP headers are needed")
     d = tmp_path_factory.mktemp("divisor")
     src, exe = d / "divisor.cpp", d / "divisor"
-    src.write_text(DRIVER)
+    src.write_text(PROGRAM)
     subprocess.run([gxx, "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__",
                     "-I/opt/rocm/include",
                     "-I" + os.path.join(ROOT, "sparsewavecomp_amd", "csrc"),
